@@ -55,13 +55,18 @@ enum irx_family {
     IRX_FAM_ROWOP = 4,         /* row statistics, then an elementwise pass over the row */
     IRX_FAM_MATMUL = 5,        /* C[M,N] = A[M,K] B[K,N] */
     IRX_FAM_ATTENTION = 6,     /* O = softmax(Q K^T * scale [causal]) V over [B,H,S,D] */
-    IRX_FAM_KIR = 7            /* any other graph the reference lowers: its statements written out
+    IRX_FAM_KIR = 7,           /* any other graph the reference lowers: its statements written out
                                 * as the graph's own sm_100a kernel (NVRTC), on the KIR's launch
                                 * geometry; runs as one launch (shard 0 of any count) */
+    /* the serving operators, compiled from a descriptor instead of KIR (further down) */
+    IRX_FAM_DECODE = 8,        /* attention of one new token per sequence over a paged cache */
+    IRX_FAM_KV_APPEND = 9,     /* new tokens' keys and values into their pages */
+    IRX_FAM_KV_COPY = 10,      /* page copies of a paged cache */
+    IRX_FAM_MATVEC4 = 11       /* y = x W^T with 4-bit weights and group scales */
 };
 
-enum irx_dtype { IRX_DT_F32 = 1, IRX_DT_BF16 = 2 };
-enum irx_argkind { IRX_ARG_IN = 0, IRX_ARG_CONST = 1, IRX_ARG_OUT = 2 };
+enum irx_dtype { IRX_DT_F32 = 1, IRX_DT_BF16 = 2, IRX_DT_I32 = 4, IRX_DT_U8 = 5 };
+enum irx_argkind { IRX_ARG_IN = 0, IRX_ARG_CONST = 1, IRX_ARG_OUT = 2, IRX_ARG_WORK = 3 };
 
 /* "irptx-b200 <version>". Replaces `irptx --version` (src/main.c:56-59). */
 IRX_API const char *irx_version(void);
@@ -93,8 +98,92 @@ IRX_API int irx_plan_describe(const irx_plan_t *plan, char *buf, size_t cap);
  * attention; causal attention counts half the score matrix). */
 IRX_API int irx_plan_work(const irx_plan_t *plan, double *bytes, double *flops);
 
+/* ---- serving operators ----
+ *
+ * What a decoding program runs between KIR graphs. Each is compiled from a descriptor into an
+ * ordinary plan: irx_plan_arg, _describe, _work, _units, irx_launch and irx_launch_shard take it,
+ * with the argument order stated below. They are device-side only: irx_run_host refuses them (E093).
+ * Nothing on the host reads lengths, tables or positions, so a launch can be captured in a CUDA
+ * graph and replayed while their contents change. Indices are checked on the device: one outside
+ * the cache is skipped and reported by irx_check as E093. No counterpart in the reference.
+ *
+ * A paged cache is two pools, keys and values, of `pages` pages of page_size tokens, each token
+ * `heads` rows of head_dim contiguous elements. The strides, in elements, place page p, head h and
+ * slot t of a page at p * page_stride + h * head_stride + t * token_stride; they must not make
+ * rows overlap. All three zero mean [pages, heads, page_size, head_dim], packed. The table is int32
+ * [batch, table_cols]: the page of tokens [i * page_size, (i + 1) * page_size) of a sequence is
+ * its entry i. Only entries that a length or position reaches are read. */
+typedef struct irx_kv_cache {
+    int dtype;                       /* IRX_DT_BF16 or IRX_DT_F32 */
+    int heads, head_dim, page_size;  /* key-value heads; head_dim up to 256 */
+    long long pages;
+    long long page_stride, head_stride, token_stride;
+    int batch, table_cols;           /* unused by irx_compile_kv_copy */
+} irx_kv_cache_t;
+
+/* Decode attention: the newest token of each sequence (position lens[b] - 1) attends to its cache.
+ * Args: q [batch, heads, head_dim] (q_stride elements from one sequence to the next; 0: packed),
+ * k pool, v pool, table, lens int32 [batch], out [batch, heads, head_dim] (packed, the cache's
+ * dtype), with `lse` != 0 the natural log of each row's sum of exps, f32 [batch, heads], and last
+ * the workspace (IRX_DT_U8; its elements are its bytes). Query head h reads key-value head
+ * h / (heads / cache heads). window > 0 hides the keys before position lens[b] - window, except
+ * the first `sinks`. A sequence of length 0 gives zeros (and -inf). The workspace must be zero
+ * before its first launch and is left ready for the next; launches that may overlap need one
+ * each. The result is the same bits for the same inputs on the same GPU. Units: key-value heads. */
+IRX_API int irx_compile_decode(const irx_kv_cache_t *cache, int heads, long long q_stride, float scale, int window, int sinks,
+                               int lse, irx_plan_t *plan);
+
+/* Append: token i's keys and values go to sequence seq[i], position pos[i]; pos[i] < 0 is padding.
+ * Args: k, v [tokens, heads, head_dim] (`stride` elements from one token to the next; 0: packed),
+ * seq, pos int32 [tokens], table, k pool, v pool (the pools are updated in place). Two tokens of one
+ * launch must not go to one place. Units: tokens. */
+IRX_API int irx_compile_kv_append(const irx_kv_cache_t *cache, long long tokens, long long stride, irx_plan_t *plan);
+
+/* Page copy, in both pools and in `layers` layers whose pools lie layer_stride elements apart
+ * (0: packed): for each pair (src, dst), page dst becomes a copy of page src. (-1, -1) is padding. A
+ * page must not be the destination of one pair and in another pair of the launch; irx_pages
+ * makes such lists. Args: pairs int32 [pairs, 2], k pools, v pools (updated in place). Units: pairs. */
+IRX_API int irx_compile_kv_copy(const irx_kv_cache_t *cache, long long pairs, int layers, long long layer_stride, irx_plan_t *plan);
+
+/* y[m, n] = sum over k of x[m, k] * s[n, k / group] * (q[n, k] - z[n, k / group]).
+ * Args: x [m, k] (x_stride elements between rows; 0: packed), w uint8 [n, ceil(k / 2)] (w_stride bytes
+ * between rows; 0: packed), two weights to a byte, the even k in its low four bits; scales [n,
+ * ceil(k / group)]; with `zeros` != 0 the zero points, uint8 of the same shape, values 0 to 15 (8
+ * otherwise); y [m, n], packed, of x's dtype. Weights are used as they are (not rounded again), sums
+ * are f32. Units: rows of w. */
+typedef struct irx_matvec4 {
+    int dtype, scale_dtype;          /* IRX_DT_BF16 or IRX_DT_F32 */
+    long long m, n, k;
+    int group, zeros;
+    long long x_stride, w_stride;
+} irx_matvec4_t;
+IRX_API int irx_compile_matvec4(const irx_matvec4_t *desc, irx_plan_t *plan);
+
+/* The host side of a paged cache: pages handed out, shared by forks, copied when a shared page is
+ * written to, returned and compacted. It keeps numbers only; the caller uploads irx_pages_table
+ * (int32 [max_seqs, table_cols], -1 where nothing is held) and runs the (src, dst) pairs through
+ * a plan of irx_compile_kv_copy before the launches that follow. One owner; not thread-safe.
+ * irx_pages_new, _table: NULL on failure. irx_pages_open, _fork: the new sequence's row, or -1.
+ * irx_pages_extend grows a sequence by `tokens` (all or nothing; E094 when the pool is out of
+ * pages) and sets pair to the copy its first new token needs, or (-1, -1). irx_pages_close returns
+ * a sequence's pages. irx_pages_compact moves the live pages to the front of the pool and returns
+ * how many moves it wrote into `pairs` (at most cap), or -1 with nothing changed. irx_pages_len
+ * is -1 for a sequence that is not open. */
+typedef struct irx_pages irx_pages_t;
+IRX_API irx_pages_t *irx_pages_new(int pages, int page_size, int max_seqs, int table_cols);
+IRX_API void irx_pages_delete(irx_pages_t *m);
+IRX_API int irx_pages_open(irx_pages_t *m);
+IRX_API int irx_pages_extend(irx_pages_t *m, int seq, int tokens, int pair[2]);
+IRX_API int irx_pages_fork(irx_pages_t *m, int seq);
+IRX_API int irx_pages_close(irx_pages_t *m, int seq);
+IRX_API int irx_pages_compact(irx_pages_t *m, int *pairs, int cap);
+IRX_API int irx_pages_free(const irx_pages_t *m);
+IRX_API int irx_pages_len(const irx_pages_t *m, int seq);
+IRX_API const int *irx_pages_table(const irx_pages_t *m);
+
 /* How many independent shard units the plan has: elements/8 (pointwise), rows (reductions,
- * row ops), 256-column blocks (matmul), batch*head (attention), element blocks (full sum). */
+ * row ops), 256-column blocks (matmul), batch*head (attention), element blocks (full sum); the
+ * serving operators state theirs above. */
 IRX_API long long irx_plan_units(const irx_plan_t *plan);
 
 /* Queue the plan on `stream` with one device pointer per KIR arg (args[i] for arg i). Outputs

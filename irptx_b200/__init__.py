@@ -19,15 +19,15 @@ import re
 from dataclasses import dataclass
 
 __all__ = ["compile", "compile_generic", "Plan", "IrxError", "IrxUnavailable", "library_path", "version", "check",
-           "FAMILIES", "kir_author"]
+           "FAMILIES", "kir_author", "KvCache", "Pages", "decode", "kv_append", "kv_copy", "matvec4", "pack4"]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB = None
 
 FAMILIES = {0: "none", 1: "pointwise", 2: "reduce_all", 3: "reduce_rows", 4: "rowop", 5: "matmul",
-            6: "attention", 7: "kir"}
-_DT = {1: "f32", 2: "bf16"}
-_KIND = {0: "in", 1: "const", 2: "out"}
+            6: "attention", 7: "kir", 8: "decode", 9: "kv_append", 10: "kv_copy", 11: "matvec4"}
+_DT = {1: "f32", 2: "bf16", 4: "i32", 5: "u8"}
+_KIND = {0: "in", 1: "const", 2: "out", 3: "work"}
 PLAN_BYTES = 4096
 
 
@@ -84,6 +84,24 @@ def _lib():
     lib.irx_plan_shard.argtypes = [vp, u, u, ctypes.POINTER(ctypes.c_longlong), ctypes.POINTER(ctypes.c_longlong),
                                    ctypes.POINTER(i)]
     lib.irx_inject.argtypes = [i, ctypes.c_ulonglong]
+    ll, ip = ctypes.c_longlong, ctypes.POINTER(ctypes.c_int)
+    lib.irx_compile_decode.argtypes = [vp, i, ll, ctypes.c_float, i, i, i, vp]
+    lib.irx_compile_kv_append.argtypes = [vp, ll, ll, vp]
+    lib.irx_compile_kv_copy.argtypes = [vp, ll, i, ll, vp]
+    lib.irx_compile_matvec4.argtypes = [vp, vp]
+    lib.irx_pages_new.argtypes = [i, i, i, i]
+    lib.irx_pages_new.restype = vp
+    lib.irx_pages_delete.argtypes = [vp]
+    lib.irx_pages_delete.restype = None
+    lib.irx_pages_open.argtypes = [vp]
+    lib.irx_pages_extend.argtypes = [vp, i, i, ip]
+    lib.irx_pages_fork.argtypes = [vp, i]
+    lib.irx_pages_close.argtypes = [vp, i]
+    lib.irx_pages_compact.argtypes = [vp, ip, i]
+    lib.irx_pages_free.argtypes = [vp]
+    lib.irx_pages_len.argtypes = [vp, i]
+    lib.irx_pages_table.argtypes = [vp]
+    lib.irx_pages_table.restype = ip
     lib.irx_quiet(1)
     _LIB = lib
     return lib
@@ -301,3 +319,4 @@ def check(stream=None):
 
 
 from . import kir_author  # noqa: E402
+from .serve import KvCache, Pages, decode, kv_append, kv_copy, matvec4, pack4  # noqa: E402

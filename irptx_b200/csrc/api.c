@@ -88,7 +88,9 @@ int irx_plan_arg(const irx_plan_t *plan, unsigned i, int *kind, int *dtype, long
     return 0;
 }
 
-static int esz(int dt) { return dt == DT_BF16 ? 2 : 4; }
+static int esz(int dt) { return dt == DT_BF16 ? 2 : dt == DT_U8 ? 1 : 4; }
+
+static int serving(const irx_plan_int_t *p) { return p->fam >= FAM_DECODE && p->fam <= FAM_MATVEC4; }
 
 static void prog_text(const irx_prog_t *g, char *b, size_t cap)
 {
@@ -165,6 +167,12 @@ int irx_plan_describe(const irx_plan_t *plan, char *buf, size_t cap)
         snprintf(buf, cap, "kir grid=%d block=%d cells=%lld args=%d kernel=irx_kir(%016llx)", (int)p->u.kk.grid,
                  (int)p->u.kk.block, (long long)p->u.kk.cells, p->narg, (unsigned long long)p->u.kk.key);
         break;
+    case FAM_DECODE:
+    case FAM_KV_APPEND:
+    case FAM_KV_COPY:
+    case FAM_MATVEC4:
+        irx_serve_text(p, buf, cap);
+        break;
     default:
         snprintf(buf, cap, "none");
     }
@@ -207,6 +215,12 @@ int irx_plan_work(const irx_plan_t *plan, double *bytes, double *flops)
     case FAM_KIR:                        /* every argument read or written once */
         for (i = 0; i < p->narg; i++) b += (double)p->arg_elems[i] * esz(p->arg_dt[i]);
         break;
+    case FAM_DECODE:
+    case FAM_KV_APPEND:
+    case FAM_KV_COPY:
+    case FAM_MATVEC4:
+        irx_serve_work(p, &b, &f);
+        break;
     default:
         break;
     }
@@ -229,6 +243,10 @@ long long irx_plan_units(const irx_plan_t *plan)
     case FAM_MATMUL: return (p->u.mm.n + MM_TILE_N - 1) / MM_TILE_N;
     case FAM_ATTENTION: return p->u.at.b * p->u.at.h;
     case FAM_KIR: return 1;              /* one launch of the KIR's own geometry */
+    case FAM_DECODE: return p->u.dec.c.heads;
+    case FAM_KV_APPEND:
+    case FAM_KV_COPY: return p->u.kv.n;
+    case FAM_MATVEC4: return p->u.mv.n;
     default: return 0;
     }
 }
@@ -463,6 +481,7 @@ static int launch_kir(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, void *c
     return irx_dev_launch_fn(fn, (unsigned)p->u.kk.grid, (unsigned)p->u.kk.block, st, &prm, 0);
 }
 
+int irx_launch_serve(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsigned ns, void *const *args, void *st);
 int irx_launch_mm(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsigned ns, void *const *args, void *st);
 int irx_launch_attn(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsigned ns, void *const *args, void *st);
 
@@ -477,7 +496,7 @@ int irx_launch_shard(const irx_plan_t *plan, unsigned shard, unsigned nshards, v
     int rc;
     irx_clear_error();
     if (!p) return irx_fail(E093, "a launch of a plan that was never compiled");
-    if (!args || nargs != p->narg) return irx_fail(E093, "a launch whose argument count is not the KIR's");
+    if (!args || nargs != p->narg) return irx_fail(E093, p->fam >= FAM_DECODE ? "a launch whose argument count is not the plan's" : "a launch whose argument count is not the KIR's");
     if (!nshards || shard >= nshards) return irx_fail(E093, "a shard index outside its shard count");
     for (i = 0; i < nargs; i++) if (!args[i]) return irx_fail(E093, "a launch with a null device pointer");
     if (irx_dev_get(&d)) return 1;
@@ -490,6 +509,10 @@ int irx_launch_shard(const irx_plan_t *plan, unsigned shard, unsigned nshards, v
     case FAM_MATMUL: rc = irx_launch_mm(p, d, shard, nshards, args, stream); break;
     case FAM_ATTENTION: rc = irx_launch_attn(p, d, shard, nshards, args, stream); break;
     case FAM_KIR: rc = launch_kir(p, d, shard, args, stream); break;
+    case FAM_DECODE:
+    case FAM_KV_APPEND:
+    case FAM_KV_COPY:
+    case FAM_MATVEC4: rc = irx_launch_serve(p, d, shard, nshards, args, stream); break;
     default: rc = irx_fail(E000, "a plan of no known family");
     }
     pthread_mutex_unlock(&LLOCK);
@@ -717,6 +740,7 @@ int irx_run_host_shard(const irx_plan_t *plan, unsigned shard, unsigned nshards,
     unsigned i;
     irx_clear_error();
     if (!p) return irx_fail(E093, "a run of a plan that was never compiled");
+    if (serving(p)) return irx_fail(E093, "a run from host memory of a serving operator, whose cache and weights stay on the device");
     if (!host_args || nargs != p->narg) return irx_fail(E093, "a run whose argument count is not the KIR's");
     if (!nshards || shard >= nshards) return irx_fail(E093, "a shard index outside its shard count");
     for (i = 0; i < nargs; i++) {
@@ -759,6 +783,7 @@ int irx_run_host_chunks(const irx_plan_t *plan, unsigned shard, unsigned nshards
     long long u0, u1;
     irx_clear_error();
     if (!p) return irx_fail(E093, "the chunks of a plan that was never compiled"), -1;
+    if (serving(p)) return irx_fail(E093, "the chunks of a serving operator, which has no host path"), -1;
     if (!nshards || shard >= nshards) return irx_fail(E093, "a shard index outside its shard count"), -1;
     irx_unit_range(irx_plan_units(plan), shard, nshards, &u0, &u1);
     return pipe_chunks(p, nshards, u0, u1, uni);

@@ -81,8 +81,9 @@ typedef struct {
     uint32_t fld0, nfld;
 } kn_t;
 
-typedef enum { KA_IN = 0, KA_CONST, KA_OUT } ka_kind_t;
-typedef enum { DT_NONE = 0, DT_F32, DT_BF16, DT_OTHER } dt_t;
+typedef enum { KA_IN = 0, KA_CONST, KA_OUT, KA_WORK } ka_kind_t;
+/* DT_I32 and DT_U8 are only the serving operators' (tables, lengths, packed weights): no KIR has them */
+typedef enum { DT_NONE = 0, DT_F32, DT_BF16, DT_OTHER, DT_I32, DT_U8 } dt_t;
 
 typedef struct {
     uint32_t name;
@@ -130,7 +131,8 @@ typedef struct { uint8_t kind; uint8_t pad[3]; uint32_t v; int32_t off; } irx_un
 /* ---- plans ---- */
 typedef enum {
     FAM_NONE = 0, FAM_POINTWISE, FAM_REDUCE_ALL, FAM_REDUCE_ROWS, FAM_ROWOP,
-    FAM_MATMUL, FAM_ATTENTION, FAM_KIR
+    FAM_MATMUL, FAM_ATTENTION, FAM_KIR,
+    FAM_DECODE, FAM_KV_APPEND, FAM_KV_COPY, FAM_MATVEC4
 } irx_fam_t;
 
 /* Every family that runs op programs has one uniform program (`uprog`). It runs once
@@ -207,6 +209,37 @@ typedef struct {
     uint32_t src_len;
 } irx_kirk_t;
 
+/* The serving operators (serve.c): compiled from a descriptor, not from KIR. */
+typedef struct {
+    int32_t  heads, dim, page_size, batch, cols;
+    int64_t  pages, page_stride, head_stride, token_stride;   /* strides in elements */
+    uint8_t  dt;
+} irx_kvc_t;
+
+typedef struct {
+    irx_kvc_t c;
+    int64_t  q_stride;                 /* elements from one sequence's query heads to the next one's */
+    int32_t  heads, window, sinks;
+    int32_t  dp, nt, split;            /* padded head size; 8-row blocks of a work unit; units per kv head */
+    int32_t  max_ctas;                 /* the workspace holds the partials of this many blocks */
+    uint32_t scale_bits;
+    uint8_t  lse;
+} irx_dec_t;
+
+typedef struct {
+    irx_kvc_t c;
+    int64_t  n;                        /* tokens (append) or page pairs (copy) */
+    int64_t  stride;                   /* append: elements between two new tokens' rows */
+    int64_t  layer_stride;             /* copy: elements between two layers' pools */
+    int32_t  layers;
+} irx_kv_t;
+
+typedef struct {
+    int64_t  m, n, k, x_stride, w_stride;   /* x_stride in elements, w_stride in bytes */
+    int32_t  group, groups;
+    uint8_t  dt, sdt, zeros;
+} irx_mv4_t;
+
 typedef struct {
     uint32_t magic;
     uint8_t  fam;
@@ -215,10 +248,13 @@ typedef struct {
     uint8_t  arg_zero[KIR_MAX_ARG];   /* 1: the KIR lists the output on a `zero` line */
     int64_t  arg_elems[KIR_MAX_ARG];
     char     kname[KIR_MAX_NAME + 1];
-    union { irx_pw_t pw; irx_red_t red; irx_row_t row; irx_mm_t mm; irx_at_t at; irx_kirk_t kk; } u;
+    union { irx_pw_t pw; irx_red_t red; irx_row_t row; irx_mm_t mm; irx_at_t at; irx_kirk_t kk;
+            irx_dec_t dec; irx_kv_t kv; irx_mv4_t mv; } u;
 } irx_plan_int_t;
 
 int irx_kirgen(const kir_t *k, irx_plan_int_t *p);
+void irx_serve_text(const irx_plan_int_t *p, char *buf, size_t cap);
+void irx_serve_work(const irx_plan_int_t *p, double *bytes, double *flops);
 
 /* Shard s of ns of a plan's units (irx_plan_units): the one split of every launcher; narrowed to
  * [a, b) on this thread while irx_unit_window(a, b) is set (b < 0 clears it). */

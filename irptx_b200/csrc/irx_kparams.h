@@ -15,6 +15,7 @@
 /* Device-side error word, written by a kernel whose bounded wait ran out. */
 #define IRX_KERR_TIMEOUT   1u
 #define IRX_KERR_TMEM      2u
+#define IRX_KERR_INDEX     4u      /* a page, sequence, position or length outside the cache */
 
 typedef struct {
     const void *ptr;        /* UNI_ARG: the const buffer */
@@ -104,5 +105,72 @@ typedef struct {
     unsigned   *sched;              /* persistent form: the next unit to hand out (zeroed per launch) */
     uint8_t     causal, k_t, scale_div, pad[5];
 } irx_kat_t;
+
+/* Decode attention: blocks whose partials the workspace holds, and its layout: 2 slots a block, each
+ * rows x dp accumulators then rows (max, sum) pairs, then the tickets (a work unit each) and the
+ * group counters (a slot each). */
+#define IRX_DEC_MAX_CTAS 512
+#define IRX_DEC_KEYS 64             /* keys of a chunk, the grain the work is cut in */
+
+/* Ring depth and shared memory of the two decode kernels, by padded head size and 8-row blocks
+ * (the launcher and the kernels agree on them; the share is the block's part of the work). */
+#define IRX_DEC_SHARE 128
+#define IRX_DEC_TC_ST(dp, nt) ((dp) == 64 ? 4 : (dp) == 128 && (nt) == 1 ? 3 : 2)
+#define IRX_DEC_ST_ST(dp) ((dp) == 256 ? 1 : 2)
+#define IRX_DEC_TC_SMEM(dp, nt, st) (4 * (st) * 2 * 16 * (dp) * 2 + 4 * 8 * ((dp) + 4) * 4 + 4 * 8 * (nt) * 8 + IRX_DEC_SHARE)
+#define IRX_DEC_ST_SMEM(dp, nt, st) (8 * (st) * 8 * (2 * (dp) + 16) * 4 + 8 * 8 * (dp) * 4 + 8 * (nt) * (dp) * 4 + \
+                                     8 * 8 * (nt) * 8 * 4 + 8 * 8 * (nt) * 8 + IRX_DEC_SHARE)
+
+typedef struct {
+    const void *q, *k, *v;
+    const int32_t *table, *lens;
+    void       *o;
+    float      *lse;                /* NULL: not asked for */
+    float      *part;
+    unsigned   *ticket, *gcount;
+    unsigned   *err;
+    int64_t     q_stride, page_stride, head_stride, token_stride, pages;
+    int32_t     batch, cols, page_size, heads, group, d;
+    int32_t     h0, h1;             /* kv heads of this launch (a shard) */
+    int32_t     split;              /* work units per kv head */
+    int32_t     window, sinks;
+    float       scale2;             /* scale * log2(e) */
+    uint8_t     dt, vec, pad[2];    /* vec: rows can be moved 16 bytes at a time */
+} irx_kdec_t;
+
+/* Cache append: one warp per (token, part of the token's row). */
+typedef struct {
+    const void *kn, *vn;
+    const int32_t *seq, *pos, *table;
+    void       *k, *v;
+    unsigned   *err;
+    int64_t     stride, page_stride, head_stride, token_stride, pages;   /* in vectors */
+    int64_t     t0, t1;             /* tokens of this launch */
+    int32_t     batch, cols, page_size, heads, dv;      /* dv: vectors of a head's row */
+    int32_t     parts;              /* warps per token */
+} irx_kapp_t;
+
+/* Page copy: runs of `run` vectors at (i1, i2) of every (pair, layer) of both pools. */
+typedef struct {
+    const int32_t *pairs;
+    void       *k, *v;
+    unsigned   *err;
+    int64_t     page_stride, layer_stride, s1, s2, pages;                 /* in vectors */
+    int64_t     p0, p1;             /* pairs of this launch */
+    int64_t     run, tiles;         /* tiles: blocks' worth of work per (pair, layer, pool) */
+    int32_t     n1, n2, layers, pad;
+} irx_kcpy_t;
+
+/* 4-bit matrix-vector products. */
+typedef struct {
+    const void *x;
+    const uint8_t *w, *z;           /* z: NULL when every zero point is 8 */
+    const void *s;
+    void       *y;
+    int64_t     m, n, k, x_stride, w_stride;
+    int64_t     n0, n1;             /* rows of w of this launch */
+    int32_t     group, groups;
+    uint8_t     dt, sdt, pad[6];
+} irx_kmv4_t;
 
 #endif /* IRX_KPARAMS_H */

@@ -5,3 +5,6 @@
 #include "rowop.cu"
 #include "gemm.cu"
 #include "attn.cu"
+#include "kvpages.cu"
+#include "decode.cu"
+#include "matvec4.cu"

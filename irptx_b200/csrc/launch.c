@@ -158,7 +158,15 @@ static const char *const KNAMES[K_COUNT] = {
     "irx_red_rows_p0", "irx_red_rows_p1", "irx_red_all_p0", "irx_red_all_p1",
     "irx_rowop", "irx_row_rmsnorm", "irx_row_softmax", "irx_row_l2norm",
     "irx_mm_f32", "irx_mm_bf16", "irx_mm_bf16_simt", "irx_attn_f32", "irx_attn_bf16", "irx_attn_bf16_simt",
-    "irx_mm_bf16_pair", "irx_mm_bf16_wide"
+    "irx_mm_bf16_pair", "irx_mm_bf16_wide",
+    "irx_dec_tc_64_1", "irx_dec_tc_64_2", "irx_dec_tc_128_1", "irx_dec_tc_128_2", "irx_dec_tc_256_1",
+    "irx_dec_st_64_1", "irx_dec_st_64_2", "irx_dec_st_128_1", "irx_dec_st_128_2", "irx_dec_st_256_1",
+    "irx_kv_append_16", "irx_kv_append_4", "irx_kv_append_2",
+    "irx_kv_copy_16", "irx_kv_copy_4", "irx_kv_copy_2",
+    "irx_mv4_32_1", "irx_mv4z_32_1", "irx_mv4_32_2", "irx_mv4z_32_2",
+    "irx_mv4_64_1", "irx_mv4z_64_1", "irx_mv4_64_2", "irx_mv4z_64_2",
+    "irx_mv4_128_1", "irx_mv4z_128_1", "irx_mv4_128_2", "irx_mv4z_128_2",
+    "irx_mv4_any"
 };
 
 static irx_dev_t CTX[MAX_CTX];
@@ -536,6 +544,8 @@ int irx_dev_check_err(irx_dev_t *d, void *s)
     if (e) {
         irx_dev_memset32(d->err, 0, 1, s);
         irx_dev_sync(s);
+        if (e & IRX_KERR_INDEX && !(e & ~IRX_KERR_INDEX))
+            return irx_fail(E093, "a page, sequence, position or length outside the cache (the access was skipped)");
         return irx_fail(E092, e & IRX_KERR_TIMEOUT ? "a kernel whose bounded device wait ran out (error word set)"
                                                    : "a kernel that set its device error word");
     }

@@ -13,6 +13,10 @@ enum {
     K_ROWOP = K_RED_ALL + 2, K_ROW_RMSNORM, K_ROW_SOFTMAX, K_ROW_L2NORM,
     K_MM_F32, K_MM_BF16, K_MM_BF16_SIMT, K_ATTN_F32, K_ATTN_BF16, K_ATTN_BF16_SIMT,
     K_MM_BF16_PAIR, K_MM_BF16_WIDE,
+    /* the serving operators: decode by padded head size and 8-row blocks, cache moves by vector
+     * width, matrix-vector products by (group grain, zero points, tokens) */
+    K_DEC_TC, K_DEC_ST = K_DEC_TC + 5, K_KV_APPEND = K_DEC_ST + 5, K_KV_COPY = K_KV_APPEND + 3,
+    K_MV4 = K_KV_COPY + 3, K_MV4_ANY = K_MV4 + 12,
     K_COUNT
 };
 
@@ -43,6 +47,7 @@ typedef struct {
     CUfunction fn[K_COUNT];
     unsigned   smem_set[K_COUNT];      /* the dynamic shared memory limit last set per kernel */
     int        sms, smem_optin;
+    int        occ[K_COUNT];           /* the serving kernels' resident blocks per SM (0: not asked yet) */
     CUdeviceptr scratch, err;
     unsigned    slot0;                 /* next scratch slot (under the launch lock) */
     CUdeviceptr arena;                 /* irx_run_host's device copies, grown on demand */
