@@ -161,8 +161,13 @@ typedef struct {
     int32_t     n1, n2, layers, pad;
 } irx_kcpy_t;
 
-/* 4-bit matrix-vector products. */
+/* 4-bit matrix-vector products: ring depth and shared memory by 8-column blocks of tokens. */
+#define IRX_MV4_STAGES 4
+#define IRX_MV4_SMEM(nt) (IRX_MV4_STAGES * (128 * 128 + (nt) * 8 * (512 + 64)) + 1024 + 64)
+
 typedef struct {
+    CUtensorMap tma_w;              /* w's bytes of this launch's rows, in boxes of 128 x 128 */
+    unsigned   *err;
     const void *x;
     const uint8_t *w, *z;           /* z: NULL when every zero point is 8 */
     const void *s;
@@ -170,7 +175,9 @@ typedef struct {
     int64_t     m, n, k, x_stride, w_stride;
     int64_t     n0, n1;             /* rows of w of this launch */
     int32_t     group, groups;
-    uint8_t     dt, sdt, pad[6];
+    int32_t     ck;                 /* blocks of a cluster: slices of k */
+    uint8_t     dt, sdt, gshift, pad;
+    uint64_t    gmul;               /* group of k: (k / 32 * gmul) >> gshift */
 } irx_kmv4_t;
 
 #endif /* IRX_KPARAMS_H */

@@ -22,120 +22,133 @@ __device__ __forceinline__ void mv4_unpack(uint32_t w, __nv_bfloat162 z, uint32_
 {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const uint32_t u = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+        uint32_t u;
+        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(u) : "r"(w), "r"(0x000f000fu), "r"(0x43004300u));   // (w & m) | c
         const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&u), z);
         r[i] = *reinterpret_cast<const uint32_t *>(&d);
+        w >>= 4;
     }
 }
 
-template <int B> struct mv4_vec;
-template <> struct mv4_vec<16> { using T = uint4; };
-template <> struct mv4_vec<8> { using T = uint2; };
-template <> struct mv4_vec<4> { using T = unsigned; };
-
-// GV: weights that share a scale, as far as the kernel is concerned (128, 64 or 32; group is a
-// multiple of it). A warp's step is 128 weights of 16 RT rows: in each GV-wide piece the four lanes
-// of a row take GV/4 weights each, so that one instruction never mixes two groups.
-template <int GV, int RT>
-struct Mv4Step {
-    static constexpr int P = 128 / GV, WB = GV / 8;      // pieces; bytes of a lane's load
-    typename mv4_vec<WB>::T w[RT][2][P];
-    float s[RT][2];                                      // this lane's piece's scale (piece t * P / 4)
-    unsigned z[RT][2];
+// The tiling. A block takes 128 rows of w and a slice of k, in stages of 256 k: 128 bytes of every
+// row, with the tokens' values of those k, through a ring of asynchronous copies, so that bytes
+// are in flight whatever the warps do. Its 8 warps are 4 groups of 32 rows times 2 halves of a
+// stage. The weights of a stage come by one TMA copy, which also fills zeros past the ends and
+// swizzles the 16-byte pieces for ldmatrix. The slices of k of the same rows are a cluster's blocks, which add up through
+// distributed shared memory in a fixed order: that is how a matrix of few rows still fills the
+// GPU, with no workspace and the same bits every time.
+//
+// A stage's 16 bytes of a row are 32 weights; ldmatrix hands lane (g, t) the 8 weights t of row g, so
+// an instruction's four lanes always lie in one group of 32, whatever the group size is (GV: 128,
+// 64 or 32, the widest that divides it).
+//
+// f32 tokens are carried as three bf16 columns each, high, middle and low part, whose sum is the
+// f32 value to its last bit (unless that is below bf16's range): the same products, exact, and
+// the three columns' sums are added at the end.
+template <int NT>
+struct Mv4Smem {
+    static constexpr int XS = 512 + 64;                  // bytes of a column's stage: 64 off the banks' period
+    static constexpr int W = 128 * 128, X = NT * 8 * XS, RING = W * IRX_MV4_STAGES, BARS = RING + X * IRX_MV4_STAGES;
+    static_assert(BARS + 1024 + 64 == IRX_MV4_SMEM(NT), "the launcher's shared memory size");
+    static constexpr int RS = NT * 8 + 4;                // floats of a row of the sums
+    static_assert(2 * 128 * RS * 4 <= BARS, "the sums fit the ring");
 };
 
-template <int GV, int RT, bool Z>
-__device__ __forceinline__ void mv4_load(const irx_kmv4_t &p, int64_t row0, int64_t kb, int g, int t, Mv4Step<GV, RT> &S)
+// The scales (as they lie in memory: turning them into numbers at once would wait for them) and zero
+// points of a warp's rows g, g + 8, g + 16, g + 24, for this lane's piece of the stage.
+struct Mv4Scale {
+    uint32_t s[4], z[4];
+};
+
+// k / 32 / (group / 32) by a multiplication: exact below 2^26 (the launcher's constants).
+template <int GV>
+__device__ __forceinline__ void mv4_scales(const irx_kmv4_t &p, const uint32_t (&at)[4], uint32_t k0, int t, Mv4Scale &S)
 {
-    using St = Mv4Step<GV, RT>;
-    using V = typename mv4_vec<St::WB>::T;
+    const uint32_t k = k0 + (t * (128 / GV) / 4) * GV;
+    const uint32_t grp = (uint32_t)(((uint64_t)(k >> 5) * p.gmul) >> p.gshift);
+    if (k < (uint32_t)p.k) {
+        if (p.sdt == DT_BF16) {
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++)
+            for (int i = 0; i < 4; i++) S.s[i] = __ldg(reinterpret_cast<const unsigned short *>(p.s) + (at[i] + grp));
+        } else {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int64_t row = row0 + rt * 16 + h * 8 + g;
-            const bool in = row < p.n1;
-            const uint8_t *w = p.w + row * p.w_stride;
-#pragma unroll
-            for (int i = 0; i < St::P; i++) {
-                const int64_t k = kb * 128 + i * GV + t * (GV / 4);
-                V v{};
-                if (in && k < p.k) v = __ldcs(reinterpret_cast<const V *>(w + k / 2));
-                S.w[rt][h][i] = v;
-            }
-            const int64_t ks = kb * 128 + (t * St::P / 4) * GV;
-            float s = 0.0f;
-            unsigned z = 8;
-            if (in && ks < p.k) {
-                const int64_t e = row * p.groups + (uint32_t)ks / (uint32_t)p.group;
-                s = irx_ld1(p.s, p.sdt, e);
-                if (Z) z = p.z[e];
-            }
-            S.s[rt][h] = s;
-            S.z[rt][h] = z;
+            for (int i = 0; i < 4; i++) S.s[i] = __ldg(reinterpret_cast<const uint32_t *>(p.s) + (at[i] + grp));
         }
+        if (p.z) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) S.z[i] = __ldg(p.z + (at[i] + grp));
+        }
+    }
 }
 
-template <int GV, int NT, int RT, bool Z>
-__device__ __forceinline__ void mv4_step(const irx_kmv4_t &p, int64_t m0, int64_t kb, int g, int t,
-                                         const Mv4Step<GV, RT> &S, float (&acc)[RT][NT][4])
+// The first product of a sum: the accumulators start at zero.
+__device__ __forceinline__ void mma_16816_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
-    using St = Mv4Step<GV, RT>;
-    constexpr int W = St::WB / 4;                        // words of a lane's load
-    const int lane = g * 4 + t;
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+template <int GV, int NT>
+__device__ __forceinline__ void mv4_stage(uint32_t ws, const unsigned char *xs, int wr, int wk, int lane, const Mv4Scale &S, bool zs, int sshift,
+                                          float (&acc)[2][NT][4])
+{
+    using M = Mv4Smem<NT>;
+    constexpr int P = 128 / GV;                          // pieces of a warp's 128 k
+    const int g = lane >> 2, t = lane & 3;
+    uint32_t w[2][2][4];
 #pragma unroll
-    for (int i = 0; i < St::P; i++) {
-        float part[RT][NT][4];
-        __nv_bfloat162 z[RT][2];
-        float s[RT][2];
+    for (int rt = 0; rt < 2; rt++)
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++)
+        for (int j = 0; j < 2; j++) {
+            const int row = wr * 32 + rt * 16 + (lane & 15), ch = wk * 4 + j * 2 + (lane >> 4);
+            ldsm4(w[rt][j], ws + row * 128 + ((ch ^ (row & 7)) << 4));
+        }
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+        float part[2][NT][4];
+        __nv_bfloat162 z[2][2];
+        float s[2][2];
+#pragma unroll
+        for (int rt = 0; rt < 2; rt++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 unsigned zz = 8;
-                if (St::P > 1) {
-                    const int from = (lane & ~3) + i * 4 / St::P;
-                    s[rt][h] = __shfl_sync(0xffffffffu, S.s[rt][h], from);
-                    if (Z) zz = __shfl_sync(0xffffffffu, S.z[rt][h], from);
-                } else {
-                    s[rt][h] = S.s[rt][h];
-                    if (Z) zz = S.z[rt][h];
-                }
+                const int from = (lane & ~3) + i * (4 / P);
+                const uint32_t sb = P > 1 ? __shfl_sync(0xffffffffu, S.s[rt * 2 + h], from) : S.s[rt * 2 + h];
+                s[rt][h] = __uint_as_float(sb << sshift);
+                if (zs) zz = P > 1 ? __shfl_sync(0xffffffffu, S.z[rt * 2 + h], from) : S.z[rt * 2 + h];
                 const uint32_t zb = 0x43004300u | ((zz & 15u) * 0x00010001u);
                 z[rt][h] = *reinterpret_cast<const __nv_bfloat162 *>(&zb);
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) part[rt][nt][2 * h] = part[rt][nt][2 * h + 1] = 0.0f;
             }
 #pragma unroll
-        for (int w = 0; w < W; w++) {
-            const int64_t k = kb * 128 + i * GV + t * (GV / 4) + w * 8;
+        for (int q = 0; q < 4 / P; q++) {
+            const int step = i * (4 / P) + q;
             uint32_t b[NT][4];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                const int64_t m = m0 + nt * 8 + g;
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (m < p.m && k < p.k)
-                    x = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const __nv_bfloat16 *>(p.x) + m * p.x_stride + k));
-                b[nt][0] = __byte_perm(x.x, x.z, 0x5410);
-                b[nt][1] = __byte_perm(x.x, x.z, 0x7632);
-                b[nt][2] = __byte_perm(x.y, x.w, 0x5410);
-                b[nt][3] = __byte_perm(x.y, x.w, 0x7632);
+                const uint4 x = *reinterpret_cast<const uint4 *>(xs + (nt * 8 + g) * M::XS + (wk * 128 + step * 32 + t * 8) * 2);
+                b[nt][0] = x.x;
+                b[nt][1] = x.y;
+                b[nt][2] = x.z;
+                b[nt][3] = x.w;
             }
 #pragma unroll
-            for (int rt = 0; rt < RT; rt++) {
+            for (int rt = 0; rt < 2; rt++) {
                 uint32_t lo[4], hi[4];
-                mv4_unpack(reinterpret_cast<const uint32_t *>(&S.w[rt][0][i])[w], z[rt][0], lo);
-                mv4_unpack(reinterpret_cast<const uint32_t *>(&S.w[rt][1][i])[w], z[rt][1], hi);
+                mv4_unpack(w[rt][step >> 1][(step & 1) * 2], z[rt][0], lo);
+                mv4_unpack(w[rt][step >> 1][(step & 1) * 2 + 1], z[rt][1], hi);
                 const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]}, a1[4] = {lo[2], hi[2], lo[3], hi[3]};
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    mma_16816(part[rt][nt], a0, b[nt][0], b[nt][1]);
+                    if (q == 0) mma_16816_first(part[rt][nt], a0, b[nt][0], b[nt][1]);
+                    else mma_16816(part[rt][nt], a0, b[nt][0], b[nt][1]);
                     mma_16816(part[rt][nt], a1, b[nt][2], b[nt][3]);
                 }
             }
         }
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++)
+        for (int rt = 0; rt < 2; rt++)
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -143,50 +156,178 @@ __device__ __forceinline__ void mv4_step(const irx_kmv4_t &p, int64_t m0, int64_
     }
 }
 
-template <int GV, int NT, int RT, bool Z>
+// Four floats of any block of the cluster; not volatile, so that several can be on their way at once (the
+// cluster barriers on both sides are).
+__device__ __forceinline__ float4 ld_cluster4(uint32_t a)
+{
+    float4 x;
+    asm("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(a));
+    return x;
+}
+
+template <int GV, int NT, bool F32>
 __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
 {
-    __shared__ float red[MV4_WARPS][RT * 16][NT * 8 + 1];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int64_t nb = (p.n1 - p.n0 + RT * 16 - 1) / (RT * 16);
-    const int64_t row0 = p.n0 + (blockIdx.x % nb) * (RT * 16), m0 = (blockIdx.x / nb) * (NT * 8);
-    const int64_t steps = (p.k + 127) / 128;
-    float acc[RT][NT][4];
+    using M = Mv4Smem<NT>;
+    extern __shared__ unsigned char sm_raw[];
+    unsigned char *sm = sm_raw + ((1024u - (irx_smem_u32(sm_raw) & 1023u)) & 1023u);   // the swizzle's period
+    constexpr int ST = IRX_MV4_STAGES, COLS = NT * 8, TOK = F32 ? COLS / 3 : COLS;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wr = warp & 3, wk = warp >> 2, g = lane >> 2, t = lane & 3;
+    const int rank = (int)blockIdx.x % p.ck;
+    const int64_t tile = blockIdx.x / p.ck, nb = (p.n1 - p.n0 + 127) / 128;
+    const int64_t row0 = p.n0 + (tile % nb) * 128, m0 = (tile / nb) * TOK;
+    const int k_all = (int)p.k, steps = (int)((p.k + 255) / 256);
+    const int s0 = (int)((int64_t)rank * steps / p.ck), s1 = (int)((int64_t)(rank + 1) * steps / p.ck);
+    float acc[2][NT][4];
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++)
+    for (int rt = 0; rt < 2; rt++)
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int j = 0; j < 4; j++) acc[rt][nt][j] = 0.0f;
+    uint64_t *full = reinterpret_cast<uint64_t *>(sm + M::BARS);
+    if (tid == 0) {
+        for (int i = 0; i < ST; i++) irx_mbar_init(full + i, 1);
+        irx_fence_mbar_init();
+        tma_prefetch_desc(&p.tma_w);
+    }
     irx_pdl_enter();
-    // the warps take the row's steps in turn, so neighbours read neighbouring bytes; a step's bytes are
-    // loaded two steps ahead of their use
-    Mv4Step<GV, RT> S[2];
-    int64_t kb = warp;
-    mv4_load<GV, RT, Z>(p, row0, kb, g, t, S[0]);
-    mv4_load<GV, RT, Z>(p, row0, kb + MV4_WARPS, g, t, S[1]);
-    for (; kb < steps; kb += 2 * MV4_WARPS) {
-        mv4_step<GV, NT, RT, Z>(p, m0, kb, g, t, S[0], acc);
-        mv4_load<GV, RT, Z>(p, row0, kb + 2 * MV4_WARPS, g, t, S[0]);
-        if (kb + MV4_WARPS >= steps) break;
-        mv4_step<GV, NT, RT, Z>(p, m0, kb + MV4_WARPS, g, t, S[1], acc);
-        mv4_load<GV, RT, Z>(p, row0, kb + 3 * MV4_WARPS, g, t, S[1]);
-    }
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) red[warp][rt * 16 + g + (j >> 1) * 8][nt * 8 + 2 * t + (j & 1)] = acc[rt][nt][j];
     __syncthreads();
-    for (int i = threadIdx.x; i < RT * 16 * NT * 8; i += MV4_WARPS * 32) {
-        const int r = i % (RT * 16), c = i / (RT * 16);
-        if (row0 + r >= p.n1 || m0 + c >= p.m) continue;
-        float v = red[0][r][c];
+
+    auto fetch = [&](int s) {                            // stage s into its slot, by one thread
+        if (tid == 0 && s < s1) {
+            irx_mbar_expect_tx(full + (s - s0) % ST, M::W);
+            tma_load_2d(sm + ((s - s0) % ST) * M::W, &p.tma_w, s * 128, (int)row0, full + (s - s0) % ST);
+        }
+    };
+    // The tokens' part, a stage ahead in registers, stored in the order in which the weights unpack: bf16 8
+    // k of columns tid / 32 + 8 i at a time, f32 the stage's k = tid of every token, in three parts
+    // (truncations, so that the parts of an infinity or a NaN stay what they should).
+    uint4 xb[F32 ? 1 : NT];
+    float xr[F32 ? TOK : 1];
+    const int64_t xoff = F32 ? m0 * p.x_stride + tid : (m0 + (tid >> 5)) * p.x_stride + (tid & 31) * 8;
+    auto xload = [&](int s) {
+        if (F32) {
+            const float *x = reinterpret_cast<const float *>(p.x) + xoff + (int64_t)s * 256;
 #pragma unroll
-        for (int w = 1; w < MV4_WARPS; w++) v += red[w][r][c];
-        irx_st1(p.y, p.dt, (m0 + c) * p.n + row0 + r, v);
+            for (int m = 0; m < TOK; m++) {
+                xr[m] = 0.0f;
+                if (s < s1 && m0 + m < p.m && s * 256 + tid < k_all) xr[m] = __ldg(x + m * p.x_stride);
+            }
+        } else {
+            const __nv_bfloat16 *x = reinterpret_cast<const __nv_bfloat16 *>(p.x) + xoff + (int64_t)s * 256;
+#pragma unroll
+            for (int i = 0; i < NT; i++) {
+                xb[i] = make_uint4(0, 0, 0, 0);
+                if (s < s1 && m0 + (tid >> 5) + 8 * i < p.m && s * 256 + (tid & 31) * 8 < k_all)
+                    xb[i] = __ldg(reinterpret_cast<const uint4 *>(x + 8 * i * p.x_stride));
+            }
+        }
+    };
+    auto xstore = [&](int s) {
+        unsigned char *st = sm + M::RING + ((s - s0) % ST) * M::X;
+        if (F32) {
+            const int k8 = tid & 7;
+            st += ((tid & ~7) + (k8 < 4 ? 2 * k8 : 2 * k8 - 7)) * 2;
+#pragma unroll
+            for (int m = 0; m < TOK; m++) {
+                const __nv_bfloat16 hi = __float2bfloat16_rz(xr[m]);
+                const float r1 = isinf(xr[m]) ? 0.0f : xr[m] - __bfloat162float(hi);
+                const __nv_bfloat16 mid = __float2bfloat16_rz(r1);
+                const __nv_bfloat16 lo = __float2bfloat16_rz(r1 - __bfloat162float(mid));
+                *reinterpret_cast<__nv_bfloat16 *>(st + (3 * m) * M::XS) = hi;
+                *reinterpret_cast<__nv_bfloat16 *>(st + (3 * m + 1) * M::XS) = mid;
+                *reinterpret_cast<__nv_bfloat16 *>(st + (3 * m + 2) * M::XS) = lo;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NT; i++)
+                *reinterpret_cast<uint4 *>(st + ((tid >> 5) + 8 * i) * M::XS + (tid & 31) * 16) =
+                    make_uint4(__byte_perm(xb[i].x, xb[i].z, 0x5410), __byte_perm(xb[i].x, xb[i].z, 0x7632),
+                               __byte_perm(xb[i].y, xb[i].w, 0x5410), __byte_perm(xb[i].y, xb[i].w, 0x7632));
+        }
+    };
+    Mv4Scale S[2] = {};
+    uint32_t at[4];                                      // rows past the end read the last row's: their sums go nowhere
+#pragma unroll
+    for (int i = 0; i < 4; i++) at[i] = (uint32_t)(min(row0 + wr * 32 + i * 8 + g, p.n1 - 1) * p.groups);
+    const int sshift = p.sdt == DT_BF16 ? 16 : 0;
+    if (F32) {                                           // columns that no token has stay zero
+        for (int i = tid; i < ST * M::X / 16; i += MV4_WARPS * 32) *reinterpret_cast<uint4 *>(sm + M::RING + i * 16) = make_uint4(0, 0, 0, 0);
+        __syncthreads();
     }
+#pragma unroll
+    for (int i = 0; i < ST - 1; i++) fetch(s0 + i);
+    mv4_scales<GV>(p, at, (uint32_t)s0 * 256 + wk * 128, t, S[0]);
+    mv4_scales<GV>(p, at, (uint32_t)(s0 + 1) * 256 + wk * 128, t, S[1]);
+    xload(s0);
+    xstore(s0);
+    xload(s0 + 1);
+    int ok = 1;
+    for (int s = s0; s < s1; s += 2) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            if (s + u >= s1) break;
+            const int slot = (s + u - s0) % ST;
+            ok = ok && irx_mbar_wait(full + slot, ((s + u - s0) / ST) & 1);
+            __syncthreads();                             // the tokens are there too; the stage before is free
+            fetch(s + u + ST - 1);
+            mv4_stage<GV, NT>(irx_smem_u32(sm) + slot * M::W, sm + M::RING + slot * M::X, wr, wk, lane, S[u], p.z != nullptr, sshift, acc);
+            mv4_scales<GV>(p, at, (uint32_t)(s + u + 2) * 256 + wk * 128, t, S[u]);
+            if (s + u + 1 < s1) {
+                xstore(s + u + 1);
+                xload(s + u + 2);
+            }
+        }
+    }
+    if (!ok) {                                           // a wait ran out: report it, and let copies in flight land
+        irx_flag(p.err, IRX_KERR_TIMEOUT);
+        for (int s = max(s0, s1 - ST); s < s1; s++) irx_mbar_wait(full + (s - s0) % ST, ((s - s0) / ST) & 1);
+    }
+    __syncthreads();
+    // the second half's sums go through shared memory to the first half's warps, which leave the block's
+    // 128 x COLS sums there; then every block of the cluster adds up its share of the rows
+    float *red = reinterpret_cast<float *>(sm);
+#pragma unroll
+    for (int half = 1; half >= 0; half--) {
+        if (wk == half) {
+#pragma unroll
+            for (int rt = 0; rt < 2; rt++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        float *a = red + (wr * 32 + rt * 16 + g + (j >> 1) * 8) * M::RS + nt * 8 + 2 * t + (j & 1);
+                        *a = half ? acc[rt][nt][j] : acc[rt][nt][j] + *a;
+                    }
+        }
+        if (half) __syncthreads();
+    }
+    if (p.ck > 1) cluster_sync(); else __syncthreads();
+    const int rows = 128 / p.ck, r0 = rank * rows;
+    const float *fin = red + r0 * M::RS;
+    if (p.ck > 1) {
+        float *sum = red + 128 * M::RS;
+        for (int i = tid; i < rows * (COLS / 4); i += MV4_WARPS * 32) {
+            const int r = i / (COLS / 4), c = (i % (COLS / 4)) * 4;
+            const float *a = red + (r0 + r) * M::RS + c;
+            float4 v = ld_cluster4(cluster_addr(a, 0));
+            for (int q = 1; q < p.ck; q++) {
+                const float4 x = ld_cluster4(cluster_addr(a, q));
+                v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+            }
+            *reinterpret_cast<float4 *>(sum + r * M::RS + c) = v;
+        }
+        __syncthreads();
+        fin = sum;
+    }
+    for (int i = tid; i < rows * TOK; i += MV4_WARPS * 32) {
+        const int r = i % rows, m = i / rows;
+        const float *a = fin + r * M::RS + (F32 ? 3 * m : m);
+        const float v = F32 ? a[0] + (a[1] + a[2]) : a[0];
+        if (row0 + r0 + r < p.n1 && m0 + m < p.m) irx_st1(p.y, p.dt, (m0 + m) * p.n + row0 + r0 + r, v);
+    }
+    if (p.ck > 1) cluster_sync();                        // no block leaves while its sums are still read
 }
 
 // Any sizes, strides and types: a warp per row of w and four tokens, two weights a lane and step.
@@ -221,11 +362,11 @@ __device__ __forceinline__ void mv4_any_body(const irx_kmv4_t &p)
     }
 }
 
-#define MV4_K(GV, NT, RT) \
-    extern "C" __global__ void __launch_bounds__(MV4_WARPS * 32) irx_mv4_##GV##_##NT(const __grid_constant__ irx_kmv4_t p) \
-    { mv4_body<GV, NT, RT, false>(p); } \
-    extern "C" __global__ void __launch_bounds__(MV4_WARPS * 32) irx_mv4z_##GV##_##NT(const __grid_constant__ irx_kmv4_t p) \
-    { mv4_body<GV, NT, RT, true>(p); }
+#define MV4_K(GV, NT) \
+    extern "C" __global__ void __launch_bounds__(MV4_WARPS * 32, 2) irx_mv4_bf16_##GV##_##NT(const __grid_constant__ irx_kmv4_t p) \
+    { mv4_body<GV, NT, false>(p); } \
+    extern "C" __global__ void __launch_bounds__(MV4_WARPS * 32, 2) irx_mv4_f32_##GV##_##NT(const __grid_constant__ irx_kmv4_t p) \
+    { mv4_body<GV, NT, true>(p); }
 
-MV4_K(32, 1, 1) MV4_K(32, 2, 2) MV4_K(64, 1, 1) MV4_K(64, 2, 2) MV4_K(128, 1, 1) MV4_K(128, 2, 2)
+MV4_K(32, 1) MV4_K(32, 2) MV4_K(64, 1) MV4_K(64, 2) MV4_K(128, 1) MV4_K(128, 2)
 extern "C" __global__ void __launch_bounds__(MV4_WARPS * 32) irx_mv4_any(const __grid_constant__ irx_kmv4_t p) { mv4_any_body(p); }

@@ -163,9 +163,8 @@ static const char *const KNAMES[K_COUNT] = {
     "irx_dec_st_64_1", "irx_dec_st_64_2", "irx_dec_st_128_1", "irx_dec_st_128_2", "irx_dec_st_256_1",
     "irx_kv_append_16", "irx_kv_append_4", "irx_kv_append_2",
     "irx_kv_copy_16", "irx_kv_copy_4", "irx_kv_copy_2",
-    "irx_mv4_32_1", "irx_mv4z_32_1", "irx_mv4_32_2", "irx_mv4z_32_2",
-    "irx_mv4_64_1", "irx_mv4z_64_1", "irx_mv4_64_2", "irx_mv4z_64_2",
-    "irx_mv4_128_1", "irx_mv4z_128_1", "irx_mv4_128_2", "irx_mv4z_128_2",
+    "irx_mv4_bf16_32_1", "irx_mv4_bf16_32_2", "irx_mv4_bf16_64_1", "irx_mv4_bf16_64_2", "irx_mv4_bf16_128_1", "irx_mv4_bf16_128_2",
+    "irx_mv4_f32_32_1", "irx_mv4_f32_32_2", "irx_mv4_f32_64_1", "irx_mv4_f32_64_2", "irx_mv4_f32_128_1", "irx_mv4_f32_128_2",
     "irx_mv4_any"
 };
 

@@ -391,12 +391,30 @@ static int launch_mv4(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsigne
     k.n0 = u0; k.n1 = u1;
     k.group = a->group; k.groups = a->groups;
     k.dt = a->dt; k.sdt = a->sdt;
-    if (a->dt == DT_BF16 && a->k % 32 == 0 && a->group % 32 == 0 && a->w_stride % 16 == 0 && a->x_stride % 8 == 0 &&
-        a_to(k.x, 16) && a_to(k.w, 16)) {
-        const int gv = a->group % 128 == 0 ? 2 : a->group % 64 == 0 ? 1 : 0, nt = a->m > 8 ? 2 : 1;
-        grid = ((u1 - u0 + 16 * nt - 1) / (16 * nt)) * ((a->m + 8 * nt - 1) / (8 * nt));
-        if (grid > MAX_COUNT) return irx_fail(E042, "a matvec4 past one launch's blocks");
-        return irx_dev_launch(d, K_MV4 + gv * 4 + (nt - 1) * 2 + a->zeros, (unsigned)grid, 256, 0, 1, st, &k);
+    k.err = (unsigned *)(size_t)d->err;
+    if (a->k % 32 == 0 && a->group % 32 == 0 && a->w_stride % 16 == 0 && a_to(k.w, 16) && a->n * a->groups <= MAX_COUNT &&
+        (a->dt == DT_F32 || (a->x_stride % 8 == 0 && a_to(k.x, 16)))) {
+        /* columns: one a token, three for f32 tokens; 8 or 16 of them at a time. The slices of k: as
+         * many blocks as fit the GPU at two an SM, in clusters of up to 8 */
+        const int f32 = a->dt == DT_F32, gv = a->group % 128 == 0 ? 2 : a->group % 64 == 0 ? 1 : 0;
+        const int nt = a->m > (f32 ? 2 : 8) ? 2 : 1, tok = f32 ? (nt == 1 ? 2 : 5) : 8 * nt;
+        const int64_t tiles = ((u1 - u0 + 127) / 128) * ((a->m + tok - 1) / tok), steps = (a->k + 255) / 256;
+        int ck = 1;
+        while (ck < 8 && tiles * ck * 2 <= 2 * d->sms && ck * 2 <= steps) ck *= 2;
+        if (tiles * ck > MAX_COUNT) return irx_fail(E042, "a matvec4 past one launch's blocks");
+        const cuuint64_t dims[2] = {(cuuint64_t)a->k / 2, (cuuint64_t)u1}, strides[1] = {(cuuint64_t)a->w_stride};
+        const cuuint32_t box[2] = {128, 128};
+        if (irx_dev_tmap(&k.tma_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void *)(size_t)k.w, dims, strides, box,
+                         CU_TENSOR_MAP_SWIZZLE_128B)) return 1;
+        k.ck = ck;
+        {   /* division by d = group / 32 of numbers below 2^26: ceil(2^(26 + l) / d), l = ceil(log2 d) */
+            const uint64_t d32 = (uint64_t)a->group / 32;
+            int l = 0;
+            while ((1ull << l) < d32) l++;
+            k.gshift = (uint8_t)(26 + l);
+            k.gmul = ((1ull << (26 + l)) + d32 - 1) / d32;
+        }
+        return irx_dev_launch(d, K_MV4 + 6 * f32 + gv * 2 + nt - 1, (unsigned)(tiles * ck), 256, IRX_MV4_SMEM(nt), (unsigned)ck, st, &k);
     }
     if (serve_grid(d, K_MV4_ANY, 256, 0, ((u1 - u0) * ((a->m + 3) / 4) + 7) / 8, &grid)) return 1;
     return irx_dev_launch(d, K_MV4_ANY, (unsigned)grid, 256, 0, 1, st, &k);
