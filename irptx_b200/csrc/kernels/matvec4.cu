@@ -177,7 +177,8 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
     const int64_t tile = blockIdx.x / p.ck, nb = (p.n1 - p.n0 + 127) / 128;
     const int64_t row0 = p.n0 + (tile % nb) * 128, m0 = (tile / nb) * TOK;
     const int k_all = (int)p.k, steps = (int)((p.k + 255) / 256);
-    const int s0 = (int)((int64_t)rank * steps / p.ck), s1 = (int)((int64_t)(rank + 1) * steps / p.ck);
+    // this block's stages: rank, rank + ck, ..., so that the cluster reads neighbouring bytes of a row at a time
+    const int ck = p.ck, n_st = (steps - rank + ck - 1) / ck;
     float acc[2][NT][4];
 #pragma unroll
     for (int rt = 0; rt < 2; rt++)
@@ -195,9 +196,9 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
     __syncthreads();
 
     auto fetch = [&](int s) {                            // stage s into its slot, by one thread
-        if (tid == 0 && s < s1) {
-            irx_mbar_expect_tx(full + (s - s0) % ST, M::W);
-            tma_load_2d(sm + ((s - s0) % ST) * M::W, &p.tma_w, s * 128, (int)row0, full + (s - s0) % ST);
+        if (tid == 0 && s < n_st) {
+            irx_mbar_expect_tx(full + s % ST, M::W);
+            tma_load_2d(sm + (s % ST) * M::W, &p.tma_w, (s * ck + rank) * 128, (int)row0, full + s % ST);
         }
     };
     // The tokens' part, a stage ahead in registers, stored in the order in which the weights unpack: bf16 8
@@ -208,24 +209,24 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
     const int64_t xoff = F32 ? m0 * p.x_stride + tid : (m0 + (tid >> 5)) * p.x_stride + (tid & 31) * 8;
     auto xload = [&](int s) {
         if (F32) {
-            const float *x = reinterpret_cast<const float *>(p.x) + xoff + (int64_t)s * 256;
+            const float *x = reinterpret_cast<const float *>(p.x) + xoff + (int64_t)(s * ck + rank) * 256;
 #pragma unroll
             for (int m = 0; m < TOK; m++) {
                 xr[m] = 0.0f;
-                if (s < s1 && m0 + m < p.m && s * 256 + tid < k_all) xr[m] = __ldg(x + m * p.x_stride);
+                if (s < n_st && m0 + m < p.m && (s * ck + rank) * 256 + tid < k_all) xr[m] = __ldg(x + m * p.x_stride);
             }
         } else {
-            const __nv_bfloat16 *x = reinterpret_cast<const __nv_bfloat16 *>(p.x) + xoff + (int64_t)s * 256;
+            const __nv_bfloat16 *x = reinterpret_cast<const __nv_bfloat16 *>(p.x) + xoff + (int64_t)(s * ck + rank) * 256;
 #pragma unroll
             for (int i = 0; i < NT; i++) {
                 xb[i] = make_uint4(0, 0, 0, 0);
-                if (s < s1 && m0 + (tid >> 5) + 8 * i < p.m && s * 256 + (tid & 31) * 8 < k_all)
+                if (s < n_st && m0 + (tid >> 5) + 8 * i < p.m && (s * ck + rank) * 256 + (tid & 31) * 8 < k_all)
                     xb[i] = __ldg(reinterpret_cast<const uint4 *>(x + 8 * i * p.x_stride));
             }
         }
     };
     auto xstore = [&](int s) {
-        unsigned char *st = sm + M::RING + ((s - s0) % ST) * M::X;
+        unsigned char *st = sm + M::RING + (s % ST) * M::X;
         if (F32) {
             const int k8 = tid & 7;
             st += ((tid & ~7) + (k8 < 4 ? 2 * k8 : 2 * k8 - 7)) * 2;
@@ -257,24 +258,24 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
         __syncthreads();
     }
 #pragma unroll
-    for (int i = 0; i < ST - 1; i++) fetch(s0 + i);
-    mv4_scales<GV>(p, at, (uint32_t)s0 * 256 + wk * 128, t, S[0]);
-    mv4_scales<GV>(p, at, (uint32_t)(s0 + 1) * 256 + wk * 128, t, S[1]);
-    xload(s0);
-    xstore(s0);
-    xload(s0 + 1);
+    for (int i = 0; i < ST - 1; i++) fetch(i);
+    mv4_scales<GV>(p, at, (uint32_t)rank * 256 + wk * 128, t, S[0]);
+    mv4_scales<GV>(p, at, (uint32_t)(ck + rank) * 256 + wk * 128, t, S[1]);
+    xload(0);
+    xstore(0);
+    xload(1);
     int ok = 1;
-    for (int s = s0; s < s1; s += 2) {
+    for (int s = 0; s < n_st; s += 2) {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            if (s + u >= s1) break;
-            const int slot = (s + u - s0) % ST;
-            ok = ok && irx_mbar_wait(full + slot, ((s + u - s0) / ST) & 1);
+            if (s + u >= n_st) break;
+            const int slot = (s + u) % ST;
+            ok = ok && irx_mbar_wait(full + slot, ((s + u) / ST) & 1);
             __syncthreads();                             // the tokens are there too; the stage before is free
             fetch(s + u + ST - 1);
             mv4_stage<GV, NT>(irx_smem_u32(sm) + slot * M::W, sm + M::RING + slot * M::X, wr, wk, lane, S[u], p.z != nullptr, sshift, acc);
-            mv4_scales<GV>(p, at, (uint32_t)(s + u + 2) * 256 + wk * 128, t, S[u]);
-            if (s + u + 1 < s1) {
+            mv4_scales<GV>(p, at, (uint32_t)((s + u + 2) * ck + rank) * 256 + wk * 128, t, S[u]);
+            if (s + u + 1 < n_st) {
                 xstore(s + u + 1);
                 xload(s + u + 2);
             }
@@ -282,7 +283,7 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
     }
     if (!ok) {                                           // a wait ran out: report it, and let copies in flight land
         irx_flag(p.err, IRX_KERR_TIMEOUT);
-        for (int s = max(s0, s1 - ST); s < s1; s++) irx_mbar_wait(full + (s - s0) % ST, ((s - s0) / ST) & 1);
+        for (int s = max(0, n_st - ST); s < n_st; s++) irx_mbar_wait(full + s % ST, (s / ST) & 1);
     }
     __syncthreads();
     // the second half's sums go through shared memory to the first half's warps, which leave the block's
@@ -303,16 +304,16 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
         }
         if (half) __syncthreads();
     }
-    if (p.ck > 1) cluster_sync(); else __syncthreads();
-    const int rows = 128 / p.ck, r0 = rank * rows;
+    if (ck > 1) cluster_sync(); else __syncthreads();
+    const int rows = 128 / ck, r0 = rank * rows;
     const float *fin = red + r0 * M::RS;
-    if (p.ck > 1) {
+    if (ck > 1) {
         float *sum = red + 128 * M::RS;
         for (int i = tid; i < rows * (COLS / 4); i += MV4_WARPS * 32) {
             const int r = i / (COLS / 4), c = (i % (COLS / 4)) * 4;
             const float *a = red + (r0 + r) * M::RS + c;
             float4 v = ld_cluster4(cluster_addr(a, 0));
-            for (int q = 1; q < p.ck; q++) {
+            for (int q = 1; q < ck; q++) {
                 const float4 x = ld_cluster4(cluster_addr(a, q));
                 v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
             }
@@ -327,7 +328,7 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
         const float v = F32 ? a[0] + (a[1] + a[2]) : a[0];
         if (row0 + r0 + r < p.n1 && m0 + m < p.m) irx_st1(p.y, p.dt, (m0 + m) * p.n + row0 + r0 + r, v);
     }
-    if (p.ck > 1) cluster_sync();                        // no block leaves while its sums are still read
+    if (ck > 1) cluster_sync();                        // no block leaves while its sums are still read
 }
 
 // Any sizes, strides and types: a warp per row of w and four tokens, two weights a lane and step.
