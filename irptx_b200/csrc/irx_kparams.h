@@ -175,7 +175,7 @@ typedef struct {
     int64_t     m, n, k, x_stride, w_stride;
     int64_t     n0, n1;             /* rows of w of this launch */
     int32_t     group, groups;
-    int32_t     ck;                 /* blocks of a cluster: slices of k */
+    int32_t     lck;                /* log2 of a cluster's blocks: slices of k */
     uint8_t     dt, sdt, gshift, pad;
     uint64_t    gmul;               /* group of k: (k / 32 * gmul) >> gshift */
 } irx_kmv4_t;

@@ -173,12 +173,11 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
     unsigned char *sm = sm_raw + ((1024u - (irx_smem_u32(sm_raw) & 1023u)) & 1023u);   // the swizzle's period
     constexpr int ST = IRX_MV4_STAGES, COLS = NT * 8, TOK = F32 ? COLS / 3 : COLS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wr = warp & 3, wk = warp >> 2, g = lane >> 2, t = lane & 3;
-    const int rank = (int)blockIdx.x % p.ck;
-    const int64_t tile = blockIdx.x / p.ck, nb = (p.n1 - p.n0 + 127) / 128;
-    const int64_t row0 = p.n0 + (tile % nb) * 128, m0 = (tile / nb) * TOK;
-    const int k_all = (int)p.k, steps = (int)((p.k + 255) / 256);
+    const int lck = p.lck, ck = 1 << lck, rank = (int)blockIdx.x & (ck - 1);
+    const unsigned tile = blockIdx.x >> lck, nb = (unsigned)((p.n1 - p.n0 + 127) >> 7), mt = nb == 1 ? tile : tile / nb;
+    const int row0 = (int)p.n0 + (int)(tile - mt * nb) * 128, n1 = (int)p.n1, m0 = (int)mt * TOK, m_all = (int)p.m;
     // this block's stages: rank, rank + ck, ..., so that the cluster reads neighbouring bytes of a row at a time
-    const int ck = p.ck, n_st = (steps - rank + ck - 1) / ck;
+    const int k_all = (int)p.k, steps = (k_all + 255) >> 8, n_st = (steps - rank + ck - 1) >> lck;
     float acc[2][NT][4];
 #pragma unroll
     for (int rt = 0; rt < 2; rt++)
@@ -198,7 +197,7 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
     auto fetch = [&](int s) {                            // stage s into its slot, by one thread
         if (tid == 0 && s < n_st) {
             irx_mbar_expect_tx(full + s % ST, M::W);
-            tma_load_2d(sm + (s % ST) * M::W, &p.tma_w, (s * ck + rank) * 128, (int)row0, full + s % ST);
+            tma_load_2d(sm + (s % ST) * M::W, &p.tma_w, (s * ck + rank) * 128, row0, full + s % ST);
         }
     };
     // The tokens' part, a stage ahead in registers, stored in the order in which the weights unpack: bf16 8
@@ -206,24 +205,28 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
     // (truncations, so that the parts of an infinity or a NaN stay what they should).
     uint4 xb[F32 ? 1 : NT];
     float xr[F32 ? TOK : 1];
-    const int64_t xoff = F32 ? m0 * p.x_stride + tid : (m0 + (tid >> 5)) * p.x_stride + (tid & 31) * 8;
-    auto xload = [&](int s) {
+    const char *xsrc = reinterpret_cast<const char *>(p.x) +
+        (F32 ? ((int64_t)m0 * p.x_stride + tid + rank * 256) * 4 : ((int64_t)(m0 + (tid >> 5)) * p.x_stride + (tid & 31) * 8 + rank * 256) * 2);
+    const int64_t xrow = p.x_stride * (F32 ? 4 : 16), xadv = (int64_t)ck * 256 * (F32 ? 4 : 2);
+    int xk = rank * 256 + (F32 ? tid : (tid & 31) * 8);   // the k that the next load starts at
+    const int xleft = m_all - m0 - (F32 ? 0 : tid >> 5);
+    auto xload = [&]() {
+        const bool kin = xk < k_all;
         if (F32) {
-            const float *x = reinterpret_cast<const float *>(p.x) + xoff + (int64_t)(s * ck + rank) * 256;
 #pragma unroll
             for (int m = 0; m < TOK; m++) {
                 xr[m] = 0.0f;
-                if (s < n_st && m0 + m < p.m && (s * ck + rank) * 256 + tid < k_all) xr[m] = __ldg(x + m * p.x_stride);
+                if (kin && m < xleft) xr[m] = __ldg(reinterpret_cast<const float *>(xsrc + m * xrow));
             }
         } else {
-            const __nv_bfloat16 *x = reinterpret_cast<const __nv_bfloat16 *>(p.x) + xoff + (int64_t)(s * ck + rank) * 256;
 #pragma unroll
             for (int i = 0; i < NT; i++) {
                 xb[i] = make_uint4(0, 0, 0, 0);
-                if (s < n_st && m0 + (tid >> 5) + 8 * i < p.m && (s * ck + rank) * 256 + (tid & 31) * 8 < k_all)
-                    xb[i] = __ldg(reinterpret_cast<const uint4 *>(x + 8 * i * p.x_stride));
+                if (kin && 8 * i < xleft) xb[i] = __ldg(reinterpret_cast<const uint4 *>(xsrc + i * xrow));
             }
         }
+        xk += ck * 256;
+        xsrc += xadv;
     };
     auto xstore = [&](int s) {
         unsigned char *st = sm + M::RING + (s % ST) * M::X;
@@ -251,7 +254,7 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
     Mv4Scale S[2] = {};
     uint32_t at[4];                                      // rows past the end read the last row's: their sums go nowhere
 #pragma unroll
-    for (int i = 0; i < 4; i++) at[i] = (uint32_t)(min(row0 + wr * 32 + i * 8 + g, p.n1 - 1) * p.groups);
+    for (int i = 0; i < 4; i++) at[i] = (uint32_t)min(row0 + wr * 32 + i * 8 + g, n1 - 1) * (uint32_t)p.groups;
     const int sshift = p.sdt == DT_BF16 ? 16 : 0;
     if (F32) {                                           // columns that no token has stay zero
         for (int i = tid; i < ST * M::X / 16; i += MV4_WARPS * 32) *reinterpret_cast<uint4 *>(sm + M::RING + i * 16) = make_uint4(0, 0, 0, 0);
@@ -261,9 +264,9 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
     for (int i = 0; i < ST - 1; i++) fetch(i);
     mv4_scales<GV>(p, at, (uint32_t)rank * 256 + wk * 128, t, S[0]);
     mv4_scales<GV>(p, at, (uint32_t)(ck + rank) * 256 + wk * 128, t, S[1]);
-    xload(0);
+    xload();
     xstore(0);
-    xload(1);
+    xload();
     int ok = 1;
     for (int s = 0; s < n_st; s += 2) {
 #pragma unroll
@@ -277,7 +280,7 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
             mv4_scales<GV>(p, at, (uint32_t)((s + u + 2) * ck + rank) * 256 + wk * 128, t, S[u]);
             if (s + u + 1 < n_st) {
                 xstore(s + u + 1);
-                xload(s + u + 2);
+                xload();
             }
         }
     }
@@ -305,7 +308,7 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
         if (half) __syncthreads();
     }
     if (ck > 1) cluster_sync(); else __syncthreads();
-    const int rows = 128 / ck, r0 = rank * rows;
+    const int lrows = 7 - lck, rows = 1 << lrows, r0 = rank << lrows;
     const float *fin = red + r0 * M::RS;
     if (ck > 1) {
         float *sum = red + 128 * M::RS;
@@ -323,10 +326,10 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
         fin = sum;
     }
     for (int i = tid; i < rows * TOK; i += MV4_WARPS * 32) {
-        const int r = i % rows, m = i / rows;
+        const int r = i & (rows - 1), m = i >> lrows;
         const float *a = fin + r * M::RS + (F32 ? 3 * m : m);
         const float v = F32 ? a[0] + (a[1] + a[2]) : a[0];
-        if (row0 + r0 + r < p.n1 && m0 + m < p.m) irx_st1(p.y, p.dt, (m0 + m) * p.n + row0 + r0 + r, v);
+        if (row0 + r0 + r < n1 && m0 + m < m_all) irx_st1(p.y, p.dt, (int64_t)(m0 + m) * p.n + row0 + r0 + r, v);
     }
     if (ck > 1) cluster_sync();                        // no block leaves while its sums are still read
 }

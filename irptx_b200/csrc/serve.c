@@ -399,14 +399,14 @@ static int launch_mv4(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsigne
         const int f32 = a->dt == DT_F32, gv = a->group % 128 == 0 ? 2 : a->group % 64 == 0 ? 1 : 0;
         const int nt = a->m > (f32 ? 2 : 8) ? 2 : 1, tok = f32 ? (nt == 1 ? 2 : 5) : 8 * nt;
         const int64_t tiles = ((u1 - u0 + 127) / 128) * ((a->m + tok - 1) / tok), steps = (a->k + 255) / 256;
-        int ck = 1;
-        while (ck < 8 && tiles * ck * 2 <= 2 * d->sms && ck * 2 <= steps) ck *= 2;
-        if (tiles * ck > MAX_COUNT) return irx_fail(E042, "a matvec4 past one launch's blocks");
+        int lck = 0;
+        while (lck < 3 && (tiles << (lck + 1)) <= 2 * d->sms && (2 << lck) <= steps) lck++;
+        if (tiles << lck > MAX_COUNT) return irx_fail(E042, "a matvec4 past one launch's blocks");
         const cuuint64_t dims[2] = {(cuuint64_t)a->k / 2, (cuuint64_t)u1}, strides[1] = {(cuuint64_t)a->w_stride};
         const cuuint32_t box[2] = {128, 128};
         if (irx_dev_tmap(&k.tma_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void *)(size_t)k.w, dims, strides, box,
                          CU_TENSOR_MAP_SWIZZLE_128B)) return 1;
-        k.ck = ck;
+        k.lck = lck;
         {   /* division by d = group / 32 of numbers below 2^26: ceil(2^(26 + l) / d), l = ceil(log2 d) */
             const uint64_t d32 = (uint64_t)a->group / 32;
             int l = 0;
@@ -414,7 +414,7 @@ static int launch_mv4(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsigne
             k.gshift = (uint8_t)(26 + l);
             k.gmul = ((1ull << (26 + l)) + d32 - 1) / d32;
         }
-        return irx_dev_launch(d, K_MV4 + 6 * f32 + gv * 2 + nt - 1, (unsigned)(tiles * ck), 256, IRX_MV4_SMEM(nt), (unsigned)ck, st, &k);
+        return irx_dev_launch(d, K_MV4 + 6 * f32 + gv * 2 + nt - 1, (unsigned)(tiles << lck), 256, IRX_MV4_SMEM(nt), 1u << lck, st, &k);
     }
     if (serve_grid(d, K_MV4_ANY, 256, 0, ((u1 - u0) * ((a->m + 3) / 4) + 7) / 8, &grid)) return 1;
     return irx_dev_launch(d, K_MV4_ANY, (unsigned)grid, 256, 0, 1, st, &k);
