@@ -20,54 +20,71 @@
 
 #define DEC_JOIN 16
 
-struct DecCur {                       // a place in the laid-out chunks: chunk j of unit u of sequence b
-    int b, u, j, nch, nvis, lo, sk;   // of sequence b: chunks, visible keys, window start, sinks before it
+// A place in the laid-out chunks: chunk j of the unit (kv head h0 + h, row block rb) of sequence b. A
+// chunk is a block of IRX_DEC_KEYS positions: the first `cs` of a sequence's chunks are the blocks that
+// hold sinks, the others the blocks from wb on; keys outside the mask are dropped in their tile.
+struct DecCur {
+    int b, h, rb, j;
+    int nch, n, lo, sk, cs, wb;       // of sequence b: chunks, tokens, window start, sinks before it
 };
 
-__device__ __forceinline__ int dec_len(const irx_kdec_t &p, int b)
+__device__ __forceinline__ int dec_len(const irx_kdec_t &p, int n)
 {
-    const int n = p.lens[b];
     const int64_t cap = (int64_t)p.cols * p.page_size;
     return n < 0 ? 0 : (int64_t)n > cap ? (int)cap : n;
 }
 
-__device__ __forceinline__ int dec_vis(const irx_kdec_t &p, int n, int &lo, int &sk)
+__device__ __forceinline__ int dec_blocks(int n) { return n / IRX_DEC_KEYS + (n % IRX_DEC_KEYS != 0); }
+
+// Sequence c.b's numbers, from its length.
+__device__ __forceinline__ void dec_enter(const irx_kdec_t &p, DecCur &c, int len)
 {
-    lo = sk = 0;
-    if (p.window > 0 && n > p.window) {
-        lo = n - p.window;
-        sk = p.sinks < lo ? p.sinks : lo;
-        return sk + p.window;
+    c.n = dec_len(p, len);
+    c.lo = c.sk = c.cs = c.wb = 0;
+    if (p.window > 0 && c.n > p.window) {
+        c.lo = c.n - p.window;
+        c.sk = min(p.sinks, c.lo);
+        c.cs = dec_blocks(c.sk);
+        c.wb = max(c.lo / IRX_DEC_KEYS, c.cs);
     }
-    return n;
+    c.nch = c.cs + dec_blocks(c.n) - c.wb;
 }
 
-__device__ __forceinline__ int dec_chunks(int nvis) { return (nvis + IRX_DEC_KEYS - 1) / IRX_DEC_KEYS; }
-
-__device__ __forceinline__ void dec_enter(const irx_kdec_t &p, DecCur &c)      // sequence c.b's numbers
-{
-    c.nvis = dec_vis(p, dec_len(p, c.b), c.lo, c.sk);
-    c.nch = dec_chunks(c.nvis);
-}
-
-__device__ __forceinline__ void dec_next(const irx_kdec_t &p, DecCur &c, int upb)
+__device__ __forceinline__ void dec_next(const irx_kdec_t &p, DecCur &c)
 {
     if (++c.j < c.nch) return;
     c.j = 0;
-    if (++c.u < upb) return;
-    c.u = 0;
+    if (++c.rb < p.split) return;
+    c.rb = 0;
+    if (++c.h < p.h1 - p.h0) return;
+    c.h = 0;
     do {
-        if (++c.b >= p.batch) { c.nvis = c.lo = c.sk = 0; c.nch = 0x7fffffff; return; }   // past the end
-        dec_enter(p, c);
+        if (++c.b >= p.batch) { c.n = 0; c.nch = 0x7fffffff; return; }        // past the end
+        dec_enter(p, c, p.lens[c.b]);
     } while (c.nch == 0);
 }
 
+// The first position of the cursor's chunk j, and whether a tile of `keys` positions from pos shows any
+// key, or shows all of them.
+__device__ __forceinline__ int dec_pos(const DecCur &c, int j) { return (j < c.cs ? j : j - c.cs + c.wb) * IRX_DEC_KEYS; }
+__device__ __forceinline__ bool dec_any(const DecCur &c, int pos, int keys) { return pos < c.n && (pos > c.lo - keys || pos < c.sk); }
+__device__ __forceinline__ bool dec_all(const DecCur &c, int pos, int keys) { return c.n - pos >= keys && (pos >= c.lo || c.sk - pos >= keys); }
+__device__ __forceinline__ bool dec_sees(const DecCur &c, int pos) { return pos < c.n && (pos >= c.lo || pos < c.sk); }
+
 struct DecShare {
-    long long c0, c1, total;          // this block's chunks and all chunks
+    long long c0, c1, q;              // this block's chunks; the first r blocks have q + 1, the others q
     long long wsum[8];                // a warp each
-    int geff, b, u, j, last;
-    unsigned arrived;
+    int geff, r, b, u, j;
+    int last[2];
+    // the shares of units that other blocks hold too: [0] the one that began before this block, [1] the
+    // one that goes on after it; pieces = 0: none
+    struct { long long unit; int first, pieces, b, head0, live; } pend[2];
 };
+
+__device__ __forceinline__ long long dec_div(long long a, long long b)         // not below 0; mostly 32 bits
+{
+    return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
 
 // The block's chunk range and where it starts: every block sums the chunks of all sequences (a
 // segment of them per thread, then a scan), so nothing has to run before the kernel.
@@ -77,11 +94,12 @@ __device__ __forceinline__ void dec_partition(const irx_kdec_t &p, int upb, DecS
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = THREADS / 32;
     const int seg = (p.batch + THREADS - 1) / THREADS, b0 = tid * seg, b1 = min(p.batch, b0 + seg);
     long long sum = 0;
+    DecCur w;
     for (int b = b0; b < b1; b++) {
-        int lo, sk;
-        const int raw = p.lens[b], n = dec_len(p, b);
-        if (raw != n && blockIdx.x == 0) irx_flag(p.err, IRX_KERR_INDEX);
-        sum += dec_chunks(dec_vis(p, n, lo, sk));
+        const int raw = p.lens[b];
+        dec_enter(p, w, raw);
+        if (raw != w.n && blockIdx.x == 0) irx_flag(p.err, IRX_KERR_INDEX);
+        sum += w.nch;
     }
     long long inc = sum;
 #pragma unroll
@@ -91,38 +109,52 @@ __device__ __forceinline__ void dec_partition(const irx_kdec_t &p, int upb, DecS
     }
     if (lane == 31) S.wsum[warp] = inc;
     __syncthreads();
-    if (tid == 0) {
-        long long a = 0;
-        for (int w = 0; w < nw; w++) { const long long v = S.wsum[w]; S.wsum[w] = a; a += v; }
-        S.total = a * upb;
-        S.geff = (int)min((long long)gridDim.x, S.total);
-        S.c0 = S.c1 = 0;
-        if ((int)blockIdx.x < S.geff) {
-            S.c0 = blockIdx.x * S.total / S.geff;
-            S.c1 = (blockIdx.x + 1) * S.total / S.geff;
-        }
+    long long total = 0, before = 0;
+#pragma unroll
+    for (int i = 0; i < nw; i++) {
+        if (i == warp) before = total;
+        total += S.wsum[i];
     }
-    __syncthreads();
-    if (S.c0 == S.c1) return;
-    const long long ex = (S.wsum[warp] + inc - sum) * upb;
-    if (S.c0 >= ex && S.c0 < ex + sum * upb) {           // exactly one thread's segment holds c0
-        long long r = S.c0 - ex;
+    total *= upb;
+    const int geff = (int)min((long long)gridDim.x, total), i = blockIdx.x;
+    const long long q = geff ? dec_div(total, geff) : 0;
+    const int r = (int)(total - q * geff);
+    const long long c0 = i < geff ? i * q + min(i, r) : 0, c1 = i < geff ? c0 + q + (i < r) : 0;
+    if (tid == 0) {
+        S.c0 = c0; S.c1 = c1; S.q = q; S.r = r; S.geff = geff;
+        S.pend[0].pieces = S.pend[1].pieces = 0;
+    }
+    const long long ex = (before + inc - sum) * upb;
+    if (c0 < c1 && c0 >= ex && c0 < ex + sum * upb) {    // exactly one thread's segment holds c0
+        long long at = c0 - ex;
         for (int b = b0; b < b1; b++) {
-            int lo, sk;
-            const long long nch = dec_chunks(dec_vis(p, dec_len(p, b), lo, sk));
-            if (r < nch * upb) { S.b = b; S.u = (int)(r / nch); S.j = (int)(r % nch); break; }
-            r -= nch * upb;
+            dec_enter(p, w, p.lens[b]);
+            if (at < (long long)w.nch * upb) {
+                const long long u = dec_div(at, w.nch);
+                S.b = b; S.u = (int)u; S.j = (int)(at - u * w.nch);
+                break;
+            }
+            at -= (long long)w.nch * upb;
         }
     }
     __syncthreads();
 }
 
-// The block that holds chunk c (block i starts at floor(i * total / geff)).
-__device__ __forceinline__ int dec_block_of(const DecShare &S, long long c) { return (int)(((c + 1) * S.geff - 1) / S.total); }
+__device__ __forceinline__ void dec_start(const irx_kdec_t &p, const DecShare &S, DecCur &c)
+{
+    c.b = S.b;
+    c.h = S.u / p.split;
+    c.rb = S.u % p.split;
+    c.j = S.j;
+    dec_enter(p, c, p.lens[c.b]);
+}
 
-// Byte-free part of a tile's addressing: the element offset of visible key jj of sequence b, kv head
-// hk, given its page; -1 when there is none.
-__device__ __forceinline__ int dec_pos(const DecCur &c, int jj) { return jj < c.sk ? jj : jj - c.sk + c.lo; }
+// The block that holds chunk c.
+__device__ __forceinline__ int dec_block_of(const DecShare &S, long long c)
+{
+    const long long big = (long long)S.r * (S.q + 1);
+    return (int)(c < big ? dec_div(c, S.q + 1) : S.r + dec_div(c - big, S.q));
+}
 
 // Partials: slot s holds `rows` x dp accumulators, then rows (max, sum) pairs. Maxima are of
 // scale2 * q.k, the log2 domain.
@@ -152,100 +184,72 @@ __device__ __forceinline__ void dec_store_out(const irx_kdec_t &p, int b, int he
     for (int i = 0; i < 4; i++) if (d0 + i < p.d) irx_st1(p.o, p.dt, o + i, a[i]);
 }
 
-// Fold `cnt` partials, slot(i) = i ? s0 + i * step + adj : s_first, in order, by the whole block. With
-// `final` the result is the unit's output, else it becomes the partial of the first slot.
-// `sw` holds cnt x ROWS weights and ROWS (max, sum) pairs.
+// Fold `cnt` partials, in slots first, rest0 + step, rest0 + 2 step, ..., in that order, by the whole block.
+// With `fin` the result is the unit's output, else it becomes the partial of the first slot. Every thread
+// weighs the partials of its own row, so that all its loads are on their way at once and no
+// barrier is needed.
 template <int DP, int ROWS, int THREADS>
 __device__ __forceinline__ void dec_fold(const irx_kdec_t &p, int first, int rest0, int step, int cnt, bool fin, int b,
-                                         int head0, int live, float *sw)
+                                         int head0, int live, float2 *sw)
 {
-    const int tid = threadIdx.x;
-    float *mx = sw + cnt * ROWS;
-    __syncthreads();
-    for (int i = tid; i < cnt * ROWS; i += THREADS) {
-        const int k = i / ROWS, r = i % ROWS;
-        const int s = k ? rest0 + k * step : first;
-        sw[i] = __ldcg(dec_slot(p, s, ROWS, DP) + ROWS * DP + 2 * r);
-    }
-    __syncthreads();
-    if (tid < ROWS) {
-        float m = -INFINITY, l = 0.0f;
-        for (int k = 0; k < cnt; k++) m = fmaxf(m, sw[k * ROWS + tid]);
-        const float base = m == -INFINITY ? 0.0f : m;
-        for (int k = 0; k < cnt; k++) {
-            const int s = k ? rest0 + k * step : first;
-            const float f = exp2f(sw[k * ROWS + tid] - base);
-            sw[k * ROWS + tid] = f;
-            l += f * __ldcg(dec_slot(p, s, ROWS, DP) + ROWS * DP + 2 * tid + 1);
-        }
-        mx[2 * tid] = m;
-        mx[2 * tid + 1] = l;
-    }
-    __syncthreads();
-    for (int it = tid; it < ROWS * DP / 4; it += THREADS) {
+    for (int it = threadIdx.x; it < live * (DP / 4); it += THREADS) {
         const int r = it / (DP / 4), d0 = (it % (DP / 4)) * 4;
-        if (r >= live || d0 >= p.d) continue;
+        if (d0 >= p.d) continue;
         float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float m = -INFINITY, l = 0.0f;
         for (int k0 = 0; k0 < cnt; k0 += 8) {
             float4 v[8];
+            float2 s[8];
 #pragma unroll
-            for (int k = 0; k < 8; k++)
+            for (int k = 0; k < 8; k++) {
+                s[k] = make_float2(-INFINITY, 0.0f);
                 if (k0 + k < cnt) {
-                    const int s = k0 + k ? rest0 + (k0 + k) * step : first;
-                    v[k] = __ldcg(reinterpret_cast<const float4 *>(dec_slot(p, s, ROWS, DP) + r * DP + d0));
+                    const float *o = dec_slot(p, k0 + k ? rest0 + (k0 + k) * step : first, ROWS, DP);
+                    s[k] = __ldcg(reinterpret_cast<const float2 *>(o + ROWS * DP) + r);
+                    v[k] = __ldcg(reinterpret_cast<const float4 *>(o + r * DP + d0));
                 }
+            }
+            float mn = m;
+#pragma unroll
+            for (int k = 0; k < 8; k++) mn = fmaxf(mn, s[k].x);
+            const float base = mn == -INFINITY ? 0.0f : mn, f0 = exp2f(m - base);
+            a.x *= f0; a.y *= f0; a.z *= f0; a.w *= f0;
+            l *= f0;
+            m = mn;
 #pragma unroll
             for (int k = 0; k < 8; k++)
                 if (k0 + k < cnt) {
-                    const float f = sw[(k0 + k) * ROWS + r];
+                    const float f = exp2f(s[k].x - base);
+                    l += f * s[k].y;
                     a.x += f * v[k].x; a.y += f * v[k].y; a.z += f * v[k].z; a.w += f * v[k].w;
                 }
         }
         if (fin) {
-            const float l = mx[2 * r + 1];
-            dec_store_out(p, b, head0 + r, d0, make_float4(a.x / l, a.y / l, a.z / l, a.w / l));
-            if (p.lse && d0 == 0)
-                p.lse[(int64_t)b * p.heads + head0 + r] = (mx[2 * r] + log2f(l)) * 0.6931471805599453f;
+            const float inv = 1.0f / l;
+            dec_store_out(p, b, head0 + r, d0, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
+            if (p.lse && d0 == 0) p.lse[(int64_t)b * p.heads + head0 + r] = (m + log2f(l)) * 0.6931471805599453f;
         } else {
-            *reinterpret_cast<float4 *>(dec_slot(p, first, ROWS, DP) + r * DP + d0) = a;
+            __stcg(reinterpret_cast<float4 *>(dec_slot(p, first, ROWS, DP) + r * DP + d0), a);
+            if (d0 == 0) sw[r] = make_float2(m, l);
         }
     }
-    if (!fin && tid < ROWS) {
-        float *ml = dec_slot(p, first, ROWS, DP) + ROWS * DP + 2 * tid;
-        ml[0] = mx[2 * tid];
-        ml[1] = mx[2 * tid + 1];
-    }
-}
-
-// One arrival on a counter: true in every thread of the last of `want` blocks to arrive, which
-// leaves the counter at zero and sees what the others wrote before they arrived.
-__device__ __forceinline__ bool dec_arrive(unsigned *ctr, unsigned want, DecShare &S)
-{
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const unsigned a = atomicAdd(ctr, 1u);
-        S.last = a == want - 1;
-        if (S.last) *ctr = 0;
-    }
-    __syncthreads();
-    if (!S.last) return false;
-    __threadfence();
-    return true;
+    if (fin) return;
+    __syncthreads();                                     // every thread has read the first slot's pairs
+    if (threadIdx.x < live) __stcg(reinterpret_cast<float2 *>(dec_slot(p, first, ROWS, DP) + ROWS * DP) + threadIdx.x, sw[threadIdx.x]);
 }
 
 // A unit's share of this block is done. `acc(r, d0, k)` gives the block's four accumulators of row r
-// from d0 (item k of this thread), `ml(r)` its (max, sum). Chunk c is the share's last one.
+// from d0 (item k of this thread), `ml(r)` its (max, sum). Chunk c is the share's last one. A unit
+// that is all here is written out; a part of one becomes a partial, which dec_join looks after at
+// the end of the block: waiting for the arrival count here would stall the block's loads.
 template <int DP, int ROWS, int THREADS, class Acc, class Ml>
-__device__ __forceinline__ void dec_finish(const irx_kdec_t &p, DecShare &S, const DecCur &cur, long long c, int upb,
-                                           float *sw, Acc acc, Ml ml)
+__device__ __forceinline__ void dec_finish(const irx_kdec_t &p, DecShare &S, const DecCur &cur, long long c, int upb, Acc acc, Ml ml)
 {
     const int tid = threadIdx.x;
-    const int hk = p.h0 + cur.u / p.split, rb = cur.u % p.split;
-    const int head0 = hk * p.group + rb * ROWS, live = min(ROWS, p.group - rb * ROWS);
+    const int head0 = (p.h0 + cur.h) * p.group + cur.rb * ROWS, live = min(ROWS, p.group - cur.rb * ROWS);
     const long long ua = c - cur.j, ub = ua + cur.nch;       // the unit's chunks
     const bool alone = ua >= S.c0 && ub <= S.c1;
-    const int slot = 2 * (int)blockIdx.x + (ua >= S.c0 ? 1 : 0);
+    const int which = ua >= S.c0 ? 1 : 0, slot = 2 * (int)blockIdx.x + which;
 #pragma unroll
     for (int k = 0; k < (ROWS * DP / 4 + THREADS - 1) / THREADS; k++) {
         const int it = tid + k * THREADS, r = it / (DP / 4), d0 = (it % (DP / 4)) * 4;
@@ -253,30 +257,69 @@ __device__ __forceinline__ void dec_finish(const irx_kdec_t &p, DecShare &S, con
         const float4 a = acc(r, d0, k);
         const float2 s = ml(r);
         if (alone) {
-            dec_store_out(p, cur.b, head0 + r, d0, make_float4(a.x / s.y, a.y / s.y, a.z / s.y, a.w / s.y));
+            const float inv = 1.0f / s.y;
+            dec_store_out(p, cur.b, head0 + r, d0, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
             if (p.lse && d0 == 0) p.lse[(int64_t)cur.b * p.heads + head0 + r] = (s.x + log2f(s.y)) * 0.6931471805599453f;
         } else {
             float *o = dec_slot(p, slot, ROWS, DP);
             __stcg(reinterpret_cast<float4 *>(o + r * DP + d0), a);
-            if (d0 == 0) __stcg(reinterpret_cast<float2 *>(o + ROWS * DP + 2 * r), s);
+            if (d0 == 0) __stcg(reinterpret_cast<float2 *>(o + ROWS * DP) + r, s);
         }
     }
-    if (alone) return;
-    const int first = dec_block_of(S, ua), pieces = dec_block_of(S, ub - 1) - first + 1;
-    const int64_t unit = (int64_t)cur.b * upb + cur.u;
-    if (pieces <= DEC_JOIN) {
-        if (dec_arrive(p.ticket + unit, (unsigned)pieces, S))
-            dec_fold<DP, ROWS, THREADS>(p, 2 * first + 1, 2 * first, 2, pieces, true, cur.b, head0, live, sw);
-        return;
+    if (!alone && tid == 0) {
+        const int first = dec_block_of(S, ua);
+        S.pend[which].unit = (long long)cur.b * upb + cur.h * p.split + cur.rb;
+        S.pend[which].first = first;
+        S.pend[which].pieces = dec_block_of(S, ub - 1) - first + 1;
+        S.pend[which].b = cur.b;
+        S.pend[which].head0 = head0;
+        S.pend[which].live = live;
     }
-    // partials fold in groups of DEC_JOIN, each into its first slot, and the groups' folds into the output
-    const int g = ((int)blockIdx.x - first) / DEC_JOIN, ng = (pieces + DEC_JOIN - 1) / DEC_JOIN;
-    const int g0 = first + g * DEC_JOIN, gn = min(DEC_JOIN, pieces - g * DEC_JOIN);
-    const int gslot = 2 * g0 + (g ? 0 : 1);
-    if (!dec_arrive(p.gcount + gslot, (unsigned)gn, S)) return;
-    dec_fold<DP, ROWS, THREADS>(p, gslot, 2 * g0, 2, gn, false, cur.b, head0, live, sw);
-    if (!dec_arrive(p.ticket + unit, (unsigned)ng, S)) return;
-    dec_fold<DP, ROWS, THREADS>(p, 2 * first + 1, 2 * first, 2 * DEC_JOIN, ng, true, cur.b, head0, live, sw);
+}
+
+// The end of a block: its partials arrive at their units' counters; the last block to arrive folds a
+// unit's partials, and leaves the counter at zero. Up to DEC_JOIN partials fold at once; more
+// fold in groups of DEC_JOIN first, each into its first slot, by the last block of the group.
+template <int DP, int ROWS, int THREADS>
+__device__ __forceinline__ void dec_join(const irx_kdec_t &p, DecShare &S, float2 *sw)
+{
+    // one arrival that publishes what the block's threads wrote before the last barrier, and shows the last
+    // block to arrive what all the others published
+    auto arrive = [&](unsigned *ctr, int want) {
+        unsigned a;
+        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(a) : "l"(ctr) : "memory");
+        if (a == (unsigned)want - 1) *ctr = 0;
+        return a == (unsigned)want - 1 ? 1 : 0;
+    };
+    if (!(S.pend[0].pieces | S.pend[1].pieces)) return;  // (a barrier ended the last unit's share)
+    if (threadIdx.x < 2) {
+        const auto &e = S.pend[threadIdx.x];
+        int last = 0;
+        if (e.pieces > DEC_JOIN) {
+            const int g = ((int)blockIdx.x - e.first) / DEC_JOIN;
+            last = arrive(p.gcount + 2 * (e.first + g * DEC_JOIN) + (g ? 0 : 1), min(DEC_JOIN, e.pieces - g * DEC_JOIN));
+        } else if (e.pieces) {
+            last = arrive(p.ticket + e.unit, e.pieces);
+        }
+        S.last[threadIdx.x] = last;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = 0; i < 2; i++) {
+        const auto e = S.pend[i];
+        if (!S.last[i]) continue;
+        if (e.pieces > DEC_JOIN) {
+            const int g = ((int)blockIdx.x - e.first) / DEC_JOIN, g0 = e.first + g * DEC_JOIN, ng = (e.pieces + DEC_JOIN - 1) / DEC_JOIN;
+            dec_fold<DP, ROWS, THREADS>(p, 2 * g0 + (g ? 0 : 1), 2 * g0, 2, min(DEC_JOIN, e.pieces - g * DEC_JOIN), false, e.b, e.head0, e.live, sw);
+            __syncthreads();
+            if (threadIdx.x == 0) S.last[i] = arrive(p.ticket + e.unit, ng);
+            __syncthreads();
+            if (!S.last[i]) continue;
+            dec_fold<DP, ROWS, THREADS>(p, 2 * e.first + 1, 2 * e.first, 2 * DEC_JOIN, ng, true, e.b, e.head0, e.live, sw);
+        } else {
+            dec_fold<DP, ROWS, THREADS>(p, 2 * e.first + 1, 2 * e.first, 2, e.pieces, true, e.b, e.head0, e.live, sw);
+        }
+    }
 }
 
 // Sequences with no tokens: zeros, and -inf for the log-sum.
@@ -292,23 +335,48 @@ __device__ __forceinline__ void dec_empty(const irx_kdec_t &p)
     }
 }
 
-// The page of the key `jj` (visible index) of the cursor's sequence, or -1 (flagged) when the table
-// holds no page of the pool there.
-__device__ __forceinline__ int dec_page(const irx_kdec_t &p, const DecCur &c, int jj, unsigned &slot)
+// Where a warp's key rows of the tiles to come lie: for each tile of its ring, for each of the tile's keys,
+// the key's page (copied from the table asynchronously, a whole ring ahead of its use, so that no load of
+// keys waits for the table) and the rest of its offset, -1 where there is no such key.
+template <int KEYS>
+struct DecRows {
+    long long off[KEYS];
+    int page[KEYS];
+};
+
+// pos / page_size by a multiplication, exact below 2^31 (the launcher's constants).
+__device__ __forceinline__ unsigned dec_page_of(const irx_kdec_t &p, int pos) { return (unsigned)(((uint64_t)(unsigned)pos * p.pmul) >> p.pshift); }
+
+template <int KEYS>
+__device__ __forceinline__ void dec_lookup(const irx_kdec_t &p, const DecCur &c, bool more, int pos0, DecRows<KEYS> &R)
 {
-    const unsigned pos = (unsigned)dec_pos(c, jj), pi = pos / (unsigned)p.page_size;
-    slot = pos - pi * (unsigned)p.page_size;
-    const int page = p.table[(int64_t)c.b * p.cols + pi];
-    return page < 0 ? -1 : page;
+    const int lane = threadIdx.x & 31;
+    if (lane < KEYS) {
+        const int pos = pos0 + lane;
+        long long off = -1;
+        if (more && dec_sees(c, pos)) {
+            const unsigned pi = dec_page_of(p, pos);
+            off = (long long)((unsigned)pos - pi * (unsigned)p.page_size) * p.token_stride + (long long)(p.h0 + c.h) * p.head_stride;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
+                         :: "r"(irx_smem_u32(&R.page[lane])), "l"(p.table + ((int64_t)c.b * p.cols + pi)) : "memory");
+        }
+        R.off[lane] = off;
+    }
 }
 
-__device__ __forceinline__ int64_t dec_offset(const irx_kdec_t &p, int page, unsigned slot, int hk)
+// The element offset of the tile's key `i`: -1 when there is none, -2 (flagged) when the table's page is
+// not one of the pool's.
+template <int KEYS>
+__device__ __forceinline__ long long dec_row(const irx_kdec_t &p, const DecRows<KEYS> &R, int i)
 {
+    const long long off = R.off[i];
+    if (off < 0) return -1;
+    const int page = R.page[i];
     if (page < 0 || page >= p.pages) {
         irx_flag(p.err, IRX_KERR_INDEX);
-        return -1;
+        return -2;
     }
-    return (int64_t)page * p.page_stride + (int64_t)slot * p.token_stride + (int64_t)hk * p.head_stride;
+    return off + (long long)page * p.page_stride;
 }
 
 // ---- bf16: matrix instructions ----
@@ -363,93 +431,159 @@ template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.as
 template <int DP, int NT, int ST>
 struct DecTc {
     static constexpr int THREADS = DEC_TC_WARPS * 32, ROWS = 8 * NT, TILE = 16 * DP * 2, QS = DP + 4;
-    // ring, then one 8-row block of the warps' accumulators (reused for a fold's weights), then
-    // (max, sum) pairs and the share
+    // ring, then one 8-row block of two warps' accumulators then
+    // (max, sum) pairs, the share, the rings' row places and barriers
     static constexpr int RING = DEC_TC_WARPS * ST * 2 * TILE;
-    static constexpr int MERGE = DEC_TC_WARPS * 8 * QS * 4;
+    static constexpr int MERGE = DEC_TC_WARPS / 2 * 8 * QS * 4;
     static constexpr int ML = DEC_TC_WARPS * ROWS * 8;
-    static constexpr int SMEM = RING + MERGE + ML + IRX_DEC_SHARE;
+    static constexpr int PLACES = RING + MERGE + ML + IRX_DEC_SHARE, BARS = PLACES + DEC_TC_WARPS * ST * (int)sizeof(DecRows<16>);
+    static constexpr int SMEM = 1024 + BARS + DEC_TC_WARPS * ST * 8;
     static_assert(SMEM == IRX_DEC_TC_SMEM(DP, NT, ST), "the launcher's shared memory size");
-    static_assert((IRX_DEC_MAX_CTAS / DEC_JOIN + 2) * ROWS * 4 <= MERGE && sizeof(DecShare) <= IRX_DEC_SHARE, "shared memory");
+    static_assert(sizeof(DecShare) <= IRX_DEC_SHARE, "shared memory");
 };
 
-template <int DP, int NT, int ST>
+// A tile lies in 64-dim columns of 16 rows x 128 bytes, 16-byte pieces swizzled by row, as TMA's 128-byte
+// swizzle leaves them. TMA: pages of a multiple of 8 slots, whose 8 or 16 rows are one box; a few
+// instructions fill a tile, where 16-byte copies with their addresses take as many as the products.
+template <int DP, int NT, int ST, bool TMA>
 __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
 {
     using T = DecTc<DP, NT, ST>;
-    extern __shared__ __align__(128) unsigned char sm[];
-    unsigned char *ring = sm;
+    extern __shared__ unsigned char sm_raw[];
+    unsigned char *sm = sm_raw + ((1024u - (irx_smem_u32(sm_raw) & 1023u)) & 1023u);   // the swizzle's period
     float *merge = reinterpret_cast<float *>(sm + T::RING);
     float2 *wml = reinterpret_cast<float2 *>(sm + T::RING + T::MERGE);
     DecShare &S = *reinterpret_cast<DecShare *>(sm + T::RING + T::MERGE + T::ML);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    DecRows<16> *rows = reinterpret_cast<DecRows<16> *>(sm + T::PLACES) + warp * ST;
+    uint64_t *bar = reinterpret_cast<uint64_t *>(sm + T::BARS) + warp * ST;
     const int upb = (p.h1 - p.h0) * p.split;
 
+    if (TMA && lane == 0) {
+        for (int i = 0; i < ST; i++) irx_mbar_init(bar + i, 1);
+        irx_fence_mbar_init();
+        tma_prefetch_desc(&p.tma_k);
+        tma_prefetch_desc(&p.tma_v);
+    }
     irx_pdl_enter();
     dec_partition<T::THREADS>(p, upb, S);
     if (S.c0 < S.c1) {
-        DecCur ld, cu;
-        ld.b = S.b; ld.u = S.u; ld.j = S.j;
-        dec_enter(p, ld);
-        cu = ld;
-        const __nv_bfloat16 *kg = reinterpret_cast<const __nv_bfloat16 *>(p.k), *vg = reinterpret_cast<const __nv_bfloat16 *>(p.v);
-        const uint32_t myring = irx_smem_u32(ring) + warp * (ST * 2 * T::TILE);
+        DecCur tl, cu;                                       // the tile to be loaded (without TMA: looked up) next, the one in work
+        dec_start(p, S, tl);
+        cu = tl;
+        unsigned char *myring = sm + warp * (ST * 2 * T::TILE);
+        const uint32_t ring = irx_smem_u32(myring);
+        long long tc = S.c0;                                 // the chunk that `tl` is at
+        int ok = 1;
+
+        // TMA: each lane holds the page and slot of one box of the next 32 boxes of this warp's tiles in the unit
+        const int two = TMA && p.box == 8 ? 1 : 0;           // boxes of a tile: 1 + two
+        int pg = -2, tok = 0, at = 0;
+        auto pages = [&]() {
+            const int j = tl.j + (lane >> two), pos = dec_pos(tl, j) + warp * 16 + (two ? (lane & 1) * 8 : 0);
+            pg = -2;                                         // no such box
+            if (tc < S.c1 && j < tl.nch && pos < tl.n) {
+                const unsigned pi = dec_page_of(p, pos);
+                tok = (int)((unsigned)pos - pi * (unsigned)p.page_size);
+                pg = p.table[(int64_t)tl.b * p.cols + pi];
+                if (pg < 0) pg = -1;
+            }
+            at = 0;
+        };
+        // without: each key row's place, a ring ahead
         constexpr int CPR = DP / 8, RPI = 32 / CPR, NI = 16 / RPI;
         const int lrow = lane / CPR, lch = lane % CPR;
         const bool cin = lch * 8 < p.d;
-        long long lc = S.c0;                                 // the chunk that `ld` is at
-        int pg = -1;
-        unsigned slot = 0;
-        // each lane looks up one key row's page a tile ahead of its use
-        auto lookup = [&]() {
-            const int jj = ld.j * IRX_DEC_KEYS + warp * 16 + (lane & 15);
-            pg = -2;                                         // no such key
-            if (lc < S.c1 && jj < ld.nvis) pg = dec_page(p, ld, jj, slot);
+        auto lookup = [&](int st) {
+            dec_lookup<16>(p, tl, tc < S.c1, dec_pos(tl, tl.j) + warp * 16, rows[st]);
+            if (tc < S.c1) {
+                tc++;
+                dec_next(p, tl);
+            }
         };
         auto fetch = [&](int st) {
-            if (lc < S.c1) {
-                const int64_t off = pg == -2 ? -1 : dec_offset(p, pg, slot, p.h0 + ld.u / p.split);
-                if (__any_sync(0xffffffffu, pg != -2)) {
-                    const uint32_t kd = myring + st * (2 * T::TILE), vd = kd + T::TILE;
+            if (TMA) {
+                if (tc >= S.c1) return;
+                if (dec_any(tl, dec_pos(tl, tl.j) + warp * 16, 16)) {
+                    const bool mine = lane >> two == at && pg != -2, good = mine && pg >= 0 && pg < p.pages;
+                    const unsigned have = __ballot_sync(0xffffffffu, good);
+                    if (__any_sync(0xffffffffu, mine && !good)) {      // no page of the pool: flagged, read as zeros
+                        if (lane == 0) irx_flag(p.err, IRX_KERR_INDEX);
+                        for (int i = lane; i < 2 * T::TILE / 16; i += 32)
+                            *reinterpret_cast<uint4 *>(myring + st * (2 * T::TILE) + i * 16) = make_uint4(0, 0, 0, 0);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    if (lane == 0) irx_mbar_expect_tx(bar + st, __popc(have) * 2 * (DP / 64) * 128 * p.box);
+                    __syncwarp();
+                    if (good) {
+                        unsigned char *kd = myring + st * (2 * T::TILE) + (two ? (lane & 1) * 1024 : 0);
 #pragma unroll
-                    for (int i = 0; i < NI; i++) {
-                        const int row = i * RPI + lrow;
-                        const int64_t o = __shfl_sync(0xffffffffu, off, row);
-                        const uint32_t d = row * (DP * 2) + ((lch ^ (row & 7)) << 4);
-                        const int64_t e = o >= 0 && cin ? o + lch * 8 : 0;
-                        const uint32_t nb = o >= 0 && cin ? 16 : 0;
-                        cp16(kd + d, kg + e, nb);
-                        cp16(vd + d, vg + e, nb);
+                        for (int i = 0; i < DP / 64; i++) {
+                            tma_load_4d(kd + i * 2048, &p.tma_k, i * 64, tok, p.h0 + tl.h, pg, bar + st);
+                            tma_load_4d(kd + T::TILE + i * 2048, &p.tma_v, i * 64, tok, p.h0 + tl.h, pg, bar + st);
+                        }
                     }
                 }
-                lc++;
-                dec_next(p, ld, upb);
-                lookup();
+                tc++;
+                dec_next(p, tl);
+                at++;
+                if (tl.j == 0 || at == 32 >> two) pages();
+                return;
             }
+            const long long off = dec_row<16>(p, rows[st], lane & 15);
+            if (__any_sync(0xffffffffu, off != -1)) {
+                const uint32_t kd = ring + st * (2 * T::TILE), vd = kd + T::TILE;
+#pragma unroll
+                for (int i = 0; i < NI; i++) {
+                    const int row = i * RPI + lrow;
+                    const long long o = __shfl_sync(0xffffffffu, off, row);
+                    const uint32_t d = (lch >> 3) * 2048 + row * 128 + (((lch & 7) ^ (row & 7)) << 4);
+                    const int64_t e = o >= 0 && cin ? o + lch * 8 : 0;
+                    const uint32_t nb = o >= 0 && cin ? 16 : 0;
+                    cp16(kd + d, reinterpret_cast<const __nv_bfloat16 *>(p.k) + e, nb);
+                    cp16(vd + d, reinterpret_cast<const __nv_bfloat16 *>(p.v) + e, nb);
+                }
+            }
+            __syncwarp();
+            lookup(st);
             cp_commit();
         };
-        lookup();
+        if (TMA) {
+            pages();
+        } else {
+            for (int s = 0; s < ST; s++) lookup(s);
+            cp_commit();
+            cp_wait<0>();
+            __syncwarp();
+        }
         for (int s = 0; s < ST; s++) fetch(s);
 
         uint32_t q[DP / 16][NT][2];
         float o[DP / 16][NT][4], m[NT][2], l[NT][2];
         int st = 0;
+        unsigned phase = 0;                                  // a bit per slot
         bool fresh = true;
+        auto load_q = [&](const DecCur &w) {                 // a unit's query rows
+            const __nv_bfloat16 *qg = reinterpret_cast<const __nv_bfloat16 *>(p.q) + (int64_t)w.b * p.q_stride;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                const int r = w.rb * T::ROWS + nt * 8 + g;
+                const __nv_bfloat16 *row = qg + (int64_t)((p.h0 + w.h) * p.group + r) * p.d;
+#pragma unroll
+                for (int ks = 0; ks < DP / 16; ks++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int d0 = ks * 16 + h * 8 + 2 * t;
+                        q[ks][nt][h] = r < p.group && d0 < p.d ? *reinterpret_cast<const uint32_t *>(row + d0) : 0u;
+                    }
+            }
+        };
+        load_q(cu);
         for (long long c = S.c0; c < S.c1; c++) {
-            if (fresh) {                                     // a unit starts: its query rows, an empty state
-                const int hk = p.h0 + cu.u / p.split, rb = cu.u % p.split;
-                const __nv_bfloat16 *qg = reinterpret_cast<const __nv_bfloat16 *>(p.q) + (int64_t)cu.b * p.q_stride;
+            if (fresh) {                                     // a unit starts: an empty state
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    const int r = rb * T::ROWS + nt * 8 + g;
-                    const __nv_bfloat16 *row = qg + (int64_t)(hk * p.group + r) * p.d;
-#pragma unroll
-                    for (int ks = 0; ks < DP / 16; ks++)
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const int d0 = ks * 16 + h * 8 + 2 * t;
-                            q[ks][nt][h] = r < p.group && d0 < p.d ? *reinterpret_cast<const uint32_t *>(row + d0) : 0u;
-                        }
                     m[nt][0] = m[nt][1] = -INFINITY;
                     l[nt][0] = l[nt][1] = 0.0f;
 #pragma unroll
@@ -459,34 +593,51 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
                 }
                 fresh = false;
             }
-            cp_wait<ST - 1>();
-            __syncwarp();
-            const int nv = cu.nvis - (cu.j * IRX_DEC_KEYS + warp * 16);
-            if (nv > 0) {
-                const uint32_t kb = myring + st * (2 * T::TILE), vb = kb + T::TILE;
-                float s[NT][4];
+            if (!TMA) {
+                cp_wait<ST - 1>();
+                __syncwarp();
+            }
+            const int pos = dec_pos(cu, cu.j) + warp * 16;
+            if (dec_any(cu, pos, 16)) {
+                const uint32_t kb = ring + st * (2 * T::TILE), vb = kb + T::TILE;
+                const bool whole = dec_all(cu, pos, 16);
+                if (TMA) {
+                    ok = ok && irx_mbar_wait(bar + st, (phase >> st) & 1);
+                    phase ^= 1u << st;
+                    if (!whole) {                            // rows that are not seen: their values may be anything, and 0 * NaN is not 0
+                        for (int i = lane; i < 16 * (DP / 8); i += 32) {
+                            const int row = i & 15;
+                            if (!dec_sees(cu, pos + row))
+                                *reinterpret_cast<uint4 *>(myring + st * (2 * T::TILE) + T::TILE + (i >> 7) * 2048 + row * 128 + ((i >> 4) & 7) * 16) =
+                                    make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async_smem();            // before the copy that comes here next
+                        __syncwarp();
+                    }
+                }
+                float s[NT][4], s2[NT][4];                   // two sums, of even and odd steps: half the chain
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[nt][i] = s2[nt][i] = 0.0f;
                 {
                     const int row = (lane & 7) + ((lane >> 3) & 1) * 8, ch = lane >> 4;
 #pragma unroll
                     for (int ks = 0; ks < DP / 16; ks++) {
                         uint32_t a[4];
-                        ldsm4(a, kb + row * (DP * 2) + (((2 * ks + ch) ^ (row & 7)) << 4));
+                        ldsm4(a, kb + (ks >> 2) * 2048 + row * 128 + (((2 * (ks & 3) + ch) ^ (row & 7)) << 4));
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) mma_16816(s[nt], a, q[ks][nt][0], q[ks][nt][1]);
+                        for (int nt = 0; nt < NT; nt++) mma_16816(ks & 1 ? s2[nt] : s[nt], a, q[ks][nt][0], q[ks][nt][1]);
                     }
                 }
+                const bool in0 = whole || dec_sees(cu, pos + g), in1 = whole || dec_sees(cu, pos + g + 8);
                 uint32_t pb[NT][2];
                 bool grew = false;
                 float al[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int key = g + (i >> 1) * 8;
-                        s[nt][i] = key < nv ? s[nt][i] * p.scale2 : -INFINITY;
-                    }
+                    for (int i = 0; i < 4; i++) s[nt][i] = (i < 2 ? in0 : in1) ? (s[nt][i] + s2[nt][i]) * p.scale2 : -INFINITY;
                     float pr[4];
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
@@ -520,7 +671,7 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
 #pragma unroll
                     for (int i = 0; i < DP / 16; i++) {
                         uint32_t a[4];
-                        ldsm4t(a, vb + row * (DP * 2) + (((2 * i + ch) ^ (row & 7)) << 4));
+                        ldsm4t(a, vb + (i >> 2) * 2048 + row * 128 + (((2 * (i & 3) + ch) ^ (row & 7)) << 4));
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) mma_16816(o[i][nt], a, pb[nt][0], pb[nt][1]);
                     }
@@ -530,7 +681,13 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
             fetch(st);
             if (++st == ST) st = 0;
             if (cu.j + 1 == cu.nch || c + 1 == S.c1) {
-                // the unit's share ends: the warps' states meet in shared memory, one 8-row block at a time
+                // the unit's share ends: the warps' states meet in shared memory, one 8-row block at a time,
+                // while the next unit's query rows are on their way
+                if (c + 1 < S.c1) {
+                    DecCur nx = cu;
+                    dec_next(p, nx);
+                    load_q(nx);
+                }
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -555,23 +712,27 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
                         f[i] = exp2f(m[nt][i] - (M == -INFINITY ? 0.0f : M));
                     }
                     if (nt) __syncthreads();
-                    float *mb = merge + warp * (8 * T::QS);
+                    // the upper two warps' go to the lower two, whose sums then meet
+                    float *mb = merge + (warp & 1) * (8 * T::QS);
 #pragma unroll
-                    for (int i = 0; i < DP / 16; i++)
+                    for (int up = 1; up >= 0; up--) {
+                        if (warp >> 1 == up) {
 #pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            mb[(2 * t + (j & 1)) * T::QS + i * 16 + g + (j >> 1) * 8] = o[i][nt][j] * f[j & 1];
-                    __syncthreads();
+                            for (int i = 0; i < DP / 16; i++)
+#pragma unroll
+                                for (int j = 0; j < 4; j++) {
+                                    float *a = mb + (2 * t + (j & 1)) * T::QS + i * 16 + g + (j >> 1) * 8;
+                                    *a = up ? o[i][nt][j] * f[j & 1] : o[i][nt][j] * f[j & 1] + *a;
+                                }
+                        }
+                        __syncthreads();
+                    }
 #pragma unroll
                     for (int k = 0; k < PT; k++) {
                         const int it = threadIdx.x + k * T::THREADS, r = it / (DP / 4), d0 = (it % (DP / 4)) * 4;
-                        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                        for (int w = 0; w < DEC_TC_WARPS; w++) {
-                            const float4 v = *reinterpret_cast<const float4 *>(merge + w * (8 * T::QS) + r * T::QS + d0);
-                            a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
-                        }
-                        keep[nt * PT + k] = a;
+                        const float4 a = *reinterpret_cast<const float4 *>(merge + r * T::QS + d0);
+                        const float4 v = *reinterpret_cast<const float4 *>(merge + 8 * T::QS + r * T::QS + d0);
+                        keep[nt * PT + k] = make_float4(a.x + v.x, a.y + v.y, a.z + v.z, a.w + v.w);
                     }
                 }
                 auto ml = [&](int r) {
@@ -585,13 +746,18 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
                     }
                     return make_float2(M, L);
                 };
-                dec_finish<DP, T::ROWS, T::THREADS>(p, S, cu, c, upb, merge, [&](int, int, int k) { return keep[k]; }, ml);
+                dec_finish<DP, T::ROWS, T::THREADS>(p, S, cu, c, upb, [&](int, int, int k) { return keep[k]; }, ml);
                 __syncthreads();                             // wml and merge are free again
                 fresh = true;
             }
-            dec_next(p, cu, upb);
+            dec_next(p, cu);
         }
-        cp_wait<0>();
+        if (!TMA) cp_wait<0>();
+        if (!ok) {                                           // a wait ran out: report it, and let copies in flight land
+            irx_flag(p.err, IRX_KERR_TIMEOUT);
+            for (int i = 0; i < ST; i++) irx_mbar_wait(bar + i, (phase >> i) & 1, 1u << 20, 100000000ull);
+        }
+        dec_join<DP, T::ROWS, T::THREADS>(p, S, wml);
     }
     dec_empty(p);
 }
@@ -612,9 +778,8 @@ struct DecSt {
     static constexpr int Q = ROWS * DP * 4;
     static constexpr int PB = DEC_ST_WARPS * ROWS * 8 * 4;
     static constexpr int ML = DEC_ST_WARPS * ROWS * 8;
-    static constexpr int SMEM = RING + MERGE + Q + PB + ML + IRX_DEC_SHARE;
+    static constexpr int SMEM = RING + MERGE + Q + PB + ML + IRX_DEC_SHARE + DEC_ST_WARPS * ST * (int)sizeof(DecRows<8>);
     static_assert(SMEM == IRX_DEC_ST_SMEM(DP, NT, ST), "the launcher's shared memory size");
-    static_assert((IRX_DEC_MAX_CTAS / DEC_JOIN + 2) * ROWS * 4 <= MERGE, "shared memory");
 };
 
 template <int DP, int NT, int ST>
@@ -627,6 +792,7 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
     float *pball = qs + T::Q / 4;
     float2 *wml = reinterpret_cast<float2 *>(pball + T::PB / 4);
     DecShare &S = *reinterpret_cast<DecShare *>(reinterpret_cast<float *>(wml) + T::ML / 4);
+    DecRows<8> *rows = reinterpret_cast<DecRows<8> *>(reinterpret_cast<float *>(wml) + (T::ML + IRX_DEC_SHARE) / 4) + (threadIdx.x >> 5) * ST;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, key = lane >> 2, quarter = lane & 3;
     const int upb = (p.h1 - p.h0) * p.split;
     constexpr int VW = DP / 32 < 4 ? DP / 32 : 4, NJ = DP / 32 / VW;
@@ -634,53 +800,52 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
     irx_pdl_enter();
     dec_partition<T::THREADS>(p, upb, S);
     if (S.c0 < S.c1) {
-        DecCur ld, cu;
-        ld.b = S.b; ld.u = S.u; ld.j = S.j;
-        dec_enter(p, ld);
-        cu = ld;
+        DecCur tl, cu;
+        dec_start(p, S, tl);
+        cu = tl;
         float *myring = reinterpret_cast<float *>(sm) + warp * (ST * T::TILE / 4);
         float *pb = pball + warp * (T::ROWS * 8);
-        long long lc = S.c0;
-        int pg = -1;
-        unsigned slot = 0;
-        auto lookup = [&]() {
-            const int jj = ld.j * IRX_DEC_KEYS + warp * 8 + (lane & 7);
-            pg = -2;
-            if (lc < S.c1 && jj < ld.nvis) pg = dec_page(p, ld, jj, slot);
+        long long tc = S.c0;
+        auto lookup = [&](int st) {
+            dec_lookup<8>(p, tl, tc < S.c1, dec_pos(tl, tl.j) + warp * 8, rows[st]);
+            if (tc < S.c1) {
+                tc++;
+                dec_next(p, tl);
+            }
         };
         auto fetch = [&](int st) {
-            if (lc < S.c1) {
-                const int64_t off = pg == -2 ? -1 : dec_offset(p, pg, slot, p.h0 + ld.u / p.split);
-                if (__any_sync(0xffffffffu, pg != -2)) {
-                    float *kd = myring + st * (T::TILE / 4), *vd = kd + 8 * T::KS;
-                    if (p.vec) {
-                        constexpr int CPR = DP / 4;              // 16-byte pieces of a row
+            const long long off = dec_row<8>(p, rows[st], lane & 7);
+            if (__any_sync(0xffffffffu, off != -1)) {
+                float *kd = myring + st * (T::TILE / 4), *vd = kd + 8 * T::KS;
+                if (p.vec) {
+                    constexpr int CPR = DP / 4;              // 16-byte pieces of a row
 #pragma unroll
-                        for (int i = 0; i < 8 * CPR / 32; i++) {
-                            const int it = i * 32 + lane, row = it / CPR, ch = it % CPR;
-                            const int64_t o = __shfl_sync(0xffffffffu, off, row);
-                            const bool in = o >= 0 && ch * 4 < p.d;
-                            const int64_t e = in ? o + ch * 4 : 0;
-                            cp16(irx_smem_u32(kd + row * T::KS + ch * 4), reinterpret_cast<const float *>(p.k) + e, in ? 16 : 0);
-                            cp16(irx_smem_u32(vd + row * DP + ch * 4), reinterpret_cast<const float *>(p.v) + e, in ? 16 : 0);
-                        }
-                    } else {
-                        for (int it = lane; it < 8 * DP; it += 32) {
-                            const int row = it / DP, d = it % DP;
-                            const int64_t o = __shfl_sync(0xffffffffu, off, row);
-                            const bool in = o >= 0 && d < p.d;
-                            kd[row * T::KS + d] = in ? irx_ld1(p.k, p.dt, o + d) : 0.0f;
-                            vd[row * DP + d] = in ? irx_ld1(p.v, p.dt, o + d) : 0.0f;
-                        }
+                    for (int i = 0; i < 8 * CPR / 32; i++) {
+                        const int it = i * 32 + lane, row = it / CPR, ch = it % CPR;
+                        const long long o = __shfl_sync(0xffffffffu, off, row);
+                        const bool in = o >= 0 && ch * 4 < p.d;
+                        const int64_t e = in ? o + ch * 4 : 0;
+                        cp16(irx_smem_u32(kd + row * T::KS + ch * 4), reinterpret_cast<const float *>(p.k) + e, in ? 16 : 0);
+                        cp16(irx_smem_u32(vd + row * DP + ch * 4), reinterpret_cast<const float *>(p.v) + e, in ? 16 : 0);
+                    }
+                } else {
+                    for (int it = lane; it < 8 * DP; it += 32) {
+                        const int row = it / DP, d = it % DP;
+                        const long long o = __shfl_sync(0xffffffffu, off, row);
+                        const bool in = o >= 0 && d < p.d;
+                        kd[row * T::KS + d] = in ? irx_ld1(p.k, p.dt, o + d) : 0.0f;
+                        vd[row * DP + d] = in ? irx_ld1(p.v, p.dt, o + d) : 0.0f;
                     }
                 }
-                lc++;
-                dec_next(p, ld, upb);
-                lookup();
             }
+            __syncwarp();
+            lookup(st);
             cp_commit();
         };
-        lookup();
+        for (int s = 0; s < ST; s++) lookup(s);
+        cp_commit();
+        cp_wait<0>();
+        __syncwarp();
         for (int s = 0; s < ST; s++) fetch(s);
 
         float o[T::ROWS][NJ * VW], m[T::ROWS], l[T::ROWS];
@@ -688,7 +853,7 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
         bool fresh = true;
         for (long long c = S.c0; c < S.c1; c++) {
             if (fresh) {
-                const int hk = p.h0 + cu.u / p.split, rb = cu.u % p.split;
+                const int hk = p.h0 + cu.h, rb = cu.rb;
                 live = min(T::ROWS, p.group - rb * T::ROWS);
                 for (int i = threadIdx.x; i < T::ROWS * DP; i += T::THREADS) {
                     const int r = i / DP, d = i % DP;
@@ -707,8 +872,9 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
             }
             cp_wait<ST - 1>();
             __syncwarp();
-            const int nv = cu.nvis - (cu.j * IRX_DEC_KEYS + warp * 8);
-            if (nv > 0) {
+            const int pos = dec_pos(cu, cu.j) + warp * 8;
+            if (dec_any(cu, pos, 8)) {
+                const bool in = dec_sees(cu, pos + key);
                 const float *kt = myring + st * (T::TILE / 4), *vt = kt + 8 * T::KS;
                 float s[T::ROWS];
 #pragma unroll
@@ -730,7 +896,7 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
                     float x = s[r];
                     x += __shfl_xor_sync(0xffffffffu, x, 1);
                     x += __shfl_xor_sync(0xffffffffu, x, 2);
-                    x = key < nv ? x * p.scale2 : -INFINITY;
+                    x = in ? x * p.scale2 : -INFINITY;
                     float mx = x;
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
@@ -825,27 +991,26 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
                     return make_float2(M, L);
                 };
                 auto acc = [&](int r, int d0, int) { return *reinterpret_cast<const float4 *>(qs + r * DP + d0); };
-                dec_finish<DP, T::ROWS, T::THREADS>(p, S, cu, c, upb, merge, acc, ml);
+                dec_finish<DP, T::ROWS, T::THREADS>(p, S, cu, c, upb, acc, ml);
                 __syncthreads();
                 fresh = true;
             }
-            dec_next(p, cu, upb);
+            dec_next(p, cu);
         }
         cp_wait<0>();
+        dec_join<DP, T::ROWS, T::THREADS>(p, S, wml);
     }
     dec_empty(p);
 }
 
-#define DEC_TC(DP, NT, ST) \
+#define DEC_TC(DP, NT) \
+    extern "C" __global__ void __launch_bounds__(DEC_TC_WARPS * 32) irx_dec_tma_##DP##_##NT(const __grid_constant__ irx_kdec_t p) \
+    { dec_tc_body<DP, NT, IRX_DEC_TC_ST(DP, NT), true>(p); } \
     extern "C" __global__ void __launch_bounds__(DEC_TC_WARPS * 32) irx_dec_tc_##DP##_##NT(const __grid_constant__ irx_kdec_t p) \
-    { dec_tc_body<DP, NT, ST>(p); }
-#define DEC_STK(DP, NT, ST) \
+    { dec_tc_body<DP, NT, IRX_DEC_TC_ST(DP, NT), false>(p); }
+#define DEC_STK(DP, NT) \
     extern "C" __global__ void __launch_bounds__(DEC_ST_WARPS * 32) irx_dec_st_##DP##_##NT(const __grid_constant__ irx_kdec_t p) \
-    { dec_st_body<DP, NT, ST>(p); }
+    { dec_st_body<DP, NT, IRX_DEC_ST_ST(DP)>(p); }
 
-DEC_TC(64, 1, IRX_DEC_TC_ST(64, 1)) DEC_TC(64, 2, IRX_DEC_TC_ST(64, 2))
-DEC_TC(128, 1, IRX_DEC_TC_ST(128, 1)) DEC_TC(128, 2, IRX_DEC_TC_ST(128, 2))
-DEC_TC(256, 1, IRX_DEC_TC_ST(256, 1))
-DEC_STK(64, 1, IRX_DEC_ST_ST(64)) DEC_STK(64, 2, IRX_DEC_ST_ST(64))
-DEC_STK(128, 1, IRX_DEC_ST_ST(128)) DEC_STK(128, 2, IRX_DEC_ST_ST(128))
-DEC_STK(256, 1, IRX_DEC_ST_ST(256))
+DEC_TC(64, 1) DEC_TC(64, 2) DEC_TC(128, 1) DEC_TC(128, 2) DEC_TC(256, 1)
+DEC_STK(64, 1) DEC_STK(64, 2) DEC_STK(128, 1) DEC_STK(128, 2) DEC_STK(256, 1)
