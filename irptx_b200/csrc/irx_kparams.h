@@ -117,12 +117,11 @@ typedef struct {
 #define IRX_DEC_SHARE 256
 #define IRX_DEC_TC_ST(dp, nt) ((dp) == 64 ? 4 : (dp) == 128 && (nt) == 1 ? 3 : 2)
 #define IRX_DEC_ST_ST(dp) ((dp) == 256 ? 1 : 2)
-#define IRX_DEC_TC_SMEM(dp, nt, st) (1024 + 4 * (st) * 8 + 4 * (st) * 2 * 16 * (dp) * 2 + 2 * 8 * ((dp) + 4) * 4 + 4 * 8 * (nt) * 8 + IRX_DEC_SHARE + 4 * (st) * 192)
+#define IRX_DEC_TC_SMEM(dp, nt, st) (4 * (st) * 2 * 16 * (dp) * 2 + 2 * 8 * ((dp) + 4) * 4 + 4 * 8 * (nt) * 8 + IRX_DEC_SHARE + 4 * (st) * 192)
 #define IRX_DEC_ST_SMEM(dp, nt, st) (8 * (st) * 8 * (2 * (dp) + 16) * 4 + 8 * 8 * (dp) * 4 + 8 * (nt) * (dp) * 4 + \
                                      8 * 8 * (nt) * 8 * 4 + 8 * 8 * (nt) * 8 + IRX_DEC_SHARE + 8 * (st) * 96)
 
 typedef struct {
-    CUtensorMap tma_k, tma_v;       /* a pool as [page, head, slot, dim], in boxes of `box` slots x 64 dims */
     const void *q, *k, *v;
     const int32_t *table, *lens;
     void       *o;
@@ -136,7 +135,7 @@ typedef struct {
     int32_t     split;              /* work units per kv head */
     int32_t     window, sinks;
     float       scale2;             /* scale * log2(e) */
-    uint8_t     dt, vec, box, pshift;   /* vec: rows can be moved 16 bytes at a time */
+    uint8_t     dt, vec, pshift, pad;   /* vec: rows can be moved 16 bytes at a time */
     uint64_t    pmul;               /* page of a position: (position * pmul) >> pshift */
 } irx_kdec_t;
 

@@ -81,6 +81,12 @@ struct DecShare {
     struct { long long unit; int first, pieces, b, head0, live; } pend[2];
 };
 
+// What a unit takes on the line that is dealt out: its chunks and EXTRA more, about what its end costs
+// (its warps meet, write and begin anew). Without them blocks that hold many short units finish late:
+// measured at 31 sequences of 1 to 4096 tokens, the last block at 52 us, the median one at 39.
+template <int EXTRA>
+__device__ __forceinline__ long long dec_cost(int nch) { return nch ? nch + EXTRA : 0; }
+
 __device__ __forceinline__ long long dec_div(long long a, long long b)         // not below 0; mostly 32 bits
 {
     return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
@@ -88,7 +94,7 @@ __device__ __forceinline__ long long dec_div(long long a, long long b)         /
 
 // The block's chunk range and where it starts: every block sums the chunks of all sequences (a
 // segment of them per thread, then a scan), so nothing has to run before the kernel.
-template <int THREADS>
+template <int THREADS, int EXTRA>
 __device__ __forceinline__ void dec_partition(const irx_kdec_t &p, int upb, DecShare &S)
 {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = THREADS / 32;
@@ -99,7 +105,7 @@ __device__ __forceinline__ void dec_partition(const irx_kdec_t &p, int upb, DecS
         const int raw = p.lens[b];
         dec_enter(p, w, raw);
         if (raw != w.n && blockIdx.x == 0) irx_flag(p.err, IRX_KERR_INDEX);
-        sum += w.nch;
+        sum += dec_cost<EXTRA>(w.nch);
     }
     long long inc = sum;
 #pragma unroll
@@ -129,25 +135,37 @@ __device__ __forceinline__ void dec_partition(const irx_kdec_t &p, int upb, DecS
         long long at = c0 - ex;
         for (int b = b0; b < b1; b++) {
             dec_enter(p, w, p.lens[b]);
-            if (at < (long long)w.nch * upb) {
-                const long long u = dec_div(at, w.nch);
-                S.b = b; S.u = (int)u; S.j = (int)(at - u * w.nch);
+            const long long cost = dec_cost<EXTRA>(w.nch);
+            if (at < cost * upb) {
+                const long long u = dec_div(at, cost);
+                S.b = b; S.u = (int)u; S.j = (int)(at - u * cost);
                 break;
             }
-            at -= (long long)w.nch * upb;
+            at -= cost * upb;
         }
     }
     __syncthreads();
 }
 
-__device__ __forceinline__ void dec_start(const irx_kdec_t &p, const DecShare &S, DecCur &c)
+// The block's first chunk, at place c0 of the line.
+template <int EXTRA>
+__device__ __forceinline__ long long dec_start(const irx_kdec_t &p, const DecShare &S, DecCur &c)
 {
     c.b = S.b;
     c.h = S.u / p.split;
     c.rb = S.u % p.split;
     c.j = S.j;
     dec_enter(p, c, p.lens[c.b]);
+    if (c.j < c.nch) return S.c0;
+    const long long at = S.c0 + (c.nch + EXTRA - c.j);   // the share begins in a unit's end: with the next unit then
+    c.j = c.nch - 1;
+    dec_next(p, c);
+    return at;
 }
+
+// The place of the next chunk on the line, from a chunk at place c.
+template <int EXTRA>
+__device__ __forceinline__ long long dec_step(const DecCur &w, long long c) { return c + (w.j + 1 < w.nch ? 1 : 1 + EXTRA); }
 
 // The block that holds chunk c.
 __device__ __forceinline__ int dec_block_of(const DecShare &S, long long c)
@@ -432,105 +450,51 @@ template <int DP, int NT, int ST>
 struct DecTc {
     static constexpr int THREADS = DEC_TC_WARPS * 32, ROWS = 8 * NT, TILE = 16 * DP * 2, QS = DP + 4;
     // ring, then one 8-row block of two warps' accumulators then
-    // (max, sum) pairs, the share, the rings' row places and barriers
+    // (max, sum) pairs, the share and the rings' row places
     static constexpr int RING = DEC_TC_WARPS * ST * 2 * TILE;
     static constexpr int MERGE = DEC_TC_WARPS / 2 * 8 * QS * 4;
     static constexpr int ML = DEC_TC_WARPS * ROWS * 8;
-    static constexpr int PLACES = RING + MERGE + ML + IRX_DEC_SHARE, BARS = PLACES + DEC_TC_WARPS * ST * (int)sizeof(DecRows<16>);
-    static constexpr int SMEM = 1024 + BARS + DEC_TC_WARPS * ST * 8;
+    static constexpr int PLACES = RING + MERGE + ML + IRX_DEC_SHARE;
+    static constexpr int SMEM = PLACES + DEC_TC_WARPS * ST * (int)sizeof(DecRows<16>);
     static_assert(SMEM == IRX_DEC_TC_SMEM(DP, NT, ST), "the launcher's shared memory size");
     static_assert(sizeof(DecShare) <= IRX_DEC_SHARE, "shared memory");
 };
 
-// A tile lies in 64-dim columns of 16 rows x 128 bytes, 16-byte pieces swizzled by row, as TMA's 128-byte
-// swizzle leaves them. TMA: pages of a multiple of 8 slots, whose 8 or 16 rows are one box; a few
-// instructions fill a tile, where 16-byte copies with their addresses take as many as the products.
-template <int DP, int NT, int ST, bool TMA>
+// A tile lies in 64-dim columns of 16 rows x 128 bytes, 16-byte pieces swizzled by row against bank conflicts.
+// (Filling tiles by TMA, a page's 8 or 16 rows a box, measured no better: 171 against 164 us for two
+// sequences of 125k tokens, 54 against 52 for 31 of 2k.)
+template <int DP, int NT, int ST>
 __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
 {
     using T = DecTc<DP, NT, ST>;
-    extern __shared__ unsigned char sm_raw[];
-    unsigned char *sm = sm_raw + ((1024u - (irx_smem_u32(sm_raw) & 1023u)) & 1023u);   // the swizzle's period
+    constexpr int EX = DP == 64 ? 3 : DP == 128 ? 2 : 1;
+    extern __shared__ __align__(128) unsigned char sm[];
     float *merge = reinterpret_cast<float *>(sm + T::RING);
     float2 *wml = reinterpret_cast<float2 *>(sm + T::RING + T::MERGE);
     DecShare &S = *reinterpret_cast<DecShare *>(sm + T::RING + T::MERGE + T::ML);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     DecRows<16> *rows = reinterpret_cast<DecRows<16> *>(sm + T::PLACES) + warp * ST;
-    uint64_t *bar = reinterpret_cast<uint64_t *>(sm + T::BARS) + warp * ST;
     const int upb = (p.h1 - p.h0) * p.split;
 
-    if (TMA && lane == 0) {
-        for (int i = 0; i < ST; i++) irx_mbar_init(bar + i, 1);
-        irx_fence_mbar_init();
-        tma_prefetch_desc(&p.tma_k);
-        tma_prefetch_desc(&p.tma_v);
-    }
     irx_pdl_enter();
-    dec_partition<T::THREADS>(p, upb, S);
+    dec_partition<T::THREADS, EX>(p, upb, S);
     if (S.c0 < S.c1) {
-        DecCur tl, cu;                                       // the tile to be loaded (without TMA: looked up) next, the one in work
-        dec_start(p, S, tl);
+        DecCur tl, cu;                                       // the tile whose rows are looked up next, the one in work
+        const long long cfirst = dec_start<EX>(p, S, tl);
         cu = tl;
-        unsigned char *myring = sm + warp * (ST * 2 * T::TILE);
-        const uint32_t ring = irx_smem_u32(myring);
-        long long tc = S.c0;                                 // the chunk that `tl` is at
-        int ok = 1;
-
-        // TMA: each lane holds the page and slot of one box of the next 32 boxes of this warp's tiles in the unit
-        const int two = TMA && p.box == 8 ? 1 : 0;           // boxes of a tile: 1 + two
-        int pg = -2, tok = 0, at = 0;
-        auto pages = [&]() {
-            const int j = tl.j + (lane >> two), pos = dec_pos(tl, j) + warp * 16 + (two ? (lane & 1) * 8 : 0);
-            pg = -2;                                         // no such box
-            if (tc < S.c1 && j < tl.nch && pos < tl.n) {
-                const unsigned pi = dec_page_of(p, pos);
-                tok = (int)((unsigned)pos - pi * (unsigned)p.page_size);
-                pg = p.table[(int64_t)tl.b * p.cols + pi];
-                if (pg < 0) pg = -1;
-            }
-            at = 0;
-        };
-        // without: each key row's place, a ring ahead
+        const uint32_t ring = irx_smem_u32(sm) + warp * (ST * 2 * T::TILE);
+        long long tc = cfirst;                                 // the chunk that `tl` is at
         constexpr int CPR = DP / 8, RPI = 32 / CPR, NI = 16 / RPI;
         const int lrow = lane / CPR, lch = lane % CPR;
         const bool cin = lch * 8 < p.d;
         auto lookup = [&](int st) {
             dec_lookup<16>(p, tl, tc < S.c1, dec_pos(tl, tl.j) + warp * 16, rows[st]);
             if (tc < S.c1) {
-                tc++;
+                tc = dec_step<EX>(tl, tc);
                 dec_next(p, tl);
             }
         };
         auto fetch = [&](int st) {
-            if (TMA) {
-                if (tc >= S.c1) return;
-                if (dec_any(tl, dec_pos(tl, tl.j) + warp * 16, 16)) {
-                    const bool mine = lane >> two == at && pg != -2, good = mine && pg >= 0 && pg < p.pages;
-                    const unsigned have = __ballot_sync(0xffffffffu, good);
-                    if (__any_sync(0xffffffffu, mine && !good)) {      // no page of the pool: flagged, read as zeros
-                        if (lane == 0) irx_flag(p.err, IRX_KERR_INDEX);
-                        for (int i = lane; i < 2 * T::TILE / 16; i += 32)
-                            *reinterpret_cast<uint4 *>(myring + st * (2 * T::TILE) + i * 16) = make_uint4(0, 0, 0, 0);
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                    }
-                    if (lane == 0) irx_mbar_expect_tx(bar + st, __popc(have) * 2 * (DP / 64) * 128 * p.box);
-                    __syncwarp();
-                    if (good) {
-                        unsigned char *kd = myring + st * (2 * T::TILE) + (two ? (lane & 1) * 1024 : 0);
-#pragma unroll
-                        for (int i = 0; i < DP / 64; i++) {
-                            tma_load_4d(kd + i * 2048, &p.tma_k, i * 64, tok, p.h0 + tl.h, pg, bar + st);
-                            tma_load_4d(kd + T::TILE + i * 2048, &p.tma_v, i * 64, tok, p.h0 + tl.h, pg, bar + st);
-                        }
-                    }
-                }
-                tc++;
-                dec_next(p, tl);
-                at++;
-                if (tl.j == 0 || at == 32 >> two) pages();
-                return;
-            }
             const long long off = dec_row<16>(p, rows[st], lane & 15);
             if (__any_sync(0xffffffffu, off != -1)) {
                 const uint32_t kd = ring + st * (2 * T::TILE), vd = kd + T::TILE;
@@ -549,20 +513,15 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
             lookup(st);
             cp_commit();
         };
-        if (TMA) {
-            pages();
-        } else {
-            for (int s = 0; s < ST; s++) lookup(s);
-            cp_commit();
-            cp_wait<0>();
-            __syncwarp();
-        }
+        for (int s = 0; s < ST; s++) lookup(s);
+        cp_commit();
+        cp_wait<0>();
+        __syncwarp();
         for (int s = 0; s < ST; s++) fetch(s);
 
         uint32_t q[DP / 16][NT][2];
         float o[DP / 16][NT][4], m[NT][2], l[NT][2];
         int st = 0;
-        unsigned phase = 0;                                  // a bit per slot
         bool fresh = true;
         auto load_q = [&](const DecCur &w) {                 // a unit's query rows
             const __nv_bfloat16 *qg = reinterpret_cast<const __nv_bfloat16 *>(p.q) + (int64_t)w.b * p.q_stride;
@@ -579,8 +538,8 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
                     }
             }
         };
-        load_q(cu);
-        for (long long c = S.c0; c < S.c1; c++) {
+        if (cfirst < S.c1) load_q(cu);
+        for (long long c = cfirst; c < S.c1;) {
             if (fresh) {                                     // a unit starts: an empty state
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
@@ -593,28 +552,12 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
                 }
                 fresh = false;
             }
-            if (!TMA) {
-                cp_wait<ST - 1>();
-                __syncwarp();
-            }
+            cp_wait<ST - 1>();
+            __syncwarp();
             const int pos = dec_pos(cu, cu.j) + warp * 16;
             if (dec_any(cu, pos, 16)) {
                 const uint32_t kb = ring + st * (2 * T::TILE), vb = kb + T::TILE;
                 const bool whole = dec_all(cu, pos, 16);
-                if (TMA) {
-                    ok = ok && irx_mbar_wait(bar + st, (phase >> st) & 1);
-                    phase ^= 1u << st;
-                    if (!whole) {                            // rows that are not seen: their values may be anything, and 0 * NaN is not 0
-                        for (int i = lane; i < 16 * (DP / 8); i += 32) {
-                            const int row = i & 15;
-                            if (!dec_sees(cu, pos + row))
-                                *reinterpret_cast<uint4 *>(myring + st * (2 * T::TILE) + T::TILE + (i >> 7) * 2048 + row * 128 + ((i >> 4) & 7) * 16) =
-                                    make_uint4(0, 0, 0, 0);
-                        }
-                        fence_proxy_async_smem();            // before the copy that comes here next
-                        __syncwarp();
-                    }
-                }
                 float s[NT][4], s2[NT][4];                   // two sums, of even and odd steps: half the chain
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
@@ -680,10 +623,11 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
             __syncwarp();
             fetch(st);
             if (++st == ST) st = 0;
-            if (cu.j + 1 == cu.nch || c + 1 == S.c1) {
+            const long long cnext = dec_step<EX>(cu, c);
+            if (cu.j + 1 == cu.nch || cnext >= S.c1) {
                 // the unit's share ends: the warps' states meet in shared memory, one 8-row block at a time,
                 // while the next unit's query rows are on their way
-                if (c + 1 < S.c1) {
+                if (cnext < S.c1) {
                     DecCur nx = cu;
                     dec_next(p, nx);
                     load_q(nx);
@@ -751,12 +695,9 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
                 fresh = true;
             }
             dec_next(p, cu);
+            c = cnext;
         }
-        if (!TMA) cp_wait<0>();
-        if (!ok) {                                           // a wait ran out: report it, and let copies in flight land
-            irx_flag(p.err, IRX_KERR_TIMEOUT);
-            for (int i = 0; i < ST; i++) irx_mbar_wait(bar + i, (phase >> i) & 1, 1u << 20, 100000000ull);
-        }
+        cp_wait<0>();
         dec_join<DP, T::ROWS, T::THREADS>(p, S, wml);
     }
     dec_empty(p);
@@ -786,6 +727,7 @@ template <int DP, int NT, int ST>
 __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
 {
     using T = DecSt<DP, NT, ST>;
+    constexpr int EX = 1;
     extern __shared__ __align__(128) unsigned char sm[];
     float *merge = reinterpret_cast<float *>(sm + T::RING);
     float *qs = merge + T::MERGE / 4;
@@ -798,18 +740,18 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
     constexpr int VW = DP / 32 < 4 ? DP / 32 : 4, NJ = DP / 32 / VW;
 
     irx_pdl_enter();
-    dec_partition<T::THREADS>(p, upb, S);
+    dec_partition<T::THREADS, EX>(p, upb, S);
     if (S.c0 < S.c1) {
         DecCur tl, cu;
-        dec_start(p, S, tl);
+        const long long cfirst = dec_start<EX>(p, S, tl);
         cu = tl;
         float *myring = reinterpret_cast<float *>(sm) + warp * (ST * T::TILE / 4);
         float *pb = pball + warp * (T::ROWS * 8);
-        long long tc = S.c0;
+        long long tc = cfirst;
         auto lookup = [&](int st) {
             dec_lookup<8>(p, tl, tc < S.c1, dec_pos(tl, tl.j) + warp * 8, rows[st]);
             if (tc < S.c1) {
-                tc++;
+                tc = dec_step<EX>(tl, tc);
                 dec_next(p, tl);
             }
         };
@@ -851,7 +793,7 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
         float o[T::ROWS][NJ * VW], m[T::ROWS], l[T::ROWS];
         int st = 0, live = 0;
         bool fresh = true;
-        for (long long c = S.c0; c < S.c1; c++) {
+        for (long long c = cfirst; c < S.c1;) {
             if (fresh) {
                 const int hk = p.h0 + cu.h, rb = cu.rb;
                 live = min(T::ROWS, p.group - rb * T::ROWS);
@@ -946,7 +888,8 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
             __syncwarp();
             fetch(st);
             if (++st == ST) st = 0;
-            if (cu.j + 1 == cu.nch || c + 1 == S.c1) {
+            const long long cnext = dec_step<EX>(cu, c);
+            if (cu.j + 1 == cu.nch || cnext >= S.c1) {
 #pragma unroll
                 for (int r = 0; r < T::ROWS; r++) {
                     float x = l[r];
@@ -996,6 +939,7 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
                 fresh = true;
             }
             dec_next(p, cu);
+            c = cnext;
         }
         cp_wait<0>();
         dec_join<DP, T::ROWS, T::THREADS>(p, S, wml);
@@ -1004,10 +948,8 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
 }
 
 #define DEC_TC(DP, NT) \
-    extern "C" __global__ void __launch_bounds__(DEC_TC_WARPS * 32) irx_dec_tma_##DP##_##NT(const __grid_constant__ irx_kdec_t p) \
-    { dec_tc_body<DP, NT, IRX_DEC_TC_ST(DP, NT), true>(p); } \
     extern "C" __global__ void __launch_bounds__(DEC_TC_WARPS * 32) irx_dec_tc_##DP##_##NT(const __grid_constant__ irx_kdec_t p) \
-    { dec_tc_body<DP, NT, IRX_DEC_TC_ST(DP, NT), false>(p); }
+    { dec_tc_body<DP, NT, IRX_DEC_TC_ST(DP, NT)>(p); }
 #define DEC_STK(DP, NT) \
     extern "C" __global__ void __launch_bounds__(DEC_ST_WARPS * 32) irx_dec_st_##DP##_##NT(const __grid_constant__ irx_kdec_t p) \
     { dec_st_body<DP, NT, IRX_DEC_ST_ST(DP)>(p); }

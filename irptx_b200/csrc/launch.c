@@ -159,7 +159,6 @@ static const char *const KNAMES[K_COUNT] = {
     "irx_rowop", "irx_row_rmsnorm", "irx_row_softmax", "irx_row_l2norm",
     "irx_mm_f32", "irx_mm_bf16", "irx_mm_bf16_simt", "irx_attn_f32", "irx_attn_bf16", "irx_attn_bf16_simt",
     "irx_mm_bf16_pair", "irx_mm_bf16_wide",
-    "irx_dec_tma_64_1", "irx_dec_tma_64_2", "irx_dec_tma_128_1", "irx_dec_tma_128_2", "irx_dec_tma_256_1",
     "irx_dec_tc_64_1", "irx_dec_tc_64_2", "irx_dec_tc_128_1", "irx_dec_tc_128_2", "irx_dec_tc_256_1",
     "irx_dec_st_64_1", "irx_dec_st_64_2", "irx_dec_st_128_1", "irx_dec_st_128_2", "irx_dec_st_256_1",
     "irx_kv_append_16", "irx_kv_append_4", "irx_kv_append_2",

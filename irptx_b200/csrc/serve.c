@@ -209,20 +209,6 @@ static int launch_decode(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
     rows = a->nt;
     if (k.vec && a->c.dt == DT_BF16) {
         kk = K_DEC_TC + i;
-        if (a->c.page_size % 8 == 0 && a->c.page_stride < (1ll << 39) && a->c.head_stride < (1ll << 39) &&
-            a->c.token_stride < (1ll << 39)) {           /* whole boxes of a page: by TMA */
-            const irx_kvc_t *c = &a->c;
-            const cuuint64_t dims[4] = {(cuuint64_t)c->dim, (cuuint64_t)c->page_size, (cuuint64_t)c->heads, (cuuint64_t)c->pages};
-            /* an axis of one may have any stride: give it one that the map takes */
-            const cuuint64_t strides[3] = {(cuuint64_t)c->token_stride * 2, (cuuint64_t)(c->heads > 1 ? c->head_stride : c->token_stride) * 2,
-                                           (cuuint64_t)(c->pages > 1 ? c->page_stride : c->token_stride) * 2};
-            cuuint32_t box[4] = {64, 16, 1, 1};
-            box[1] = k.box = c->page_size % 16 ? 8 : 16;
-            if (irx_dev_tmap(&k.tma_k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void *)k.k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B) ||
-                irx_dev_tmap(&k.tma_v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void *)k.v, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
-                return 1;
-            kk = K_DEC_TMA + i;
-        }
         smem = (size_t)IRX_DEC_TC_SMEM(DP[i], rows, IRX_DEC_TC_ST(DP[i], rows));
         if (serve_grid(d, kk, 128, smem, a->max_ctas, &grid)) return 1;
         return irx_dev_launch(d, kk, (unsigned)grid, 128, (unsigned)smem, 1, st, &k);
@@ -467,7 +453,7 @@ void irx_serve_text(const irx_plan_int_t *p, char *buf, size_t cap)
         snprintf(buf, cap, "decode batch=%d heads=%d kv_heads=%d d=%d page=%d pages=%lld window=%d sinks=%d lse=%d scale=%g "
                  "dtype=%s kernel=irx_dec_%s_%d_%d", a->c.batch, a->heads, a->c.heads, a->c.dim, a->c.page_size,
                  (long long)a->c.pages, a->window, a->sinks, a->lse, (double)sc, dname(a->c.dt),
-                 a->c.dt != DT_BF16 || a->c.dim % 8 ? "st" : a->c.page_size % 8 ? "tc" : "tma", a->dp, a->nt);
+                 a->c.dt != DT_BF16 || a->c.dim % 8 ? "st" : "tc", a->dp, a->nt);
     } else if (p->fam == FAM_MATVEC4) {
         const irx_mv4_t *a = &p->u.mv;
         snprintf(buf, cap, "matvec4 m=%lld n=%lld k=%lld group=%d zeros=%d dtype=%s", (long long)a->m, (long long)a->n,
