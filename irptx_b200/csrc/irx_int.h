@@ -220,7 +220,9 @@ typedef struct {
     irx_kvc_t c;
     int64_t  q_stride;                 /* elements from one sequence's query heads to the next one's */
     int32_t  heads, window, sinks;
-    int32_t  dp, nt, split;            /* padded head size; 8-row blocks of a work unit; units per kv head */
+    int32_t  dp;                       /* padded head size */
+    int32_t  rows[2], split[2];        /* query rows of a work unit and units per kv head, by kernel: [0]
+                                        * matrix instructions, [1] FP32 units */
     int32_t  max_ctas;                 /* the workspace holds the partials of this many blocks */
     uint32_t scale_bits;
     uint8_t  lse;

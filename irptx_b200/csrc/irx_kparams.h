@@ -110,16 +110,18 @@ typedef struct {
  * rows x dp accumulators then rows (max, sum) pairs, then the tickets (a work unit each) and the
  * group counters (a slot each). */
 #define IRX_DEC_MAX_CTAS 512
-#define IRX_DEC_KEYS 64             /* keys of a chunk, the grain the work is cut in */
 
-/* Ring depth and shared memory of the two decode kernels, by padded head size and 8-row blocks
- * (the launcher and the kernels agree on them; the share is the block's part of the work). */
+/* Ring depth, 16-key blocks of a warp's tile and shared memory of the two decode kernels, by padded head
+ * size and query rows of a work unit (the launcher and the kernels agree on them; the share is the
+ * block's part of the work). */
 #define IRX_DEC_SHARE 256
-#define IRX_DEC_TC_ST(dp, nt) ((dp) == 64 ? 4 : (dp) == 128 && (nt) == 1 ? 3 : 2)
+#define IRX_DEC_TC_KM(dp) ((dp) == 64 ? 2 : 1)
+#define IRX_DEC_TC_ST(dp, nt) ((dp) == 256 || ((dp) == 128 && (nt) == 2) ? 2 : 3)
 #define IRX_DEC_ST_ST(dp) ((dp) == 256 ? 1 : 2)
-#define IRX_DEC_TC_SMEM(dp, nt, st) (4 * (st) * 2 * 16 * (dp) * 2 + 2 * 8 * ((dp) + 4) * 4 + 4 * 8 * (nt) * 8 + IRX_DEC_SHARE + 4 * (st) * 192)
-#define IRX_DEC_ST_SMEM(dp, nt, st) (8 * (st) * 8 * (2 * (dp) + 16) * 4 + 8 * 8 * (dp) * 4 + 8 * (nt) * (dp) * 4 + \
-                                     8 * 8 * (nt) * 8 * 4 + 8 * 8 * (nt) * 8 + IRX_DEC_SHARE + 8 * (st) * 96)
+#define IRX_DEC_TC_SMEM(dp, nt, km, st) (4 * (st) * 2 * 16 * (km) * (dp) * 2 + 2 * 8 * ((dp) + 4) * 4 + 4 * 8 * (nt) * 8 + \
+                                         IRX_DEC_SHARE + 4 * (st) * 192 * (km))
+#define IRX_DEC_ST_SMEM(dp, rows, st) (8 * (st) * 8 * (2 * (dp) + 16) * 4 + 8 * (rows) * (dp) * 4 + (rows) * (dp) * 4 + \
+                                       8 * (rows) * 8 * 4 + 8 * (rows) * 8 + IRX_DEC_SHARE + 8 * (st) * 96)
 
 typedef struct {
     const void *q, *k, *v;

@@ -21,7 +21,7 @@
 #define DEC_JOIN 16
 
 // A place in the laid-out chunks: chunk j of the unit (kv head h0 + h, row block rb) of sequence b. A
-// chunk is a block of IRX_DEC_KEYS positions: the first `cs` of a sequence's chunks are the blocks that
+// chunk is a block of K positions (what a block of threads takes in one step): the first `cs` of a sequence's chunks are the blocks that
 // hold sinks, the others the blocks from wb on; keys outside the mask are dropped in their tile.
 struct DecCur {
     int b, h, rb, j;
@@ -34,9 +34,11 @@ __device__ __forceinline__ int dec_len(const irx_kdec_t &p, int n)
     return n < 0 ? 0 : (int64_t)n > cap ? (int)cap : n;
 }
 
-__device__ __forceinline__ int dec_blocks(int n) { return n / IRX_DEC_KEYS + (n % IRX_DEC_KEYS != 0); }
+template <int K>
+__device__ __forceinline__ int dec_blocks(int n) { return n / K + (n % K != 0); }
 
 // Sequence c.b's numbers, from its length.
+template <int K>
 __device__ __forceinline__ void dec_enter(const irx_kdec_t &p, DecCur &c, int len)
 {
     c.n = dec_len(p, len);
@@ -44,12 +46,13 @@ __device__ __forceinline__ void dec_enter(const irx_kdec_t &p, DecCur &c, int le
     if (p.window > 0 && c.n > p.window) {
         c.lo = c.n - p.window;
         c.sk = min(p.sinks, c.lo);
-        c.cs = dec_blocks(c.sk);
-        c.wb = max(c.lo / IRX_DEC_KEYS, c.cs);
+        c.cs = dec_blocks<K>(c.sk);
+        c.wb = max(c.lo / K, c.cs);
     }
-    c.nch = c.cs + dec_blocks(c.n) - c.wb;
+    c.nch = c.cs + dec_blocks<K>(c.n) - c.wb;
 }
 
+template <int K>
 __device__ __forceinline__ void dec_next(const irx_kdec_t &p, DecCur &c)
 {
     if (++c.j < c.nch) return;
@@ -60,13 +63,14 @@ __device__ __forceinline__ void dec_next(const irx_kdec_t &p, DecCur &c)
     c.h = 0;
     do {
         if (++c.b >= p.batch) { c.n = 0; c.nch = 0x7fffffff; return; }        // past the end
-        dec_enter(p, c, p.lens[c.b]);
+        dec_enter<K>(p, c, p.lens[c.b]);
     } while (c.nch == 0);
 }
 
 // The first position of the cursor's chunk j, and whether a tile of `keys` positions from pos shows any
 // key, or shows all of them.
-__device__ __forceinline__ int dec_pos(const DecCur &c, int j) { return (j < c.cs ? j : j - c.cs + c.wb) * IRX_DEC_KEYS; }
+template <int K>
+__device__ __forceinline__ int dec_pos(const DecCur &c, int j) { return (j < c.cs ? j : j - c.cs + c.wb) * K; }
 __device__ __forceinline__ bool dec_any(const DecCur &c, int pos, int keys) { return pos < c.n && (pos > c.lo - keys || pos < c.sk); }
 __device__ __forceinline__ bool dec_all(const DecCur &c, int pos, int keys) { return c.n - pos >= keys && (pos >= c.lo || c.sk - pos >= keys); }
 __device__ __forceinline__ bool dec_sees(const DecCur &c, int pos) { return pos < c.n && (pos >= c.lo || pos < c.sk); }
@@ -94,7 +98,7 @@ __device__ __forceinline__ long long dec_div(long long a, long long b)         /
 
 // The block's chunk range and where it starts: every block sums the chunks of all sequences (a
 // segment of them per thread, then a scan), so nothing has to run before the kernel.
-template <int THREADS, int EXTRA>
+template <int THREADS, int K, int EXTRA>
 __device__ __forceinline__ void dec_partition(const irx_kdec_t &p, int upb, DecShare &S)
 {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = THREADS / 32;
@@ -103,7 +107,7 @@ __device__ __forceinline__ void dec_partition(const irx_kdec_t &p, int upb, DecS
     DecCur w;
     for (int b = b0; b < b1; b++) {
         const int raw = p.lens[b];
-        dec_enter(p, w, raw);
+        dec_enter<K>(p, w, raw);
         if (raw != w.n && blockIdx.x == 0) irx_flag(p.err, IRX_KERR_INDEX);
         sum += dec_cost<EXTRA>(w.nch);
     }
@@ -134,7 +138,7 @@ __device__ __forceinline__ void dec_partition(const irx_kdec_t &p, int upb, DecS
     if (c0 < c1 && c0 >= ex && c0 < ex + sum * upb) {    // exactly one thread's segment holds c0
         long long at = c0 - ex;
         for (int b = b0; b < b1; b++) {
-            dec_enter(p, w, p.lens[b]);
+            dec_enter<K>(p, w, p.lens[b]);
             const long long cost = dec_cost<EXTRA>(w.nch);
             if (at < cost * upb) {
                 const long long u = dec_div(at, cost);
@@ -148,18 +152,18 @@ __device__ __forceinline__ void dec_partition(const irx_kdec_t &p, int upb, DecS
 }
 
 // The block's first chunk, at place c0 of the line.
-template <int EXTRA>
+template <int K, int EXTRA>
 __device__ __forceinline__ long long dec_start(const irx_kdec_t &p, const DecShare &S, DecCur &c)
 {
     c.b = S.b;
     c.h = S.u / p.split;
     c.rb = S.u % p.split;
     c.j = S.j;
-    dec_enter(p, c, p.lens[c.b]);
+    dec_enter<K>(p, c, p.lens[c.b]);
     if (c.j < c.nch) return S.c0;
     const long long at = S.c0 + (c.nch + EXTRA - c.j);   // the share begins in a unit's end: with the next unit then
     c.j = c.nch - 1;
-    dec_next(p, c);
+    dec_next<K>(p, c);
     return at;
 }
 
@@ -401,7 +405,7 @@ __device__ __forceinline__ long long dec_row(const irx_kdec_t &p, const DecRows<
 // The transposed products: S^T[16 keys x 8 rows] = K Q^T and O^T[16 dims x 8 rows] += V^T P^T, so that
 // the few query rows sit on the instruction's narrow side (8) and keys or dims on its wide one.
 // S^T's accumulators become P^T's operand by an 8x8 transpose across the warp. Each warp
-// owns 16 keys of a chunk and its own ring of ST tiles filled by 16-byte asynchronous copies, so
+// owns 16 keys of a chunk (32 at head size 64, where 16 are too little work for what a tile costs) and its own ring of ST tiles filled by 16-byte asynchronous copies, so
 // warps meet only where a unit ends. mma.sync runs far below tcgen05's rate, but at 8 to 16 rows
 // the products take 16 to 32 instructions per 8 KB (D = 128), which HBM delivers in about 360
 // cycles per SM: the tensor pipe is idle most of the time and tcgen05's 128-row tiles would be
@@ -446,63 +450,63 @@ template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.as
 
 #define DEC_TC_WARPS 4
 
-template <int DP, int NT, int ST>
+template <int DP, int NT, int KM, int ST>
 struct DecTc {
-    static constexpr int THREADS = DEC_TC_WARPS * 32, ROWS = 8 * NT, TILE = 16 * DP * 2, QS = DP + 4;
+    static constexpr int THREADS = DEC_TC_WARPS * 32, ROWS = 8 * NT, KEYS = 16 * KM, K = DEC_TC_WARPS * KEYS, TILE = KEYS * DP * 2, QS = DP + 4;
     // ring, then one 8-row block of two warps' accumulators then
     // (max, sum) pairs, the share and the rings' row places
     static constexpr int RING = DEC_TC_WARPS * ST * 2 * TILE;
     static constexpr int MERGE = DEC_TC_WARPS / 2 * 8 * QS * 4;
     static constexpr int ML = DEC_TC_WARPS * ROWS * 8;
     static constexpr int PLACES = RING + MERGE + ML + IRX_DEC_SHARE;
-    static constexpr int SMEM = PLACES + DEC_TC_WARPS * ST * (int)sizeof(DecRows<16>);
-    static_assert(SMEM == IRX_DEC_TC_SMEM(DP, NT, ST), "the launcher's shared memory size");
+    static constexpr int SMEM = PLACES + DEC_TC_WARPS * ST * (int)sizeof(DecRows<KEYS>);
+    static_assert(SMEM == IRX_DEC_TC_SMEM(DP, NT, KM, ST), "the launcher's shared memory size");
     static_assert(sizeof(DecShare) <= IRX_DEC_SHARE, "shared memory");
 };
 
-// A tile lies in 64-dim columns of 16 rows x 128 bytes, 16-byte pieces swizzled by row against bank conflicts.
+// A tile, 16 KM keys, lies in 64-dim columns of 128 bytes a key, 16-byte pieces swizzled by row against bank conflicts.
 // (Filling tiles by TMA, a page's 8 or 16 rows a box, measured no better: 171 against 164 us for two
 // sequences of 125k tokens, 54 against 52 for 31 of 2k.)
-template <int DP, int NT, int ST>
+template <int DP, int NT, int KM, int ST>
 __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
 {
-    using T = DecTc<DP, NT, ST>;
+    using T = DecTc<DP, NT, KM, ST>;
     constexpr int EX = DP == 64 ? 3 : DP == 128 ? 2 : 1;
     extern __shared__ __align__(128) unsigned char sm[];
     float *merge = reinterpret_cast<float *>(sm + T::RING);
     float2 *wml = reinterpret_cast<float2 *>(sm + T::RING + T::MERGE);
     DecShare &S = *reinterpret_cast<DecShare *>(sm + T::RING + T::MERGE + T::ML);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    DecRows<16> *rows = reinterpret_cast<DecRows<16> *>(sm + T::PLACES) + warp * ST;
+    DecRows<T::KEYS> *rows = reinterpret_cast<DecRows<T::KEYS> *>(sm + T::PLACES) + warp * ST;
     const int upb = (p.h1 - p.h0) * p.split;
 
     irx_pdl_enter();
-    dec_partition<T::THREADS, EX>(p, upb, S);
+    dec_partition<T::THREADS, T::K, EX>(p, upb, S);
     if (S.c0 < S.c1) {
         DecCur tl, cu;                                       // the tile whose rows are looked up next, the one in work
-        const long long cfirst = dec_start<EX>(p, S, tl);
+        const long long cfirst = dec_start<T::K, EX>(p, S, tl);
         cu = tl;
         const uint32_t ring = irx_smem_u32(sm) + warp * (ST * 2 * T::TILE);
         long long tc = cfirst;                                 // the chunk that `tl` is at
-        constexpr int CPR = DP / 8, RPI = 32 / CPR, NI = 16 / RPI;
+        constexpr int CPR = DP / 8, RPI = 32 / CPR, NI = T::KEYS / RPI;
         const int lrow = lane / CPR, lch = lane % CPR;
         const bool cin = lch * 8 < p.d;
         auto lookup = [&](int st) {
-            dec_lookup<16>(p, tl, tc < S.c1, dec_pos(tl, tl.j) + warp * 16, rows[st]);
+            dec_lookup<T::KEYS>(p, tl, tc < S.c1, dec_pos<T::K>(tl, tl.j) + warp * T::KEYS, rows[st]);
             if (tc < S.c1) {
                 tc = dec_step<EX>(tl, tc);
-                dec_next(p, tl);
+                dec_next<T::K>(p, tl);
             }
         };
         auto fetch = [&](int st) {
-            const long long off = dec_row<16>(p, rows[st], lane & 15);
+            const long long off = dec_row<T::KEYS>(p, rows[st], lane & (T::KEYS - 1));
             if (__any_sync(0xffffffffu, off != -1)) {
                 const uint32_t kd = ring + st * (2 * T::TILE), vd = kd + T::TILE;
 #pragma unroll
                 for (int i = 0; i < NI; i++) {
                     const int row = i * RPI + lrow;
                     const long long o = __shfl_sync(0xffffffffu, off, row);
-                    const uint32_t d = (lch >> 3) * 2048 + row * 128 + (((lch & 7) ^ (row & 7)) << 4);
+                    const uint32_t d = (lch >> 3) * (T::KEYS * 128) + row * 128 + (((lch & 7) ^ (row & 7)) << 4);
                     const int64_t e = o >= 0 && cin ? o + lch * 8 : 0;
                     const uint32_t nb = o >= 0 && cin ? 16 : 0;
                     cp16(kd + d, reinterpret_cast<const __nv_bfloat16 *>(p.k) + e, nb);
@@ -554,37 +558,54 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
             }
             cp_wait<ST - 1>();
             __syncwarp();
-            const int pos = dec_pos(cu, cu.j) + warp * 16;
-            if (dec_any(cu, pos, 16)) {
+            const int pos = dec_pos<T::K>(cu, cu.j) + warp * T::KEYS;
+            if (dec_any(cu, pos, T::KEYS)) {
                 const uint32_t kb = ring + st * (2 * T::TILE), vb = kb + T::TILE;
-                const bool whole = dec_all(cu, pos, 16);
-                float s[NT][4], s2[NT][4];                   // two sums, of even and odd steps: half the chain
+                const bool whole = dec_all(cu, pos, T::KEYS);
+                // S^T: two sums per 16 keys where there are 16 only, of even and odd steps: half the chain
+                float s[KM][NT][4], s2[NT][4];
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) s[nt][i] = s2[nt][i] = 0.0f;
+                    for (int i = 0; i < 4; i++) {
+                        s2[nt][i] = 0.0f;
+#pragma unroll
+                        for (int km = 0; km < KM; km++) s[km][nt][i] = 0.0f;
+                    }
                 {
                     const int row = (lane & 7) + ((lane >> 3) & 1) * 8, ch = lane >> 4;
 #pragma unroll
-                    for (int ks = 0; ks < DP / 16; ks++) {
-                        uint32_t a[4];
-                        ldsm4(a, kb + (ks >> 2) * 2048 + row * 128 + (((2 * (ks & 3) + ch) ^ (row & 7)) << 4));
+                    for (int ks = 0; ks < DP / 16; ks++)
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) mma_16816(ks & 1 ? s2[nt] : s[nt], a, q[ks][nt][0], q[ks][nt][1]);
-                    }
+                        for (int km = 0; km < KM; km++) {
+                            uint32_t a[4];
+                            ldsm4(a, kb + (ks >> 2) * (T::KEYS * 128) + (km * 16 + row) * 128 + (((2 * (ks & 3) + ch) ^ (row & 7)) << 4));
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) mma_16816(KM == 1 && (ks & 1) ? s2[nt] : s[km][nt], a, q[ks][nt][0], q[ks][nt][1]);
+                        }
                 }
-                const bool in0 = whole || dec_sees(cu, pos + g), in1 = whole || dec_sees(cu, pos + g + 8);
-                uint32_t pb[NT][2];
+                bool in[KM][2];
+#pragma unroll
+                for (int km = 0; km < KM; km++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) in[km][h] = whole || dec_sees(cu, pos + km * 16 + h * 8 + g);
+                uint32_t pb[KM][NT][2];
                 bool grew = false;
                 float al[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) s[nt][i] = (i < 2 ? in0 : in1) ? (s[nt][i] + s2[nt][i]) * p.scale2 : -INFINITY;
-                    float pr[4];
-#pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        float x = fmaxf(s[nt][i], s[nt][i + 2]);
+                        float x = -INFINITY;
+#pragma unroll
+                        for (int km = 0; km < KM; km++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                float &v = s[km][nt][i + 2 * h];
+                                if (KM == 1) v += s2[nt][i + 2 * h];
+                                v = in[km][h] ? v * p.scale2 : -INFINITY;
+                                x = fmaxf(x, v);
+                            }
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -592,13 +613,24 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
                         al[nt][i] = exp2f(m[nt][i] - base);
                         grew = grew || mn > m[nt][i];
                         m[nt][i] = mn;
-                        pr[i] = __bfloat162float(__float2bfloat16_rn(exp2f(s[nt][i] - base)));
-                        pr[i + 2] = __bfloat162float(__float2bfloat16_rn(exp2f(s[nt][i + 2] - base)));
-                        l[nt][i] = l[nt][i] * al[nt][i] + (pr[i] + pr[i + 2]);
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int km = 0; km < KM; km++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                float &v = s[km][nt][i + 2 * h];
+                                v = __bfloat162float(__float2bfloat16_rn(exp2f(v - base)));
+                                sum += v;
+                            }
+                        l[nt][i] = l[nt][i] * al[nt][i] + sum;
                     }
-                    const __nv_bfloat162 p0 = __floats2bfloat162_rn(pr[0], pr[1]), p1 = __floats2bfloat162_rn(pr[2], pr[3]);
-                    pb[nt][0] = trans8(*reinterpret_cast<const uint32_t *>(&p0));
-                    pb[nt][1] = trans8(*reinterpret_cast<const uint32_t *>(&p1));
+#pragma unroll
+                    for (int km = 0; km < KM; km++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const __nv_bfloat162 pr = __floats2bfloat162_rn(s[km][nt][2 * h], s[km][nt][2 * h + 1]);
+                            pb[km][nt][h] = trans8(*reinterpret_cast<const uint32_t *>(&pr));
+                        }
                 }
                 if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
@@ -612,12 +644,14 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
                 {
                     const int row = (lane & 7) + (lane >> 4) * 8, ch = (lane >> 3) & 1;
 #pragma unroll
-                    for (int i = 0; i < DP / 16; i++) {
-                        uint32_t a[4];
-                        ldsm4t(a, vb + (i >> 2) * 2048 + row * 128 + (((2 * (i & 3) + ch) ^ (row & 7)) << 4));
+                    for (int km = 0; km < KM; km++)
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) mma_16816(o[i][nt], a, pb[nt][0], pb[nt][1]);
-                    }
+                        for (int i = 0; i < DP / 16; i++) {
+                            uint32_t a[4];
+                            ldsm4t(a, vb + (i >> 2) * (T::KEYS * 128) + (km * 16 + row) * 128 + (((2 * (i & 3) + ch) ^ (row & 7)) << 4));
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) mma_16816(o[i][nt], a, pb[km][nt][0], pb[km][nt][1]);
+                        }
                 }
             }
             __syncwarp();
@@ -629,7 +663,7 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
                 // while the next unit's query rows are on their way
                 if (cnext < S.c1) {
                     DecCur nx = cu;
-                    dec_next(p, nx);
+                    dec_next<T::K>(p, nx);
                     load_q(nx);
                 }
 #pragma unroll
@@ -694,7 +728,7 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
                 __syncthreads();                             // wml and merge are free again
                 fresh = true;
             }
-            dec_next(p, cu);
+            dec_next<T::K>(p, cu);
             c = cnext;
         }
         cp_wait<0>();
@@ -710,23 +744,23 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
 // across. f32 products and sums throughout.
 #define DEC_ST_WARPS 8
 
-template <int DP, int NT, int ST>
+template <int DP, int ROWS, int ST>
 struct DecSt {
-    static constexpr int THREADS = DEC_ST_WARPS * 32, ROWS = 8 * NT, KS = DP + 16;
+    static constexpr int THREADS = DEC_ST_WARPS * 32, K = DEC_ST_WARPS * 8, KS = DP + 16;
     static constexpr int TILE = 8 * (KS + DP) * 4;
     static constexpr int RING = DEC_ST_WARPS * ST * TILE;
-    static constexpr int MERGE = DEC_ST_WARPS * 8 * DP * 4;
+    static constexpr int MERGE = DEC_ST_WARPS * ROWS * DP * 4;
     static constexpr int Q = ROWS * DP * 4;
     static constexpr int PB = DEC_ST_WARPS * ROWS * 8 * 4;
     static constexpr int ML = DEC_ST_WARPS * ROWS * 8;
     static constexpr int SMEM = RING + MERGE + Q + PB + ML + IRX_DEC_SHARE + DEC_ST_WARPS * ST * (int)sizeof(DecRows<8>);
-    static_assert(SMEM == IRX_DEC_ST_SMEM(DP, NT, ST), "the launcher's shared memory size");
+    static_assert(SMEM == IRX_DEC_ST_SMEM(DP, ROWS, ST), "the launcher's shared memory size");
 };
 
-template <int DP, int NT, int ST>
+template <int DP, int ROWS, int ST>
 __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
 {
-    using T = DecSt<DP, NT, ST>;
+    using T = DecSt<DP, ROWS, ST>;
     constexpr int EX = 1;
     extern __shared__ __align__(128) unsigned char sm[];
     float *merge = reinterpret_cast<float *>(sm + T::RING);
@@ -740,19 +774,19 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
     constexpr int VW = DP / 32 < 4 ? DP / 32 : 4, NJ = DP / 32 / VW;
 
     irx_pdl_enter();
-    dec_partition<T::THREADS, EX>(p, upb, S);
+    dec_partition<T::THREADS, T::K, EX>(p, upb, S);
     if (S.c0 < S.c1) {
         DecCur tl, cu;
-        const long long cfirst = dec_start<EX>(p, S, tl);
+        const long long cfirst = dec_start<T::K, EX>(p, S, tl);
         cu = tl;
         float *myring = reinterpret_cast<float *>(sm) + warp * (ST * T::TILE / 4);
-        float *pb = pball + warp * (T::ROWS * 8);
+        float *pb = pball + warp * (ROWS * 8);
         long long tc = cfirst;
         auto lookup = [&](int st) {
-            dec_lookup<8>(p, tl, tc < S.c1, dec_pos(tl, tl.j) + warp * 8, rows[st]);
+            dec_lookup<8>(p, tl, tc < S.c1, dec_pos<T::K>(tl, tl.j) + warp * 8, rows[st]);
             if (tc < S.c1) {
                 tc = dec_step<EX>(tl, tc);
-                dec_next(p, tl);
+                dec_next<T::K>(p, tl);
             }
         };
         auto fetch = [&](int st) {
@@ -790,20 +824,20 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
         __syncwarp();
         for (int s = 0; s < ST; s++) fetch(s);
 
-        float o[T::ROWS][NJ * VW], m[T::ROWS], l[T::ROWS];
+        float o[ROWS][NJ * VW], m[ROWS], l[ROWS];
         int st = 0, live = 0;
         bool fresh = true;
         for (long long c = cfirst; c < S.c1;) {
             if (fresh) {
                 const int hk = p.h0 + cu.h, rb = cu.rb;
-                live = min(T::ROWS, p.group - rb * T::ROWS);
-                for (int i = threadIdx.x; i < T::ROWS * DP; i += T::THREADS) {
+                live = min(ROWS, p.group - rb * ROWS);
+                for (int i = threadIdx.x; i < ROWS * DP; i += T::THREADS) {
                     const int r = i / DP, d = i % DP;
                     qs[i] = r < live && d < p.d
-                          ? irx_ld1(p.q, p.dt, (int64_t)cu.b * p.q_stride + (int64_t)(hk * p.group + rb * T::ROWS + r) * p.d + d) : 0.0f;
+                          ? irx_ld1(p.q, p.dt, (int64_t)cu.b * p.q_stride + (int64_t)(hk * p.group + rb * ROWS + r) * p.d + d) : 0.0f;
                 }
 #pragma unroll
-                for (int r = 0; r < T::ROWS; r++) {
+                for (int r = 0; r < ROWS; r++) {
                     m[r] = -INFINITY;
                     l[r] = 0.0f;
 #pragma unroll
@@ -814,18 +848,18 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
             }
             cp_wait<ST - 1>();
             __syncwarp();
-            const int pos = dec_pos(cu, cu.j) + warp * 8;
+            const int pos = dec_pos<T::K>(cu, cu.j) + warp * 8;
             if (dec_any(cu, pos, 8)) {
                 const bool in = dec_sees(cu, pos + key);
                 const float *kt = myring + st * (T::TILE / 4), *vt = kt + 8 * T::KS;
-                float s[T::ROWS];
+                float s[ROWS];
 #pragma unroll
-                for (int r = 0; r < T::ROWS; r++) s[r] = 0.0f;
+                for (int r = 0; r < ROWS; r++) s[r] = 0.0f;
 #pragma unroll 4
                 for (int i = 0; i < DP / 16; i++) {
                     const float4 k4 = *reinterpret_cast<const float4 *>(kt + key * T::KS + (4 * i + quarter) * 4);
 #pragma unroll
-                    for (int r = 0; r < T::ROWS; r++) {
+                    for (int r = 0; r < ROWS; r++) {
                         const float4 q4 = *reinterpret_cast<const float4 *>(qs + r * DP + (4 * i + quarter) * 4);
                         s[r] = fmaf(q4.x, k4.x, s[r]);
                         s[r] = fmaf(q4.y, k4.y, s[r]);
@@ -834,7 +868,7 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
                     }
                 }
 #pragma unroll
-                for (int r = 0; r < T::ROWS; r++) {
+                for (int r = 0; r < ROWS; r++) {
                     float x = s[r];
                     x += __shfl_xor_sync(0xffffffffu, x, 1);
                     x += __shfl_xor_sync(0xffffffffu, x, 2);
@@ -873,7 +907,7 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
                             }
                         }
 #pragma unroll
-                    for (int r = 0; r < T::ROWS; r++) {
+                    for (int r = 0; r < ROWS; r++) {
                         const float4 e = *reinterpret_cast<const float4 *>(pb + r * 8 + kk);
 #pragma unroll
                         for (int j = 0; j < NJ * VW; j++) {
@@ -891,68 +925,63 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
             const long long cnext = dec_step<EX>(cu, c);
             if (cu.j + 1 == cu.nch || cnext >= S.c1) {
 #pragma unroll
-                for (int r = 0; r < T::ROWS; r++) {
+                for (int r = 0; r < ROWS; r++) {
                     float x = l[r];
                     x += __shfl_xor_sync(0xffffffffu, x, 4);
                     x += __shfl_xor_sync(0xffffffffu, x, 8);
                     x += __shfl_xor_sync(0xffffffffu, x, 16);
-                    if (lane == 0) wml[warp * T::ROWS + r] = make_float2(m[r], x);
+                    if (lane == 0) wml[warp * ROWS + r] = make_float2(m[r], x);
                 }
                 __syncthreads();
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    if (nt) __syncthreads();
+                for (int r = 0; r < ROWS; r++) {
+                    float M = -INFINITY;
 #pragma unroll
-                    for (int r8 = 0; r8 < 8; r8++) {
-                        const int r = nt * 8 + r8;
-                        float M = -INFINITY;
+                    for (int w = 0; w < DEC_ST_WARPS; w++) M = fmaxf(M, wml[w * ROWS + r].x);
+                    const float f = exp2f(m[r] - (M == -INFINITY ? 0.0f : M));
 #pragma unroll
-                        for (int w = 0; w < DEC_ST_WARPS; w++) M = fmaxf(M, wml[w * T::ROWS + r].x);
-                        const float f = exp2f(m[r] - (M == -INFINITY ? 0.0f : M));
+                    for (int j = 0; j < NJ * VW; j++)
+                        merge[(warp * ROWS + r) * DP + (j / VW) * 128 + lane * VW + j % VW] = o[r][j] * f;
+                }
+                __syncthreads();
+                for (int it = threadIdx.x; it < ROWS * DP; it += T::THREADS) {
+                    float a = 0.0f;
 #pragma unroll
-                        for (int j = 0; j < NJ * VW; j++)
-                            merge[(warp * 8 + r8) * DP + (j / VW) * 128 + lane * VW + j % VW] = o[r][j] * f;
-                    }
-                    __syncthreads();
-                    for (int it = threadIdx.x; it < 8 * DP; it += T::THREADS) {
-                        float a = 0.0f;
-#pragma unroll
-                        for (int w = 0; w < DEC_ST_WARPS; w++) a += merge[w * 8 * DP + it];
-                        qs[nt * 8 * DP + it] = a;                // the query rows are done with
-                    }
+                    for (int w = 0; w < DEC_ST_WARPS; w++) a += merge[w * ROWS * DP + it];
+                    qs[it] = a;                                  // the query rows are done with
                 }
                 __syncthreads();
                 auto ml = [&](int r) {
                     float M = -INFINITY, L = 0.0f;
 #pragma unroll
-                    for (int w = 0; w < DEC_ST_WARPS; w++) M = fmaxf(M, wml[w * T::ROWS + r].x);
+                    for (int w = 0; w < DEC_ST_WARPS; w++) M = fmaxf(M, wml[w * ROWS + r].x);
 #pragma unroll
                     for (int w = 0; w < DEC_ST_WARPS; w++) {
-                        const float2 x = wml[w * T::ROWS + r];
+                        const float2 x = wml[w * ROWS + r];
                         L += x.y * exp2f(x.x - (M == -INFINITY ? 0.0f : M));
                     }
                     return make_float2(M, L);
                 };
                 auto acc = [&](int r, int d0, int) { return *reinterpret_cast<const float4 *>(qs + r * DP + d0); };
-                dec_finish<DP, T::ROWS, T::THREADS>(p, S, cu, c, upb, acc, ml);
+                dec_finish<DP, ROWS, T::THREADS>(p, S, cu, c, upb, acc, ml);
                 __syncthreads();
                 fresh = true;
             }
-            dec_next(p, cu);
+            dec_next<T::K>(p, cu);
             c = cnext;
         }
         cp_wait<0>();
-        dec_join<DP, T::ROWS, T::THREADS>(p, S, wml);
+        dec_join<DP, ROWS, T::THREADS>(p, S, wml);
     }
     dec_empty(p);
 }
 
 #define DEC_TC(DP, NT) \
     extern "C" __global__ void __launch_bounds__(DEC_TC_WARPS * 32) irx_dec_tc_##DP##_##NT(const __grid_constant__ irx_kdec_t p) \
-    { dec_tc_body<DP, NT, IRX_DEC_TC_ST(DP, NT)>(p); }
-#define DEC_STK(DP, NT) \
-    extern "C" __global__ void __launch_bounds__(DEC_ST_WARPS * 32) irx_dec_st_##DP##_##NT(const __grid_constant__ irx_kdec_t p) \
-    { dec_st_body<DP, NT, IRX_DEC_ST_ST(DP)>(p); }
+    { dec_tc_body<DP, NT, IRX_DEC_TC_KM(DP), IRX_DEC_TC_ST(DP, NT)>(p); }
+#define DEC_STK(DP, ROWS) \
+    extern "C" __global__ void __launch_bounds__(DEC_ST_WARPS * 32) irx_dec_st_##DP##_##ROWS(const __grid_constant__ irx_kdec_t p) \
+    { dec_st_body<DP, ROWS, IRX_DEC_ST_ST(DP)>(p); }
 
 DEC_TC(64, 1) DEC_TC(64, 2) DEC_TC(128, 1) DEC_TC(128, 2) DEC_TC(256, 1)
-DEC_STK(64, 1) DEC_STK(64, 2) DEC_STK(128, 1) DEC_STK(128, 2) DEC_STK(256, 1)
+DEC_STK(64, 4) DEC_STK(64, 8) DEC_STK(128, 4) DEC_STK(128, 8) DEC_STK(256, 4) DEC_STK(256, 8)

@@ -160,7 +160,7 @@ static const char *const KNAMES[K_COUNT] = {
     "irx_mm_f32", "irx_mm_bf16", "irx_mm_bf16_simt", "irx_attn_f32", "irx_attn_bf16", "irx_attn_bf16_simt",
     "irx_mm_bf16_pair", "irx_mm_bf16_wide",
     "irx_dec_tc_64_1", "irx_dec_tc_64_2", "irx_dec_tc_128_1", "irx_dec_tc_128_2", "irx_dec_tc_256_1",
-    "irx_dec_st_64_1", "irx_dec_st_64_2", "irx_dec_st_128_1", "irx_dec_st_128_2", "irx_dec_st_256_1",
+    "irx_dec_st_64_4", "irx_dec_st_64_8", "irx_dec_st_128_4", "irx_dec_st_128_8", "irx_dec_st_256_4", "irx_dec_st_256_8",
     "irx_kv_append_16", "irx_kv_append_4", "irx_kv_append_2",
     "irx_kv_copy_16", "irx_kv_copy_4", "irx_kv_copy_2",
     "irx_mv4_bf16_32_1", "irx_mv4_bf16_32_2", "irx_mv4_bf16_64_1", "irx_mv4_bf16_64_2", "irx_mv4_bf16_128_1", "irx_mv4_bf16_128_2",

@@ -15,7 +15,7 @@ enum {
     K_MM_BF16_PAIR, K_MM_BF16_WIDE,
     /* the serving operators: decode by padded head size and 8-row blocks, cache moves by vector
      * width, matrix-vector products by type, group grain and 8-column blocks */
-    K_DEC_TC, K_DEC_ST = K_DEC_TC + 5, K_KV_APPEND = K_DEC_ST + 5, K_KV_COPY = K_KV_APPEND + 3,
+    K_DEC_TC, K_DEC_ST = K_DEC_TC + 5, K_KV_APPEND = K_DEC_ST + 6, K_KV_COPY = K_KV_APPEND + 3,
     K_MV4 = K_KV_COPY + 3, K_MV4_ANY = K_MV4 + 12,
     K_COUNT
 };

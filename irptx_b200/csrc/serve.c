@@ -100,11 +100,15 @@ static int cache_of(irx_kvc_t *o, const irx_kv_cache_t *c, int tabled)
 
 /* ---- decode ---- */
 
-static int64_t dec_units(const irx_dec_t *a) { return (int64_t)a->c.batch * a->c.heads * a->split; }
+/* The workspace serves either kernel: an unaligned bf16 launch takes the second. */
+static int64_t dec_units(const irx_dec_t *a)
+{
+    return (int64_t)a->c.batch * a->c.heads * (a->split[0] > a->split[1] ? a->split[0] : a->split[1]);
+}
 
 static int64_t dec_part_bytes(const irx_dec_t *a)
 {
-    return 2ll * a->max_ctas * (8 * a->nt) * (a->dp + 2) * 4;
+    return 2ll * a->max_ctas * (a->rows[0] > a->rows[1] ? a->rows[0] : a->rows[1]) * (a->dp + 2) * 4;
 }
 
 int irx_compile_decode(const irx_kv_cache_t *cache, int heads, long long q_stride, float scale, int window, int sinks, int lse,
@@ -113,7 +117,7 @@ int irx_compile_decode(const irx_kv_cache_t *cache, int heads, long long q_strid
     irx_plan_int_t *p = begin(plan, FAM_DECODE, "decode");
     irx_dec_t *a;
     int64_t per, chunks, qrow;
-    int g;
+    int g, i;
     if (!p) return 1;
     a = &p->u.dec;
     if (cache_of(&a->c, cache, 1)) return 1;
@@ -132,10 +136,11 @@ int irx_compile_decode(const irx_kv_cache_t *cache, int heads, long long q_strid
     memcpy(&a->scale_bits, &scale, 4);
     g = heads / a->c.heads;
     a->dp = a->c.dim <= 64 ? 64 : a->c.dim <= 128 ? 128 : 256;
-    a->nt = g > 8 && a->dp <= 128 ? 2 : 1;
-    a->split = (g + 8 * a->nt - 1) / (8 * a->nt);
+    a->rows[0] = g > 8 && a->dp <= 128 ? 16 : 8;
+    a->rows[1] = g > 4 ? 8 : 4;
+    for (i = 0; i < 2; i++) a->split[i] = (g + a->rows[i] - 1) / a->rows[i];
     /* no more blocks than chunks of a full cache: what the workspace has to hold */
-    per = ((int64_t)a->c.cols * a->c.page_size + IRX_DEC_KEYS - 1) / IRX_DEC_KEYS;
+    per = ((int64_t)a->c.cols * a->c.page_size + 63) / 64;
     chunks = dec_units(a) > IRX_DEC_MAX_CTAS ? IRX_DEC_MAX_CTAS : dec_units(a) * per;
     a->max_ctas = chunks < IRX_DEC_MAX_CTAS ? (int32_t)chunks : IRX_DEC_MAX_CTAS;
     if (dec_units(a) > MAX_COUNT) return irx_fail(E042, "more than 2^31 - 1 rows of work");
@@ -165,12 +170,10 @@ static int launch_decode(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
 {
     const irx_dec_t *a = &p->u.dec;
     static irx_kdec_t k;
-    static const int DP[5] = {64, 64, 128, 128, 256};
     const int es = esz(a->c.dt), al = 16 / es, last = p->narg - 1;
-    const int i = a->dp == 64 ? a->nt - 1 : a->dp == 128 ? 1 + a->nt : 4;
     long long u0, u1;
     int64_t grid;
-    int rows, kk;
+    int rows, kk, st_;
     size_t smem;
     float scale;
     memset(&k, 0, sizeof k);
@@ -192,7 +195,6 @@ static int launch_decode(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
     k.batch = a->c.batch; k.cols = a->c.cols; k.page_size = a->c.page_size;
     k.heads = a->heads; k.group = a->heads / a->c.heads; k.d = a->c.dim;
     k.h0 = (int32_t)u0; k.h1 = (int32_t)u1;
-    k.split = a->split;
     k.window = a->window; k.sinks = a->sinks;
     k.scale2 = (float)((double)scale * 1.4426950408889634);
     k.dt = a->c.dt;
@@ -206,17 +208,19 @@ static int launch_decode(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
         k.pshift = (uint8_t)(31 + l);
         k.pmul = ((1ull << l << 31) + ps - 1) / ps;
     }
-    rows = a->nt;
-    if (k.vec && a->c.dt == DT_BF16) {
-        kk = K_DEC_TC + i;
-        smem = (size_t)IRX_DEC_TC_SMEM(DP[i], rows, IRX_DEC_TC_ST(DP[i], rows));
-        if (serve_grid(d, kk, 128, smem, a->max_ctas, &grid)) return 1;
-        return irx_dev_launch(d, kk, (unsigned)grid, 128, (unsigned)smem, 1, st, &k);
+    st_ = !k.vec || a->c.dt != DT_BF16;
+    rows = a->rows[st_];
+    k.split = a->split[st_];
+    if (!st_) {
+        const int nt = rows / 8;
+        kk = K_DEC_TC + (a->dp == 64 ? nt - 1 : a->dp == 128 ? 1 + nt : 4);
+        smem = (size_t)IRX_DEC_TC_SMEM(a->dp, nt, IRX_DEC_TC_KM(a->dp), IRX_DEC_TC_ST(a->dp, nt));
+    } else {
+        kk = K_DEC_ST + (a->dp == 64 ? 0 : a->dp == 128 ? 2 : 4) + (rows == 8);
+        smem = (size_t)IRX_DEC_ST_SMEM(a->dp, rows, IRX_DEC_ST_ST(a->dp));
     }
-    kk = K_DEC_ST + i;
-    smem = (size_t)IRX_DEC_ST_SMEM(DP[i], rows, IRX_DEC_ST_ST(DP[i]));
-    if (serve_grid(d, kk, 256, smem, a->max_ctas, &grid)) return 1;
-    return irx_dev_launch(d, kk, (unsigned)grid, 256, (unsigned)smem, 1, st, &k);
+    if (serve_grid(d, kk, st_ ? 256 : 128, smem, a->max_ctas, &grid)) return 1;
+    return irx_dev_launch(d, kk, (unsigned)grid, st_ ? 256 : 128, (unsigned)smem, 1, st, &k);
 }
 
 /* ---- the cache's moves ---- */
@@ -448,12 +452,13 @@ void irx_serve_text(const irx_plan_int_t *p, char *buf, size_t cap)
 {
     if (p->fam == FAM_DECODE) {
         const irx_dec_t *a = &p->u.dec;
+        const int st = a->c.dt != DT_BF16 || a->c.dim % 8;
         float sc;
         memcpy(&sc, &a->scale_bits, 4);
         snprintf(buf, cap, "decode batch=%d heads=%d kv_heads=%d d=%d page=%d pages=%lld window=%d sinks=%d lse=%d scale=%g "
                  "dtype=%s kernel=irx_dec_%s_%d_%d", a->c.batch, a->heads, a->c.heads, a->c.dim, a->c.page_size,
                  (long long)a->c.pages, a->window, a->sinks, a->lse, (double)sc, dname(a->c.dt),
-                 a->c.dt != DT_BF16 || a->c.dim % 8 ? "st" : "tc", a->dp, a->nt);
+                 st ? "st" : "tc", a->dp, st ? a->rows[1] : a->rows[0] / 8);
     } else if (p->fam == FAM_MATVEC4) {
         const irx_mv4_t *a = &p->u.mv;
         snprintf(buf, cap, "matvec4 m=%lld n=%lld k=%lld group=%d zeros=%d dtype=%s", (long long)a->m, (long long)a->n,
