@@ -456,3 +456,56 @@ def test_launch_refusals(cuda, irx):
     with pytest.raises(irx.IrxError):
         plan.run_host([np.zeros(4, np.float32)] * len(args))
     irx.check()
+
+
+# ---- caches past 32 bits ----
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_offsets_past_32_bits(cuda, irx, dtype):
+    """Two pages more than 2^31 elements apart, written by append, copied and attended to."""
+    torch = cuda
+    kv, d, page = 2, 64, 16
+    far = (1 << 31) + 4096
+    cache = irx.KvCache(dtype, kv, d, page, 3, batch=1, table_cols=3, strides=(far // 2, page * d, d))
+    k = torch.empty(far + 4096, dtype=tdt(torch, dtype), device="cuda").as_strided(cache.shape, cache.strides + (1,))
+    v = torch.empty(far + 4096, dtype=tdt(torch, dtype), device="cuda").as_strided(cache.shape, cache.strides + (1,))
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    n = 2 * page
+    new = [torch.empty(n, kv, d, device="cuda").normal_(generator=gen).to(k.dtype) for _ in range(2)]
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32, device="cuda")
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    irx.kv_append(cache, n).launch(new + [torch.zeros_like(pos), pos, table, k, v])
+    assert torch.equal(k[2].transpose(0, 1), new[0][:page]) and torch.equal(v[0].transpose(0, 1), new[1][page:])
+    irx.kv_copy(cache, 1).launch([torch.tensor([[2, 1]], dtype=torch.int32, device="cuda"), k[None], v[None]])
+    assert torch.equal(k[1], k[2]) and torch.equal(v[1], v[2])
+    q = torch.empty(1, 4, d, device="cuda").normal_(generator=gen).to(k.dtype)
+    plan, outs = irx.decode(cache, 4), []
+    for order in ([2, 0, 0], [1, 0, 0]):                 # the far page, and its copy
+        outs.append(torch.empty_like(q))
+        plan.launch([q, k, v, torch.tensor([order], dtype=torch.int32, device="cuda"), torch.tensor([n], dtype=torch.int32, device="cuda"),
+                     outs[-1], plan.workspace()])
+    irx.check()
+    assert torch.equal(outs[0], outs[1])
+    kk, vv = new[0].double(), new[1].double()
+    for h in range(4):
+        s = (q[0, h].double() @ kk[:, h // 2].T) / math.sqrt(d)
+        p = torch.softmax(s, -1)
+        want, spread = p @ vv[:, h // 2], p @ vv[:, h // 2].abs()
+        big = (q[0, h].double().abs() @ kk[:, h // 2].abs().T).max() / math.sqrt(d)
+        assert bool(((outs[0][0, h].double() - want).abs() <= decode_tol(dtype, d, n, want, spread, big.reshape(())[None])).all())
+
+
+# ---- together, as a decoding program runs them ----
+
+def test_example_decodes_like_the_dense_model(cuda):
+    """Prompt, forks with copy on write, a replayed step graph, a closed sequence and a compaction. The
+    bound: each of the two layers rounds its activations to bf16 about ten times (2^-9 of their size
+    each, adding like noise), which stays well below a twentieth of the largest logit; a page or
+    position gone wrong changes logits by their own size."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "decode_layers.py")
+    spec = importlib.util.spec_from_file_location("decode_layers", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    assert mod.main(out=lambda *_: None) < 0.05
