@@ -48,38 +48,12 @@ __device__ __forceinline__ void mv4_unpack(uint32_t w, __nv_bfloat162 z, uint32_
 template <int NT>
 struct Mv4Smem {
     static constexpr int XS = 512 + 64;                  // bytes of a column's stage: 64 off the banks' period
-    static constexpr int W = 128 * 128, X = NT * 8 * XS, RING = W * IRX_MV4_STAGES, BARS = RING + X * IRX_MV4_STAGES;
+    static constexpr int W = 128 * 128, X = NT * 8 * XS, RING = W * IRX_MV4_STAGES, SCALES = RING + X * IRX_MV4_STAGES;
+    static constexpr int ZEROS = SCALES + 2 * 128 * 9 * 4, BARS = ZEROS + 2 * 128 * 8;
     static_assert(BARS + 1024 + 64 == IRX_MV4_SMEM(NT), "the launcher's shared memory size");
     static constexpr int RS = NT * 8 + 4;                // floats of a row of the sums
-    static_assert(2 * 128 * RS * 4 <= BARS, "the sums fit the ring");
+    static_assert(2 * 128 * RS * 4 <= SCALES, "the sums fit the ring");
 };
-
-// The scales (as they lie in memory: turning them into numbers at once would wait for them) and zero
-// points of a warp's rows g, g + 8, g + 16, g + 24, for this lane's piece of the stage.
-struct Mv4Scale {
-    uint32_t s[4], z[4];
-};
-
-// k / 32 / (group / 32) by a multiplication: exact below 2^26 (the launcher's constants).
-template <int GV>
-__device__ __forceinline__ void mv4_scales(const irx_kmv4_t &p, const uint32_t (&at)[4], uint32_t k0, int t, Mv4Scale &S)
-{
-    const uint32_t k = k0 + (t * (128 / GV) / 4) * GV;
-    const uint32_t grp = (uint32_t)(((uint64_t)(k >> 5) * p.gmul) >> p.gshift);
-    if (k < (uint32_t)p.k) {
-        if (p.sdt == DT_BF16) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) S.s[i] = __ldg(reinterpret_cast<const unsigned short *>(p.s) + (at[i] + grp));
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++) S.s[i] = __ldg(reinterpret_cast<const uint32_t *>(p.s) + (at[i] + grp));
-        }
-        if (p.z) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) S.z[i] = __ldg(p.z + (at[i] + grp));
-        }
-    }
-}
 
 // The first product of a sum: the accumulators start at zero.
 __device__ __forceinline__ void mma_16816_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
@@ -90,7 +64,7 @@ __device__ __forceinline__ void mma_16816_first(float (&c)[4], const uint32_t (&
 }
 
 template <int GV, int NT>
-__device__ __forceinline__ void mv4_stage(uint32_t ws, const unsigned char *xs, int wr, int wk, int lane, const Mv4Scale &S, bool zs, int sshift,
+__device__ __forceinline__ void mv4_stage(uint32_t ws, const unsigned char *xs, const float *sc, const unsigned char *zp, int wr, int wk, int lane,
                                           float (&acc)[2][NT][4])
 {
     using M = Mv4Smem<NT>;
@@ -113,11 +87,9 @@ __device__ __forceinline__ void mv4_stage(uint32_t ws, const unsigned char *xs, 
         for (int rt = 0; rt < 2; rt++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                unsigned zz = 8;
-                const int from = (lane & ~3) + i * (4 / P);
-                const uint32_t sb = P > 1 ? __shfl_sync(0xffffffffu, S.s[rt * 2 + h], from) : S.s[rt * 2 + h];
-                s[rt][h] = __uint_as_float(sb << sshift);
-                if (zs) zz = P > 1 ? __shfl_sync(0xffffffffu, S.z[rt * 2 + h], from) : S.z[rt * 2 + h];
+                const int row = wr * 32 + rt * 16 + h * 8 + g;
+                const unsigned zz = zp ? zp[row * 8 + i] : 8u;
+                s[rt][h] = sc[row * 9 + i];
                 const uint32_t zb = 0x43004300u | ((zz & 15u) * 0x00010001u);
                 z[rt][h] = *reinterpret_cast<const __nv_bfloat162 *>(&zb);
             }
@@ -251,37 +223,70 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
                                __byte_perm(xb[i].y, xb[i].w, 0x5410), __byte_perm(xb[i].y, xb[i].w, 0x7632));
         }
     };
-    Mv4Scale S[2] = {};
+    // Scales and zero points: 8 pieces of GV k a row serve a run of 4, 2 or 1 stages. A thread loads four
+    // pieces, eight neighbouring threads a row's, a run ahead in registers (as they lie in memory), and
+    // stores them as numbers when the run before them is done with: every lane loading its own rows'
+    // each stage took as long as half the products.
+    constexpr int P = 128 / GV, RUN = 4 / P;
+    float *scales = reinterpret_cast<float *>(sm + M::SCALES);
+    unsigned char *zeros = sm + M::ZEROS;
+    uint32_t sr[4], zr[4];
     uint32_t at[4];                                      // rows past the end read the last row's: their sums go nowhere
 #pragma unroll
-    for (int i = 0; i < 4; i++) at[i] = (uint32_t)min(row0 + wr * 32 + i * 8 + g, n1 - 1) * (uint32_t)p.groups;
-    const int sshift = p.sdt == DT_BF16 ? 16 : 0;
+    for (int i = 0; i < 4; i++) at[i] = (uint32_t)min(row0 + (tid >> 3) + 32 * i, n1 - 1) * (uint32_t)p.groups;
+    auto sload = [&](int r) {                            // run r; k / 32 / (group / 32) is a multiplication, exact below 2^26
+        const int pc = tid & 7;
+        const uint32_t k = min((uint32_t)(((r * RUN + pc / (2 * P)) * ck + rank) * 256 + (pc % (2 * P)) * GV), (uint32_t)k_all - 1);
+        const uint32_t grp = (uint32_t)(((uint64_t)(k >> 5) * p.gmul) >> p.gshift);
+        if (p.sdt == DT_BF16) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) sr[i] = __ldg(reinterpret_cast<const unsigned short *>(p.s) + (at[i] + grp));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) sr[i] = __ldg(reinterpret_cast<const uint32_t *>(p.s) + (at[i] + grp));
+        }
+        if (p.z) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) zr[i] = __ldg(p.z + (at[i] + grp));
+        }
+    };
+    auto sstore = [&](int r) {
+        const int shift = p.sdt == DT_BF16 ? 16 : 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int row = (r & 1) * 128 + (tid >> 3) + 32 * i;
+            scales[row * 9 + (tid & 7)] = __uint_as_float(sr[i] << shift);
+            if (p.z) zeros[row * 8 + (tid & 7)] = (unsigned char)zr[i];
+        }
+    };
     if (F32) {                                           // columns that no token has stay zero
         for (int i = tid; i < ST * M::X / 16; i += MV4_WARPS * 32) *reinterpret_cast<uint4 *>(sm + M::RING + i * 16) = make_uint4(0, 0, 0, 0);
         __syncthreads();
     }
 #pragma unroll
     for (int i = 0; i < ST - 1; i++) fetch(i);
-    mv4_scales<GV>(p, at, (uint32_t)rank * 256 + wk * 128, t, S[0]);
-    mv4_scales<GV>(p, at, (uint32_t)(ck + rank) * 256 + wk * 128, t, S[1]);
+    sload(0);
     xload();
+    sstore(0);
+    sload(1);
     xstore(0);
     xload();
     int ok = 1;
-    for (int s = 0; s < n_st; s += 2) {
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            if (s + u >= n_st) break;
-            const int slot = (s + u) % ST;
-            ok = ok && irx_mbar_wait(full + slot, ((s + u) / ST) & 1);
-            __syncthreads();                             // the tokens are there too; the stage before is free
-            fetch(s + u + ST - 1);
-            mv4_stage<GV, NT>(irx_smem_u32(sm) + slot * M::W, sm + M::RING + slot * M::X, wr, wk, lane, S[u], p.z != nullptr, sshift, acc);
-            mv4_scales<GV>(p, at, (uint32_t)((s + u + 2) * ck + rank) * 256 + wk * 128, t, S[u]);
-            if (s + u + 1 < n_st) {
-                xstore(s + u + 1);
-                xload();
+    for (int c = 0; c < n_st; c++) {
+        const int slot = c % ST, run = c / RUN, sub = c % RUN;
+        ok = ok && irx_mbar_wait(full + slot, (c / ST) & 1);
+        __syncthreads();                                 // tokens and scales are there too; the stage before is free
+        fetch(c + ST - 1);
+        mv4_stage<GV, NT>(irx_smem_u32(sm) + slot * M::W, sm + M::RING + slot * M::X,
+                          scales + (run & 1) * (128 * 9) + sub * (2 * P) + wk * P,
+                          p.z ? zeros + (run & 1) * (128 * 8) + sub * (2 * P) + wk * P : nullptr, wr, wk, lane, acc);
+        if (c + 1 < n_st) {
+            if (sub == RUN - 1) {
+                sstore(run + 1);
+                sload(run + 2);
             }
+            xstore(c + 1);
+            xload();
         }
     }
     if (!ok) {                                           // a wait ran out: report it, and let copies in flight land
