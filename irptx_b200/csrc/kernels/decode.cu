@@ -410,8 +410,10 @@ __device__ __forceinline__ long long dec_row(const irx_kdec_t &p, const DecRows<
 // the products take 16 to 32 instructions per 8 KB (D = 128), which HBM delivers in about 360
 // cycles per SM: the tensor pipe is idle most of the time and tcgen05's 128-row tiles would be
 // filled with padding.
-// P is rounded to bf16 for the product (as V is bf16), the sum of exps takes the same rounded
-// values so that the weights still sum to one.
+// P enters the product as two bf16 numbers, its upper half truncated and the rest rounded, 16 bits in
+// all: the tensor pipe has room for the second product, and the output is then as near the
+// definition as one rounded once at the end. (The rest is kept above zero, so that an infinite value
+// does not meet 0 there.)
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
@@ -589,7 +591,7 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
                 for (int km = 0; km < KM; km++)
 #pragma unroll
                     for (int h = 0; h < 2; h++) in[km][h] = whole || dec_sees(cu, pos + km * 16 + h * 8 + g);
-                uint32_t pb[KM][NT][2];
+                uint32_t pb[KM][NT][2], pl[KM][NT][2];       // P^T's upper and lower halves
                 bool grew = false;
                 float al[NT][2];
 #pragma unroll
@@ -619,7 +621,7 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
 #pragma unroll
                             for (int h = 0; h < 2; h++) {
                                 float &v = s[km][nt][i + 2 * h];
-                                v = __bfloat162float(__float2bfloat16_rn(exp2f(v - base)));
+                                v = exp2f(v - base);
                                 sum += v;
                             }
                         l[nt][i] = l[nt][i] * al[nt][i] + sum;
@@ -628,8 +630,12 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
                     for (int km = 0; km < KM; km++)
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            const __nv_bfloat162 pr = __floats2bfloat162_rn(s[km][nt][2 * h], s[km][nt][2 * h + 1]);
-                            pb[km][nt][h] = trans8(*reinterpret_cast<const uint32_t *>(&pr));
+                            const float x = s[km][nt][2 * h], y = s[km][nt][2 * h + 1];
+                            const uint32_t hi = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+                            const __nv_bfloat162 lo = __floats2bfloat162_rn(fmaxf(x - __uint_as_float(hi << 16), 1.2e-38f),
+                                                                            fmaxf(y - __uint_as_float(hi & 0xffff0000u), 1.2e-38f));
+                            pb[km][nt][h] = trans8(hi);
+                            pl[km][nt][h] = trans8(*reinterpret_cast<const uint32_t *>(&lo));
                         }
                 }
                 if (__any_sync(0xffffffffu, grew)) {
@@ -650,7 +656,10 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
                             uint32_t a[4];
                             ldsm4t(a, vb + (i >> 2) * (T::KEYS * 128) + (km * 16 + row) * 128 + (((2 * (i & 3) + ch) ^ (row & 7)) << 4));
 #pragma unroll
-                            for (int nt = 0; nt < NT; nt++) mma_16816(o[i][nt], a, pb[km][nt][0], pb[km][nt][1]);
+                            for (int nt = 0; nt < NT; nt++) {
+                                mma_16816(o[i][nt], a, pb[km][nt][0], pb[km][nt][1]);
+                                mma_16816(o[i][nt], a, pl[km][nt][0], pl[km][nt][1]);
+                            }
                         }
                 }
             }
