@@ -447,6 +447,11 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void *src, uint32_t byt
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(dst), "l"(src) : "memory");
+}
+
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
 
@@ -502,17 +507,30 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
         };
         auto fetch = [&](int st) {
             const long long off = dec_row<T::KEYS>(p, rows[st], lane & (T::KEYS - 1));
-            if (__any_sync(0xffffffffu, off != -1)) {
-                const uint32_t kd = ring + st * (2 * T::TILE), vd = kd + T::TILE;
+            const uint32_t kd = ring + st * (2 * T::TILE);
+            if (DP < 256 && __all_sync(0xffffffffu, off >= 0) && p.d == DP) {      // every row whole: offsets by way of shared memory
+                if (lane < T::KEYS) rows[st].off[lane] = off;
+                __syncwarp();
+                const char *src = reinterpret_cast<const char *>(p.k) + lch * 16;
+                const long long dv = reinterpret_cast<const char *>(p.v) - reinterpret_cast<const char *>(p.k);
+#pragma unroll
+                for (int i = 0; i < NI; i++) {
+                    const int row = i * RPI + lrow;
+                    const char *k = src + rows[st].off[row] * 2;
+                    const uint32_t d = kd + (lch >> 3) * (T::KEYS * 128) + row * 128 + (((lch & 7) ^ (row & 7)) << 4);
+                    cp16(d, k);
+                    cp16(d + T::TILE, k + dv);
+                }
+            } else if (__any_sync(0xffffffffu, off != -1)) {
 #pragma unroll
                 for (int i = 0; i < NI; i++) {
                     const int row = i * RPI + lrow;
                     const long long o = __shfl_sync(0xffffffffu, off, row);
-                    const uint32_t d = (lch >> 3) * (T::KEYS * 128) + row * 128 + (((lch & 7) ^ (row & 7)) << 4);
+                    const uint32_t d = kd + (lch >> 3) * (T::KEYS * 128) + row * 128 + (((lch & 7) ^ (row & 7)) << 4);
                     const int64_t e = o >= 0 && cin ? o + lch * 8 : 0;
                     const uint32_t nb = o >= 0 && cin ? 16 : 0;
-                    cp16(kd + d, reinterpret_cast<const __nv_bfloat16 *>(p.k) + e, nb);
-                    cp16(vd + d, reinterpret_cast<const __nv_bfloat16 *>(p.v) + e, nb);
+                    cp16(d, reinterpret_cast<const __nv_bfloat16 *>(p.k) + e, nb);
+                    cp16(d + T::TILE, reinterpret_cast<const __nv_bfloat16 *>(p.v) + e, nb);
                 }
             }
             __syncwarp();
