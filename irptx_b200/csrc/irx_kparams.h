@@ -153,6 +153,9 @@ typedef struct {
     int32_t     parts;              /* warps per token */
 } irx_kapp_t;
 
+#define IRX_APPEND_VEC 2            /* vectors of keys, and of values, a lane of a warp moves */
+#define IRX_COPY_TILE 512           /* vectors a block of the page copy moves at a time */
+
 /* Page copy: runs of `run` vectors at (i1, i2) of every (pair, layer) of both pools. */
 typedef struct {
     const int32_t *pairs;

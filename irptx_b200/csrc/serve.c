@@ -306,7 +306,7 @@ static int launch_append(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
     k.t0 = u0; k.t1 = u1;
     k.batch = c->batch; k.cols = c->cols; k.page_size = c->page_size; k.heads = c->heads;
     k.dv = c->dim / vb;
-    k.parts = (c->heads * k.dv + 127) / 128;
+    k.parts = (c->heads * k.dv + 32 * IRX_APPEND_VEC - 1) / (32 * IRX_APPEND_VEC);
     warps = (u1 - u0) * k.parts;
     if ((warps + 3) / 4 > MAX_COUNT) return irx_fail(E042, "an append past one launch's blocks");
     return irx_dev_launch(d, K_KV_APPEND + w, (unsigned)((warps + 3) / 4), 128, 0, 1, st, &k);
@@ -345,7 +345,7 @@ static int launch_copy(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsign
     k.p0 = u0; k.p1 = u1;
     k.run = run / vb;
     k.n1 = (int32_t)n1; k.n2 = (int32_t)n2; k.layers = a->layers;
-    k.tiles = (k.run * n1 * n2 + 1023) / 1024;
+    k.tiles = (k.run * n1 * n2 + IRX_COPY_TILE - 1) / IRX_COPY_TILE;
     want = (u1 - u0) * k.tiles * a->layers * 2;
     if (serve_grid(d, K_KV_COPY + w, 256, 0, want, &grid)) return 1;
     return irx_dev_launch(d, K_KV_COPY + w, (unsigned)grid, 256, 0, 1, st, &k);
