@@ -168,7 +168,7 @@ typedef struct {
 } irx_kcpy_t;
 
 /* 4-bit matrix-vector products: ring depth and shared memory by 8-column blocks of tokens. */
-#define IRX_MV4_STAGES 4
+#define IRX_MV4_STAGES 3
 #define IRX_MV4_SMEM(nt) (IRX_MV4_STAGES * (128 * 128 + (nt) * 8 * (512 + 64)) + 2 * 128 * (9 * 4 + 8) + 1024 + 64)
 
 typedef struct {
@@ -181,7 +181,7 @@ typedef struct {
     int64_t     m, n, k, x_stride, w_stride;
     int64_t     n0, n1;             /* rows of w of this launch */
     int32_t     group, groups;
-    int32_t     lck;                /* log2 of a cluster's blocks: slices of k */
+    int32_t     ck;                 /* blocks of a cluster, 1 to 8: slices of k */
     uint8_t     dt, sdt, gshift, pad;
     uint64_t    gmul;               /* group of k: (k / 32 * gmul) >> gshift */
 } irx_kmv4_t;

@@ -76,14 +76,7 @@ __device__ __forceinline__ void mv4_stage(uint32_t ws, const unsigned char *xs, 
     using M = Mv4Smem<NT>;
     constexpr int P = 128 / GV;                          // pieces of a warp's 128 k
     const int g = lane >> 2, t = lane & 3;
-    uint32_t w[2][2][4];
-#pragma unroll
-    for (int rt = 0; rt < 2; rt++)
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const int row = wr * 32 + rt * 16 + (lane & 15), ch = wk * 4 + j * 2 + (lane >> 4);
-            ldsm4(w[rt][j], ws + row * 128 + ((ch ^ (row & 7)) << 4));
-        }
+    uint32_t w[2][4];                                    // of two steps, both row tiles
 #pragma unroll
     for (int i = 0; i < P; i++) {
         float part[2][NT][4];
@@ -102,6 +95,13 @@ __device__ __forceinline__ void mv4_stage(uint32_t ws, const unsigned char *xs, 
 #pragma unroll
         for (int q = 0; q < 4 / P; q++) {
             const int step = i * (4 / P) + q;
+            if ((step & 1) == 0) {
+#pragma unroll
+                for (int rt = 0; rt < 2; rt++) {
+                    const int row = wr * 32 + rt * 16 + (lane & 15), ch = wk * 4 + step + (lane >> 4);
+                    ldsm4(w[rt], ws + row * 128 + ((ch ^ (row & 7)) << 4));
+                }
+            }
             uint32_t b[NT][4];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
@@ -114,8 +114,8 @@ __device__ __forceinline__ void mv4_stage(uint32_t ws, const unsigned char *xs, 
 #pragma unroll
             for (int rt = 0; rt < 2; rt++) {
                 uint32_t lo[4], hi[4];
-                mv4_unpack(w[rt][step >> 1][(step & 1) * 2], z[rt][0], lo);
-                mv4_unpack(w[rt][step >> 1][(step & 1) * 2 + 1], z[rt][1], hi);
+                mv4_unpack(w[rt][(step & 1) * 2], z[rt][0], lo);
+                mv4_unpack(w[rt][(step & 1) * 2 + 1], z[rt][1], hi);
                 const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]}, a1[4] = {lo[2], hi[2], lo[3], hi[3]};
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
@@ -151,11 +151,11 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
     unsigned char *sm = sm_raw + ((1024u - (irx_smem_u32(sm_raw) & 1023u)) & 1023u);   // the swizzle's period
     constexpr int ST = IRX_MV4_STAGES, COLS = NT * 8, TOK = F32 ? COLS / 3 : COLS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wr = warp & 3, wk = warp >> 2, g = lane >> 2, t = lane & 3;
-    const int lck = p.lck, ck = 1 << lck, rank = (int)blockIdx.x & (ck - 1);
-    const unsigned tile = blockIdx.x >> lck, nb = (unsigned)((p.n1 - p.n0 + 127) >> 7), mt = nb == 1 ? tile : tile / nb;
+    const int ck = p.ck, rank = (int)(blockIdx.x % (unsigned)ck);
+    const unsigned tile = blockIdx.x / (unsigned)ck, nb = (unsigned)((p.n1 - p.n0 + 127) >> 7), mt = nb == 1 ? tile : tile / nb;
     const int row0 = (int)p.n0 + (int)(tile - mt * nb) * 128, n1 = (int)p.n1, m0 = (int)mt * TOK, m_all = (int)p.m;
     // this block's stages: rank, rank + ck, ..., so that the cluster reads neighbouring bytes of a row at a time
-    const int k_all = (int)p.k, steps = (k_all + 255) >> 8, n_st = (steps - rank + ck - 1) >> lck;
+    const int k_all = (int)p.k, steps = (k_all + 255) >> 8, n_st = (steps - rank + ck - 1) / ck;
     float acc[2][NT][4];
 #pragma unroll
     for (int rt = 0; rt < 2; rt++)
@@ -319,7 +319,7 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
         if (half) __syncthreads();
     }
     if (ck > 1) cluster_sync(); else __syncthreads();
-    const int lrows = 7 - lck, rows = 1 << lrows, r0 = rank << lrows;
+    const int r0 = rank * ((127 + ck) / ck), rows = min((127 + ck) / ck, 128 - r0);   // (not below 0: ck is 8 at most)
     const float *fin = red + r0 * M::RS;
     if (ck > 1) {
         float *sum = red + 128 * M::RS;
@@ -337,7 +337,7 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
         fin = sum;
     }
     for (int i = tid; i < rows * TOK; i += MV4_WARPS * 32) {
-        const int r = i & (rows - 1), m = i >> lrows;
+        const int m = i / rows, r = i - m * rows;
         const float *a = fin + r * M::RS + (F32 ? 3 * m : m);
         const float v = F32 ? a[0] + (a[1] + a[2]) : a[0];
         if (row0 + r0 + r < n1 && m0 + m < m_all) irx_st1(p.y, p.dt, (int64_t)(m0 + m) * p.n + row0 + r0 + r, v);

@@ -47,6 +47,7 @@ typedef struct {
     CUfunction fn[K_COUNT];
     unsigned   smem_set[K_COUNT];      /* the dynamic shared memory limit last set per kernel */
     int        sms, smem_optin;
+    short      mv4_fit[12][2][9];      /* matvec4: clusters of 1 to 8 blocks that fit at 1, 2 blocks an SM (0: not asked) */
     int        occ[K_COUNT];           /* the serving kernels' resident blocks per SM (0: not asked yet) */
     CUdeviceptr scratch, err;
     unsigned    slot0;                 /* next scratch slot (under the launch lock) */

@@ -386,6 +386,40 @@ int irx_compile_matvec4(const irx_matvec4_t *m, irx_plan_t *plan)
     return finish(p);
 }
 
+/* How many slices of k, and how much shared memory. Up to two blocks an SM a block's speed is bound by its own
+ * latencies, so the most slices (a cluster's blocks, 1 to 8) whose clusters all fit at once. The GPU
+ * packs clusters as tightly as shared memory lets it, which leaves SMs idle when the grid does not
+ * fill it, so a launch asks for as much as keeps its blocks at the fewest an SM that hold them all.
+ * Measured (bf16, one token, 14336 k): 74 tiles in 4 slices at two an SM, where 71 clusters fit, 31 us, 71
+ * tiles 21.5; 64 tiles in 4 slices 20, in 2 slices 38. Three an SM measured slower where two fit (14337
+ * rows of 4096, 4 tokens: 17.0 us in 3 slices against 14.9 in 2). */
+static int mv4_split(irx_dev_t *d, int i, unsigned need, int64_t tiles, int64_t steps, unsigned *ck, unsigned *smem)
+{
+    unsigned r, c, best = 0;
+    *ck = 1;
+    *smem = need;
+    for (r = 1; r <= 2; r++) {
+        /* what an SM can share out (228 KB, 1 KB of it taken by each block) over r blocks */
+        unsigned room = (unsigned)(228 / r - 1) * 1024;
+        if (room > (unsigned)d->smem_optin) room = (unsigned)d->smem_optin;
+        if (room < need) break;
+        for (c = 1; c <= 8 && c <= steps; c++) {
+            short *fit = &d->mv4_fit[i][r - 1][c];
+            if (!*fit) {
+                int n = 1;
+                if (irx_dev_max_clusters(d, K_MV4 + i, 4096 * c, 256, room, c, &n)) return 1;
+                *fit = (short)(n < 32767 ? n : 32767);
+            }
+            if (tiles <= *fit && c > best) {
+                best = c;
+                *ck = c;
+                *smem = room;
+            }
+        }
+    }
+    return 0;
+}
+
 static int launch_mv4(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsigned ns, void *const *args, void *st)
 {
     const irx_mv4_t *a = &p->u.mv;
@@ -405,19 +439,18 @@ static int launch_mv4(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsigne
     k.err = (unsigned *)(size_t)d->err;
     if (a->k % 32 == 0 && a->group % 32 == 0 && a->w_stride % 16 == 0 && a_to(k.w, 16) && a->n * a->groups <= MAX_COUNT &&
         (a->dt == DT_F32 || (a->x_stride % 8 == 0 && a_to(k.x, 16)))) {
-        /* columns: one a token, three for f32 tokens; 8 or 16 of them at a time. The slices of k: as
-         * many blocks as fit the GPU at two an SM, in clusters of up to 8 */
+        /* columns: one a token, three for f32 tokens; 8 or 16 of them at a time */
         const int f32 = a->dt == DT_F32, gv = a->group % 128 == 0 ? 2 : a->group % 64 == 0 ? 1 : 0;
         const int nt = a->m > (f32 ? 2 : 8) ? 2 : 1, tok = f32 ? (nt == 1 ? 2 : 5) : 8 * nt;
         const int64_t tiles = ((u1 - u0 + 127) / 128) * ((a->m + tok - 1) / tok), steps = (a->k + 255) / 256;
-        int lck = 0;
-        while (lck < 3 && (tiles << (lck + 1)) <= 2 * d->sms && (2 << lck) <= steps) lck++;
-        if (tiles << lck > MAX_COUNT) return irx_fail(E042, "a matvec4 past one launch's blocks");
+        unsigned ck, smem;
+        if (mv4_split(d, 6 * f32 + gv * 2 + nt - 1, (unsigned)IRX_MV4_SMEM(nt), tiles, steps, &ck, &smem)) return 1;
+        if (tiles * ck > MAX_COUNT) return irx_fail(E042, "a matvec4 past one launch's blocks");
         const cuuint64_t dims[2] = {(cuuint64_t)a->k / 2, (cuuint64_t)u1}, strides[1] = {(cuuint64_t)a->w_stride};
         const cuuint32_t box[2] = {128, 128};
         if (irx_dev_tmap(&k.tma_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void *)(size_t)k.w, dims, strides, box,
                          CU_TENSOR_MAP_SWIZZLE_128B)) return 1;
-        k.lck = lck;
+        k.ck = (int32_t)ck;
         {   /* division by d = group / 32 of numbers below 2^26: ceil(2^(26 + l) / d), l = ceil(log2 d) */
             const uint64_t d32 = (uint64_t)a->group / 32;
             int l = 0;
@@ -425,7 +458,7 @@ static int launch_mv4(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsigne
             k.gshift = (uint8_t)(26 + l);
             k.gmul = ((1ull << (26 + l)) + d32 - 1) / d32;
         }
-        return irx_dev_launch(d, K_MV4 + 6 * f32 + gv * 2 + nt - 1, (unsigned)(tiles << lck), 256, IRX_MV4_SMEM(nt), 1u << lck, st, &k);
+        return irx_dev_launch(d, K_MV4 + 6 * f32 + gv * 2 + nt - 1, (unsigned)(tiles * ck), 256, smem, ck, st, &k);
     }
     if (serve_grid(d, K_MV4_ANY, 256, 0, ((u1 - u0) * ((a->m + 3) / 4) + 7) / 8, &grid)) return 1;
     return irx_dev_launch(d, K_MV4_ANY, (unsigned)grid, 256, 0, 1, st, &k);
