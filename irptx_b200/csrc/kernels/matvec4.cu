@@ -16,8 +16,9 @@
 // Which k an operand slot stands for does not matter as long as both operands agree, so each lane
 // keeps the order in which its bytes come (k0 with k4, k1 with k5, ...), and the tokens are
 // paired the same way with byte permutes. (tcgen05 with the unpacked weights in tensor memory as its
-// A operand measured no better, 28 us against 26 at the first size and 8.9 against 5.8 at the last: the unpacking is the same work,
-// and each chunk's hand-over to the one thread that issues products adds latency.)
+// A operand measured no better, 28 us against 26 at the first size and 8.9 against 5.8 at the last: the
+// unpacking is the same work, and each chunk's hand-over to the one thread that issues products
+// adds latency.)
 #pragma once
 #include "decode.cu"
 
@@ -40,9 +41,9 @@ __device__ __forceinline__ void mv4_unpack(uint32_t w, __nv_bfloat162 z, uint32_
 // row, with the tokens' values of those k, through a ring of asynchronous copies, so that bytes
 // are in flight whatever the warps do. Its 8 warps are 4 groups of 32 rows times 2 halves of a
 // stage. The weights of a stage come by one TMA copy, which also fills zeros past the ends and
-// swizzles the 16-byte pieces for ldmatrix. The slices of k of the same rows are a cluster's blocks, which add up through
-// distributed shared memory in a fixed order: that is how a matrix of few rows still fills the
-// GPU, with no workspace and the same bits every time.
+// swizzles the 16-byte pieces for ldmatrix. The slices of k of the same rows are a cluster's blocks,
+// which add up through distributed shared memory in a fixed order: that is how a matrix of few
+// rows still fills the GPU, with no workspace and the same bits every time.
 //
 // A stage's 16 bytes of a row are 32 weights; ldmatrix hands lane (g, t) the 8 weights t of row g, so
 // an instruction's four lanes always lie in one group of 32, whatever the group size is (GV: 128,

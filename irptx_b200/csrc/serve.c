@@ -15,6 +15,7 @@
 #define MAX_DIM 256
 #define MAX_COUNT 0x7fffffffll
 #define MAX_STRIDE (1ll << 40)
+#define MAX_32 (1ll << 30)
 
 static int esz(int dt) { return dt == DT_BF16 ? 2 : dt == DT_U8 ? 1 : 4; }
 
@@ -24,7 +25,10 @@ static irx_plan_int_t *begin(irx_plan_t *plan, int fam, const char *name)
 {
     irx_plan_int_t *p = (irx_plan_int_t *)plan;
     irx_clear_error();
-    if (!plan) { irx_fail(E093, "a compile with no plan storage"); return NULL; }
+    if (!plan) {
+        irx_fail(E093, "a compile with no plan storage");
+        return NULL;
+    }
     memset(plan, 0, sizeof *plan);
     p->fam = (uint8_t)fam;
     snprintf(p->kname, sizeof p->kname, "%s", name);
@@ -437,8 +441,10 @@ static int launch_mv4(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsigne
     k.group = a->group; k.groups = a->groups;
     k.dt = a->dt; k.sdt = a->sdt;
     k.err = (unsigned *)(size_t)d->err;
-    if (a->k % 32 == 0 && a->group % 32 == 0 && a->w_stride % 16 == 0 && a_to(k.w, 16) && a->n * a->groups <= MAX_COUNT &&
-        (a->dt == DT_F32 || (a->x_stride % 8 == 0 && a_to(k.x, 16)))) {
+    /* the kernels below count rows, tokens and k in 32 bits, some of them past the end */
+    if (a->m <= MAX_32 && a->n <= MAX_32 && a->k <= MAX_32 && a->n * a->groups <= MAX_COUNT && a->k % 32 == 0 &&
+        a->group % 32 == 0 && a->w_stride % 16 == 0 && a_to(k.w, 16) && (a->dt == DT_F32 ||
+        (a->x_stride % 8 == 0 && a_to(k.x, 16)))) {
         /* columns: one a token, three for f32 tokens; 8 or 16 of them at a time */
         const int f32 = a->dt == DT_F32, gv = a->group % 128 == 0 ? 2 : a->group % 64 == 0 ? 1 : 0;
         const int nt = a->m > (f32 ? 2 : 8) ? 2 : 1, tok = f32 ? (nt == 1 ? 2 : 5) : 8 * nt;

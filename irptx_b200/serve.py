@@ -139,13 +139,16 @@ class OpPlan(_irx.Plan):
             return args.arr
         if len(args) != len(self.args):
             _refuse(93, f"a launch with {len(args)} args; the plan has {len(self.args)}")
-        out = []
+        out, device = [], None
         for a, x in zip(self.args, args):
             if isinstance(x, int):
                 out.append(x)
                 continue
-            if not x.is_cuda:
-                _refuse(93, f"arg {a.name}: a tensor on {x.device}, not on a GPU")
+            if device is None and x.is_cuda:
+                import torch
+                device = torch.cuda.current_device()
+            if not x.is_cuda or x.get_device() != device:
+                _refuse(93, f"arg {a.name}: a tensor on {x.device}, not on the current GPU")
             if str(x.dtype) != _TORCH[a.dtype]:
                 _refuse(93, f"arg {a.name}: dtype {x.dtype}, the plan says {a.dtype}")
             if tuple(x.shape) != a.shape:
