@@ -114,14 +114,14 @@ typedef struct {
 /* Ring depth, 16-key blocks of a warp's tile and shared memory of the two decode kernels, by padded head
  * size and query rows of a work unit (the launcher and the kernels agree on them; the share is the
  * block's part of the work). */
-#define IRX_DEC_SHARE 256
+#define IRX_DEC_SHARE 320
 #define IRX_DEC_TC_KM(dp) ((dp) == 64 ? 2 : 1)
 #define IRX_DEC_TC_ST(dp, nt) ((dp) == 256 || ((dp) == 128 && (nt) == 2) ? 2 : 3)
-#define IRX_DEC_ST_ST(dp) ((dp) == 256 ? 1 : 2)
+#define IRX_DEC_ST_NW(dp) ((dp) == 256 ? 8 : 16)
 #define IRX_DEC_TC_SMEM(dp, nt, km, st) (4 * (st) * 2 * 16 * (km) * (dp) * 2 + 2 * 8 * ((dp) + 4) * 4 + 4 * 8 * (nt) * 8 + \
                                          IRX_DEC_SHARE + 4 * (st) * 192 * (km))
-#define IRX_DEC_ST_SMEM(dp, rows, st) (8 * (st) * 8 * (2 * (dp) + 16) * 4 + 8 * (rows) * (dp) * 4 + (rows) * (dp) * 4 + \
-                                       8 * (rows) * 8 * 4 + 8 * (rows) * 8 + IRX_DEC_SHARE + 8 * (st) * 96)
+#define IRX_DEC_ST_SMEM(dp, rows, st) (IRX_DEC_ST_NW(dp) * ((st) * 8 * (2 * (dp) + 16) * 4 + (rows) * (dp) * 4 + 8 * (rows) * 4 + \
+                                       8 * (rows) + (st) * 96) + (rows) * (dp) * 4 + IRX_DEC_SHARE)
 
 typedef struct {
     const void *q, *k, *v;

@@ -83,7 +83,7 @@ __device__ __forceinline__ bool dec_sees(const DecCur &c, int pos) { return pos 
 
 struct DecShare {
     long long c0, c1, q;              // this block's chunks; the first r blocks have q + 1, the others q
-    long long wsum[8];                // a warp each
+    long long wsum[16];               // a warp each
     int geff, r, b, u, j;
     int last[2];
     // the shares of units that other blocks hold too: [0] the one that began before this block, [1] the
@@ -771,22 +771,22 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
 }
 
 // ---- f32, and rows that cannot be moved 16 bytes at a time: FP32 units ----
-// The same cut of the work with 8 warps of 8 keys. A warp's four lanes per key each take every
+// The same cut of the work with 16 warps of 8 keys (8 at head size 256), one tile each: the warps cover each
+// other's waits (with 8 warps and two tiles each, 181 us against 132 for six sequences of 30k tokens). A warp's four lanes per key each take every
 // fourth 16 bytes of the key's row for all query rows (the rows sit in shared memory and are
 // broadcast), then every lane owns DP/32 dims of the accumulators and reads the values' rows
 // across. f32 products and sums throughout.
-#define DEC_ST_WARPS 8
 
 template <int DP, int ROWS, int ST>
 struct DecSt {
-    static constexpr int THREADS = DEC_ST_WARPS * 32, K = DEC_ST_WARPS * 8, KS = DP + 16;
+    static constexpr int NW = IRX_DEC_ST_NW(DP), THREADS = NW * 32, K = NW * 8, KS = DP + 16;
     static constexpr int TILE = 8 * (KS + DP) * 4;
-    static constexpr int RING = DEC_ST_WARPS * ST * TILE;
-    static constexpr int MERGE = DEC_ST_WARPS * ROWS * DP * 4;
+    static constexpr int RING = NW * ST * TILE;
+    static constexpr int MERGE = NW * ROWS * DP * 4;
     static constexpr int Q = ROWS * DP * 4;
-    static constexpr int PB = DEC_ST_WARPS * ROWS * 8 * 4;
-    static constexpr int ML = DEC_ST_WARPS * ROWS * 8;
-    static constexpr int SMEM = RING + MERGE + Q + PB + ML + IRX_DEC_SHARE + DEC_ST_WARPS * ST * (int)sizeof(DecRows<8>);
+    static constexpr int PB = NW * ROWS * 8 * 4;
+    static constexpr int ML = NW * ROWS * 8;
+    static constexpr int SMEM = RING + MERGE + Q + PB + ML + IRX_DEC_SHARE + NW * ST * (int)sizeof(DecRows<8>);
     static_assert(SMEM == IRX_DEC_ST_SMEM(DP, ROWS, ST), "the launcher's shared memory size");
 };
 
@@ -888,7 +888,7 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
                 float s[ROWS];
 #pragma unroll
                 for (int r = 0; r < ROWS; r++) s[r] = 0.0f;
-#pragma unroll 4
+#pragma unroll (ROWS / 4)
                 for (int i = 0; i < DP / 16; i++) {
                     const float4 k4 = *reinterpret_cast<const float4 *>(kt + key * T::KS + (4 * i + quarter) * 4);
 #pragma unroll
@@ -970,7 +970,7 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
                 for (int r = 0; r < ROWS; r++) {
                     float M = -INFINITY;
 #pragma unroll
-                    for (int w = 0; w < DEC_ST_WARPS; w++) M = fmaxf(M, wml[w * ROWS + r].x);
+                    for (int w = 0; w < T::NW; w++) M = fmaxf(M, wml[w * ROWS + r].x);
                     const float f = exp2f(m[r] - (M == -INFINITY ? 0.0f : M));
 #pragma unroll
                     for (int j = 0; j < NJ * VW; j++)
@@ -980,16 +980,16 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
                 for (int it = threadIdx.x; it < ROWS * DP; it += T::THREADS) {
                     float a = 0.0f;
 #pragma unroll
-                    for (int w = 0; w < DEC_ST_WARPS; w++) a += merge[w * ROWS * DP + it];
+                    for (int w = 0; w < T::NW; w++) a += merge[w * ROWS * DP + it];
                     qs[it] = a;                                  // the query rows are done with
                 }
                 __syncthreads();
                 auto ml = [&](int r) {
                     float M = -INFINITY, L = 0.0f;
 #pragma unroll
-                    for (int w = 0; w < DEC_ST_WARPS; w++) M = fmaxf(M, wml[w * ROWS + r].x);
+                    for (int w = 0; w < T::NW; w++) M = fmaxf(M, wml[w * ROWS + r].x);
 #pragma unroll
-                    for (int w = 0; w < DEC_ST_WARPS; w++) {
+                    for (int w = 0; w < T::NW; w++) {
                         const float2 x = wml[w * ROWS + r];
                         L += x.y * exp2f(x.x - (M == -INFINITY ? 0.0f : M));
                     }
@@ -1013,8 +1013,8 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
     extern "C" __global__ void __launch_bounds__(DEC_TC_WARPS * 32) irx_dec_tc_##DP##_##NT(const __grid_constant__ irx_kdec_t p) \
     { dec_tc_body<DP, NT, IRX_DEC_TC_KM(DP), IRX_DEC_TC_ST(DP, NT)>(p); }
 #define DEC_STK(DP, ROWS) \
-    extern "C" __global__ void __launch_bounds__(DEC_ST_WARPS * 32) irx_dec_st_##DP##_##ROWS(const __grid_constant__ irx_kdec_t p) \
-    { dec_st_body<DP, ROWS, IRX_DEC_ST_ST(DP)>(p); }
+    extern "C" __global__ void __launch_bounds__(IRX_DEC_ST_NW(DP) * 32) irx_dec_st_##DP##_##ROWS(const __grid_constant__ irx_kdec_t p) \
+    { dec_st_body<DP, ROWS, 1>(p); }
 
 DEC_TC(64, 1) DEC_TC(64, 2) DEC_TC(128, 1) DEC_TC(128, 2) DEC_TC(256, 1)
 DEC_STK(64, 4) DEC_STK(64, 8) DEC_STK(128, 4) DEC_STK(128, 8) DEC_STK(256, 4) DEC_STK(256, 8)

@@ -177,7 +177,7 @@ static int launch_decode(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
     const int es = esz(a->c.dt), al = 16 / es, last = p->narg - 1;
     long long u0, u1;
     int64_t grid;
-    int rows, kk, st_;
+    int rows, kk, st_, block = 128;
     size_t smem;
     float scale;
     memset(&k, 0, sizeof k);
@@ -221,10 +221,11 @@ static int launch_decode(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
         smem = (size_t)IRX_DEC_TC_SMEM(a->dp, nt, IRX_DEC_TC_KM(a->dp), IRX_DEC_TC_ST(a->dp, nt));
     } else {
         kk = K_DEC_ST + (a->dp == 64 ? 0 : a->dp == 128 ? 2 : 4) + (rows == 8);
-        smem = (size_t)IRX_DEC_ST_SMEM(a->dp, rows, IRX_DEC_ST_ST(a->dp));
+        smem = (size_t)IRX_DEC_ST_SMEM(a->dp, rows, 1);
+        block = 32 * IRX_DEC_ST_NW(a->dp);
     }
-    if (serve_grid(d, kk, st_ ? 256 : 128, smem, a->max_ctas, &grid)) return 1;
-    return irx_dev_launch(d, kk, (unsigned)grid, st_ ? 256 : 128, (unsigned)smem, 1, st, &k);
+    if (serve_grid(d, kk, block, smem, a->max_ctas, &grid)) return 1;
+    return irx_dev_launch(d, kk, (unsigned)grid, (unsigned)block, (unsigned)smem, 1, st, &k);
 }
 
 /* ---- the cache's moves ---- */
