@@ -173,10 +173,10 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
     irx_pdl_enter();
     __syncthreads();
 
-    auto fetch = [&](int s) {                            // stage s into its slot, by one thread
+    auto fetch = [&](int s, int slot) {                  // stage s into its slot, by one thread
         if (tid == 0 && s < n_st) {
-            irx_mbar_expect_tx(full + s % ST, M::W);
-            tma_load_2d(sm + (s % ST) * M::W, &p.tma_w, (s * ck + rank) * 128, row0, full + s % ST);
+            irx_mbar_expect_tx(full + slot, M::W);
+            tma_load_2d(sm + slot * M::W, &p.tma_w, (s * ck + rank) * 128, row0, full + slot);
         }
     };
     // The tokens' part, a stage ahead in registers, stored in the order in which the weights unpack: bf16 8
@@ -207,8 +207,8 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
         xk += ck * 256;
         xsrc += xadv;
     };
-    auto xstore = [&](int s) {
-        unsigned char *st = sm + M::RING + (s % ST) * M::X;
+    auto xstore = [&](int slot) {
+        unsigned char *st = sm + M::RING + slot * M::X;
         if (F32) {
             const int k8 = tid & 7;
             st += ((tid & ~7) + (k8 < 4 ? 2 * k8 : 2 * k8 - 7)) * 2;
@@ -271,7 +271,7 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
         __syncthreads();
     }
 #pragma unroll
-    for (int i = 0; i < ST - 1; i++) fetch(i);
+    for (int i = 0; i < ST - 1; i++) fetch(i, i);
     sload(0);
     xload();
     sstore(0);
@@ -279,11 +279,13 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
     xstore(0);
     xload();
     int ok = 1;
+    int slot = 0;
+    unsigned phase = 0;
     for (int c = 0; c < n_st; c++) {
-        const int slot = c % ST, run = c / RUN, sub = c % RUN;
-        ok = ok && irx_mbar_wait(full + slot, (c / ST) & 1);
+        const int run = c / RUN, sub = c % RUN, next = slot + 1 == ST ? 0 : slot + 1;
+        ok = ok && irx_mbar_wait(full + slot, phase);
         __syncthreads();                                 // tokens and scales are there too; the stage before is free
-        fetch(c + ST - 1);
+        fetch(c + ST - 1, slot ? slot - 1 : ST - 1);
         mv4_stage<GV, NT>(irx_smem_u32(sm) + slot * M::W, sm + M::RING + slot * M::X,
                           scales + (run & 1) * (128 * 9) + sub * (2 * P) + wk * P,
                           p.z ? zeros + (run & 1) * (128 * 8) + sub * (2 * P) + wk * P : nullptr, wr, wk, lane, acc);
@@ -292,9 +294,11 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
                 sstore(run + 1);
                 sload(run + 2);
             }
-            xstore(c + 1);
+            xstore(next);
             xload();
         }
+        slot = next;
+        phase ^= next == 0;
     }
     if (!ok) {                                           // a wait ran out: report it, and let copies in flight land
         irx_flag(p.err, IRX_KERR_TIMEOUT);
