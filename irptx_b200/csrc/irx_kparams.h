@@ -169,7 +169,7 @@ typedef struct {
 
 /* 4-bit matrix-vector products: ring depth and shared memory by 8-column blocks of tokens. */
 #define IRX_MV4_STAGES 3
-#define IRX_MV4_SMEM(nt) (IRX_MV4_STAGES * (128 * 128 + (nt) * 8 * (512 + 64)) + 2 * 128 * (9 * 4 + 8) + 1024 + 64)
+#define IRX_MV4_SMEM(nt) (IRX_MV4_STAGES * (128 * 128 + (nt) * 8 * (512 + 64)) + 2 * 128 * (9 * 4 + ((nt) == 1 ? 9 * 4 : 8)) + 1024 + 64)
 
 typedef struct {
     CUtensorMap tma_w;              /* w's bytes of this launch's rows, in boxes of 128 x 128 */

@@ -7,7 +7,7 @@
 // operations, 3 shifts and 4 subtractions whatever m is, and with 9 to 16 tokens the matrix pipe
 // (a quarter busy) and the logic pipe (a third) are each used in bursts by the few warps that fit. A
 // call of a few megabytes is bound by latency. Measured, bf16: [13 x 14336] x [8192 x 14336] (61 MB)
-// 24.8 us, 2.5 TB/s; [4 x 4096] x [14337 x 4096] with zero points 14.9 us; one token, 4096 x 4096, 6.0 us.
+// 24.3 us, 2.5 TB/s; [4 x 4096] x [14337 x 4096] with zero points 14.6 us; one token, 4096 x 4096, 6.0 us.
 //
 // The products run on matrix instructions with the weights as the wide operand (16 rows of w) and
 // the tokens as the narrow one (8). A weight becomes the exact bf16 number q - z: the
@@ -20,6 +20,7 @@
 // unpacking is the same work, and each chunk's hand-over to the one thread that issues products
 // adds latency.)
 #pragma once
+#include <type_traits>
 #include "decode.cu"
 
 #define MV4_WARPS 8
@@ -54,9 +55,12 @@ __device__ __forceinline__ void mv4_unpack(uint32_t w, __nv_bfloat162 z, uint32_
 // the three columns' sums are added at the end.
 template <int NT>
 struct Mv4Smem {
+    // zero points: as the pairs that are subtracted where there is room, bytes with 16 columns
+    using Zero = typename std::conditional<NT == 1, uint32_t, unsigned char>::type;
+    static constexpr int ZB = (int)sizeof(Zero), ZS = NT == 1 ? 9 : 8;
     static constexpr int XS = 512 + 64;                  // bytes of a column's stage: 64 off the banks' period
     static constexpr int W = 128 * 128, X = NT * 8 * XS, RING = W * IRX_MV4_STAGES, SCALES = RING + X * IRX_MV4_STAGES;
-    static constexpr int ZEROS = SCALES + 2 * 128 * 9 * 4, BARS = ZEROS + 2 * 128 * 8;
+    static constexpr int ZEROS = SCALES + 2 * 128 * 9 * 4, BARS = ZEROS + 2 * 128 * ZS * ZB;
     static_assert(BARS + 1024 + 64 == IRX_MV4_SMEM(NT), "the launcher's shared memory size");
     static constexpr int RS = NT * 8 + 4;                // floats of a row of the sums
     static_assert(2 * 128 * RS * 4 <= SCALES, "the sums fit the ring");
@@ -71,7 +75,7 @@ __device__ __forceinline__ void mma_16816_first(float (&c)[4], const uint32_t (&
 }
 
 template <int GV, int NT>
-__device__ __forceinline__ void mv4_stage(uint32_t ws, const unsigned char *xs, const float *sc, const unsigned char *zp, int wr, int wk, int lane,
+__device__ __forceinline__ void mv4_stage(uint32_t ws, const unsigned char *xs, const float *sc, const typename Mv4Smem<NT>::Zero *zp, int wr, int wk, int lane,
                                           float (&acc)[2][NT][4])
 {
     using M = Mv4Smem<NT>;
@@ -88,9 +92,12 @@ __device__ __forceinline__ void mv4_stage(uint32_t ws, const unsigned char *xs, 
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int row = wr * 32 + rt * 16 + h * 8 + g;
-                const unsigned zz = zp ? zp[row * 8 + i] : 8u;
+                uint32_t zb = 0x43084308u;               // 128 + 8
+                if (zp) {
+                    zb = zp[row * M::ZS + i];
+                    if (NT > 1) zb = 0x43004300u | ((zb & 15u) * 0x00010001u);
+                }
                 s[rt][h] = sc[row * 9 + i];
-                const uint32_t zb = 0x43004300u | ((zz & 15u) * 0x00010001u);
                 z[rt][h] = *reinterpret_cast<const __nv_bfloat162 *>(&zb);
             }
 #pragma unroll
@@ -236,7 +243,7 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
     // each stage took as long as half the products.
     constexpr int P = 128 / GV, RUN = 4 / P;
     float *scales = reinterpret_cast<float *>(sm + M::SCALES);
-    unsigned char *zeros = sm + M::ZEROS;
+    typename M::Zero *zeros = reinterpret_cast<typename M::Zero *>(sm + M::ZEROS);
     uint32_t sr[4], zr[4];
     uint32_t at[4];                                      // rows past the end read the last row's: their sums go nowhere
 #pragma unroll
@@ -263,7 +270,7 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
         for (int i = 0; i < 4; i++) {
             const int row = (r & 1) * 128 + (tid >> 3) + 32 * i;
             scales[row * 9 + (tid & 7)] = __uint_as_float(sr[i] << shift);
-            if (p.z) zeros[row * 8 + (tid & 7)] = (unsigned char)zr[i];
+            if (p.z) zeros[row * M::ZS + (tid & 7)] = (typename M::Zero)(NT == 1 ? 0x43004300u | ((zr[i] & 15u) * 0x00010001u) : zr[i]);
         }
     };
     if (F32) {                                           // columns that no token has stay zero
@@ -288,7 +295,7 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
         fetch(c + ST - 1, slot ? slot - 1 : ST - 1);
         mv4_stage<GV, NT>(irx_smem_u32(sm) + slot * M::W, sm + M::RING + slot * M::X,
                           scales + (run & 1) * (128 * 9) + sub * (2 * P) + wk * P,
-                          p.z ? zeros + (run & 1) * (128 * 8) + sub * (2 * P) + wk * P : nullptr, wr, wk, lane, acc);
+                          p.z ? zeros + (run & 1) * (128 * M::ZS) + sub * (2 * P) + wk * P : nullptr, wr, wk, lane, acc);
         if (c + 1 < n_st) {
             if (sub == RUN - 1) {
                 sstore(run + 1);
