@@ -8,8 +8,8 @@
 // Bound: every visible key and value row is read once and takes 4 * group operations per
 // element, so HBM bounds it (group operations a byte in bf16). The work is therefore cut by
 // keys, not by rows: the visible keys of all (sequence, kv head, row block) units are laid end to
-// end in chunks of IRX_DEC_KEYS keys and the chunks are dealt out evenly, a contiguous range to
-// each block of one resident wave, whatever the lengths are. A block whose range covers a whole
+// end in chunks of 64 or 128 keys and the chunks are dealt out evenly, a contiguous range to each
+// block of one resident wave, whatever the lengths are. A block whose range covers a whole
 // unit writes its output; a unit that several blocks share is joined by the last of them to
 // arrive, which folds the blocks' partials in key order, so the result does not depend on which
 // block that was. Past DEC_JOIN partials they are folded in groups first, by the last block of
@@ -27,8 +27,9 @@
 #define DEC_JOIN 16
 
 // A place in the laid-out chunks: chunk j of the unit (kv head h0 + h, row block rb) of sequence b. A
-// chunk is a block of K positions (what a block of threads takes in one step): the first `cs` of a sequence's chunks are the blocks that
-// hold sinks, the others the blocks from wb on; keys outside the mask are dropped in their tile.
+// chunk is K positions from a multiple of K (what a thread block takes in one step): the first `cs`
+// of a sequence's chunks are those that hold sinks, the others those from number wb on; keys outside
+// the mask are dropped in their tile.
 struct DecCur {
     int b, h, rb, j;
     int nch, n, lo, sk, cs, wb;       // of sequence b: chunks, tokens, window start, sinks before it
@@ -410,9 +411,9 @@ __device__ __forceinline__ long long dec_row(const irx_kdec_t &p, const DecRows<
 // ---- bf16: matrix instructions ----
 // The transposed products: S^T[16 keys x 8 rows] = K Q^T and O^T[16 dims x 8 rows] += V^T P^T, so that
 // the few query rows sit on the instruction's narrow side (8) and keys or dims on its wide one.
-// S^T's accumulators become P^T's operand by an 8x8 transpose across the warp. Each warp
-// owns 16 keys of a chunk (32 at head size 64, where 16 are too little work for what a tile costs) and its own ring of ST tiles filled by 16-byte asynchronous copies, so
-// warps meet only where a unit ends. mma.sync runs far below tcgen05's rate, but at 8 to 16 rows
+// S^T's accumulators become P^T's operand by an 8x8 transpose across the warp. Each warp owns 16
+// keys of a chunk (32 at head size 64, where 16 are too little work for what a tile costs) and its
+// own ring of ST tiles filled by 16-byte asynchronous copies, so warps meet only where a unit ends. mma.sync runs far below tcgen05's rate, but at 8 to 16 rows
 // the products take 16 to 32 instructions per 8 KB (D = 128), which HBM delivers in about 360
 // cycles per SM: the tensor pipe is idle most of the time and tcgen05's 128-row tiles would be
 // filled with padding.
@@ -466,8 +467,7 @@ template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.as
 template <int DP, int NT, int KM, int ST>
 struct DecTc {
     static constexpr int THREADS = DEC_TC_WARPS * 32, ROWS = 8 * NT, KEYS = 16 * KM, K = DEC_TC_WARPS * KEYS, TILE = KEYS * DP * 2, QS = DP + 4;
-    // ring, then one 8-row block of two warps' accumulators then
-    // (max, sum) pairs, the share and the rings' row places
+    // ring, one 8-row block of two warps' accumulators, (max, sum) pairs, the share, the rings' row places
     static constexpr int RING = DEC_TC_WARPS * ST * 2 * TILE;
     static constexpr int MERGE = DEC_TC_WARPS / 2 * 8 * QS * 4;
     static constexpr int ML = DEC_TC_WARPS * ROWS * 8;
@@ -477,7 +477,8 @@ struct DecTc {
     static_assert(sizeof(DecShare) <= IRX_DEC_SHARE, "shared memory");
 };
 
-// A tile, 16 KM keys, lies in 64-dim columns of 128 bytes a key, 16-byte pieces swizzled by row against bank conflicts.
+// A tile, 16 KM keys, lies in 64-dim columns of 128 bytes a key, 16-byte pieces swizzled by row against
+// bank conflicts.
 // (Filling tiles by TMA, a page's 8 or 16 rows a box, measured no better: 171 against 164 us for two
 // sequences of 125k tokens, 54 against 52 for 31 of 2k.)
 template <int DP, int NT, int KM, int ST>
@@ -771,11 +772,12 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
 }
 
 // ---- f32, and rows that cannot be moved 16 bytes at a time: FP32 units ----
-// The same cut of the work with 16 warps of 8 keys (8 at head size 256), one tile each: the warps cover each
-// other's waits (with 8 warps and two tiles each, 181 us against 132 for six sequences of 30k tokens). A warp's four lanes per key each take every
-// fourth 16 bytes of the key's row for all query rows (the rows sit in shared memory and are
-// broadcast), then every lane owns DP/32 dims of the accumulators and reads the values' rows
-// across. f32 products and sums throughout.
+// The same cut of the work with 16 warps of 8 keys (8 warps at head size 256), a tile each: the warps
+// cover each other's waits (8 warps with two tiles each took 181 us against 132 for six sequences
+// of 30k tokens, 4 f32 heads of 128, 738 MB: 5.6 TB/s). A warp's four lanes per key each take every fourth 16
+// bytes of the key's row for all query rows (the rows sit in shared memory and are broadcast),
+// then every lane owns DP/32 dims of the accumulators and reads the values' rows across. f32
+// products and sums throughout; with 8 rows a unit they bound it (222 us there).
 
 template <int DP, int ROWS, int ST>
 struct DecSt {
