@@ -141,8 +141,8 @@ IRX_API int irx_compile_kv_append(const irx_kv_cache_t *cache, long long tokens,
 
 /* Page copy, in both pools and in `layers` layers whose pools lie layer_stride elements apart
  * (0: packed): for each pair (src, dst), page dst becomes a copy of page src. (-1, -1) is padding. A
- * page must not be the destination of one pair and in another pair of the launch; irx_pages
- * makes such lists. Args: pairs int32 [pairs, 2], k pools, v pools (updated in place). Units: pairs. */
+ * page must not be the destination of one pair and in another pair of the launch (irx_pages
+ * makes such lists, below). Args: pairs int32 [pairs, 2], k pools, v pools (updated in place). Units: pairs. */
 IRX_API int irx_compile_kv_copy(const irx_kv_cache_t *cache, long long pairs, int layers, long long layer_stride, irx_plan_t *plan);
 
 /* y[m, n] = sum over k of x[m, k] * s[n, k / group] * (q[n, k] - z[n, k / group]).
@@ -160,15 +160,21 @@ typedef struct irx_matvec4 {
 IRX_API int irx_compile_matvec4(const irx_matvec4_t *desc, irx_plan_t *plan);
 
 /* The host side of a paged cache: pages handed out, shared by forks, copied when a shared page is
- * written to, returned and compacted. It keeps numbers only; the caller uploads irx_pages_table
- * (int32 [max_seqs, table_cols], -1 where nothing is held) and runs the (src, dst) pairs through
- * a plan of irx_compile_kv_copy before the launches that follow. One owner; not thread-safe.
+ * written to, returned and compacted. It keeps numbers only. A step calls what it needs, gathers the
+ * (src, dst) pairs that the calls return, then calls irx_pages_table (int32 [max_seqs, table_cols], -1
+ * where nothing is held) to upload it, and runs the pairs through a plan of irx_compile_kv_copy
+ * before its other launches. The pairs returned between two calls of irx_pages_table may run in one
+ * launch or in any order; they run before those returned later. Call it at every upload: until it is
+ * called, pages of those pairs are not handed out again even when nobody holds them. A copy carries
+ * what its source holds: queue a sequence's appends before its forks are extended. One owner; not
+ * thread-safe.
  * irx_pages_new, _table: NULL on failure. irx_pages_open, _fork: the new sequence's row, or -1.
  * irx_pages_extend grows a sequence by `tokens` (all or nothing; E094 when the pool is out of
  * pages) and sets pair to the copy its first new token needs, or (-1, -1). irx_pages_close returns
- * a sequence's pages. irx_pages_compact moves the live pages to the front of the pool and returns
- * how many moves it wrote into `pairs` (at most cap), or -1 with nothing changed. irx_pages_len
- * is -1 for a sequence that is not open. */
+ * a sequence's pages. irx_pages_compact moves the live pages to the front of the pool (past those that
+ * gathered pairs keep: called right after irx_pages_table, to its very front) and returns
+ * how many moves it wrote into `pairs` (at most cap), or -1 with nothing changed. irx_pages_free: pages
+ * that can be handed out now. irx_pages_len is -1 for a sequence that is not open. */
 typedef struct irx_pages irx_pages_t;
 IRX_API irx_pages_t *irx_pages_new(int pages, int page_size, int max_seqs, int table_cols);
 IRX_API void irx_pages_delete(irx_pages_t *m);
@@ -179,7 +185,7 @@ IRX_API int irx_pages_close(irx_pages_t *m, int seq);
 IRX_API int irx_pages_compact(irx_pages_t *m, int *pairs, int cap);
 IRX_API int irx_pages_free(const irx_pages_t *m);
 IRX_API int irx_pages_len(const irx_pages_t *m, int seq);
-IRX_API const int *irx_pages_table(const irx_pages_t *m);
+IRX_API const int *irx_pages_table(irx_pages_t *m);
 
 /* How many independent shard units the plan has: elements/8 (pointwise), rows (reductions,
  * row ops), 256-column blocks (matmul), batch*head (attention), element blocks (full sum); the

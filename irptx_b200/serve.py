@@ -247,8 +247,12 @@ def pack4(q):
 
 class Pages:
     """The host side of a paged cache (``irx_pages_*``): which pages each sequence holds, shared by
-    forks and copied when a shared page is written to. It keeps numbers only: upload :attr:`table`
-    and run the returned (src, dst) pairs through :func:`kv_copy` before the launches that follow."""
+    forks and copied when a shared page is written to. It keeps numbers only: a step gathers the (src,
+    dst) pairs that its calls return, reads :attr:`table` to upload it, and runs the pairs through
+    :func:`kv_copy` before its other launches. The pairs returned between two readings of the table
+    may run in one launch or in any order; pages of theirs that nobody holds any more are free again
+    once the table has been read. A copy carries what its source holds: queue a sequence's appends
+    before its forks are extended."""
 
     def __init__(self, pages: int, page_size: int, max_seqs: int, table_cols: int):
         self._h = None
@@ -292,7 +296,8 @@ class Pages:
 
     def compact(self):
         """Move the live pages to the front of the pool: the (src, dst) copies that have to run before
-        the table is used again (every destination was free)."""
+        the table is used again (every destination was free). Pages of pairs returned since the table
+        was last read stay where they are: read it first for a pool without holes."""
         buf = (ctypes.c_int * (2 * self.pages))()
         n = _irx._lib().irx_pages_compact(self._h, buf, self.pages)
         if n < 0:
@@ -301,6 +306,7 @@ class Pages:
 
     @property
     def free(self) -> int:
+        """Pages that can be handed out now."""
         return int(_irx._lib().irx_pages_free(self._h))
 
     def length(self, seq: int) -> int:
@@ -309,7 +315,8 @@ class Pages:
 
     @property
     def table(self):
-        """A copy of the page table, int32 [max_seqs, table_cols], -1 where nothing is held."""
+        """A copy of the page table, int32 [max_seqs, table_cols], -1 where nothing is held. Reading it
+        ends a step's gathering: the pairs returned before run before those returned after."""
         import numpy as np
         t = _irx._lib().irx_pages_table(self._h)
         return np.ctypeslib.as_array(t, (self.max_seqs, self.table_cols)).astype(np.int32)
