@@ -76,6 +76,8 @@ class KvCache:
         if len(strides) != 3:
             _refuse(42, "cache strides that are not three numbers")
         self.strides = tuple(_int("stride", s, 62) for s in strides)
+        if self.strides == (0, 0, 0) and max(self.pages, self.heads, self.page_size) > 1:      # the ABI's word for packed
+            _refuse(41, "a cache whose strides make rows overlap")
         self.shape = (self.pages,) + inner + (self.head_dim,)
 
     def _desc(self) -> _CacheDesc:
