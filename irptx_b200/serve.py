@@ -71,12 +71,13 @@ class KvCache:
         self.heads, self.head_dim, self.page_size = _int("heads", heads), _int("head_dim", head_dim), _int("page_size", page_size)
         self.pages, self.batch, self.table_cols = _int("pages", pages), _int("batch", batch), _int("table_cols", table_cols)
         inner = (self.heads, self.page_size) if order == "head" else (self.page_size, self.heads)
-        if strides is not None and not any(strides) and max(self.pages, self.heads, self.page_size) > 1:
-            _refuse(41, "a cache whose strides make rows overlap")        # (to the C ABI three zeros mean packed)
-        if strides is None:
+        given = strides is not None
+        if not given:
             strides = (inner[0] * inner[1] * self.head_dim, inner[1] * self.head_dim, self.head_dim)
         if len(strides) != 3:
             _refuse(42, "cache strides that are not three numbers")
+        if given and not any(strides) and max(self.pages, self.heads, self.page_size) > 1:
+            _refuse(41, "a cache whose strides make rows overlap")        # (to the C ABI three zeros mean packed)
         self.strides = tuple(_int("stride", s, 62) for s in strides)
         self.shape = (self.pages,) + inner + (self.head_dim,)
 

@@ -14,3 +14,8 @@ def test_three_zero_strides_are_an_overlap(irx, order):
         refused(irx, 41, build, **k)
     for p in build(pages=1, heads=1, page_size=1):        # one row
         assert max(a.elems for a in p.args if a.name in ("k", "k_pool", "k_pools")) >= 64
+
+
+@pytest.mark.parametrize("strides", [(), (0, 0), (0, 0, 0, 0)])
+def test_strides_are_three_numbers(irx, strides):
+    refused(irx, 42, cache, irx, strides=strides)
