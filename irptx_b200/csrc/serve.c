@@ -16,6 +16,7 @@
 #define MAX_COUNT 0x7fffffffll
 #define MAX_STRIDE (1ll << 40)
 #define MAX_32 (1ll << 30)
+#define MAX_SPAN 9e17                      /* elements; sums of a few stay below 2^63 */
 
 static int esz(int dt) { return dt == DT_BF16 ? 2 : dt == DT_U8 ? 1 : 4; }
 
@@ -95,8 +96,8 @@ static int cache_of(irx_kvc_t *o, const irx_kv_cache_t *c, int tabled)
     if (o->page_stride < 0 || o->head_stride < 0 || o->token_stride < 0 || o->page_stride > MAX_STRIDE ||
         o->head_stride > MAX_STRIDE || o->token_stride > MAX_STRIDE)
         return irx_fail(E042, "a cache stride below 0 or above 2^40");
-    if ((double)o->pages * o->page_stride > 9e17 || (double)o->heads * o->head_stride > 9e17 ||
-        (double)o->page_size * o->token_stride > 9e17)
+    if ((double)o->pages * o->page_stride > MAX_SPAN || (double)o->heads * o->head_stride > MAX_SPAN ||
+        (double)o->page_size * o->token_stride > MAX_SPAN)
         return irx_fail(E042, "a cache larger than an address space");
     if (rows_overlap(o)) return irx_fail(E041, "a cache whose strides make rows overlap");
     return 0;
@@ -132,6 +133,7 @@ int irx_compile_decode(const irx_kv_cache_t *cache, int heads, long long q_strid
     qrow = (int64_t)heads * a->c.dim;
     if (q_stride < 0 || q_stride > MAX_STRIDE || (q_stride && q_stride < qrow))
         return irx_fail(E042, "query rows that overlap");
+    if ((double)a->c.batch * (q_stride ? q_stride : qrow) > MAX_SPAN) return irx_fail(E042, "queries larger than an address space");
     a->heads = heads;
     a->q_stride = q_stride ? q_stride : qrow;
     a->window = window;
@@ -242,6 +244,7 @@ int irx_compile_kv_append(const irx_kv_cache_t *cache, long long tokens, long lo
     if (tokens < 1 || tokens > MAX_COUNT) return irx_fail(E042, "an append of no tokens");
     if (row > (1 << 20)) return irx_fail(E042, "a token's keys past 2^20 elements");
     if (stride < 0 || stride > MAX_STRIDE || (stride && stride < row)) return irx_fail(E042, "new tokens' rows that overlap");
+    if ((double)tokens * (stride ? stride : row) > MAX_SPAN) return irx_fail(E042, "new tokens larger than an address space");
     a->n = tokens;
     a->stride = stride ? stride : row;
     add(p, KA_IN, a->c.dt, (tokens - 1) * a->stride + row);
@@ -270,7 +273,9 @@ int irx_compile_kv_copy(const irx_kv_cache_t *cache, long long pairs, int layers
     a->layers = layers;
     a->layer_stride = layer_stride ? layer_stride : a->c.pages * a->c.page_stride;
     if (layers > 1 && a->layer_stride < span(&a->c)) return irx_fail(E041, "layers whose pools overlap");
-    if ((double)layers * a->layer_stride > 9e17) return irx_fail(E042, "a cache larger than an address space");
+    if ((double)layers * a->layer_stride > MAX_SPAN) return irx_fail(E042, "a cache larger than an address space");
+    if ((double)pairs * layers * a->c.heads * a->c.page_size * a->c.dim > MAX_SPAN)
+        return irx_fail(E042, "a copy of more elements than 64 bits count");
     add(p, KA_IN, DT_I32, 2 * pairs);
     add(p, KA_OUT, a->c.dt, (layers - 1) * a->layer_stride + span(&a->c));
     add(p, KA_OUT, a->c.dt, (layers - 1) * a->layer_stride + span(&a->c));
@@ -381,7 +386,7 @@ int irx_compile_matvec4(const irx_matvec4_t *m, irx_plan_t *plan)
     a->groups = (int32_t)groups;
     a->dt = (uint8_t)m->dtype; a->sdt = (uint8_t)m->scale_dtype;
     a->zeros = m->zeros != 0;
-    if ((double)a->m * a->n > 9e17 || (double)a->n * a->w_stride > 9e17 || (double)a->m * a->x_stride > 9e17)
+    if ((double)a->m * a->n > MAX_SPAN || (double)a->n * a->w_stride > MAX_SPAN || (double)a->m * a->x_stride > MAX_SPAN)
         return irx_fail(E042, "a matvec4 larger than an address space");
     add(p, KA_IN, a->dt, (a->m - 1) * a->x_stride + a->k);
     add(p, KA_IN, DT_U8, (a->n - 1) * a->w_stride + (a->k + 1) / 2);
