@@ -25,10 +25,10 @@ def test_products_past_64_bits_are_refused(irx):
     top, far = (1 << 31) - 1, 1 << 40
     one = cache(irx)
     refused(irx, 42, irx.kv_append, one, top, stride=far)
-    refused(irx, 42, irx.decode, cache(irx, batch=top), 2, q_stride=far)
+    refused(irx, 42, irx.decode, cache(irx, batch=1 << 29), 2, q_stride=far)
     refused(irx, 42, irx.decode, cache(irx, batch=top), (1 << 31) - 2)
     wide = cache(irx, heads=1, page_size=1, pages=2)
     refused(irx, 42, irx.kv_copy, cache(irx, heads=1 << 10, page_size=1 << 10, pages=2, head_dim=256), top, layers=1 << 22)
-    for plan in (irx.kv_append(one, top, stride=1 << 28), irx.decode(cache(irx, batch=top), 2, q_stride=1 << 28),
+    for plan in (irx.kv_append(one, top, stride=1 << 28), irx.decode(cache(irx, batch=1 << 29), 2, q_stride=1 << 28),
                  irx.kv_copy(wide, top, layers=1 << 20)):
         assert all(0 < a.elems < 1 << 62 for a in plan.args)
