@@ -129,7 +129,10 @@ typedef struct irx_kv_cache {
  * h / (heads / cache heads). window > 0 hides the keys before position lens[b] - window, except
  * the first `sinks`. A sequence of length 0 gives zeros (and -inf). The workspace must be zero
  * before its first launch and is left ready for the next; launches that may overlap need one
- * each. The result is the same bits for the same inputs on the same GPU. Units: key-value heads. */
+ * each. Keys whose table entry names no page of the pool are left out as the mask's are (a sequence
+ * that keeps none of its keys: NaN, and -inf), and a length outside 0 to table_cols * page_size
+ * counts as the nearer end; both are reported. The result is the same bits for the same inputs on
+ * the same GPU. Units: key-value heads. */
 IRX_API int irx_compile_decode(const irx_kv_cache_t *cache, int heads, long long q_stride, float scale, int window, int sinks,
                                int lse, irx_plan_t *plan);
 

@@ -119,9 +119,9 @@ typedef struct {
 #define IRX_DEC_TC_ST(dp, nt) ((dp) == 256 || ((dp) == 128 && (nt) == 2) ? 2 : 3)
 #define IRX_DEC_ST_NW(dp) ((dp) == 256 ? 8 : 16)
 #define IRX_DEC_TC_SMEM(dp, nt, km, st) (4 * (st) * 2 * 16 * (km) * (dp) * 2 + 2 * 8 * ((dp) + 4) * 4 + 4 * 8 * (nt) * 8 + \
-                                         IRX_DEC_SHARE + 4 * (st) * 192 * (km))
+                                         IRX_DEC_SHARE + 4 * (st) * (192 * (km) + 8))
 #define IRX_DEC_ST_SMEM(dp, rows, st) (IRX_DEC_ST_NW(dp) * ((st) * 8 * (2 * (dp) + 16) * 4 + (rows) * (dp) * 4 + 8 * (rows) * 4 + \
-                                       8 * (rows) + (st) * 96) + (rows) * (dp) * 4 + IRX_DEC_SHARE)
+                                       8 * (rows) + (st) * 104) + (rows) * (dp) * 4 + IRX_DEC_SHARE)
 
 typedef struct {
     const void *q, *k, *v;

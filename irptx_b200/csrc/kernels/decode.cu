@@ -367,10 +367,13 @@ __device__ __forceinline__ void dec_empty(const irx_kdec_t &p)
 // Where a warp's key rows of the tiles to come lie: for each tile of its ring, for each of the tile's keys,
 // the key's page (copied from the table asynchronously, a whole ring ahead of its use, so that no load of
 // keys waits for the table) and the rest of its offset, -1 where there is no such key.
+// `bad`: of the tile that is in the slot now, the keys that the table puts outside the pool, a bit each (the
+// matrix kernel reads it only where there are any).
 template <int KEYS>
 struct DecRows {
     long long off[KEYS];
     int page[KEYS];
+    unsigned bad, pad;
 };
 
 // pos / page_size by a multiplication, exact below 2^31 (the launcher's constants).
@@ -394,7 +397,7 @@ __device__ __forceinline__ void dec_lookup(const irx_kdec_t &p, const DecCur &c,
 }
 
 // The element offset of the tile's key `i`: -1 when there is none, -2 (flagged) when the table's page is
-// not one of the pool's.
+// not one of the pool's. Such a key is left out of the softmax, as one outside the mask is.
 template <int KEYS>
 __device__ __forceinline__ long long dec_row(const irx_kdec_t &p, const DecRows<KEYS> &R, int i)
 {
@@ -505,6 +508,7 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
         constexpr int CPR = DP / 8, RPI = 32 / CPR, NI = T::KEYS / RPI;
         const int lrow = lane / CPR, lch = lane % CPR;
         const bool cin = lch * 8 < p.d;
+        unsigned bads = 0;                                     // slots whose tile has bad keys
         auto lookup = [&](int st) {
             dec_lookup<T::KEYS>(p, tl, tc < S.c1, dec_pos<T::K>(tl, tl.j) + warp * T::KEYS, rows[st]);
             if (tc < S.c1) {
@@ -528,7 +532,11 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
                     cp16(d, k);
                     cp16(d + T::TILE, k + dv);
                 }
+                bads &= ~(1u << st);
             } else if (__any_sync(0xffffffffu, off != -1)) {
+                const unsigned bad = __ballot_sync(0xffffffffu, off == -2);
+                if (lane == 0) rows[st].bad = bad;
+                bads = (bads & ~(1u << st)) | (bad ? 1u << st : 0);
 #pragma unroll
                 for (int i = 0; i < NI; i++) {
                     const int row = i * RPI + lrow;
@@ -588,7 +596,8 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
             const int pos = dec_pos<T::K>(cu, cu.j) + warp * T::KEYS;
             if (dec_any(cu, pos, T::KEYS)) {
                 const uint32_t kb = ring + st * (2 * T::TILE), vb = kb + T::TILE;
-                const bool whole = dec_all(cu, pos, T::KEYS);
+                const bool whole = dec_all(cu, pos, T::KEYS) && !(bads >> st & 1);
+                const unsigned bad = bads >> st & 1 ? rows[st].bad : 0;
                 // S^T: two sums per 16 keys where there are 16 only, of even and odd steps: half the chain
                 float s[KM][NT][4], s2[NT][4];
 #pragma unroll
@@ -615,7 +624,7 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
 #pragma unroll
                 for (int km = 0; km < KM; km++)
 #pragma unroll
-                    for (int h = 0; h < 2; h++) in[km][h] = whole || dec_sees(cu, pos + km * 16 + h * 8 + g);
+                    for (int h = 0; h < 2; h++) in[km][h] = whole || (dec_sees(cu, pos + km * 16 + h * 8 + g) && !(bad >> (km * 16 + h * 8 + g) & 1));
                 uint32_t pb[KM][NT][2], pl[KM][NT][2];       // P^T's upper and lower halves
                 bool grew = false;
                 float al[NT][2];
@@ -828,6 +837,8 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
             const long long off = dec_row<8>(p, rows[st], lane & 7);
             if (__any_sync(0xffffffffu, off != -1)) {
                 float *kd = myring + st * (T::TILE / 4), *vd = kd + 8 * T::KS;
+                const unsigned bad = __ballot_sync(0xffffffffu, off == -2);
+                if (lane == 0) rows[st].bad = bad;
                 if (p.vec) {
                     constexpr int CPR = DP / 4;              // 16-byte pieces of a row
 #pragma unroll
@@ -885,7 +896,7 @@ __device__ __forceinline__ void dec_st_body(const irx_kdec_t &p)
             __syncwarp();
             const int pos = dec_pos<T::K>(cu, cu.j) + warp * 8;
             if (dec_any(cu, pos, 8)) {
-                const bool in = dec_sees(cu, pos + key);
+                const bool in = dec_sees(cu, pos + key) && !(rows[st].bad >> key & 1);
                 const float *kt = myring + st * (T::TILE / 4), *vt = kt + 8 * T::KS;
                 float s[ROWS];
 #pragma unroll
