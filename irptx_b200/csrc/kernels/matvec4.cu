@@ -10,7 +10,7 @@
 // 24.3 us, 2.5 TB/s; [4 x 4096] x [14337 x 4096] with zero points 14.6 us; one token, 4096 x 4096, 6.0 us.
 //
 // The products run on matrix instructions with the weights as the wide operand (16 rows of w) and
-// the tokens as the narrow one (8). A weight becomes the exact bf16 number q - z: the
+// the tokens as the narrow one (8). A weight becomes the exact bf16 number q - z (over 2^11): the
 // four bits placed in the mantissa of 128 give 128 + q, from which 128 + z is subtracted. So no
 // weight is rounded; a group's products are summed in f32 and the scale is applied to that sum.
 // Which k an operand slot stands for does not matter as long as both operands agree, so each lane
@@ -24,6 +24,11 @@
 #include "decode.cu"
 
 #define MV4_WARPS 8
+// Two bf16 numbers of 128 / 2^11, whose last mantissa place is 1 / 2^11: the weights enter the products as
+// (q - z) / 2^11, so that a group's sum, up to 15 * 128 tokens before its scale, stays in range for
+// every finite token; 2^11 is given back with the last sum.
+#define MV4_ONE 0x3d803d80u
+#define MV4_BACK 2048.0f
 
 // 8 weights of one row: pairs (0, 4), (1, 5), (2, 6), (3, 7) minus the zero point pair.
 __device__ __forceinline__ void mv4_unpack(uint32_t w, __nv_bfloat162 z, uint32_t (&r)[4])
@@ -31,7 +36,7 @@ __device__ __forceinline__ void mv4_unpack(uint32_t w, __nv_bfloat162 z, uint32_
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         uint32_t u;
-        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(u) : "r"(w), "r"(0x000f000fu), "r"(0x43004300u));   // (w & m) | c
+        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(u) : "r"(w), "r"(0x000f000fu), "r"(MV4_ONE));   // (w & m) | c
         const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&u), z);
         r[i] = *reinterpret_cast<const uint32_t *>(&d);
         w >>= 4;
@@ -92,10 +97,10 @@ __device__ __forceinline__ void mv4_stage(uint32_t ws, const unsigned char *xs, 
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int row = wr * 32 + rt * 16 + h * 8 + g;
-                uint32_t zb = 0x43084308u;               // 128 + 8
+                uint32_t zb = MV4_ONE + 0x00080008u;     // a zero point of 8
                 if (zp) {
                     zb = zp[row * M::ZS + i];
-                    if (NT > 1) zb = 0x43004300u | ((zb & 15u) * 0x00010001u);
+                    if (NT > 1) zb = MV4_ONE | ((zb & 15u) * 0x00010001u);
                 }
                 s[rt][h] = sc[row * 9 + i];
                 z[rt][h] = *reinterpret_cast<const __nv_bfloat162 *>(&zb);
@@ -270,7 +275,7 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
         for (int i = 0; i < 4; i++) {
             const int row = (r & 1) * 128 + (tid >> 3) + 32 * i;
             scales[row * 9 + (tid & 7)] = __uint_as_float(sr[i] << shift);
-            if (p.z) zeros[row * M::ZS + (tid & 7)] = (typename M::Zero)(NT == 1 ? 0x43004300u | ((zr[i] & 15u) * 0x00010001u) : zr[i]);
+            if (p.z) zeros[row * M::ZS + (tid & 7)] = (typename M::Zero)(NT == 1 ? MV4_ONE | ((zr[i] & 15u) * 0x00010001u) : zr[i]);
         }
     };
     if (F32) {                                           // columns that no token has stay zero
@@ -352,7 +357,7 @@ __device__ __forceinline__ void mv4_body(const irx_kmv4_t &p)
         const int m = i / rows, r = i - m * rows;
         const float *a = fin + r * M::RS + (F32 ? 3 * m : m);
         const float v = F32 ? a[0] + (a[1] + a[2]) : a[0];
-        if (row0 + r0 + r < n1 && m0 + m < m_all) irx_st1(p.y, p.dt, (int64_t)(m0 + m) * p.n + row0 + r0 + r, v);
+        if (row0 + r0 + r < n1 && m0 + m < m_all) irx_st1(p.y, p.dt, (int64_t)(m0 + m) * p.n + row0 + r0 + r, v * MV4_BACK);
     }
     if (ck > 1) cluster_sync();                        // no block leaves while its sums are still read
 }
