@@ -422,8 +422,9 @@ __device__ __forceinline__ long long dec_row(const irx_kdec_t &p, const DecRows<
 // filled with padding.
 // P enters the product as two bf16 numbers, its upper half truncated and the rest rounded, 16 bits in
 // all: the tensor pipe has room for the second product, and the output is then as near the
-// definition as one rounded once at the end. (The rest of a weight that is not 0 is kept at 2^-20 of it at
-// least, so that an infinite value does not meet 0 there; a constant would count under values of 2^100.)
+// definition as one rounded once at the end. (The rest of a weight that is not 0 is kept above 0, so that an
+// infinite value does not meet 0 there: at 2^-126, or 2^-16 of the weight where that is less, since
+// a weight of 0 must add nothing under values of 2^120.)
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
@@ -666,8 +667,8 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
                         for (int h = 0; h < 2; h++) {
                             const float x = s[km][nt][2 * h], y = s[km][nt][2 * h + 1];
                             const uint32_t hi = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
-                            const __nv_bfloat162 lo = __floats2bfloat162_rn(fmaxf(x - __uint_as_float(hi << 16), x * 0x1p-20f),
-                                                                            fmaxf(y - __uint_as_float(hi & 0xffff0000u), y * 0x1p-20f));
+                            const __nv_bfloat162 lo = __floats2bfloat162_rn(fmaxf(x - __uint_as_float(hi << 16), fminf(x * 0x1p-16f, 0x1p-126f)),
+                                                                            fmaxf(y - __uint_as_float(hi & 0xffff0000u), fminf(y * 0x1p-16f, 0x1p-126f)));
                             pb[km][nt][h] = trans8(hi);
                             pl[km][nt][h] = trans8(*reinterpret_cast<const uint32_t *>(&lo));
                         }
