@@ -187,7 +187,8 @@ class Decoder:
 
 
 def main(prompt_len=37, steps=21, out=print):
-    """Returns the largest relative error of the answers' last logits against the dense model."""
+    """Returns the largest relative error of the answers' last logits against the dense model, infinity when
+    one of them is not a number."""
     m = Decoder()
     prompt = [(17 * i * i + 5 * i + 3) % m.embed.shape[0] for i in range(prompt_len)]
     first, logits = m.prompt(prompt)
@@ -215,7 +216,8 @@ def main(prompt_len=37, steps=21, out=print):
             for s, a in answers.items():
                 if s != ended:
                     want = m.dense(a)
-                    worst = max(worst, float((logits[s].double() - want).abs().max() / want.abs().max()))
+                    off = float((logits[s].double() - want).abs().max() / want.abs().max())
+                    worst = max(worst, off if math.isfinite(off) else math.inf)      # (max would drop a NaN)
         for s in answers:
             if s != ended:
                 answers[s].append(int(m.token[s]))
