@@ -38,3 +38,9 @@ def _reference_core_for_gpu_tests(request):
     from oracle import refptx
     if not refptx.core_available():
         pytest.fail("the reference core oracle/_ref/irptx is missing: build it (make -C oracle) before the GPU tests")
+
+
+def pytest_collection_modifyitems(items):
+    """Modules whose GPU tests compare with no reference core (they say so by a fixture of the name above)
+    go first, so that a run that stops at the first failure has run them when the core is missing."""
+    items.sort(key=lambda i: not (i.get_closest_marker("gpu") and hasattr(i.module, "_reference_core_for_gpu_tests")))
