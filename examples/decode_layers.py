@@ -108,8 +108,11 @@ class Decoder:
     def copy_pages(self, pairs):
         """Run the page copies that the manager asked for, and upload its table."""
         if pairs:
-            plan = irx.kv_copy(self.cache, len(pairs), layers=self.layers)
-            plan.launch([torch.tensor(pairs, dtype=torch.int32, device="cuda"), self.k, self.v])
+            n = -(-len(pairs) // 8) * 8                  # padded, so that a few plans serve every list
+            if ("copy", n) not in self.kir:
+                self.kir["copy", n] = irx.kv_copy(self.cache, n, layers=self.layers)
+            pairs = pairs + [(-1, -1)] * (n - len(pairs))
+            self.kir["copy", n].launch([torch.tensor(pairs, dtype=torch.int32, device="cuda"), self.k, self.v])
         self.table.copy_(torch.from_numpy(self.pages.table))
 
     def prompt(self, tokens):
