@@ -131,8 +131,10 @@ typedef struct irx_kv_cache {
  * before its first launch and is left ready for the next; launches that may overlap need one
  * each. Keys whose table entry names no page of the pool are left out as the mask's are (a sequence
  * that keeps none of its keys: NaN, and -inf), and a length outside 0 to table_cols * page_size
- * counts as the nearer end; both are reported. The result is the same bits for the same inputs on
- * the same GPU. Units: key-value heads. */
+ * counts as the nearer end; both are reported. Sums of weights times values are f32 and divided at
+ * the end: values times the keys seen have to stay in its range. The result is the same bits for the
+ * same inputs on the same GPU; a sequence's last places depend on where the others' lengths, and a
+ * shard's heads, place its cuts. Units: key-value heads. */
 IRX_API int irx_compile_decode(const irx_kv_cache_t *cache, int heads, long long q_stride, float scale, int window, int sinks,
                                int lse, irx_plan_t *plan);
 
@@ -153,7 +155,9 @@ IRX_API int irx_compile_kv_copy(const irx_kv_cache_t *cache, long long pairs, in
  * between rows; 0: packed), two weights to a byte, the even k in its low four bits; scales [n,
  * ceil(k / group)]; with `zeros` != 0 the zero points, uint8 of the same shape, values 0 to 15 (8
  * otherwise); y [m, n], packed, of x's dtype. Weights are used as they are (not rounded again), sums
- * are f32. Units: rows of w. */
+ * are f32, a group's before its scale. The weights are read once for every 16 tokens (bf16) or 5 (f32).
+ * The same launch gives the same bits; a row's last places depend on the rows and tokens of its
+ * launch, so a shard's may differ from the whole's. Units: rows of w. */
 typedef struct irx_matvec4 {
     int dtype, scale_dtype;          /* IRX_DT_BF16 or IRX_DT_F32 */
     long long m, n, k;

@@ -5,21 +5,24 @@
 // of key-value head h / group:  o = sum_j softmax_j(scale * q.k_j) v_j, zeros when n = 0, and
 // lse = ln sum_j exp(scale * q.k_j) (-inf when n = 0).
 //
-// Bound: every visible key and value row is read once and takes 4 * group operations per
-// element, so HBM bounds it (group operations a byte in bf16). The work is therefore cut by
-// keys, not by rows: the visible keys of all (sequence, kv head, row block) units are laid end to
-// end in chunks of 64 or 128 keys and the chunks are dealt out evenly, a contiguous range to each
-// block of one resident wave, whatever the lengths are. A block whose range covers a whole
+// Bound: every visible key and value row is read and takes 4 * group operations per element, so HBM
+// bounds it (group operations a byte in bf16). A unit, (sequence, kv head, row block), reads its keys
+// for 16 query rows at most (8 at head sizes past 128 and in f32): wider groups are several units and
+// read them as often. The work is cut by keys, not by rows: the visible keys of all units are laid
+// end to end in chunks of 64 or 128 keys and the chunks are dealt out evenly, a contiguous range to
+// each block of one resident wave, whatever the lengths are. A block whose range covers a whole
 // unit writes its output; a unit that several blocks share is joined by the last of them to
 // arrive, which folds the blocks' partials in key order, so the result does not depend on which
 // block that was. Past DEC_JOIN partials they are folded in groups first, by the last block of
 // each group, so a single long sequence's join is not one block's work.
 //
 // Measured (bf16, 8 kv heads of 128 and 32 query heads): two sequences of 120 to 131 thousand tokens
-// (1.0 GB) in 160 to 163 us, 6.2 to 6.3 TB/s; 31 of 1 to 4096 tokens (259 MB) in 49 us, 5.3 TB/s. Of those 49
+// (1.0 GB) in 163 us, 6.2 TB/s; 31 of 1 to 4096 tokens (259 MB) in 49 us, 5.3 TB/s. Of those 49
 // about 2 are the launch, 2.6 pass before the first keys can be asked for (lengths, then the page
 // table), the keys stream for 37 at 7 TB/s, and 5 are the ends: warps meet, partials are written,
-// counted and folded. One sequence of 17 tokens takes 5.5 us, those latencies alone.
+// counted and folded. One sequence of 17 tokens takes 5.5 us, those latencies alone. Sixteen sequences of 8192
+// tokens: 4 rows a group 90 us (5.9 TB/s), 16 rows 102, 32 rows, read twice, 183; head size 80, whose rows
+// lie in tiles of 128, 79 us (4.3 TB/s), 96 79 (5.1), 256 170 (6.3), 256 with 16 rows, read twice, 330.
 #pragma once
 #include "tc.cuh"
 #include "kvpages.cu"
@@ -417,7 +420,7 @@ __device__ __forceinline__ long long dec_row(const irx_kdec_t &p, const DecRows<
 // S^T's accumulators become P^T's operand by an 8x8 transpose across the warp. Each warp owns 16
 // keys of a chunk (32 at head size 64, where 16 are too little work for what a tile costs) and its
 // own ring of ST tiles filled by 16-byte asynchronous copies, so warps meet only where a unit ends. mma.sync runs far below tcgen05's rate, but at 8 to 16 rows
-// the products take 16 to 32 instructions per 8 KB (D = 128), which HBM delivers in about 360
+// the products take 24 to 48 instructions per 8 KB (D = 128), which HBM delivers in about 360
 // cycles per SM: the tensor pipe is idle most of the time and tcgen05's 128-row tiles would be
 // filled with padding.
 // P enters the product as two bf16 numbers, its upper half truncated and the rest rounded, 16 bits in
@@ -783,11 +786,13 @@ __device__ __forceinline__ void dec_tc_body(const irx_kdec_t &p)
 
 // ---- f32, and rows that cannot be moved 16 bytes at a time: FP32 units ----
 // The same cut of the work with 16 warps of 8 keys (8 warps at head size 256), a tile each: the warps
-// cover each other's waits (8 warps with two tiles each took 181 us against 132 for six sequences
-// of 30k tokens, 4 f32 heads of 128, 738 MB: 5.6 TB/s). A warp's four lanes per key each take every fourth 16
+// cover each other's waits (8 warps with two tiles each took 181 us against 131 for six sequences
+// of 30k tokens, 4 f32 heads of 128, 737 MB: 5.6 TB/s). A warp's four lanes per key each take every fourth 16
 // bytes of the key's row for all query rows (the rows sit in shared memory and are broadcast),
 // then every lane owns DP/32 dims of the accumulators and reads the values' rows across. f32
-// products and sums throughout; with 8 rows a unit they bound it (222 us there).
+// products and sums throughout; with 8 rows a unit they bound it (221 us there), and so they do at head size 64
+// (179 us for the same bytes). At 512 threads a thread has 128 registers, of which some are spilled (152 to
+// 352 bytes a thread, most with 8 rows at 128).
 
 template <int DP, int ROWS, int ST>
 struct DecSt {

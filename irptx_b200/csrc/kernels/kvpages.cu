@@ -4,9 +4,9 @@
 // Both only move bytes, so they are bound by HBM for large calls (floor: the moved bytes read once
 // and written once) and by the launch and the chain of dependent loads for small ones. They are
 // written on vectors of 16, 4 or 2 bytes: the launcher takes the widest that every base and
-// stride allows. Measured: 16,376 tokens of 8 heads of 128 (bf16, 125 MB moved) appended in 21.3 us,
-// 5.9 TB/s; 1023 pages of 32 KB in 4 layers and 2 pools (536 MB moved) copied in 86 us, 6.2 TB/s;
-// the smallest calls 1.9 and 2.4 us, about an empty launch.
+// stride allows. Measured: 16,376 tokens of 8 heads of 128 (bf16, 125 MB moved) appended in 21.4 us,
+// 5.8 TB/s; 1023 pages of 32 KB in 4 layers and 2 pools (536 MB moved) copied in 86 us, 6.2 TB/s;
+// the smallest calls 2.0 and 2.4 us, about an empty launch.
 #pragma once
 #include "common.cuh"
 
@@ -19,7 +19,7 @@ __device__ __forceinline__ void irx_flag(unsigned *err, unsigned bit)
 // One warp moves up to APP_VEC x 32 vectors of a token's keys and as many of its values. The data loads
 // are issued before the token's slot is known (sequence and position, then the page table): only
 // the stores wait for that chain. Two vectors of each a lane: one token of 8 heads of 128 is then two
-// warps (1.9 us for 32 tokens; 2.1 with four vectors, one warp; long calls do not change).
+// warps (0.2 us less for 32 tokens than four vectors, one warp; long calls do not change).
 #define APP_VEC IRX_APPEND_VEC
 
 template <class V>

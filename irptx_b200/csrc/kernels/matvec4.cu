@@ -2,12 +2,17 @@
 // weights q (two to a byte, the even k in the low half), group scales s and zero points z (8 when
 // there are none), for a few tokens m.
 //
-// Bound: the packed weights are read once, half a byte each for 2 m operations, so HBM sets the floor
-// up to m of a few hundred. What bounds the kernel in fact is unpacking: 8 weights take 4 logic
-// operations, 3 shifts and 4 subtractions whatever m is, and with 9 to 16 tokens the matrix pipe
-// (a quarter busy) and the logic pipe (a third) are each used in bursts by the few warps that fit. A
-// call of a few megabytes is bound by latency. Measured, bf16: [13 x 14336] x [8192 x 14336] (61 MB)
-// 24.3 us, 2.5 TB/s; [4 x 4096] x [14337 x 4096] with zero points 14.6 us; one token, 4096 x 4096, 6.0 us.
+// Bound: the packed weights are read, half a byte each for 2 m operations, so HBM sets the floor up to m of
+// a few hundred. The kernel stays at a third of it, and no single part is why: of 27.8 us in an earlier
+// build of the largest call below, 23.7 were left without the unpacking (4 logic operations, 3 shifts and
+// 4 subtractions for 8 weights, whatever m is), 17.8 without the products, 13.7 with the weights'
+// stream alone. A warp goes through a chain, unpack, then up to 8 products into one accumulator, and 16
+// warps an SM are too few to cover it (0.46 instructions issue a cycle and scheduler, the matrix pipe is
+// 24 % busy); equal slices also leave places empty (226 or 256 blocks where 296 fit). A call of a few
+// megabytes is bound by latency. Measured, bf16: [13 x 14336] x [8192 x 14336] (61 MB) 24.2 us, 2.5 TB/s;
+// [4 x 4096] x [14337 x 4096] with zero points 14.6 us; one token, 4096 x 4096, 6.0 us.
+// More than 16 tokens (5 in f32) go over the weights again for each 16 (5): 17 tokens of the largest
+// call take 42.2 us, 64 77.8, and 13 in f32 87 where 5 take 27.6.
 //
 // The products run on matrix instructions with the weights as the wide operand (16 rows of w) and
 // the tokens as the narrow one (8). A weight becomes the exact bf16 number q - z (over 2^11): the

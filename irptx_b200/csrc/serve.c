@@ -400,9 +400,9 @@ int irx_compile_matvec4(const irx_matvec4_t *m, irx_plan_t *plan)
  * latencies, so the most slices (a cluster's blocks, 1 to 8) whose clusters all fit at once. The GPU
  * packs clusters as tightly as shared memory lets it, which leaves SMs idle when the grid does not
  * fill it, so a launch asks for as much as keeps its blocks at the fewest an SM that hold them all.
- * Measured (bf16, one token, 14336 k): 74 tiles in 4 slices at two an SM, where 71 clusters fit, 31 us, 71
- * tiles 21.5; 64 tiles in 4 slices 20, in 2 slices 38. Three an SM measured slower where two fit (14337
- * rows of 4096, 4 tokens: 17.0 us in 3 slices against 14.9 in 2). */
+ * Measured (bf16, one token, 14336 k): 71 tiles in 4 slices at two an SM 22.0 us, in 3 26.8, in 2 34.0; 74
+ * tiles, of which 71 clusters of 4 fit, in 4 31.9, in 3 (the rule's) 26.8, in 2 24.9; 14337 rows of 4096, 4
+ * tokens, in 2 12.7, in 1 13.7 at one an SM, in 4 16.0. A third block an SM does not fit its shared memory. */
 static int mv4_split(irx_dev_t *d, int i, unsigned need, int64_t tiles, int64_t steps, unsigned *ck, unsigned *smem)
 {
     unsigned r, c, best = 0;
@@ -519,7 +519,8 @@ void irx_serve_text(const irx_plan_int_t *p, char *buf, size_t cap)
     }
 }
 
-/* The work of a launch; a decode's, of a full cache (the lengths are only known on the device). */
+/* The work that a launch cannot do without (weights, keys and values once, whatever the kernels read again); a
+ * decode's, of a full cache (the lengths are only known on the device). */
 void irx_serve_work(const irx_plan_int_t *p, double *bytes, double *flops)
 {
     *bytes = *flops = 0;

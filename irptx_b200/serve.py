@@ -213,7 +213,8 @@ def matvec4(m: int, n: int, k: int, group: int = 128, dtype: str = "bf16", scale
             zeros: bool = False, x_stride: int = 0, w_stride: int = 0) -> OpPlan:
     """y[m, n] = sum_k x[m, k] s[n, k // group] (q[n, k] - z[n, k // group]): [x, w, scales, (zeros,) y].
     w is uint8 [n, ceil(k / 2)], the even k in the low four bits (:func:`pack4`); z is uint8, 0 to
-    15, or 8 everywhere without ``zeros``. Meant for a few tokens: past 16 the weights are read again."""
+    15, or 8 everywhere without ``zeros``. Meant for a few tokens: the weights are read again for every 16
+    (every 5 with f32 tokens)."""
     m, n, k, group = _int("m", m, 62), _int("n", n, 62), _int("k", k, 62), _int("group", group)
     x_stride, w_stride = _int("x_stride", x_stride, 62), _int("w_stride", w_stride, 62)
     d = _Matvec4Desc(_dtype(dtype), _dtype(scale_dtype or dtype), m, n, k, group, int(bool(zeros)), x_stride, w_stride)
