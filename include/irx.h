@@ -62,7 +62,11 @@ enum irx_family {
     IRX_FAM_DECODE = 8,        /* attention of one new token per sequence over a paged cache */
     IRX_FAM_KV_APPEND = 9,     /* new tokens' keys and values into their pages */
     IRX_FAM_KV_COPY = 10,      /* page copies of a paged cache */
-    IRX_FAM_MATVEC4 = 11       /* y = x W^T with 4-bit weights and group scales */
+    IRX_FAM_MATVEC4 = 11,      /* y = x W^T with 4-bit weights and group scales */
+    IRX_FAM_ROPE = 12,         /* rotary positions */
+    IRX_FAM_ROPE_APPEND = 13,  /* rotary positions on the way into the pages */
+    IRX_FAM_PROMPT = 14,       /* causal attention over packed prompts */
+    IRX_FAM_SAMPLE = 15        /* the draw of the next token */
 };
 
 enum irx_dtype { IRX_DT_F32 = 1, IRX_DT_BF16 = 2, IRX_DT_I32 = 4, IRX_DT_U8 = 5 };
@@ -165,6 +169,84 @@ typedef struct irx_matvec4 {
     long long x_stride, w_stride;
 } irx_matvec4_t;
 IRX_API int irx_compile_matvec4(const irx_matvec4_t *desc, irx_plan_t *plan);
+
+/* Rotary positions. The first 2 * pairs numbers of a head are turned, the rest copied: pair i, the numbers
+ * (i, i + pairs) or, interleaved, (2 i, 2 i + 1), by the angle pos * freqs[i]:
+ * (x1, x2) -> amplitude * (x1 cos - x2 sin, x1 sin + x2 cos); with `backward` != 0 by the opposite
+ * angle, which turns the result's gradient into x's. freqs: host memory, radians a position, each
+ * within 1024, copied into the plan. Angles are held in 64 bits, sines, cosines and products in 32.
+ * irx_rope_freqs writes the rot / 2 frequencies base^(-2 i / rot), for a context `factor` times as long
+ * as the `original` one that a model was trained on: LINEAR divides them all by factor; NTK stretches
+ * the base by factor^(rot / (rot - 2)); YARN and BANDS divide those that turn fewer than `slow` times
+ * within the original context, keep those that turn more than `fast` times, and blend between them, YARN
+ * along the pair's number, BANDS along its turns. (original, fast, slow: YARN and BANDS only.) */
+enum irx_rope_scaling { IRX_ROPE_PLAIN = 0, IRX_ROPE_LINEAR = 1, IRX_ROPE_NTK = 2, IRX_ROPE_YARN = 3, IRX_ROPE_BANDS = 4 };
+IRX_API int irx_rope_freqs(int rot, double base, int scaling, double factor, double original, double fast, double slow,
+                           double *freqs);
+typedef struct irx_rope {
+    const double *freqs;
+    int pairs;
+    int interleaved, backward;
+    float amplitude;
+} irx_rope_t;
+
+/* Args: x [tokens, heads, head_dim] (x_stride elements from one token to the next; 0: packed), pos int32
+ * [tokens], y (y_stride likewise). A token with pos < 0 is padding: its rows of y are left as they were. y may
+ * be x itself, with the same stride. head_dim up to 256, a token's heads up to 2^20 elements. Units: tokens. */
+IRX_API int irx_compile_rope(const irx_rope_t *rope, int dtype, long long tokens, int heads, int head_dim, long long x_stride,
+                             long long y_stride, irx_plan_t *plan);
+
+/* Rotary positions on the way into the cache: token i's queries are turned into q_out, its keys are turned and its
+ * values copied to position pos[i] of sequence seq[i], in one launch. Args: q [tokens, heads, head_dim], k, v
+ * [tokens, cache heads, head_dim] (`stride` elements from one token to the next in all three, as in slices
+ * of a fused projection; 0: each packed), seq, pos int32 [tokens], table, q_out [tokens, heads, head_dim]
+ * (out_stride; 0: packed), k pool, v pool (updated in place). pos[i] < 0 is padding: nothing of it is written.
+ * A place outside the cache is skipped and reported, the token's queries are turned all the same. q_out may
+ * be q itself, with the same stride. Two tokens of one launch must not go to one place. `backward` is refused.
+ * Units: tokens. */
+IRX_API int irx_compile_rope_append(const irx_kv_cache_t *cache, const irx_rope_t *rope, long long tokens, int heads,
+                                    long long stride, long long out_stride, irx_plan_t *plan);
+
+/* Causal attention over packed prompts: sequence s is tokens [starts[s], starts[s + 1]) of the rows, and each
+ * token attends to its sequence's tokens up to itself, with window > 0 only to the last `window` of them and to
+ * the sequence's first `sinks`. Args: q [tokens, heads, head_dim] (q_stride elements from one token to the next;
+ * 0: packed), k, v [tokens, kv_heads, head_dim] (kv_stride), starts int32 [batch + 1], out [tokens, heads,
+ * head_dim] (packed), with `lse` != 0 the natural log of each row's sum of exps, f32 [tokens, heads]. Query head h
+ * reads key-value head h / (heads / kv_heads). starts are read on the device; `tokens` is the buffers' length, and
+ * rows outside every sequence are not read into any result and are left as they were. A sequence whose starts fall
+ * or leave the rows, or that begins below an earlier start, is skipped and reported; one of no tokens is none. What a mask hides has no effect, infinities
+ * and NaN among it. bf16 with head_dim a multiple of 8 and 16-byte aligned rows takes the matrix instructions
+ * (weights rounded to bf16, sums f32); everything else f32 units. head_dim up to 256. Same bits for the same
+ * launch. Units: key-value heads. */
+typedef struct irx_prompt {
+    int dtype;
+    long long tokens;
+    int batch, heads, kv_heads, head_dim;
+    long long q_stride, kv_stride;
+    float scale;
+    int window, sinks, lse;
+} irx_prompt_t;
+IRX_API int irx_compile_prompt(const irx_prompt_t *desc, irx_plan_t *plan);
+
+/* The draw of the next token. A row's tokens are ordered by their logit, equal ones by index, and weigh
+ * exp((logit - largest) / temperature). Of that order, top_k > 0 keeps the first top_k; top_p < 1 the shortest
+ * beginning of those (at least one) whose weights reach top_p of theirs; min_p > 0 those of the rest that weigh at
+ * least min_p (at most 1) times the largest. Drawn is the first kept token, by index, at which the running sum of
+ * kept weights is above u times their total. Args: logits [rows, vocab] (`stride` elements from one row to the next;
+ * 0: packed), temperature f32 [rows], top_k int32 [rows], top_p, min_p f32 [rows], u f32 [rows], uniform in [0, 1)
+ * (outside it: the nearer end), token int32 [rows], with `logprob` != 0 the log of the token's share of the kept
+ * weights, f32 [rows]. A temperature that is not above 0 takes the largest logit (the lowest index of it; log 0).
+ * A filter outside its range, or NaN, is off (top_p of 0 or below keeps one token). NaN logits count as -infinity,
+ * which is never drawn; a row of nothing else gives token -1 and -infinity; if the largest is +infinity only such
+ * tokens weigh anything. Weights are 64-bit integers, 2^kbits for the largest, kbits = 62 - ceil(log2 vocab) and at most
+ * 46: smaller ones round to nothing, and sums are exact, so the result does not depend on rows, shards or order.
+ * Units: rows. */
+typedef struct irx_sample {
+    int dtype;
+    long long rows, vocab, stride;
+    int logprob;
+} irx_sample_t;
+IRX_API int irx_compile_sample(const irx_sample_t *desc, irx_plan_t *plan);
 
 /* The host side of a paged cache: pages handed out, shared by forks, copied when a shared page is
  * written to, returned and compacted. It keeps numbers only. A step calls what it needs, gathers the

@@ -19,13 +19,15 @@ import re
 from dataclasses import dataclass
 
 __all__ = ["compile", "compile_generic", "Plan", "IrxError", "IrxUnavailable", "library_path", "version", "check",
-           "FAMILIES", "kir_author", "KvCache", "Pages", "decode", "kv_append", "kv_copy", "matvec4", "pack4"]
+           "FAMILIES", "kir_author", "KvCache", "Pages", "decode", "kv_append", "kv_copy", "matvec4", "pack4",
+           "rope_freqs", "rope", "rope_append", "prompt", "sample"]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB = None
 
 FAMILIES = {0: "none", 1: "pointwise", 2: "reduce_all", 3: "reduce_rows", 4: "rowop", 5: "matmul",
-            6: "attention", 7: "kir", 8: "decode", 9: "kv_append", 10: "kv_copy", 11: "matvec4"}
+            6: "attention", 7: "kir", 8: "decode", 9: "kv_append", 10: "kv_copy", 11: "matvec4",
+            12: "rope", 13: "rope_append", 14: "prompt", 15: "sample"}
 _DT = {1: "f32", 2: "bf16", 4: "i32", 5: "u8"}
 _KIND = {0: "in", 1: "const", 2: "out", 3: "work"}
 PLAN_BYTES = 4096
@@ -89,6 +91,12 @@ def _lib():
     lib.irx_compile_kv_append.argtypes = [vp, ll, ll, vp]
     lib.irx_compile_kv_copy.argtypes = [vp, ll, i, ll, vp]
     lib.irx_compile_matvec4.argtypes = [vp, vp]
+    f64, dp = ctypes.c_double, ctypes.POINTER(ctypes.c_double)
+    lib.irx_rope_freqs.argtypes = [i, f64, i, f64, f64, f64, f64, dp]
+    lib.irx_compile_rope.argtypes = [vp, i, ll, i, i, ll, ll, vp]
+    lib.irx_compile_rope_append.argtypes = [vp, vp, ll, i, ll, ll, vp]
+    lib.irx_compile_prompt.argtypes = [vp, vp]
+    lib.irx_compile_sample.argtypes = [vp, vp]
     lib.irx_pages_new.argtypes = [i, i, i, i]
     lib.irx_pages_new.restype = vp
     lib.irx_pages_delete.argtypes = [vp]
@@ -337,3 +345,4 @@ def check(stream=None):
 
 from . import kir_author  # noqa: E402
 from .serve import KvCache, Pages, decode, kv_append, kv_copy, matvec4, pack4  # noqa: E402
+from .step import prompt, rope, rope_append, rope_freqs, sample  # noqa: E402

@@ -90,7 +90,7 @@ int irx_plan_arg(const irx_plan_t *plan, unsigned i, int *kind, int *dtype, long
 
 static int esz(int dt) { return dt == DT_BF16 ? 2 : dt == DT_U8 ? 1 : 4; }
 
-static int serving(const irx_plan_int_t *p) { return p->fam >= FAM_DECODE && p->fam <= FAM_MATVEC4; }
+static int serving(const irx_plan_int_t *p) { return p->fam >= FAM_DECODE && p->fam <= FAM_SAMPLE; }
 
 static void prog_text(const irx_prog_t *g, char *b, size_t cap)
 {
@@ -173,6 +173,12 @@ int irx_plan_describe(const irx_plan_t *plan, char *buf, size_t cap)
     case FAM_MATVEC4:
         irx_serve_text(p, buf, cap);
         break;
+    case FAM_ROPE:
+    case FAM_ROPE_APPEND:
+    case FAM_PROMPT:
+    case FAM_SAMPLE:
+        irx_step_text(p, buf, cap);
+        break;
     default:
         snprintf(buf, cap, "none");
     }
@@ -221,6 +227,12 @@ int irx_plan_work(const irx_plan_t *plan, double *bytes, double *flops)
     case FAM_MATVEC4:
         irx_serve_work(p, &b, &f);
         break;
+    case FAM_ROPE:
+    case FAM_ROPE_APPEND:
+    case FAM_PROMPT:
+    case FAM_SAMPLE:
+        irx_step_work(p, &b, &f);
+        break;
     default:
         break;
     }
@@ -247,6 +259,10 @@ long long irx_plan_units(const irx_plan_t *plan)
     case FAM_KV_APPEND:
     case FAM_KV_COPY: return p->u.kv.n;
     case FAM_MATVEC4: return p->u.mv.n;
+    case FAM_ROPE:
+    case FAM_ROPE_APPEND: return p->u.ro.n;
+    case FAM_PROMPT: return p->u.pr.kv_heads;
+    case FAM_SAMPLE: return p->u.sm.rows;
     default: return 0;
     }
 }
@@ -482,6 +498,7 @@ static int launch_kir(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, void *c
 }
 
 int irx_launch_serve(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsigned ns, void *const *args, void *st);
+int irx_launch_step(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsigned ns, void *const *args, void *st);
 int irx_launch_mm(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsigned ns, void *const *args, void *st);
 int irx_launch_attn(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsigned ns, void *const *args, void *st);
 
@@ -513,6 +530,10 @@ int irx_launch_shard(const irx_plan_t *plan, unsigned shard, unsigned nshards, v
     case FAM_KV_APPEND:
     case FAM_KV_COPY:
     case FAM_MATVEC4: rc = irx_launch_serve(p, d, shard, nshards, args, stream); break;
+    case FAM_ROPE:
+    case FAM_ROPE_APPEND:
+    case FAM_PROMPT:
+    case FAM_SAMPLE: rc = irx_launch_step(p, d, shard, nshards, args, stream); break;
     default: rc = irx_fail(E000, "a plan of no known family");
     }
     pthread_mutex_unlock(&LLOCK);

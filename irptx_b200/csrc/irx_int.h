@@ -132,7 +132,8 @@ typedef struct { uint8_t kind; uint8_t pad[3]; uint32_t v; int32_t off; } irx_un
 typedef enum {
     FAM_NONE = 0, FAM_POINTWISE, FAM_REDUCE_ALL, FAM_REDUCE_ROWS, FAM_ROWOP,
     FAM_MATMUL, FAM_ATTENTION, FAM_KIR,
-    FAM_DECODE, FAM_KV_APPEND, FAM_KV_COPY, FAM_MATVEC4
+    FAM_DECODE, FAM_KV_APPEND, FAM_KV_COPY, FAM_MATVEC4,
+    FAM_ROPE, FAM_ROPE_APPEND, FAM_PROMPT, FAM_SAMPLE
 } irx_fam_t;
 
 /* Every family that runs op programs has one uniform program (`uprog`). It runs once
@@ -242,6 +243,29 @@ typedef struct {
     uint8_t  dt, sdt, zeros;
 } irx_mv4_t;
 
+#define IRX_ROPE_MAX 128               /* rotated pairs of a head of 256 */
+typedef struct {
+    irx_kvc_t c;                       /* rope_append only; rope: dim and dt alone */
+    int64_t  n;                        /* tokens */
+    int64_t  x_stride, y_stride;       /* elements between two tokens' rows, read and written */
+    int32_t  heads, pairs;
+    float    amp;
+    uint8_t  inter;
+    double   freq[IRX_ROPE_MAX];       /* turns a position (negative in the transposed rotation) */
+} irx_ropep_t;
+
+typedef struct {
+    int64_t  tokens, q_stride, kv_stride;
+    int32_t  batch, heads, kv_heads, dim, window, sinks;
+    uint32_t scale_bits;
+    uint8_t  dt, lse;
+} irx_prm_t;
+
+typedef struct {
+    int64_t  rows, vocab, stride;
+    uint8_t  dt, logprob;
+} irx_smp_t;
+
 typedef struct {
     uint32_t magic;
     uint8_t  fam;
@@ -251,12 +275,14 @@ typedef struct {
     int64_t  arg_elems[KIR_MAX_ARG];
     char     kname[KIR_MAX_NAME + 1];
     union { irx_pw_t pw; irx_red_t red; irx_row_t row; irx_mm_t mm; irx_at_t at; irx_kirk_t kk;
-            irx_dec_t dec; irx_kv_t kv; irx_mv4_t mv; } u;
+            irx_dec_t dec; irx_kv_t kv; irx_mv4_t mv; irx_ropep_t ro; irx_prm_t pr; irx_smp_t sm; } u;
 } irx_plan_int_t;
 
 int irx_kirgen(const kir_t *k, irx_plan_int_t *p);
 void irx_serve_text(const irx_plan_int_t *p, char *buf, size_t cap);
 void irx_serve_work(const irx_plan_int_t *p, double *bytes, double *flops);
+void irx_step_text(const irx_plan_int_t *p, char *buf, size_t cap);
+void irx_step_work(const irx_plan_int_t *p, double *bytes, double *flops);
 
 /* Shard s of ns of a plan's units (irx_plan_units): the one split of every launcher; narrowed to
  * [a, b) on this thread while irx_unit_window(a, b) is set (b < 0 clears it). */

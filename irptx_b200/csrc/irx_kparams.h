@@ -186,4 +186,56 @@ typedef struct {
     uint64_t    gmul;               /* group of k: (k / 32 * gmul) >> gshift */
 } irx_kmv4_t;
 
+/* Rotary positions, alone (kv = 0) or on the way into a paged cache: items of two vectors of a head's row. */
+typedef struct {
+    const void *q, *kn, *vn;        /* queries (or the rows to turn), new keys and values */
+    const int32_t *pos, *seq, *table;
+    void       *qo, *k, *v;
+    unsigned   *err;
+    int64_t     x_stride, kv_stride, y_stride, page_stride, head_stride, token_stride, pages;   /* in elements */
+    int64_t     t0, t1;             /* tokens of this launch */
+    int32_t     heads, kv, d, pairs;
+    int32_t     batch, cols, page_size;
+    int32_t     items;              /* items of a head's row */
+    int32_t     parts, chunk;       /* warps per token, items per warp */
+    float       amp;
+    uint8_t     inter, pad[3];
+    double      freq[128];          /* turns a position */
+} irx_krope_t;
+
+/* Attention over packed prompts. Units: tiles of query rows (token, head of the group) of a sequence and a
+ * key-value head. Shared memory of the FP32 kernel: three tiles of 64 rows and the weights. */
+#define IRX_PR_ST_SMEM(dp) ((3 * 64 * ((dp) + 4) + 64 * 68) * 4)
+
+typedef struct {
+    const void *q, *k, *v;
+    const int32_t *starts;
+    void       *o;
+    float      *lse;                /* NULL: not asked for */
+    unsigned   *err;
+    int64_t     tokens, q_stride, kv_stride;
+    int32_t     batch, heads, kv_heads, group, d;
+    int32_t     h0, h1;             /* kv heads of this launch (a shard) */
+    int32_t     window, sinks;
+    float       scale2;             /* scale * log2(e), not zero */
+    uint8_t     dt, vec, pad[2];
+} irx_kprm_t;
+
+/* The draw of a token: one cluster a row. */
+#define IRX_SMP_BINS 2048
+#define IRX_SMP_THREADS 512
+#define IRX_SMP_FIXED (IRX_SMP_BINS * 12 + 2048)   /* shared memory beside the row: histogram, reductions */
+
+typedef struct {
+    const void *x;
+    const float *temperature, *top_p, *min_p, *u;
+    const int32_t *top_k;
+    int32_t    *token;
+    float      *logprob;            /* NULL: not asked for */
+    int64_t     r0, stride, n;
+    int64_t     per;                /* elements of a block, a multiple of 8 per warp */
+    int32_t     kbits;              /* a weight of 1 is 2^kbits */
+    uint8_t     vec, pad[3];
+} irx_ksmp_t;
+
 #endif /* IRX_KPARAMS_H */

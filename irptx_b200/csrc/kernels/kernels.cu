@@ -8,3 +8,6 @@
 #include "kvpages.cu"
 #include "decode.cu"
 #include "matvec4.cu"
+#include "rope.cu"
+#include "prompt.cu"
+#include "sample.cu"

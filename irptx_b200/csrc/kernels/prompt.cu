@@ -1,0 +1,275 @@
+// prompt.cu -- causal attention over packed prompts: O = softmax(Q K^T * scale, masked) V, sequence by
+// sequence, grouped heads.
+//
+// Sequence s is the tokens [starts[s], starts[s + 1]) of the packed rows; token i of a sequence sees
+// its tokens j <= i, with a window those with j > i - window or j < sinks. The query heads that share a
+// key-value head are rows of the same tiles: row r of a (sequence, key-value head) is token
+// r / group, head r % group, so a short prompt fills a tile with its heads and every key tile
+// read serves the whole group.
+//
+// A unit is one tile of rows of one (sequence, key-value head). The blocks find their units from
+// `starts` alone, heaviest first: units are numbered by their tile's place in its sequence,
+// from the last place down, and block b takes units b, b + blocks, ...; nothing on the host and no
+// counter in memory is needed, and a row's result does not depend on which block takes it.
+#pragma once
+#include "tc.cuh"
+
+struct pr_unit { int base, len, tile, head; };          // first row of the sequence, its tokens, tile, kv head
+
+// Tokens of sequence s0 + lane (0 past the last one), and its first row. 0 too, and `bad`, when its starts fall, leave the
+// packed rows, or an earlier start is above its own: then no two sequences share a row. highest: the largest
+// start so far, INT_MIN at first. A whole warp calls it.
+__device__ __forceinline__ int pr_len(const irx_kprm_t &p, int s0, int &highest, int &base, bool &bad)
+{
+    const int lane = threadIdx.x & 31, s = s0 + lane;
+    int a = 0x80000000, b = 0;
+    if (s < p.batch) {
+        a = p.starts[s];
+        b = p.starts[s + 1];
+    }
+    int m = a;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, m, o);
+        if (lane >= o) m = max(m, x);
+    }
+    m = max(m, highest);
+    highest = __shfl_sync(0xffffffffu, m, 31);
+    base = a;
+    bad = s < p.batch && (a < 0 || b < a || b > p.tokens || m > a);
+    return s < p.batch && !bad ? b - a : 0;
+}
+
+// Tiles of a sequence of n tokens: mul rows a token, per rows a tile.
+__device__ __forceinline__ int pr_tiles(int n, int mul, int per)
+{
+    return (int)(((int64_t)n * mul + per - 1) / per);
+}
+
+// Per key-value head: units whose tile is number t or later, over all sequences. A whole warp calls it.
+__device__ __forceinline__ int pr_count(const irx_kprm_t &p, int t, int mul, int per, int &most)
+{
+    int n = 0, base, highest = 0x80000000;
+    bool bad;
+    most = 0;
+    for (int s0 = 0; s0 < p.batch; s0 += 32) {
+        const int nt = pr_tiles(pr_len(p, s0, highest, base, bad), mul, per);
+        n += max(0, nt - t);
+        most = max(most, nt);
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    return __reduce_add_sync(0xffffffffu, n);
+}
+
+// Unit u, u below pr_count(0) * heads; most: the largest sequence's tiles. A whole warp calls it.
+__device__ __forceinline__ pr_unit pr_find(const irx_kprm_t &p, int64_t u, int most, int mul, int per)
+{
+    const int nh = p.h1 - p.h0;
+    int lo = 0, hi = most, after = 0, m;
+    while (hi - lo > 1) {                                // the last t with u below the units of tiles t and later
+        const int mid = (lo + hi) >> 1, c = pr_count(p, mid, mul, per, m);
+        if ((int64_t)c * nh > u) lo = mid;
+        else {
+            hi = mid;
+            after = c;
+        }
+    }
+    const int64_t off = u - (int64_t)after * nh;
+    int skip = (int)(off / nh), highest = 0x80000000;    // among the sequences that have a tile number lo
+    pr_unit r = {0, 0, lo, p.h0 + (int)(off % nh)};
+    for (int s0 = 0; s0 < p.batch; s0 += 32) {
+        int base;
+        bool bad;
+        const int n = pr_len(p, s0, highest, base, bad);
+        const unsigned has = __ballot_sync(0xffffffffu, pr_tiles(n, mul, per) > lo);
+        const int c = __popc(has);
+        if (skip < c) {
+            const int at = __fns(has, 0, skip + 1);
+            r.base = __shfl_sync(0xffffffffu, base, at);
+            r.len = __shfl_sync(0xffffffffu, n, at);
+            break;
+        }
+        skip -= c;
+    }
+    return r;
+}
+
+// One warp reports sequences that are skipped.
+__device__ __forceinline__ void pr_report(const irx_kprm_t &p)
+{
+    int base, highest = 0x80000000;
+    for (int s0 = 0; s0 < p.batch; s0 += 32) {
+        bool bad;
+        pr_len(p, s0, highest, base, bad);
+        if (bad) atomicOr(p.err, IRX_KERR_INDEX);
+    }
+}
+
+// ---- FP32 units: f32 rows, and bf16 rows that the matrix instructions do not take ----
+//
+// 64 query rows against tiles of 64 keys, all as f32 in shared memory; 256 threads hold 4 x 4 scores and
+// 4 rows x DP / 16 columns of the output each, in registers. Rows of Q and K are padded by four
+// floats, so that the 16 key rows read together fall into different banks. Bound by the FP32 units
+// and the shared memory that feeds them.
+#define PS_ROWS 64
+#define PS_KEYS 64
+
+template <int DP>
+__device__ __forceinline__ void ps_fill(float *dst, const void *src, int dt, int64_t row0, int64_t stride, int64_t off, int n, int d, bool vec)
+{
+    // n rows of d numbers into 64 rows of DP + 4, zeros behind both
+    if (vec && dt == DT_F32) {
+        for (int e = threadIdx.x; e < 64 * (DP / 4); e += 256) {
+            const int r = e / (DP / 4), c = (e % (DP / 4)) * 4;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < n && c < d) x = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(src) + (row0 + r) * stride + off + c);
+            *reinterpret_cast<float4 *>(dst + r * (DP + 4) + c) = x;
+        }
+        return;
+    }
+    for (int e = threadIdx.x; e < 64 * DP; e += 256) {
+        const int r = e / DP, c = e % DP;
+        dst[r * (DP + 4) + c] = r < n && c < d ? irx_ld1(src, dt, (row0 + r) * stride + off + c) : 0.0f;
+    }
+}
+
+template <int DP>
+__device__ __forceinline__ void ps_body(const irx_kprm_t &p)
+{
+    irx_pdl_enter();
+    extern __shared__ __align__(16) float ps_smem[];
+    float *sq = ps_smem, *sk = sq + 64 * (DP + 4), *sv = sk + 64 * (DP + 4), *sp = sv + 64 * (DP + 4);
+    constexpr int NC = DP / 64;                          // 4-column groups of the output a thread owns
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    int most;
+    const int64_t units = (int64_t)pr_count(p, 0, p.group, PS_ROWS, most) * (p.h1 - p.h0);
+    if (blockIdx.x == 0 && threadIdx.x < 32) pr_report(p);
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const pr_unit un = pr_find(p, u, most, p.group, PS_ROWS);
+        const int64_t r0 = (int64_t)un.tile * PS_ROWS, rows = (int64_t)un.len * p.group;
+        const int nr = (int)min((int64_t)PS_ROWS, rows - r0);
+        const int first = (int)(r0 / p.group), last = (int)((r0 + nr - 1) / p.group);
+        __syncthreads();                                 // the tile before is done with
+        for (int e = threadIdx.x; e < 64 * DP; e += 256) {
+            const int r = e / DP, c = e % DP;
+            float x = 0.0f;
+            if (r < nr && c < p.d) {
+                const int64_t tok = (r0 + r) / p.group;
+                const int h = un.head * p.group + (int)((r0 + r) - tok * p.group);
+                x = irx_ld1(p.q, p.dt, (un.base + tok) * p.q_stride + (int64_t)h * p.d + c);
+            }
+            sq[r * (DP + 4) + c] = x;
+        }
+        int tok[4];
+        float m[4], l[4], o[4][NC * 4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = min(ty * 4 + i, nr - 1);
+            tok[i] = (int)((r0 + r) / p.group);
+            m[i] = -3.0e38f;
+            l[i] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NC * 4; c++) o[i][c] = 0.0f;
+        }
+        const int lo = p.window ? max(0, first - p.window + 1) : 0, sinks = min(p.sinks, lo);
+        const int nsink = (sinks + PS_KEYS - 1) / PS_KEYS, ntiles = nsink + (last - lo) / PS_KEYS + 1;
+        for (int kt = 0; kt < ntiles; kt++) {
+            const int kb = kt < nsink ? kt * PS_KEYS : lo + (kt - nsink) * PS_KEYS;
+            const int kend = kt < nsink ? sinks : last + 1, nk = min(PS_KEYS, kend - kb);
+            // a tile that some row does not see in whole: masked, and its weights of zero add nothing
+            const bool cut = kt < nsink || nk < PS_KEYS || kb + PS_KEYS - 1 > first || (p.window && kb <= last - p.window);
+            __syncthreads();
+            ps_fill<DP>(sk, p.k, p.dt, un.base + kb, p.kv_stride, (int64_t)un.head * p.d, nk, p.d, p.vec);
+            ps_fill<DP>(sv, p.v, p.dt, un.base + kb, p.kv_stride, (int64_t)un.head * p.d, nk, p.d, p.vec);
+            __syncthreads();
+            float s[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) s[i][j] = 0.0f;
+#pragma unroll 2
+            for (int c = 0; c < DP; c += 4) {
+                float4 a[4], b[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    a[i] = *reinterpret_cast<const float4 *>(sq + (ty * 4 + i) * (DP + 4) + c);
+                    b[i] = *reinterpret_cast<const float4 *>(sk + (tx + 16 * i) * (DP + 4) + c);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        s[i][j] = fmaf(a[i].w, b[j].w, fmaf(a[i].z, b[j].z, fmaf(a[i].y, b[j].y, fmaf(a[i].x, b[j].x, s[i][j]))));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float mx = -3.0e38f;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int key = kb + tx + 16 * j;
+                    s[i][j] *= p.scale2;
+                    if (cut && (key >= kend || key > tok[i] || (p.window && key <= tok[i] - p.window && key >= p.sinks))) s[i][j] = -INFINITY;
+                    mx = s[i][j] > mx || s[i][j] != s[i][j] ? s[i][j] : mx;      // a NaN stays
+                }
+#pragma unroll
+                for (int x = 8; x; x >>= 1) {
+                    const float y = __shfl_xor_sync(0xffffffffu, mx, x);
+                    mx = y > mx || y != y ? y : mx;
+                }
+                const float mn = m[i] > mx || m[i] != m[i] ? m[i] : mx, r = exp2f(m[i] - mn);
+                float sum = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    s[i][j] = exp2f(s[i][j] - mn);
+                    sum += s[i][j];
+                    sp[(ty * 4 + i) * 68 + tx + 16 * j] = s[i][j];
+                }
+#pragma unroll
+                for (int x = 8; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+                m[i] = mn;
+                l[i] = l[i] * r + sum;
+#pragma unroll
+                for (int c = 0; c < NC * 4; c++) o[i][c] *= r;
+            }
+            __syncwarp();                                // a row's weights are made and read by one half warp
+            for (int j = 0; j < PS_KEYS; j++) {
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = sp[(ty * 4 + i) * 68 + j];
+#pragma unroll
+                for (int g = 0; g < NC; g++) {
+                    const float4 x = *reinterpret_cast<const float4 *>(sv + j * (DP + 4) + g * 64 + tx * 4);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if (cut && w[i] == 0.0f) continue;
+                        o[i][g * 4] = fmaf(w[i], x.x, o[i][g * 4]);
+                        o[i][g * 4 + 1] = fmaf(w[i], x.y, o[i][g * 4 + 1]);
+                        o[i][g * 4 + 2] = fmaf(w[i], x.z, o[i][g * 4 + 2]);
+                        o[i][g * 4 + 3] = fmaf(w[i], x.w, o[i][g * 4 + 3]);
+                    }
+                }
+            }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = ty * 4 + i;
+            if (r >= nr) continue;
+            const int h = un.head * p.group + (int)((r0 + r) - (int64_t)tok[i] * p.group);
+            const int64_t row = (int64_t)(un.base + tok[i]) * p.heads + h;
+            const float inv = 1.0f / l[i];
+            if (p.lse && tx == 0) p.lse[row] = (m[i] + log2f(l[i])) * 0.6931471806f;
+#pragma unroll
+            for (int g = 0; g < NC; g++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const int col = g * 64 + tx * 4 + c;
+                    if (col < p.d) irx_st1(p.o, p.dt, row * p.d + col, o[i][g * 4 + c] * inv);
+                }
+        }
+    }
+}
+
+extern "C" __global__ void __launch_bounds__(256) irx_prompt_st_64(const __grid_constant__ irx_kprm_t p) { ps_body<64>(p); }
+extern "C" __global__ void __launch_bounds__(256) irx_prompt_st_128(const __grid_constant__ irx_kprm_t p) { ps_body<128>(p); }
+extern "C" __global__ void __launch_bounds__(256) irx_prompt_st_256(const __grid_constant__ irx_kprm_t p) { ps_body<256>(p); }

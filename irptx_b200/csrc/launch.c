@@ -165,7 +165,10 @@ static const char *const KNAMES[K_COUNT] = {
     "irx_kv_copy_16", "irx_kv_copy_4", "irx_kv_copy_2",
     "irx_mv4_bf16_32_1", "irx_mv4_bf16_32_2", "irx_mv4_bf16_64_1", "irx_mv4_bf16_64_2", "irx_mv4_bf16_128_1", "irx_mv4_bf16_128_2",
     "irx_mv4_f32_32_1", "irx_mv4_f32_32_2", "irx_mv4_f32_64_1", "irx_mv4_f32_64_2", "irx_mv4_f32_128_1", "irx_mv4_f32_128_2",
-    "irx_mv4_any"
+    "irx_mv4_any",
+    "irx_rope_bf16_8", "irx_rope_bf16_1", "irx_rope_f32_4", "irx_rope_f32_1",
+    "irx_prompt_st_64", "irx_prompt_st_128", "irx_prompt_st_256",
+    "irx_sample_bf16", "irx_sample_bf16_far", "irx_sample_f32", "irx_sample_f32_far"
 };
 
 static irx_dev_t CTX[MAX_CTX];
@@ -544,7 +547,7 @@ int irx_dev_check_err(irx_dev_t *d, void *s)
         irx_dev_memset32(d->err, 0, 1, s);
         irx_dev_sync(s);
         if (e & IRX_KERR_INDEX && !(e & ~IRX_KERR_INDEX))
-            return irx_fail(E093, "a page, sequence, position or length outside the cache (the access was skipped)");
+            return irx_fail(E093, "a page, sequence, position, length or start outside its buffer (the access was skipped)");
         return irx_fail(E092, e & IRX_KERR_TIMEOUT ? "a kernel whose bounded device wait ran out (error word set)"
                                                    : "a kernel that set its device error word");
     }

@@ -17,7 +17,9 @@ enum {
      * width, matrix-vector products by type, group grain and 8-column blocks */
     K_DEC_TC, K_DEC_ST = K_DEC_TC + 5, K_KV_APPEND = K_DEC_ST + 6, K_KV_COPY = K_KV_APPEND + 3,
     K_MV4 = K_KV_COPY + 3, K_MV4_ANY = K_MV4 + 12,
-    K_COUNT
+    /* rotary positions by type and vector, prompt attention by padded head size, the draw by type and residence */
+    K_ROPE, K_PR_ST = K_ROPE + 4, K_SMP = K_PR_ST + 3,
+    K_COUNT = K_SMP + 4
 };
 
 /* Per-context scratch: a 256-byte head (the error word) and IRX_SLOTS launch slots, each with

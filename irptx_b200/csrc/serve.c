@@ -5,49 +5,12 @@
  * own; the plan it compiles to is an ordinary one. Kernels: kernels/decode.cu, kvpages.cu and
  * matvec4.cu. */
 
-#include <stdio.h>
-#include <string.h>
-#include "irx_int.h"
-#include "irx_kparams.h"
-#include "launch.h"
-#include "../../include/irx.h"
+#include "serve.h"
 
-#define MAX_DIM 256
-#define MAX_COUNT 0x7fffffffll
-#define MAX_STRIDE (1ll << 40)
 #define MAX_32 (1ll << 30)
-#define MAX_SPAN 9e17                      /* elements; sums of a few stay below 2^63 */
-
-static int esz(int dt) { return dt == DT_BF16 ? 2 : dt == DT_U8 ? 1 : 4; }
-
-static int float_dt(int dt) { return dt == DT_BF16 || dt == DT_F32; }
-
-static irx_plan_int_t *begin(irx_plan_t *plan, int fam, const char *name)
-{
-    irx_plan_int_t *p = (irx_plan_int_t *)plan;
-    irx_clear_error();
-    if (!plan) {
-        irx_fail(E093, "a compile with no plan storage");
-        return NULL;
-    }
-    memset(plan, 0, sizeof *plan);
-    p->fam = (uint8_t)fam;
-    snprintf(p->kname, sizeof p->kname, "%s", name);
-    return p;
-}
-
-static void add(irx_plan_int_t *p, int kind, int dt, int64_t elems)
-{
-    p->arg_kind[p->narg] = (uint8_t)kind;
-    p->arg_dt[p->narg] = (uint8_t)dt;
-    p->arg_elems[p->narg] = elems;
-    p->narg++;
-}
-
-static int finish(irx_plan_int_t *p) { p->magic = IRX_PLAN_MAGIC; return 0; }
 
 /* Elements from the first to past the last of a pool. */
-static int64_t span(const irx_kvc_t *c)
+int64_t irx_cache_span(const irx_kvc_t *c)
 {
     return (c->pages - 1) * c->page_stride + (int64_t)(c->heads - 1) * c->head_stride +
            (int64_t)(c->page_size - 1) * c->token_stride + c->dim;
@@ -73,7 +36,7 @@ static int rows_overlap(const irx_kvc_t *c)
     return 0;
 }
 
-static int cache_of(irx_kvc_t *o, const irx_kv_cache_t *c, int tabled)
+int irx_cache_of(irx_kvc_t *o, const irx_kv_cache_t *c, int tabled)
 {
     if (!c) return irx_fail(E093, "an operator over no cache descriptor");
     if (!float_dt(c->dtype)) return irx_fail(E024, "a cache whose dtype is not f32 or bf16");
@@ -125,7 +88,7 @@ int irx_compile_decode(const irx_kv_cache_t *cache, int heads, long long q_strid
     int g, i;
     if (!p) return 1;
     a = &p->u.dec;
-    if (cache_of(&a->c, cache, 1)) return 1;
+    if (irx_cache_of(&a->c, cache, 1)) return 1;
     if (heads < 1 || heads % a->c.heads) return irx_fail(E042, "query heads that are not a multiple of the cache's heads");
     if (window < 0 || sinks < 0) return irx_fail(E042, "a window or sink count below 0");
     if (sinks && !window) return irx_fail(E042, "sinks without a window");
@@ -151,8 +114,8 @@ int irx_compile_decode(const irx_kv_cache_t *cache, int heads, long long q_strid
     a->max_ctas = chunks < IRX_DEC_MAX_CTAS ? (int32_t)chunks : IRX_DEC_MAX_CTAS;
     if (dec_units(a) > MAX_COUNT) return irx_fail(E042, "more than 2^31 - 1 rows of work");
     add(p, KA_IN, a->c.dt, (int64_t)(a->c.batch - 1) * a->q_stride + qrow);
-    add(p, KA_IN, a->c.dt, span(&a->c));
-    add(p, KA_IN, a->c.dt, span(&a->c));
+    add(p, KA_IN, a->c.dt, irx_cache_span(&a->c));
+    add(p, KA_IN, a->c.dt, irx_cache_span(&a->c));
     add(p, KA_IN, DT_I32, (int64_t)a->c.batch * a->c.cols);
     add(p, KA_IN, DT_I32, a->c.batch);
     add(p, KA_OUT, a->c.dt, (int64_t)a->c.batch * qrow);
@@ -161,9 +124,7 @@ int irx_compile_decode(const irx_kv_cache_t *cache, int heads, long long q_strid
     return finish(p);
 }
 
-static int a_to(const void *q, size_t n) { return ((size_t)q % n) == 0; }
-
-static int serve_grid(irx_dev_t *d, int k, int block, size_t smem, int64_t want, int64_t *g)
+int irx_serve_grid(irx_dev_t *d, int k, int block, size_t smem, int64_t want, int64_t *g)
 {
     if (!d->occ[k] && irx_dev_occupancy(d, k, block, smem, &d->occ[k])) return 1;
     *g = (int64_t)d->sms * d->occ[k];
@@ -226,7 +187,7 @@ static int launch_decode(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
         smem = (size_t)IRX_DEC_ST_SMEM(a->dp, rows, 1);
         block = 32 * IRX_DEC_ST_NW(a->dp);
     }
-    if (serve_grid(d, kk, block, smem, a->max_ctas, &grid)) return 1;
+    if (irx_serve_grid(d, kk, block, smem, a->max_ctas, &grid)) return 1;
     return irx_dev_launch(d, kk, (unsigned)grid, (unsigned)block, (unsigned)smem, 1, st, &k);
 }
 
@@ -239,7 +200,7 @@ int irx_compile_kv_append(const irx_kv_cache_t *cache, long long tokens, long lo
     int64_t row;
     if (!p) return 1;
     a = &p->u.kv;
-    if (cache_of(&a->c, cache, 1)) return 1;
+    if (irx_cache_of(&a->c, cache, 1)) return 1;
     row = (int64_t)a->c.heads * a->c.dim;
     if (tokens < 1 || tokens > MAX_COUNT) return irx_fail(E042, "an append of no tokens");
     if (row > (1 << 20)) return irx_fail(E042, "a token's keys past 2^20 elements");
@@ -252,8 +213,8 @@ int irx_compile_kv_append(const irx_kv_cache_t *cache, long long tokens, long lo
     add(p, KA_IN, DT_I32, tokens);
     add(p, KA_IN, DT_I32, tokens);
     add(p, KA_IN, DT_I32, (int64_t)a->c.batch * a->c.cols);
-    add(p, KA_OUT, a->c.dt, span(&a->c));
-    add(p, KA_OUT, a->c.dt, span(&a->c));
+    add(p, KA_OUT, a->c.dt, irx_cache_span(&a->c));
+    add(p, KA_OUT, a->c.dt, irx_cache_span(&a->c));
     p->arg_zero[5] = p->arg_zero[6] = 1;
     return finish(p);
 }
@@ -264,21 +225,21 @@ int irx_compile_kv_copy(const irx_kv_cache_t *cache, long long pairs, int layers
     irx_kv_t *a;
     if (!p) return 1;
     a = &p->u.kv;
-    if (cache_of(&a->c, cache, 0)) return 1;
+    if (irx_cache_of(&a->c, cache, 0)) return 1;
     if (pairs < 1 || pairs > MAX_COUNT) return irx_fail(E042, "a copy of no pages");
     if (layers < 1) return irx_fail(E042, "a copy in no layers");
-    if (layer_stride < 0 || layer_stride > MAX_STRIDE || (layers > 1 && layer_stride && layer_stride < span(&a->c)))
+    if (layer_stride < 0 || layer_stride > MAX_STRIDE || (layers > 1 && layer_stride && layer_stride < irx_cache_span(&a->c)))
         return irx_fail(E041, "layers whose pools overlap");
     a->n = pairs;
     a->layers = layers;
     a->layer_stride = layer_stride ? layer_stride : a->c.pages * a->c.page_stride;
-    if (layers > 1 && a->layer_stride < span(&a->c)) return irx_fail(E041, "layers whose pools overlap");
+    if (layers > 1 && a->layer_stride < irx_cache_span(&a->c)) return irx_fail(E041, "layers whose pools overlap");
     if ((double)layers * a->layer_stride > MAX_SPAN) return irx_fail(E042, "a cache larger than an address space");
     if ((double)pairs * layers * a->c.heads * a->c.page_size * a->c.dim > MAX_SPAN)
         return irx_fail(E042, "a copy of more elements than 64 bits count");
     add(p, KA_IN, DT_I32, 2 * pairs);
-    add(p, KA_OUT, a->c.dt, (layers - 1) * a->layer_stride + span(&a->c));
-    add(p, KA_OUT, a->c.dt, (layers - 1) * a->layer_stride + span(&a->c));
+    add(p, KA_OUT, a->c.dt, (layers - 1) * a->layer_stride + irx_cache_span(&a->c));
+    add(p, KA_OUT, a->c.dt, (layers - 1) * a->layer_stride + irx_cache_span(&a->c));
     p->arg_zero[1] = p->arg_zero[2] = 1;
     return finish(p);
 }
@@ -357,7 +318,7 @@ static int launch_copy(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsign
     k.n1 = (int32_t)n1; k.n2 = (int32_t)n2; k.layers = a->layers;
     k.tiles = (k.run * n1 * n2 + IRX_COPY_TILE - 1) / IRX_COPY_TILE;
     want = (u1 - u0) * k.tiles * a->layers * 2;
-    if (serve_grid(d, K_KV_COPY + w, 256, 0, want, &grid)) return 1;
+    if (irx_serve_grid(d, K_KV_COPY + w, 256, 0, want, &grid)) return 1;
     return irx_dev_launch(d, K_KV_COPY + w, (unsigned)grid, 256, 0, 1, st, &k);
 }
 
@@ -472,7 +433,7 @@ static int launch_mv4(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsigne
         }
         return irx_dev_launch(d, K_MV4 + 6 * f32 + gv * 2 + nt - 1, (unsigned)(tiles * ck), 256, smem, ck, st, &k);
     }
-    if (serve_grid(d, K_MV4_ANY, 256, 0, ((u1 - u0) * ((a->m + 3) / 4) + 7) / 8, &grid)) return 1;
+    if (irx_serve_grid(d, K_MV4_ANY, 256, 0, ((u1 - u0) * ((a->m + 3) / 4) + 7) / 8, &grid)) return 1;
     return irx_dev_launch(d, K_MV4_ANY, (unsigned)grid, 256, 0, 1, st, &k);
 }
 
@@ -490,8 +451,6 @@ int irx_launch_serve(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsigned
     default: return launch_mv4(p, d, s, ns, args, st);
     }
 }
-
-static const char *dname(int dt) { return dt == DT_BF16 ? "bf16" : "f32"; }
 
 void irx_serve_text(const irx_plan_int_t *p, char *buf, size_t cap)
 {
