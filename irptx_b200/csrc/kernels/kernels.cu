@@ -10,4 +10,5 @@
 #include "matvec4.cu"
 #include "rope.cu"
 #include "prompt.cu"
+#include "prompt_tc.cu"
 #include "sample.cu"
