@@ -9,7 +9,7 @@
 //
 // A unit is one tile of rows of one (sequence, key-value head). The blocks find their units from
 // `starts` alone, heaviest first: units are numbered by their tile's place in its sequence,
-// from the last place down, and block b takes units b, b + blocks, ...; nothing on the host and no
+// from the last place down, and the blocks take them in turns; nothing on the host and no
 // counter in memory is needed, and a row's result does not depend on which block takes it.
 #pragma once
 #include "tc.cuh"
@@ -94,6 +94,12 @@ __device__ __forceinline__ pr_unit pr_find(const irx_kprm_t &p, int64_t u, int m
     return r;
 }
 
+// This block's unit of turn i: the blocks take turns forwards and backwards, so that none has the heaviest of each.
+__device__ __forceinline__ int64_t pr_turn(int i)
+{
+    return (int64_t)i * gridDim.x + (i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+
 // One warp reports sequences that are skipped.
 __device__ __forceinline__ void pr_report(const irx_kprm_t &p)
 {
@@ -144,7 +150,9 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
     int most;
     const int64_t units = (int64_t)pr_count(p, 0, p.group, PS_ROWS, most) * (p.h1 - p.h0);
     if (blockIdx.x == 0 && threadIdx.x < 32) pr_report(p);
-    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    for (int turn = 0;; turn++) {
+        const int64_t u = pr_turn(turn);
+        if (u >= units) break;
         const pr_unit un = pr_find(p, u, most, p.group, PS_ROWS);
         const int64_t r0 = (int64_t)un.tile * PS_ROWS, rows = (int64_t)un.len * p.group;
         const int nr = (int)min((int64_t)PS_ROWS, rows - r0);

@@ -94,7 +94,7 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
         int ok = 1;
         for (int uc = 0; ok; uc++) {
             const int us = uc & 1;
-            const int64_t u = blockIdx.x + (int64_t)uc * gridDim.x;
+            const int64_t u = pr_turn(uc);
             pt_info f = {};
             if (u < units) {
                 const pr_unit un = pr_find(p, u, most, 1, 2 * tp);
@@ -148,7 +148,7 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
             ok = __shfl_sync(0xffffffffu, ok, 0);
         }
       } else if (warp == 9) {
-        if (lane == 0) {                                      // MMA: P0 V, S0', P1 V, S1' per key tile
+        if (elect_one()) {                                    // MMA: P0 V, S0', P1 V, S1' per key tile
             const uint32_t id_qk = umma_idesc_bf16(128, 128, 0), id_pv = umma_idesc_bf16(128, DP, 1);
             const uint32_t sq_a = irx_smem_u32(sq), sk_a = irx_smem_u32(sk), sv_a = irx_smem_u32(sv);
             bool ok = true;
