@@ -224,7 +224,7 @@ typedef struct {
     uint8_t     dt, vec, pad[2];
 } irx_kprm_t;
 
-/* The draw of a token: one cluster a row. */
+/* The draw of a token: one cluster a row; a thread of a block holds `words` words of 4 bytes, an odd number. */
 #define IRX_SMP_BINS 2048
 #define IRX_SMP_THREADS 512
 #define IRX_SMP_FIXED (IRX_SMP_BINS * 12 + 2048)   /* shared memory beside the row: histogram, reductions */
@@ -235,10 +235,12 @@ typedef struct {
     const int32_t *top_k;
     int32_t    *token;
     float      *logprob;            /* NULL: not asked for */
+    unsigned   *err;
     int64_t     r0, stride, n;
-    int64_t     per;                /* elements of a block, a multiple of 8 per warp */
-    int32_t     kbits;              /* a weight of 1 is 2^kbits */
-    uint8_t     vec, pad[3];
+    int32_t     words;
+    int32_t     kbits;              /* a weight of 1 is 2^kbits, at most 2^46 */
+    uint8_t     vec, pad[7];        /* rows of logits begin on 16 bytes */
+    double      tab[32];            /* 2^(kbits + j / 32) */
 } irx_ksmp_t;
 
 #endif /* IRX_KPARAMS_H */

@@ -9,82 +9,115 @@
 // at which the kept weights' running sum passes u times their total.
 //
 // One cluster of 1 to 8 blocks a row; the row is read once, into the blocks' shared memory (rows too long for
-// that are read again for each pass). A threshold is found by histograms of 2048 cells over the blocks:
-// first of (max - x) in equal steps, up to where weights round to zero, then of the bits of the cell's
-// range, until the cell is a single number. Every block adds up an equal slice of the cells.
+// that are read again for each pass), where thread t holds words t * words and on: an odd number of
+// them, so that a warp's reads fall into 32 banks. Tokens per cell of (max - x), 2048 equal cells up to where
+// weights round to zero, or their weights, show the cell in which a filter ends. When that cell and those
+// above it hold few tokens (top-k, or a peaked row), they go to the first block, which finishes alone. Otherwise
+// histograms of the cell's own range follow until it is a single number.
 #pragma once
 #include "tc.cuh"
 
 #define SMP_WARPS (IRX_SMP_THREADS / 32)
-#define SMP_NEG_INF 0x007fffffu          // the key of -infinity
+#define SMP_FEW 1024                     // tokens that one block finishes alone
 
 struct smp_shared {
-    unsigned cnt[IRX_SMP_BINS], lo[IRX_SMP_BINS], hi[IRX_SMP_BINS];      // a cell's tokens and its weight, in two words
-    double tab[32];                      // 2^(j / 32)
+    union {
+        struct { unsigned cnt[IRX_SMP_BINS], lo[IRX_SMP_BINS], hi[IRX_SMP_BINS]; };   // a cell's tokens; its weight, in two words
+        struct { uint64_t mine[SMP_FEW], list[SMP_FEW], weight_of[SMP_FEW]; };        // few tokens: this block's, the row's, their weights
+    };
+    double tab[32];
     uint64_t red[SMP_WARPS], xa[2][8];   // warps' parts; what every block of the cluster posted, two exchanges of it
     unsigned redc[SMP_WARPS], xc[2][8];
     uint64_t before, weight;             // the cell found: the weight above it, its own
-    unsigned above, count, cell;
+    unsigned above, count, cell, total;
+    unsigned few, listed, drawn;
+    uint64_t bar;
 };
 static_assert(sizeof(smp_shared) <= IRX_SMP_FIXED, "the launcher's size");
 
-// Keys order as the logits do: equal numbers (both zeros) have equal keys, NaN counts as -infinity.
-__device__ __forceinline__ unsigned smp_key(float x)
-{
-    const unsigned u = __float_as_uint(x == x ? x + 0.0f : -INFINITY);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-
-__device__ __forceinline__ float smp_value(unsigned key)
-{
-    return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
-}
+// A word's elements as numbers: NaN as -infinity, both zeros as +0, so that equal logits are equal numbers.
+template <class T> struct smp_type;
+template <> struct smp_type<float> {
+    static const int N = 1;
+    static const unsigned PAD = 0xff800000u;
+    __device__ static __forceinline__ float get(unsigned w, int)
+    {
+        const float x = __uint_as_float(w) + 0.0f;
+        return x == x ? x : -INFINITY;
+    }
+    __device__ static __forceinline__ unsigned max2(unsigned a, unsigned b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+    // keys order as the numbers do
+    __device__ static __forceinline__ unsigned key(float x)
+    {
+        const unsigned u = __float_as_uint(x);
+        return u & 0x80000000u ? ~u : u | 0x80000000u;
+    }
+    __device__ static __forceinline__ float value(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+};
+template <> struct smp_type<__nv_bfloat16> {
+    static const int N = 2;
+    static const unsigned PAD = 0xff80ff80u;
+    __device__ static __forceinline__ float get(unsigned w, int h)
+    {
+        const float x = __uint_as_float(h ? w & 0xffff0000u : w << 16) + 0.0f;
+        return x == x ? x : -INFINITY;
+    }
+    __device__ static __forceinline__ unsigned max2(unsigned a, unsigned b)
+    {
+        const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
+        return *reinterpret_cast<const unsigned *>(&m);
+    }
+    __device__ static __forceinline__ unsigned key(float x)
+    {
+        const unsigned u = __float_as_uint(x) >> 16;
+        return u & 0x8000u ? ~u & 0xffffu : u | 0x8000u;
+    }
+    __device__ static __forceinline__ float value(unsigned k) { return __uint_as_float((k & 0x8000u ? k & 0x7fffu : ~k & 0xffffu) << 16); }
+};
 
 struct smp_row {
-    double max, c, low;                  // 2^((x - max) c); below 2^low it rounds to no weight
-    double one;                          // 2^kbits
+    double max, c, low;                  // 2^((x - max) c / 32); nothing below c-scaled `low`
     float maxf, step;                    // cells of the first histogram: (max - x) * step
-    unsigned top;                        // the maximum's key
+    uint64_t one;                        // 2^kbits
     const double *tab;
 };
 
-// The weight of a logit relative to the row's largest, in 64 bits; 0 when it is too small to count.
-// 2^z = 2^(i / 32) 2^r with i = round(32 z), |r| <= 1/64: a table of 32 and the exponential series to r^5, whose
-// rest is below 2^-48.
-__device__ __forceinline__ double smp_exp(const smp_row &q, unsigned key)
+// The weight of a logit, 0 when it is too small to count. 2^(z / 32) = 2^(i / 32) 2^(r / 32), i = round(z), |r| <= 1/2:
+// a table of 32 and the exponential series to r^5, whose rest is below 2^-48. The last sum, with 2^52, leaves
+// the rounded integer in the low bits.
+__device__ __forceinline__ uint64_t smp_weight(const smp_row &q, float x)
 {
-    if (key == q.top) return 1.0;        // (infinity too)
-    const double z = ((double)smp_value(key) - q.max) * q.c;
-    if (!(z >= q.low)) return 0.0;
-    const double big = 211106232532992.0;                  // 1.5 * 2^47: a sum with it is a multiple of 1/32
+    const double z = ((double)x - q.max) * q.c;
+    const double big = 6755399441055744.0, l = 0.021660849392498290;                // 1.5 * 2^52, ln 2 / 32
     const double f = z + big;
     const int i = __double2loint(f);
-    const double y = (z - (f - big)) * 0.693147180559945309417;
-    double e = fma(y, 1.0 / 120.0, 1.0 / 24.0);
-    e = fma(e, y, 1.0 / 6.0);
-    e = fma(e, y, 0.5);
-    e = fma(e, y, 1.0);
-    e = fma(e, y, 1.0) * q.tab[i & 31];
-    return __hiloint2double(__double2hiint(e) + ((i >> 5) << 20), __double2loint(e));
+    const double r = z - (f - big), t = q.tab[i & 31];
+    double e = fma(r, l * l * l * l * l / 120.0, l * l * l * l / 24.0);
+    e = fma(e, r, l * l * l / 6.0);
+    e = fma(e, r, l * l / 2.0);
+    e = fma(e, r, l);
+    e = fma(e, r, 1.0);
+    e = fma(e, __hiloint2double(__double2hiint(t) + ((i >> 5) << 20), __double2loint(t)), 4503599627370496.0);
+    const uint64_t w = (uint64_t)__double_as_longlong(e) & 0xfffffffffffffull;
+    return x == q.maxf ? q.one : z >= q.low ? w : 0;     // (the first for infinity; NaN and -infinity weigh nothing)
 }
 
-__device__ __forceinline__ uint64_t smp_weight(const smp_row &q, double e) { return __double2ull_rn(e * q.one); }
-
-// The cell of the first histogram, IRX_SMP_BINS for what has no weight. Never falls as keys fall.
-__device__ __forceinline__ unsigned smp_cell(const smp_row &q, unsigned key)
+// The cell of the first histogram, at least IRX_SMP_BINS for what has no weight. Never falls as x falls.
+__device__ __forceinline__ unsigned smp_cell(const smp_row &q, float x)
 {
-    if (key == q.top) return 0;
-    const float f = fminf(q.maxf - smp_value(key), 3.4028234663852886e38f) * q.step;
-    return f < (float)IRX_SMP_BINS ? (unsigned)f : IRX_SMP_BINS;
+    if (x == q.maxf) return 0;
+    const float f = fminf(q.maxf - x, 3.4028234663852886e38f) * q.step;
+    return x > -INFINITY && f < (float)IRX_SMP_BINS ? (unsigned)f : IRX_SMP_BINS;
 }
 
 // The largest key of [lo, hi] whose cell is at least b, when lo's is. A whole warp calls it.
+template <class T>
 __device__ __forceinline__ unsigned smp_last(const smp_row &q, unsigned lo, unsigned hi, unsigned b)
 {
     while (lo < hi) {
         const unsigned step = (hi - lo) / 32 + 1;
         const uint64_t k = (uint64_t)lo + (uint64_t)step * (threadIdx.x & 31);
-        const unsigned yes = __ballot_sync(0xffffffffu, k <= hi && smp_cell(q, (unsigned)k) >= b);
+        const unsigned yes = __ballot_sync(0xffffffffu, k <= hi && smp_cell(q, smp_type<T>::value((unsigned)k)) >= b);
         lo += (__popc(yes) - 1) * step;
         hi = min((uint64_t)hi, (uint64_t)lo + step - 1);
     }
@@ -126,6 +159,13 @@ __device__ __forceinline__ void smp_st64(void *local, unsigned rank, uint64_t v)
     asm volatile("st.shared::cluster.u64 [%0], %1;" :: "r"(cluster_addr(local, rank)), "l"(v) : "memory");
 }
 
+__device__ __forceinline__ unsigned smp_add32(void *local, unsigned rank, unsigned v)
+{
+    unsigned old;
+    asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(cluster_addr(local, rank)), "r"(v) : "memory");
+    return old;
+}
+
 __device__ __forceinline__ void smp_cluster_sync()
 {
     __syncwarp();
@@ -144,18 +184,89 @@ __device__ __forceinline__ void smp_post(smp_shared &sh, unsigned rank, unsigned
     smp_cluster_sync();
 }
 
-// One pass over a block's elements: f(index in the block, key).
-template <class T, class F>
-__device__ __forceinline__ void smp_each(const T *x, int n, F f)
+// A block's words, by thread: in shared memory, or (FAR) in the row itself.
+template <class T, bool FAR> struct smp_data {
+    const unsigned *data;                // this thread's first word
+    const T *src;                        // the row's element 0 of this thread
+    int64_t left;                        // the row's elements from there on
+    int words;
+    __device__ __forceinline__ unsigned word(int j) const
+    {
+        if (!FAR) return data[j];
+        unsigned w = smp_type<T>::PAD;
+        if constexpr (sizeof(T) == 4) {
+            if (j < left) w = reinterpret_cast<const unsigned *>(src)[j];
+        } else {
+            const unsigned short *e = reinterpret_cast<const unsigned short *>(src);
+            if (2 * j < left) w = (w & 0xffff0000u) | e[2 * j];
+            if (2 * j + 1 < left) w = (w & 0xffffu) | (unsigned)e[2 * j + 1] << 16;
+        }
+        return w;
+    }
+    // f(number, index among this thread's elements) for each of them
+    template <class F> __device__ __forceinline__ void each(F f) const
+    {
+#pragma unroll 4
+        for (int j = 0; j < words; j++) {
+            const unsigned w = word(j);
+#pragma unroll
+            for (int h = 0; h < smp_type<T>::N; h++) f(smp_type<T>::get(w, h), j * smp_type<T>::N + h);
+        }
+    }
+};
+
+struct smp_cut { float above; unsigned ties; };     // what is kept: what is above, and the first `ties` of those equal
+
+// Sums over the block: of `w` and of `c`, by warp into red and redc. All threads get both totals.
+__device__ __forceinline__ void smp_block_sums(smp_shared &sh, uint64_t &w, unsigned &c)
 {
-    for (int i = threadIdx.x; i < n; i += IRX_SMP_THREADS) f(i, smp_key((float)x[i]));
+    w = smp_warp_sum(w);
+    c = __reduce_add_sync(0xffffffffu, c);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) {
+        sh.red[threadIdx.x >> 5] = w;
+        sh.redc[threadIdx.x >> 5] = c;
+    }
+    __syncthreads();
+    w = 0;
+    c = 0;
+#pragma unroll
+    for (int i = 0; i < SMP_WARPS; i++) {
+        w += sh.red[i];
+        c += sh.redc[i];
+    }
 }
 
-struct smp_cut { unsigned key, ties; };  // what is kept: keys above, and the first `ties` of those equal
+__device__ __forceinline__ void smp_clear(smp_shared &sh)
+{
+    __syncthreads();
+    for (int b = threadIdx.x; b < IRX_SMP_BINS; b += IRX_SMP_THREADS) {
+        sh.cnt[b] = 0;
+        sh.lo[b] = 0;
+        sh.hi[b] = 0;
+    }
+    __syncthreads();
+}
 
-// The cell of the histogram in which the running count (want: count) or weight reaches `target`, from cell 0 on;
-// false when all of them together do not. Fills sh.cell, above, before, count, weight of every block.
-__device__ __forceinline__ bool smp_find(smp_shared &sh, unsigned rank, unsigned nc, unsigned &turn, bool by_weight, uint64_t target)
+__device__ __forceinline__ void smp_tally(smp_shared &sh, unsigned cell, bool by_weight, uint64_t w)
+{
+    atomicAdd(&sh.cnt[cell], 1u);
+    if (by_weight) {
+        const unsigned wl = (unsigned)w, old = atomicAdd(&sh.lo[cell], wl), up = (unsigned)(w >> 32) + (old + wl < old);
+        if (up) atomicAdd(&sh.hi[cell], up);
+    }
+}
+
+// The cell of the blocks' histograms in which the running count, or weight, reaches `target`, from cell 0 on; false when
+// all of them together do not. With `part`, a share of all: target = the least integer not below part / 2^62 times
+// the whole weight, at least 1. Fills every block's sh.cell, above, before, count, weight.
+__device__ __forceinline__ uint64_t smp_part(uint64_t part, uint64_t v, bool up)
+{
+    const uint64_t hi = __umul64hi(part, v), lo = part * v;
+    return (hi << 2 | lo >> 62) + (up && (lo << 2) != 0);
+}
+
+__device__ __forceinline__ bool smp_find(smp_shared &sh, unsigned rank, unsigned nc, unsigned &turn, bool by_weight, uint64_t &target, uint64_t part)
 {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int slice = IRX_SMP_BINS / nc, each = (slice + IRX_SMP_THREADS - 1) / IRX_SMP_THREADS;
@@ -169,21 +280,37 @@ __device__ __forceinline__ bool smp_find(smp_shared &sh, unsigned rank, unsigned
         const int b = threadIdx.x * each + i;
         if (i < each && b < slice) {
             const int cell = rank * slice + b;
-            for (unsigned r = 0; r < nc; r++) {
-                c[i] += smp_ld32(&sh.cnt[cell], r);
-                if (by_weight) w[i] += (uint64_t)smp_ld32(&sh.lo[cell], r) + ((uint64_t)smp_ld32(&sh.hi[cell], r) << 32);
+            unsigned a[8], l[8], h[8];
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                a[r] = l[r] = h[r] = 0;
+                if (r < nc) {
+                    a[r] = smp_ld32(&sh.cnt[cell], r);
+                    if (by_weight) {
+                        l[r] = smp_ld32(&sh.lo[cell], r);
+                        h[r] = smp_ld32(&sh.hi[cell], r);
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                c[i] += a[r];
+                w[i] += (uint64_t)l[r] + ((uint64_t)h[r] << 32);
             }
         }
         cs += c[i];
         ws += w[i];
     }
-    const uint64_t ci = smp_warp_scan(cs), wi = by_weight ? smp_warp_scan(ws) : 0;
+    const unsigned ci = (unsigned)smp_warp_scan(cs);
+    const uint64_t wi = by_weight ? smp_warp_scan(ws) : 0;
     if (lane == 31) {
-        sh.redc[warp] = (unsigned)ci;
+        sh.redc[warp] = ci;
         sh.red[warp] = wi;
     }
     __syncthreads();
-    uint64_t cb = ci - cs, wb = wi - ws, ct = 0, wt = 0;
+    uint64_t wb = wi - ws, wt = 0;
+    unsigned cb = ci - cs, ct = 0;
+#pragma unroll
     for (int i = 0; i < SMP_WARPS; i++) {
         if (i < warp) {
             cb += sh.redc[i];
@@ -192,8 +319,8 @@ __device__ __forceinline__ bool smp_find(smp_shared &sh, unsigned rank, unsigned
         ct += sh.redc[i];
         wt += sh.red[i];
     }
-    smp_post(sh, rank, nc, turn, wt, (unsigned)ct);
-    uint64_t all = 0;
+    smp_post(sh, rank, nc, turn, wt, ct);
+    uint64_t all = 0, whole = 0;
     for (unsigned r = 0; r < nc; r++) {
         const uint64_t rw = sh.xa[turn][r];
         const unsigned rc = sh.xc[turn][r];
@@ -201,15 +328,17 @@ __device__ __forceinline__ bool smp_find(smp_shared &sh, unsigned rank, unsigned
             cb += rc;
             wb += rw;
         }
+        whole += rw;
         all += by_weight ? rw : rc;
     }
+    if (part) target = max(smp_part(part, whole, true), (uint64_t)1);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const uint64_t b = by_weight ? wb : cb, n = by_weight ? w[i] : c[i];
         if (b < target && target <= b + n) {             // one thread of the cluster
             for (unsigned r = 0; r < nc; r++) {
                 smp_st32(&sh.cell, r, rank * slice + threadIdx.x * each + i);
-                smp_st32(&sh.above, r, (unsigned)cb);
+                smp_st32(&sh.above, r, cb);
                 smp_st32(&sh.count, r, c[i]);
                 smp_st64(&sh.before, r, wb);
                 smp_st64(&sh.weight, r, w[i]);
@@ -222,255 +351,310 @@ __device__ __forceinline__ bool smp_find(smp_shared &sh, unsigned rank, unsigned
     return target <= all;
 }
 
-// The threshold at which the running count (weights: running weight) reaches `target`, over the keys from `from` up;
-// key 0 when all of them do not.
-template <class T>
-__device__ __forceinline__ smp_cut smp_select(smp_shared &sh, const smp_row &q, const T *x, int n, unsigned rank, unsigned nc, unsigned &turn,
-                                              bool by_weight, uint64_t target, unsigned from, unsigned floor_key)
+// After a first histogram whose cell has been found: the exact threshold in it, by histograms of its range.
+template <class T, bool FAR>
+__device__ __forceinline__ smp_cut smp_refine(smp_shared &sh, const smp_row &q, const smp_data<T, FAR> &x, unsigned rank, unsigned nc,
+                                              unsigned &turn, bool by_weight, uint64_t target)
 {
-    unsigned lo = 0, hi = 0, shift = 0;
-    uint64_t above = 0, before = 0;
-    for (int level = 0;; level++) {
-        __syncthreads();
-        for (int b = threadIdx.x; b < IRX_SMP_BINS; b += IRX_SMP_THREADS) {
-            sh.cnt[b] = 0;
-            sh.lo[b] = 0;
-            sh.hi[b] = 0;
-        }
-        __syncthreads();
-        smp_each(x, n, [&](int, unsigned key) {
-            if (key < from || key <= SMP_NEG_INF) return;
-            unsigned cell;
-            if (!level) cell = smp_cell(q, key);
-            else cell = key < lo || key > hi ? IRX_SMP_BINS : (hi - key) >> shift;
-            if (cell >= IRX_SMP_BINS) return;
-            atomicAdd(&sh.cnt[cell], 1u);
-            if (by_weight) {
-                const uint64_t w = smp_weight(q, smp_exp(q, key));
-                const unsigned wl = (unsigned)w, old = atomicAdd(&sh.lo[cell], wl), carry = old + wl < old;
-                if ((unsigned)(w >> 32) + carry) atomicAdd(&sh.hi[cell], (unsigned)(w >> 32) + carry);
-            }
+    typedef smp_type<T> ty;
+    const unsigned least = ty::key(ty::value(ty::key(-INFINITY) + 1)), top = ty::key(q.maxf);
+    unsigned hi = smp_last<T>(q, least, top, sh.cell);
+    unsigned lo = smp_cell(q, ty::value(least)) > sh.cell ? smp_last<T>(q, least, top, sh.cell + 1) + 1 : least;
+    unsigned count = sh.count;
+    uint64_t above = sh.above, before = sh.before;
+    while (lo != hi) {
+        unsigned shift = 0;
+        while (((hi - lo) >> shift) >= IRX_SMP_BINS) shift++;
+        smp_clear(sh);
+        x.each([&](float v, int) {
+            const unsigned key = ty::key(v);
+            if (key >= lo && key <= hi) smp_tally(sh, (hi - key) >> shift, by_weight, by_weight ? smp_weight(q, v) : 0);
         });
-        if (!smp_find(sh, rank, nc, turn, by_weight, target - (by_weight ? before : above))) return {0u, 0xffffffffu};
-        const unsigned cell = sh.cell, count = sh.count;
+        uint64_t left = target - (by_weight ? before : above);
+        smp_find(sh, rank, nc, turn, by_weight, left, 0);
         above += sh.above;
         before += sh.before;
-        if (!level) {
-            hi = smp_last(q, floor_key, q.top, cell);
-            lo = smp_cell(q, floor_key) > cell ? smp_last(q, floor_key, q.top, cell + 1) + 1 : floor_key;
-        } else {
-            const unsigned h = hi - (cell << shift);
-            lo = h - lo > (1u << shift) - 1u ? h - ((1u << shift) - 1u) : lo;
-            hi = h;
-        }
-        if (lo == hi) {                                  // a single number: how many of its tokens
-            uint64_t ties = target - above;
-            if (by_weight) {
-                const uint64_t w = smp_weight(q, smp_exp(q, lo));
-                ties = (target - before + w - 1) / w;
-            }
-            return {lo, (unsigned)min(ties, (uint64_t)count)};
-        }
-        shift = 0;
-        while (((hi - lo) >> shift) >= IRX_SMP_BINS) shift++;
+        count = sh.count;
+        hi -= sh.cell << shift;
+        lo = hi - lo > (1u << shift) - 1u ? hi - ((1u << shift) - 1u) : lo;
     }
+    uint64_t ties = target - above;                      // of the tokens at this number
+    if (by_weight) {
+        const uint64_t w = smp_weight(q, ty::value(lo));
+        ties = (target - before + w - 1) / w;
+    }
+    return {ty::value(lo), (unsigned)min(ties, (uint64_t)count)};
 }
 
-// floor(f * v) for f in [0, 1), v below 2^62, exact for f of at least 2^-38.
-__device__ __forceinline__ uint64_t smp_part(float f, uint64_t v, bool up)
+struct smp_settings { uint64_t k, part, least, whole; float u; };      // part: top-p in 2^-62, 0 off; least: min-p's weight
+
+// The few tokens in cells up to sh.cell, gathered in block 0: all filters and the draw.
+// whole: the row's weight, when top-k is off.
+template <class T, bool FAR>
+__device__ __forceinline__ void smp_finish(const irx_ksmp_t &p, smp_shared &sh, const smp_row &q, const smp_data<T, FAR> &x, unsigned rank,
+                                           int64_t first, int64_t row, const smp_settings &s)
 {
-    const uint64_t a = (uint64_t)((double)f * 4611686018427387904.0);           // 2^62
-    const uint64_t hi = __umul64hi(a, v), lo = a * v;
-    return (hi << 2 | lo >> 62) + (up && (lo << 2) != 0);
+    const unsigned cell = sh.cell;
+    __syncthreads();                                     // (the histograms have been read: smp_find ends with a cluster barrier)
+    x.each([&](float v, int i) {
+        if (smp_cell(q, v) <= cell) sh.mine[atomicAdd(&sh.few, 1u)] = (uint64_t)~smp_type<float>::key(v) << 32 | (unsigned)(first + i);
+    });
+    __syncthreads();
+    const unsigned n = sh.few;
+    if (threadIdx.x == 0 && n) sh.total = smp_add32(&sh.listed, 0, n);
+    __syncthreads();
+    for (unsigned i = threadIdx.x; i < n; i += IRX_SMP_THREADS) smp_st64(&sh.list[sh.total + i], 0, sh.mine[i]);
+    smp_cluster_sync();
+    if (rank) return;
+    const unsigned m = sh.listed;
+    uint64_t me[2], w[2], better[2] = {0, 0};
+    unsigned order[2] = {0, 0}, none = 0;
+#pragma unroll
+    for (int a = 0; a < 2; a++) {
+        const unsigned i = threadIdx.x + a * IRX_SMP_THREADS;
+        me[a] = i < m ? sh.list[i] : ~0ull;
+        w[a] = i < m ? smp_weight(q, smp_type<float>::value(~(unsigned)(me[a] >> 32))) : 0;
+        if (i < m) sh.weight_of[i] = w[a];
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (unsigned j = 0; j < m; j++) {                   // how many come before each, and their weight
+        const uint64_t other = sh.list[j], ow = sh.weight_of[j];
+#pragma unroll
+        for (int a = 0; a < 2; a++)
+            if (other < me[a]) {
+                order[a]++;
+                better[a] += ow;
+            }
+    }
+    uint64_t whole = s.whole;
+    bool keep[2];
+#pragma unroll
+    for (int a = 0; a < 2; a++) keep[a] = threadIdx.x + a * IRX_SMP_THREADS < m && (!s.k || order[a] < s.k);
+    if (s.k && s.part) {
+        whole = (keep[0] ? w[0] : 0) + (keep[1] ? w[1] : 0);
+        smp_block_sums(sh, whole, none);
+    }
+    const uint64_t target = s.part ? max(smp_part(s.part, whole, true), (uint64_t)1) : ~0ull;
+    uint64_t total = 0;
+#pragma unroll
+    for (int a = 0; a < 2; a++) {
+        keep[a] = keep[a] && better[a] < target && w[a] >= s.least;
+        if (!keep[a]) w[a] = 0;
+        total += w[a];
+    }
+    smp_block_sums(sh, total, none);                     // (its barriers: all have read weight_of)
+#pragma unroll
+    for (int a = 0; a < 2; a++)
+        if (threadIdx.x + a * IRX_SMP_THREADS < m) sh.weight_of[threadIdx.x + a * IRX_SMP_THREADS] = w[a];
+    __syncthreads();
+    const uint64_t at = smp_part((uint64_t)((double)s.u * 4611686018427387904.0), total, false);
+    uint64_t run[2] = {0, 0};
+#pragma unroll 4
+    for (unsigned j = 0; j < m; j++) {                   // the kept weight at lower indexes
+        const unsigned other = (unsigned)sh.list[j];
+        const uint64_t ow = sh.weight_of[j];
+#pragma unroll
+        for (int a = 0; a < 2; a++)
+            if (other < (unsigned)me[a]) run[a] += ow;
+    }
+#pragma unroll
+    for (int a = 0; a < 2; a++)
+        if (run[a] <= at && at < run[a] + w[a]) {        // one thread
+            p.token[row] = (int)(unsigned)me[a];
+            if (p.logprob) p.logprob[row] = (float)(log((double)w[a] / (double)total));
+        }
 }
 
 template <class T, bool FAR>
 __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
 {
+    typedef smp_type<T> ty;
     irx_pdl_enter();
     extern __shared__ __align__(16) unsigned char smp_raw[];
     smp_shared &sh = *reinterpret_cast<smp_shared *>(smp_raw);
+    unsigned *data = reinterpret_cast<unsigned *>(smp_raw + IRX_SMP_FIXED);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     unsigned rank = cluster_rank(), nc, turn = 0;
     asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(nc));
-    const int64_t row = p.r0 + blockIdx.x / nc, base = (int64_t)rank * p.per;
-    const int n = (int)max((int64_t)0, min(p.per, p.n - base));
+    const int64_t row = p.r0 + blockIdx.x / nc, per = (int64_t)p.words * IRX_SMP_THREADS * ty::N, base = (int64_t)rank * per;
+    const int64_t here = max((int64_t)0, min(per, p.n - base));
     const T *src = reinterpret_cast<const T *>(p.x) + row * p.stride + base;
-    T *data = reinterpret_cast<T *>(smp_raw + IRX_SMP_FIXED);
-    const T *x = FAR ? src : data;
+    const int64_t first = base + (int64_t)threadIdx.x * p.words * ty::N;               // this thread's first element
+    const smp_data<T, FAR> x = {data + threadIdx.x * p.words, src + (int64_t)threadIdx.x * p.words * ty::N, p.n - first, p.words};
+    const float t = p.temperature[row], tp = p.top_p[row], mp = p.min_p[row], un = p.u[row];
+    const int k = p.top_k[row];
 
-    // the row into shared memory; its largest logit, the lowest index of it, and its smallest finite one
-    uint64_t best = 0;
-    unsigned least = 0xffffffffu;
-    auto see = [&](int i, float v) {
-        const unsigned key = smp_key(v);
-        const uint64_t k = (uint64_t)key << 32 | (unsigned)(0x7fffffff - (base + i));
-        best = max(best, k);
-        if (key > SMP_NEG_INF) least = min(least, key);
-    };
-    if (threadIdx.x < 32) sh.tab[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
-    {
-        constexpr int V = 16 / sizeof(T);
-        const int nv = p.vec ? n / V : 0;
-        for (int i = threadIdx.x; i < nv; i += IRX_SMP_THREADS) {
-            const uint4 r = *reinterpret_cast<const uint4 *>(src + (int64_t)i * V);
-            if (!FAR) *reinterpret_cast<uint4 *>(data + i * V) = r;
-            const T *e = reinterpret_cast<const T *>(&r);
-#pragma unroll
-            for (int j = 0; j < V; j++) see(i * V + j, (float)e[j]);
+    // the row into shared memory, padded with -infinity
+    if (!FAR) {
+        const unsigned bytes = p.vec ? (unsigned)(here * sizeof(T)) & ~15u : 0;
+        if (threadIdx.x == 0) {
+            irx_mbar_init(&sh.bar, 1);
+            irx_fence_mbar_init();
+            if (bytes) {
+                irx_mbar_expect_tx(&sh.bar, bytes);
+                irx_bulk_g2s(data, src, bytes, &sh.bar);
+            }
         }
-        for (int i = nv * V + threadIdx.x; i < n; i += IRX_SMP_THREADS) {
-            const T e = src[i];
-            if (!FAR) data[i] = e;
-            see(i, (float)e);
-        }
+        T *e = reinterpret_cast<T *>(data);
+        for (int64_t i = bytes / sizeof(T) + threadIdx.x; i < per; i += IRX_SMP_THREADS) e[i] = i < here ? src[i] : (T)-INFINITY;
+        if (threadIdx.x < 32) sh.tab[threadIdx.x] = p.tab[threadIdx.x];
+        if (threadIdx.x == 0) sh.few = sh.listed = 0;
+        __syncthreads();
+        if (bytes && !irx_mbar_wait(&sh.bar, 0) && lane == 0) atomicOr(p.err, IRX_KERR_TIMEOUT);
+    } else {
+        if (threadIdx.x < 32) sh.tab[threadIdx.x] = p.tab[threadIdx.x];
+        if (threadIdx.x == 0) sh.few = sh.listed = 0;
+        __syncthreads();
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    least = __reduce_min_sync(0xffffffffu, least);
-    if (lane == 0) {
-        sh.red[warp] = best;
-        sh.redc[warp] = least;
-    }
+    unsigned most = ty::PAD;
+#pragma unroll 8
+    for (int j = 0; j < x.words; j++) most = ty::max2(most, x.word(j));
+    float top = ty::get(most, 0);
+    if (ty::N == 2) top = fmaxf(top, ty::get(most, 1));
+    const unsigned tk = __reduce_max_sync(0xffffffffu, smp_type<float>::key(top));
+    if (lane == 0) sh.redc[warp] = tk;
     __syncthreads();
-    for (int i = 0; i < SMP_WARPS; i++) {
-        best = max(best, sh.red[i]);
-        least = min(least, sh.redc[i]);
-    }
-    smp_post(sh, rank, nc, turn, best, least);
-    for (unsigned r = 0; r < nc; r++) {
-        best = max(best, sh.xa[turn][r]);
-        least = min(least, sh.xc[turn][r]);
-    }
-    smp_row q;
-    q.top = (unsigned)(best >> 32);
-    const float t = p.temperature[row];
-    if (q.top <= SMP_NEG_INF || !(t > 0.0f)) {           // nothing to draw from, or the largest logit itself
+    unsigned best = 0;
+#pragma unroll
+    for (int i = 0; i < SMP_WARPS; i++) best = max(best, sh.redc[i]);
+    smp_post(sh, rank, nc, turn, 0, best);
+    for (unsigned r = 0; r < nc; r++) best = max(best, sh.xc[turn][r]);
+    top = smp_type<float>::value(best);
+    if (top == -INFINITY || !(t > 0.0f)) {               // nothing to draw from, or the largest logit itself
+        unsigned at = 0xffffffffu;
+        if (top > -INFINITY) {
+            x.each([&](float v, int i) { if (v == top) at = min(at, (unsigned)(first + i)); });
+            at = __reduce_min_sync(0xffffffffu, at);
+            __syncthreads();
+            if (lane == 0) sh.redc[warp] = at;
+            __syncthreads();
+            for (int i = 0; i < SMP_WARPS; i++) at = min(at, sh.redc[i]);
+            smp_post(sh, rank, nc, turn, 0, at);
+            for (unsigned r = 0; r < nc; r++) at = min(at, sh.xc[turn][r]);
+        }
         if (rank == 0 && threadIdx.x == 0) {
-            const bool none = q.top <= SMP_NEG_INF;
-            p.token[row] = none ? -1 : (int)(0x7fffffff - (unsigned)best);
-            if (p.logprob) p.logprob[row] = none ? -INFINITY : 0.0f;
+            p.token[row] = (int)at;
+            if (p.logprob) p.logprob[row] = at == 0xffffffffu ? -INFINITY : 0.0f;
         }
         return;
     }
+    smp_row q;
     q.tab = sh.tab;
-    q.maxf = smp_value(q.top);
-    q.max = (double)q.maxf;
-    q.c = 1.4426950408889634074 / (double)t;
-    q.low = -(double)(p.kbits + 1);
-    q.one = (double)(1ull << p.kbits);
-    {
-        const double reach = (p.kbits + 2) / q.c, have = q.max - (double)smp_value(min(least, q.top)), r = reach < have ? reach : have;
-        q.step = r > 0.0 && r < 1e300 ? (float)min(2047.9 / r, 3.0e38) : 1.0f;
-    }
+    q.maxf = top;
+    q.max = (double)top;
+    q.c = 46.166241308446828384 / (double)t;             // 32 log2(e) / T
+    q.low = -32.0 * (p.kbits + 1);
+    q.one = 1ull << p.kbits;
+    q.step = (float)fmin(2047.9 * q.c / (32.0 * (p.kbits + 2)), 3.0e38);
+    smp_settings s;
+    s.k = k > 0 && k < p.n ? k : 0;
+    s.part = tp >= 1.0f || tp != tp ? 0 : tp > 0.0f ? max((uint64_t)((double)tp * 4611686018427387904.0), (uint64_t)1) : 1;
+    s.least = mp > 0.0f ? (uint64_t)ceil((double)fminf(mp, 1.0f) * (double)q.one) : 0;
+    s.u = un > 0.0f ? fminf(un, 0.99999994f) : 0.0f;
+    s.whole = 0;
 
-    smp_cut cut = {0u, 0xffffffffu};
-    const int k = p.top_k[row];
-    const float tp = p.top_p[row];
-    const float mp = p.min_p[row], least_p = mp > 0.0f ? fminf(mp, 1.0f) : 0.0f;
-    if (k > 0 && k < p.n) cut = smp_select(sh, q, x, n, rank, nc, turn, false, (uint64_t)k, 0u, min(least, q.top));
-    if (tp < 1.0f) {
-        // the weight of what top-k kept, of which top-p keeps its part
-        uint64_t w = 0;
-        unsigned eq = 0;
-        smp_each(x, n, [&](int, unsigned key) {
-            if (key > cut.key) w += smp_weight(q, smp_exp(q, key));
-            eq += key == cut.key;
+    smp_cut cut = {-INFINITY, 0};
+    if (s.k) {
+        smp_clear(sh);
+        x.each([&](float v, int) {
+            const unsigned cell = smp_cell(q, v);
+            if (cell < IRX_SMP_BINS) smp_tally(sh, cell, false, 0);
         });
-        w = smp_warp_sum(w);
-        eq = __reduce_add_sync(0xffffffffu, eq);
-        __syncthreads();
-        if (lane == 0) {
-            sh.red[warp] = w;
-            sh.redc[warp] = eq;
+        uint64_t target = s.k;
+        if (!smp_find(sh, rank, nc, turn, false, target, 0)) s.k = 0;      // fewer have any weight: all of those
+        else if (sh.above + sh.count <= SMP_FEW) return smp_finish(p, sh, q, x, rank, first, row, s);
+        else cut = smp_refine(sh, q, x, rank, nc, turn, false, target);
+    }
+    if (s.part) {
+        // the weights of what top-k kept, by cell; of those at its threshold only the first
+        smp_clear(sh);
+        x.each([&](float v, int) {
+            const unsigned cell = smp_cell(q, v);
+            if (v > cut.above && cell < IRX_SMP_BINS) smp_tally(sh, cell, true, smp_weight(q, v));
+        });
+        if (cut.above > -INFINITY && rank == 0) {
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                const unsigned cell = smp_cell(q, cut.above);
+                const uint64_t w = cut.ties * smp_weight(q, cut.above), sum = ((uint64_t)sh.hi[cell] << 32 | sh.lo[cell]) + w;
+                if (cell < IRX_SMP_BINS) {
+                    sh.cnt[cell] += cut.ties;
+                    sh.lo[cell] = (unsigned)sum;
+                    sh.hi[cell] = (unsigned)(sum >> 32);
+                }
+            }
         }
-        __syncthreads();
-        w = 0;
-        eq = 0;
-        for (int i = 0; i < SMP_WARPS; i++) {
-            w += sh.red[i];
-            eq += sh.redc[i];
+        uint64_t target = 0;
+        smp_find(sh, rank, nc, turn, true, target, s.part);
+        if (!s.k && sh.above + sh.count <= SMP_FEW) {
+            for (unsigned r = 0; r < nc; r++) s.whole += sh.xa[turn][r];
+            return smp_finish(p, sh, q, x, rank, first, row, s);
         }
-        smp_post(sh, rank, nc, turn, w, eq);
-        w = 0;
-        eq = 0;
-        for (unsigned r = 0; r < nc; r++) {
-            w += sh.xa[turn][r];
-            eq += sh.xc[turn][r];
-        }
-        if (cut.key) w += min(eq, cut.ties) * smp_weight(q, smp_exp(q, cut.key));
-        uint64_t target = tp > 0.0f ? smp_part(tp, w, true) : 1;
-        if (target < 1) target = 1;
-        const smp_cut c2 = smp_select(sh, q, x, n, rank, nc, turn, true, target, cut.key, min(least, q.top));
-        if (c2.key > cut.key) cut = c2;
-        else cut.ties = min(cut.ties, c2.ties);          // (the same key, or none: the whole is reached)
+        const smp_cut c = smp_refine(sh, q, x, rank, nc, turn, true, target);
+        if (c.above > cut.above) cut = c;
+        else cut.ties = min(cut.ties, c.ties);
     }
 
-    // the kept weights of every warp's stretch of the row, and where u times their total falls
-    const int stretch = (int)(p.per / SMP_WARPS), s0 = min(n, warp * stretch), s1 = min(n, s0 + stretch);
-    const double e_cut = cut.key ? smp_exp(q, cut.key) : 0.0;
-    const uint64_t w_cut = e_cut >= least_p ? smp_weight(q, e_cut) : 0;
+    // the kept weights of every thread's stretch of the row, and where u times their total falls
+    const uint64_t w_cut = cut.above > -INFINITY ? smp_weight(q, cut.above) : 0, w_eq = w_cut >= s.least ? w_cut : 0;
     uint64_t w = 0;
     unsigned eq = 0;
-    for (int i = s0 + lane; i < s1; i += 32) {
-        const unsigned key = smp_key((float)x[i]);
-        if (key > cut.key) {
-            const double e = smp_exp(q, key);
-            if (e >= least_p) w += smp_weight(q, e);
-        }
-        eq += key == cut.key;
-    }
-    w = smp_warp_sum(w);
-    eq = __reduce_add_sync(0xffffffffu, eq);
-    __syncthreads();
-    if (lane == 0) {
-        sh.red[warp] = w;
-        sh.redc[warp] = eq;
-    }
-    __syncthreads();
-    uint64_t wt = 0;
-    unsigned et = 0;
-    for (int i = 0; i < SMP_WARPS; i++) {
-        wt += sh.red[i];
-        et += sh.redc[i];
-    }
-    smp_post(sh, rank, nc, turn, wt, et);
+    x.each([&](float v, int) {
+        const uint64_t e = v > cut.above ? smp_weight(q, v) : 0;
+        if (e >= s.least) w += e;
+        eq += v == cut.above;
+    });
+    if (cut.above == -INFINITY) eq = 0;
+    const uint64_t w_mine = w;
+    const unsigned eq_mine = eq;
+    smp_block_sums(sh, w, eq);
+    smp_post(sh, rank, nc, turn, w, eq);
     uint64_t total = 0, run = 0;
-    unsigned ties = cut.ties, mine = 0;                  // ties: left to keep; mine: of them, this block's
+    unsigned ties = cut.ties, left = 0;                  // ties: left to keep; left: of them, for this block
     for (unsigned r = 0; r < nc; r++) {
         const unsigned have = min(ties, sh.xc[turn][r]);
         if (r == rank) {
             run = total;
-            mine = ties;
+            left = ties;
         }
-        total += sh.xa[turn][r] + have * w_cut;
+        total += sh.xa[turn][r] + have * w_eq;
         ties -= have;
     }
-    const float u = p.u[row];
-    const uint64_t at = smp_part(u > 0.0f ? fminf(u, 0.99999994f) : 0.0f, total, false);
+    const uint64_t at = smp_part((uint64_t)((double)s.u * 4611686018427387904.0), total, false);
+    if (at < run || at >= run + w + min(left, eq) * w_eq) return;      // one block goes on
     for (int i = 0; i < warp; i++) {
-        const unsigned have = min(mine, sh.redc[i]);
-        run += sh.red[i] + have * w_cut;
-        mine -= have;
+        const unsigned have = min(left, sh.redc[i]);
+        run += sh.red[i] + have * w_eq;
+        left -= have;
     }
-    if (at < run || at >= run + w + (uint64_t)min(mine, eq) * w_cut) return;
-    for (int i0 = s0; i0 < s1; i0 += 32) {               // one warp of the cluster
+    if (at < run || at >= run + sh.red[warp] + min(left, sh.redc[warp]) * w_eq) return;      // one warp
+    const unsigned before = (unsigned)smp_warp_scan(eq_mine) - eq_mine;
+    left -= min(left, before);
+    const uint64_t kept = w_mine + min(left, eq_mine) * w_eq, sum = smp_warp_scan(kept);
+    const int who = __ffs(__ballot_sync(0xffffffffu, run + sum > at)) - 1;             // the lane whose stretch it is
+    run = __shfl_sync(0xffffffffu, run + sum - kept, who);
+    left = __shfl_sync(0xffffffffu, left, who);
+    const smp_data<T, FAR> y = {data + (warp * 32 + who) * p.words, src + (int64_t)(warp * 32 + who) * p.words * ty::N,
+                                p.n - base - (int64_t)(warp * 32 + who) * p.words * ty::N, p.words};
+    for (int i0 = 0; i0 < p.words * ty::N; i0 += 32) {
         const int i = i0 + lane;
-        const unsigned key = i < s1 ? smp_key((float)x[i]) : 0u;
-        double e = i < s1 && key >= cut.key ? smp_exp(q, key) : 0.0;
-        const unsigned same = __ballot_sync(0xffffffffu, i < s1 && key == cut.key);
-        if (e < least_p || (key == cut.key && __popc(same & ((1u << lane) - 1u)) >= mine)) e = 0.0;
-        mine -= min(mine, (unsigned)__popc(same));
-        const uint64_t sum = smp_warp_scan(smp_weight(q, e));
-        const unsigned past = __ballot_sync(0xffffffffu, run + sum > at);
+        const float v = i < p.words * ty::N ? ty::get(y.word(i / ty::N), i % ty::N) : -INFINITY;
+        const bool same = v == cut.above && v > -INFINITY;
+        const unsigned all = __ballot_sync(0xffffffffu, same);
+        uint64_t e = v > cut.above || (same && __popc(all & ((1u << lane) - 1u)) < left) ? smp_weight(q, v) : 0;
+        if (e < s.least) e = 0;
+        left -= min(left, (unsigned)__popc(all));
+        const uint64_t up = smp_warp_scan(e);
+        const unsigned past = __ballot_sync(0xffffffffu, run + up > at);
         if (past) {
             if (lane == __ffs(past) - 1) {
-                p.token[row] = (int)(base + i);
-                if (p.logprob) p.logprob[row] = (float)(log(e) - log((double)total / q.one));
+                p.token[row] = (int)(base + (int64_t)(warp * 32 + who) * p.words * ty::N + i);
+                if (p.logprob) p.logprob[row] = (float)log((double)e / (double)total);
             }
             return;
         }
-        run += __shfl_sync(0xffffffffu, sum, 31);
+        run += __shfl_sync(0xffffffffu, up, 31);
     }
 }
 

@@ -307,10 +307,11 @@ int irx_compile_sample(const irx_sample_t *m, irx_plan_t *plan)
 static int launch_sample(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsigned ns, void *const *args, void *st)
 {
     const irx_smp_t *a = &p->u.sm;
-    const int es = esz(a->dt), warps = IRX_SMP_THREADS / 32;
+    const int epw = a->dt == DT_BF16 ? 2 : 1;              /* elements of a word */
     static irx_ksmp_t k;
     long long u0, u1;
-    int64_t nc, room = d->smem_optin - IRX_SMP_FIXED, far, smem;
+    int64_t nc, words, room = (d->smem_optin - IRX_SMP_FIXED) / 4;
+    int far, j;
     memset(&k, 0, sizeof k);
     irx_unit_range(a->rows, s, ns, &u0, &u1);
     if (u0 >= u1) return 0;
@@ -319,19 +320,21 @@ static int launch_sample(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
     k.min_p = (const float *)args[4]; k.u = (const float *)args[5];
     k.token = (int32_t *)args[6];
     k.logprob = a->logprob ? (float *)args[7] : NULL;
+    k.err = (unsigned *)(size_t)d->err;
     k.r0 = u0; k.stride = a->stride; k.n = a->vocab;
     while ((1ll << k.kbits) < a->vocab) k.kbits++;
     k.kbits = 62 - k.kbits;                                 /* a row's weights sum to at most 2^62 */
     if (k.kbits > 46) k.kbits = 46;
-    k.vec = (uint8_t)(a_to(k.x, 16) && a->stride * es % 16 == 0);
+    for (j = 0; j < 32; j++) k.tab[j] = ldexp(exp2(j / 32.0), k.kbits);
+    k.vec = (uint8_t)(a_to(k.x, 16) && a->stride * 4 / epw % 16 == 0);
     /* blocks of a cluster: the row's elements in their shared memory, at least 4096 each */
     nc = 1;
     while (nc < 8 && (a->vocab + nc - 1) / nc > 4096) nc *= 2;
-    k.per = ((a->vocab + nc - 1) / nc + 8 * warps - 1) / (8 * warps) * (8 * warps);
-    far = k.per * es > room;
-    smem = IRX_SMP_FIXED + (far ? 0 : k.per * es);
-    return irx_dev_launch(d, K_SMP + (a->dt == DT_BF16 ? 0 : 2) + (int)far, (unsigned)((u1 - u0) * nc), IRX_SMP_THREADS,
-                          (unsigned)smem, (unsigned)nc, st, &k);
+    words = (a->vocab + nc * epw * IRX_SMP_THREADS - 1) / (nc * epw * IRX_SMP_THREADS) | 1;
+    k.words = (int32_t)words;
+    far = words * IRX_SMP_THREADS > room;
+    return irx_dev_launch(d, K_SMP + (a->dt == DT_BF16 ? 0 : 2) + far, (unsigned)((u1 - u0) * nc), IRX_SMP_THREADS,
+                          (unsigned)(IRX_SMP_FIXED + (far ? 0 : words * IRX_SMP_THREADS * 4)), (unsigned)nc, st, &k);
 }
 
 /* ---- one entry for the launch switch, and the plans' descriptions ---- */
