@@ -234,8 +234,9 @@ IRX_API int irx_compile_prompt(const irx_prompt_t *desc, irx_plan_t *plan);
  * least min_p (at most 1) times the largest. Drawn is the first kept token, by index, at which the running sum of
  * kept weights is above u times their total. Args: logits [rows, vocab] (`stride` elements from one row to the next;
  * 0: packed), temperature f32 [rows], top_k int32 [rows], top_p, min_p f32 [rows], u f32 [rows], uniform in [0, 1)
- * (outside it: the nearer end), token int32 [rows], with `logprob` != 0 the log of the token's share of the kept
- * weights, f32 [rows]. A temperature that is not above 0 takes the largest logit (the lowest index of it; log 0).
+ * (outside it: the nearer end; NaN: 0), token int32 [rows], with `logprob` != 0 the log of the token's share of the kept
+ * weights, f32 [rows]. A temperature that is not above 0 takes the largest logit (the lowest index of it; log 0); one above 1e20
+ * counts as 1e20.
  * A filter outside its range, or NaN, is off (top_p of 0 or below keeps one token). NaN logits count as -infinity,
  * which is never drawn; a row of nothing else gives token -1 and -infinity; if the largest is +infinity only such
  * tokens weigh anything. Weights are 64-bit integers, 2^kbits for the largest, kbits = 62 - ceil(log2 vocab) and at most

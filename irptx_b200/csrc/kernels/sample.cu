@@ -12,8 +12,10 @@
 // that are read again for each pass), where thread t holds words t * words and on: an odd number of
 // them, so that a warp's reads fall into 32 banks. Tokens per cell of (max - x), 2048 equal cells up to where
 // weights round to zero, or their weights, show the cell in which a filter ends. When that cell and those
-// above it hold few tokens (top-k, or a peaked row), they go to the first block, which finishes alone. Otherwise
-// histograms of the cell's own range follow until it is a single number.
+// above it hold few tokens (top-k, or a peaked row), they go to the first block, which finishes alone. Otherwise the
+// cell's own tokens are resolved, by the first block when they are few, else by histograms of the cell's
+// range, and every thread adds up its stretch's kept weights. What bounds large calls is instructions, about
+// 25 of them for each weight.
 #pragma once
 #include "tc.cuh"
 
@@ -22,31 +24,39 @@
 
 struct smp_shared {
     union {
-        struct { unsigned cnt[IRX_SMP_BINS], lo[IRX_SMP_BINS], hi[IRX_SMP_BINS]; };   // a cell's tokens; its weight, in two words
+        struct { unsigned cnt[IRX_SMP_BINS], lo[IRX_SMP_BINS], hi[IRX_SMP_BINS]; };   // a cell's tokens, or its weight in two words
         struct { uint64_t mine[SMP_FEW], list[SMP_FEW], weight_of[SMP_FEW]; };        // few tokens: this block's, the row's, their weights
     };
     double tab[32];
     uint64_t red[SMP_WARPS], xa[2][8];   // warps' parts; what every block of the cluster posted, two exchanges of it
     unsigned redc[SMP_WARPS], xc[2][8];
     uint64_t before, weight;             // the cell found: the weight above it, its own
-    unsigned above, count, cell, total;
-    unsigned few, listed, drawn;
+    unsigned above, count, cell;         // tokens above it, its own
+    unsigned few, listed, at, key, ties;
     uint64_t bar;
 };
 static_assert(sizeof(smp_shared) <= IRX_SMP_FIXED, "the launcher's size");
 
-// A word's elements as numbers: NaN as -infinity, both zeros as +0, so that equal logits are equal numbers.
+// Logits as numbers that order and weigh as defined: NaN as -infinity, both zeros as +0. For rows whose largest is
+// infinite (then such logits are 0 and all others -infinity) or below -1e30 (then the largest is taken away from
+// all: exactly, wherever a weight is left) a second step follows, so that a number far below the largest exists.
+enum { SMP_PLAIN, SMP_INFINITE, SMP_LOW };
+__device__ __forceinline__ float smp_clean(float x)
+{
+    x += 0.0f;
+    return x == x ? x : -INFINITY;
+}
+__device__ __forceinline__ float smp_shift(float x, int mode, float top)
+{
+    return mode == SMP_INFINITE ? (x == INFINITY ? 0.0f : -INFINITY) : mode == SMP_LOW ? x - top : x;
+}
+
+// Keys order as the numbers do.
 template <class T> struct smp_type;
 template <> struct smp_type<float> {
     static const int N = 1;
-    static const unsigned PAD = 0xff800000u;
-    __device__ static __forceinline__ float get(unsigned w, int)
-    {
-        const float x = __uint_as_float(w) + 0.0f;
-        return x == x ? x : -INFINITY;
-    }
-    __device__ static __forceinline__ unsigned max2(unsigned a, unsigned b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
-    // keys order as the numbers do
+    __device__ static __forceinline__ float get(unsigned w, int) { return __uint_as_float(w); }
+    __device__ static __forceinline__ unsigned put(float a, float) { return __float_as_uint(a); }
     __device__ static __forceinline__ unsigned key(float x)
     {
         const unsigned u = __float_as_uint(x);
@@ -56,17 +66,8 @@ template <> struct smp_type<float> {
 };
 template <> struct smp_type<__nv_bfloat16> {
     static const int N = 2;
-    static const unsigned PAD = 0xff80ff80u;
-    __device__ static __forceinline__ float get(unsigned w, int h)
-    {
-        const float x = __uint_as_float(h ? w & 0xffff0000u : w << 16) + 0.0f;
-        return x == x ? x : -INFINITY;
-    }
-    __device__ static __forceinline__ unsigned max2(unsigned a, unsigned b)
-    {
-        const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
-        return *reinterpret_cast<const unsigned *>(&m);
-    }
+    __device__ static __forceinline__ float get(unsigned w, int h) { return __uint_as_float(h ? w & 0xffff0000u : w << 16); }
+    __device__ static __forceinline__ unsigned put(float a, float b) { return __float_as_uint(a) >> 16 | (__float_as_uint(b) & 0xffff0000u); }
     __device__ static __forceinline__ unsigned key(float x)
     {
         const unsigned u = __float_as_uint(x) >> 16;
@@ -76,18 +77,18 @@ template <> struct smp_type<__nv_bfloat16> {
 };
 
 struct smp_row {
-    double max, c, low;                  // 2^((x - max) c / 32); nothing below c-scaled `low`
-    float maxf, step;                    // cells of the first histogram: (max - x) * step
+    double max, c;                       // a weight is 2^(kbits + (x - max) c / 32)
+    float maxf, floor, step;             // at the floor and below it rounds to 0; cells: (max - x) / 2 * step
     uint64_t one;                        // 2^kbits
     const double *tab;
 };
 
-// The weight of a logit, 0 when it is too small to count. 2^(z / 32) = 2^(i / 32) 2^(r / 32), i = round(z), |r| <= 1/2:
-// a table of 32 and the exponential series to r^5, whose rest is below 2^-48. The last sum, with 2^52, leaves
-// the rounded integer in the low bits.
+// The weight of a logit. 2^(z / 32) = 2^(i / 32) 2^(r / 32), i = round(z), |r| <= 1/2: a table of 32, kbits in it, and
+// the exponential series to r^5, whose rest is below 2^-48. The last sum, with 2^52, leaves the rounded integer in
+// the low bits. The floor keeps i above -7000 (see T below), so that exponents are added without a check.
 __device__ __forceinline__ uint64_t smp_weight(const smp_row &q, float x)
 {
-    const double z = ((double)x - q.max) * q.c;
+    const double z = ((double)fmaxf(x, q.floor) - q.max) * q.c;
     const double big = 6755399441055744.0, l = 0.021660849392498290;                // 1.5 * 2^52, ln 2 / 32
     const double f = z + big;
     const int i = __double2loint(f);
@@ -97,27 +98,30 @@ __device__ __forceinline__ uint64_t smp_weight(const smp_row &q, float x)
     e = fma(e, r, l * l / 2.0);
     e = fma(e, r, l);
     e = fma(e, r, 1.0);
-    e = fma(e, __hiloint2double(__double2hiint(t) + ((i >> 5) << 20), __double2loint(t)), 4503599627370496.0);
-    const uint64_t w = (uint64_t)__double_as_longlong(e) & 0xfffffffffffffull;
-    return x == q.maxf ? q.one : z >= q.low ? w : 0;     // (the first for infinity; NaN and -infinity weigh nothing)
+    e = fma(e, __hiloint2double(__double2hiint(t) + (i & ~31) * (1 << 15), __double2loint(t)), 4503599627370496.0);
+    return (uint64_t)__double_as_longlong(e) & 0xfffffffffffffull;
 }
 
 // The cell of the first histogram, at least IRX_SMP_BINS for what has no weight. Never falls as x falls.
 __device__ __forceinline__ unsigned smp_cell(const smp_row &q, float x)
 {
-    if (x == q.maxf) return 0;
-    const float f = fminf(q.maxf - x, 3.4028234663852886e38f) * q.step;
-    return x > -INFINITY && f < (float)IRX_SMP_BINS ? (unsigned)f : IRX_SMP_BINS;
+    const float f = fmaf(fmaf(-0.5f, x, 0.5f * q.maxf), q.step, 8388608.0f);         // 2^23: the sum's low bits are the cell
+    return x > q.floor && f < 8388608.0f + IRX_SMP_BINS ? __float_as_uint(f) - 0x4b000000u : IRX_SMP_BINS;
 }
 
-// The largest key of [lo, hi] whose cell is at least b, when lo's is. A whole warp calls it.
+// A key whose number is the floor or lies below it.
 template <class T>
-__device__ __forceinline__ unsigned smp_last(const smp_row &q, unsigned lo, unsigned hi, unsigned b)
+__device__ __forceinline__ unsigned smp_least(const smp_row &q) { return smp_type<T>::key(q.floor) - (smp_type<T>::N - 1); }
+
+// The largest key of [lo, hi] for which f holds, when it holds for lo and for no key above one for which it does not. A whole
+// warp calls it.
+template <class F>
+__device__ __forceinline__ unsigned smp_last(unsigned lo, unsigned hi, F f)
 {
     while (lo < hi) {
         const unsigned step = (hi - lo) / 32 + 1;
         const uint64_t k = (uint64_t)lo + (uint64_t)step * (threadIdx.x & 31);
-        const unsigned yes = __ballot_sync(0xffffffffu, k <= hi && smp_cell(q, smp_type<T>::value((unsigned)k)) >= b);
+        const unsigned yes = __ballot_sync(0xffffffffu, k <= hi && f((unsigned)min(k, (uint64_t)hi)));
         lo += (__popc(yes) - 1) * step;
         hi = min((uint64_t)hi, (uint64_t)lo + step - 1);
     }
@@ -184,24 +188,21 @@ __device__ __forceinline__ void smp_post(smp_shared &sh, unsigned rank, unsigned
     smp_cluster_sync();
 }
 
-// A block's words, by thread: in shared memory, or (FAR) in the row itself.
+// A block's words, by thread: in shared memory, cleaned, or (FAR) in the row itself.
 template <class T, bool FAR> struct smp_data {
-    const unsigned *data;                // this thread's first word
+    unsigned *data;                      // this thread's first word
     const T *src;                        // the row's element 0 of this thread
     int64_t left;                        // the row's elements from there on
-    int words;
+    int words, mode;
+    float top;
     __device__ __forceinline__ unsigned word(int j) const
     {
         if (!FAR) return data[j];
-        unsigned w = smp_type<T>::PAD;
-        if constexpr (sizeof(T) == 4) {
-            if (j < left) w = reinterpret_cast<const unsigned *>(src)[j];
-        } else {
-            const unsigned short *e = reinterpret_cast<const unsigned short *>(src);
-            if (2 * j < left) w = (w & 0xffff0000u) | e[2 * j];
-            if (2 * j + 1 < left) w = (w & 0xffffu) | (unsigned)e[2 * j + 1] << 16;
-        }
-        return w;
+        float e[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int h = 0; h < smp_type<T>::N; h++)
+            if (j * smp_type<T>::N + h < left) e[h] = smp_shift(smp_clean((float)src[(int64_t)j * smp_type<T>::N + h]), mode, top);
+        return smp_type<T>::put(e[0], e[1]);
     }
     // f(number, index among this thread's elements) for each of them
     template <class F> __device__ __forceinline__ void each(F f) const
@@ -237,29 +238,29 @@ __device__ __forceinline__ void smp_block_sums(smp_shared &sh, uint64_t &w, unsi
     }
 }
 
-__device__ __forceinline__ void smp_clear(smp_shared &sh)
+__device__ __forceinline__ void smp_clear(smp_shared &sh, bool by_weight)
 {
     __syncthreads();
     for (int b = threadIdx.x; b < IRX_SMP_BINS; b += IRX_SMP_THREADS) {
-        sh.cnt[b] = 0;
-        sh.lo[b] = 0;
-        sh.hi[b] = 0;
+        if (!by_weight) sh.cnt[b] = 0;
+        else sh.lo[b] = sh.hi[b] = 0;
     }
     __syncthreads();
 }
 
 __device__ __forceinline__ void smp_tally(smp_shared &sh, unsigned cell, bool by_weight, uint64_t w)
 {
-    atomicAdd(&sh.cnt[cell], 1u);
-    if (by_weight) {
-        const unsigned wl = (unsigned)w, old = atomicAdd(&sh.lo[cell], wl), up = (unsigned)(w >> 32) + (old + wl < old);
-        if (up) atomicAdd(&sh.hi[cell], up);
+    if (!by_weight) {
+        atomicAdd(&sh.cnt[cell], 1u);
+        return;
     }
+    const unsigned wl = (unsigned)w, old = atomicAdd(&sh.lo[cell], wl), up = (unsigned)(w >> 32) + (old + wl < old);
+    if (up) atomicAdd(&sh.hi[cell], up);
 }
 
 // The cell of the blocks' histograms in which the running count, or weight, reaches `target`, from cell 0 on; false when
 // all of them together do not. With `part`, a share of all: target = the least integer not below part / 2^62 times
-// the whole weight, at least 1. Fills every block's sh.cell, above, before, count, weight.
+// the whole weight, at least 1. Fills every block's sh.cell, above and count, or before and weight.
 __device__ __forceinline__ uint64_t smp_part(uint64_t part, uint64_t v, bool up)
 {
     const uint64_t hi = __umul64hi(part, v), lo = part * v;
@@ -284,13 +285,11 @@ __device__ __forceinline__ bool smp_find(smp_shared &sh, unsigned rank, unsigned
 #pragma unroll
             for (int r = 0; r < 8; r++) {
                 a[r] = l[r] = h[r] = 0;
-                if (r < nc) {
-                    a[r] = smp_ld32(&sh.cnt[cell], r);
-                    if (by_weight) {
-                        l[r] = smp_ld32(&sh.lo[cell], r);
-                        h[r] = smp_ld32(&sh.hi[cell], r);
-                    }
-                }
+                if (r >= nc) continue;
+                if (by_weight) {
+                    l[r] = smp_ld32(&sh.lo[cell], r);
+                    h[r] = smp_ld32(&sh.hi[cell], r);
+                } else a[r] = smp_ld32(&sh.cnt[cell], r);
             }
 #pragma unroll
             for (int r = 0; r < 8; r++) {
@@ -351,39 +350,81 @@ __device__ __forceinline__ bool smp_find(smp_shared &sh, unsigned rank, unsigned
     return target <= all;
 }
 
-// After a first histogram whose cell has been found: the exact threshold in it, by histograms of its range.
+// After a first histogram whose cell has been found: the exact threshold in it. The cell's tokens go to block 0 when
+// they are few, else histograms of its range follow.
 template <class T, bool FAR>
-__device__ __forceinline__ smp_cut smp_refine(smp_shared &sh, const smp_row &q, const smp_data<T, FAR> &x, unsigned rank, unsigned nc,
-                                              unsigned &turn, bool by_weight, uint64_t target)
+__device__ __forceinline__ smp_cut smp_resolve(smp_shared &sh, const smp_row &q, const smp_data<T, FAR> &x, unsigned rank, unsigned nc,
+                                               unsigned &turn, bool by_weight, uint64_t target, bool gather)
 {
     typedef smp_type<T> ty;
-    const unsigned least = ty::key(ty::value(ty::key(-INFINITY) + 1)), top = ty::key(q.maxf);
-    unsigned hi = smp_last<T>(q, least, top, sh.cell);
-    unsigned lo = smp_cell(q, ty::value(least)) > sh.cell ? smp_last<T>(q, least, top, sh.cell + 1) + 1 : least;
-    unsigned count = sh.count;
-    uint64_t above = sh.above, before = sh.before;
+    const unsigned least = smp_least<T>(q), top = ty::key(q.maxf), cell = sh.cell;
+    unsigned hi = smp_last(least, top, [&](unsigned k) { return smp_cell(q, ty::value(k)) >= cell; });
+    unsigned lo = smp_last(least, top, [&](unsigned k) { return smp_cell(q, ty::value(k)) > cell; }) + 1;
+    uint64_t count = sh.count;                           // at most
+    if (by_weight) {
+        const uint64_t w = smp_weight(q, ty::value(lo));
+        count = w ? sh.weight / w : ~0ull;
+    }
+    uint64_t left = target - (by_weight ? sh.before : sh.above);
+    if (lo != hi && gather && count <= SMP_FEW) {
+        const float from = ty::value(lo), to = ty::value(hi);
+        unsigned *mine = reinterpret_cast<unsigned *>(sh.mine), *list = reinterpret_cast<unsigned *>(sh.list);
+        x.each([&](float v, int) {
+            if (v >= from && v <= to) mine[atomicAdd(&sh.few, 1u)] = ty::key(v);
+        });
+        __syncthreads();
+        const unsigned n = sh.few;
+        if (threadIdx.x == 0 && n) sh.at = smp_add32(&sh.listed, 0, n);
+        __syncthreads();
+        for (unsigned i = threadIdx.x; i < n; i += IRX_SMP_THREADS) smp_st32(&list[sh.at + i], 0, mine[i]);
+        smp_cluster_sync();
+        if (rank == 0) {
+            const unsigned m = sh.listed;
+            for (unsigned i = threadIdx.x; i < m; i += IRX_SMP_THREADS) sh.weight_of[i] = by_weight ? smp_weight(q, ty::value(list[i])) : 1;
+            __syncthreads();
+            for (unsigned i = threadIdx.x; i < m; i += IRX_SMP_THREADS) {
+                const unsigned k = list[i];
+                uint64_t above = 0;
+                unsigned same = 0;
+#pragma unroll 4
+                for (unsigned j = 0; j < m; j++) {
+                    if (list[j] > k) above += sh.weight_of[j];
+                    same += list[j] == k;
+                }
+                const uint64_t w = sh.weight_of[i];
+                if (above < left && left <= above + same * w) {        // this number's tokens, all alike
+                    const unsigned ties = (unsigned)((left - above + w - 1) / w);
+                    for (unsigned r = 0; r < nc; r++) {                // none of them is cut off: up to the number below
+                        smp_st32(&sh.key, r, ties == same ? k - 1 : k);
+                        smp_st32(&sh.ties, r, ties == same ? 0 : ties);
+                    }
+                }
+            }
+        }
+        if (threadIdx.x == 0) {
+            sh.few = 0;
+            if (rank == 0) sh.listed = 0;
+        }
+        smp_cluster_sync();
+        return {ty::value(sh.key), sh.ties};
+    }
     while (lo != hi) {
         unsigned shift = 0;
         while (((hi - lo) >> shift) >= IRX_SMP_BINS) shift++;
-        smp_clear(sh);
+        smp_clear(sh, by_weight);
+        const float from = ty::value(lo), to = ty::value(hi);
         x.each([&](float v, int) {
-            const unsigned key = ty::key(v);
-            if (key >= lo && key <= hi) smp_tally(sh, (hi - key) >> shift, by_weight, by_weight ? smp_weight(q, v) : 0);
+            if (v >= from && v <= to) smp_tally(sh, (hi - ty::key(v)) >> shift, by_weight, by_weight ? smp_weight(q, v) : 0);
         });
-        uint64_t left = target - (by_weight ? before : above);
         smp_find(sh, rank, nc, turn, by_weight, left, 0);
-        above += sh.above;
-        before += sh.before;
-        count = sh.count;
+        left -= by_weight ? sh.before : sh.above;
         hi -= sh.cell << shift;
+        count = by_weight ? sh.weight / max(smp_weight(q, ty::value(hi)), (uint64_t)1) : sh.count;
         lo = hi - lo > (1u << shift) - 1u ? hi - ((1u << shift) - 1u) : lo;
     }
-    uint64_t ties = target - above;                      // of the tokens at this number
-    if (by_weight) {
-        const uint64_t w = smp_weight(q, ty::value(lo));
-        ties = (target - before + w - 1) / w;
-    }
-    return {ty::value(lo), (unsigned)min(ties, (uint64_t)count)};
+    const uint64_t w = by_weight ? smp_weight(q, ty::value(lo)) : 1, ties = (left + w - 1) / w;
+    // (count is exact here: a single number's tokens weigh the same)
+    return ties >= count ? smp_cut{ty::value(lo - 1), 0u} : smp_cut{ty::value(lo), (unsigned)ties};
 }
 
 struct smp_settings { uint64_t k, part, least, whole; float u; };      // part: top-p in 2^-62, 0 off; least: min-p's weight
@@ -401,9 +442,9 @@ __device__ __forceinline__ void smp_finish(const irx_ksmp_t &p, smp_shared &sh, 
     });
     __syncthreads();
     const unsigned n = sh.few;
-    if (threadIdx.x == 0 && n) sh.total = smp_add32(&sh.listed, 0, n);
+    if (threadIdx.x == 0 && n) sh.at = smp_add32(&sh.listed, 0, n);
     __syncthreads();
-    for (unsigned i = threadIdx.x; i < n; i += IRX_SMP_THREADS) smp_st64(&sh.list[sh.total + i], 0, sh.mine[i]);
+    for (unsigned i = threadIdx.x; i < n; i += IRX_SMP_THREADS) smp_st64(&sh.list[sh.at + i], 0, sh.mine[i]);
     smp_cluster_sync();
     if (rank) return;
     const unsigned m = sh.listed;
@@ -481,13 +522,16 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
     const int64_t here = max((int64_t)0, min(per, p.n - base));
     const T *src = reinterpret_cast<const T *>(p.x) + row * p.stride + base;
     const int64_t first = base + (int64_t)threadIdx.x * p.words * ty::N;               // this thread's first element
-    const smp_data<T, FAR> x = {data + threadIdx.x * p.words, src + (int64_t)threadIdx.x * p.words * ty::N, p.n - first, p.words};
+    smp_data<T, FAR> x = {data + threadIdx.x * p.words, src + (int64_t)threadIdx.x * p.words * ty::N, p.n - first, p.words, SMP_PLAIN, 0.0f};
     const float t = p.temperature[row], tp = p.top_p[row], mp = p.min_p[row], un = p.u[row];
     const int k = p.top_k[row];
 
     // the row into shared memory, padded with -infinity
+    unsigned bytes = 0;
+    if (threadIdx.x < 32) sh.tab[threadIdx.x] = p.tab[threadIdx.x];
+    if (threadIdx.x == 0) sh.few = sh.listed = 0;
     if (!FAR) {
-        const unsigned bytes = p.vec ? (unsigned)(here * sizeof(T)) & ~15u : 0;
+        bytes = p.vec ? (unsigned)(here * sizeof(T)) & ~15u : 0;
         if (threadIdx.x == 0) {
             irx_mbar_init(&sh.bar, 1);
             irx_fence_mbar_init();
@@ -498,20 +542,21 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
         }
         T *e = reinterpret_cast<T *>(data);
         for (int64_t i = bytes / sizeof(T) + threadIdx.x; i < per; i += IRX_SMP_THREADS) e[i] = i < here ? src[i] : (T)-INFINITY;
-        if (threadIdx.x < 32) sh.tab[threadIdx.x] = p.tab[threadIdx.x];
-        if (threadIdx.x == 0) sh.few = sh.listed = 0;
-        __syncthreads();
-        if (bytes && !irx_mbar_wait(&sh.bar, 0) && lane == 0) atomicOr(p.err, IRX_KERR_TIMEOUT);
-    } else {
-        if (threadIdx.x < 32) sh.tab[threadIdx.x] = p.tab[threadIdx.x];
-        if (threadIdx.x == 0) sh.few = sh.listed = 0;
-        __syncthreads();
     }
-    unsigned most = ty::PAD;
-#pragma unroll 8
-    for (int j = 0; j < x.words; j++) most = ty::max2(most, x.word(j));
-    float top = ty::get(most, 0);
-    if (ty::N == 2) top = fmaxf(top, ty::get(most, 1));
+    __syncthreads();
+    if (bytes && !irx_mbar_wait(&sh.bar, 0) && lane == 0) atomicOr(p.err, IRX_KERR_TIMEOUT);
+    float top = -INFINITY;
+#pragma unroll 4
+    for (int j = 0; j < x.words; j++) {
+        const unsigned w = x.word(j);
+        float e[2];
+#pragma unroll
+        for (int h = 0; h < ty::N; h++) {
+            e[h] = smp_clean(ty::get(w, h));
+            top = fmaxf(top, e[h]);
+        }
+        if (!FAR) x.data[j] = ty::put(e[0], e[ty::N - 1]);
+    }
     const unsigned tk = __reduce_max_sync(0xffffffffu, smp_type<float>::key(top));
     if (lane == 0) sh.redc[warp] = tk;
     __syncthreads();
@@ -539,14 +584,28 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
         }
         return;
     }
+    x.mode = top == INFINITY ? SMP_INFINITE : top < -1e30f ? SMP_LOW : SMP_PLAIN;
+    x.top = top;
+    if (x.mode != SMP_PLAIN) {
+        if (!FAR)
+            for (int j = 0; j < x.words; j++) {
+                const unsigned w = x.data[j];
+                x.data[j] = ty::put(smp_shift(ty::get(w, 0), x.mode, top), smp_shift(ty::get(w, ty::N - 1), x.mode, top));
+            }
+        top = 0.0f;
+    }
+    // T is at most 1e20, so that the floor, 48 T ln 2 under the largest, is a finite number, and at least 2^-30 |max|, below
+    // which numbers next to the largest weigh nothing all the same
     smp_row q;
+    const double temp = fmax(fmin((double)t, 1e20), fabs((double)top) * 9.3132257461547852e-10);
+    const float reach = __double2float_ru((p.kbits + 2) * 0.69314718055994531 * temp);
     q.tab = sh.tab;
     q.maxf = top;
     q.max = (double)top;
-    q.c = 46.166241308446828384 / (double)t;             // 32 log2(e) / T
-    q.low = -32.0 * (p.kbits + 1);
+    q.c = 46.166241308446828384 / temp;                  // 32 log2(e) / T
+    q.floor = __fsub_rd(top, reach);
     q.one = 1ull << p.kbits;
-    q.step = (float)fmin(2047.9 * q.c / (32.0 * (p.kbits + 2)), 3.0e38);
+    q.step = (float)fmin(2.0 * 2047.6 / (double)reach, 3.0e38);
     smp_settings s;
     s.k = k > 0 && k < p.n ? k : 0;
     s.part = tp >= 1.0f || tp != tp ? 0 : tp > 0.0f ? max((uint64_t)((double)tp * 4611686018427387904.0), (uint64_t)1) : 1;
@@ -554,9 +613,9 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
     s.u = un > 0.0f ? fminf(un, 0.99999994f) : 0.0f;
     s.whole = 0;
 
-    smp_cut cut = {-INFINITY, 0};
+    smp_cut cut = {q.floor, 0};                          // (at the floor nothing weighs)
     if (s.k) {
-        smp_clear(sh);
+        smp_clear(sh, false);
         x.each([&](float v, int) {
             const unsigned cell = smp_cell(q, v);
             if (cell < IRX_SMP_BINS) smp_tally(sh, cell, false, 0);
@@ -564,48 +623,54 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
         uint64_t target = s.k;
         if (!smp_find(sh, rank, nc, turn, false, target, 0)) s.k = 0;      // fewer have any weight: all of those
         else if (sh.above + sh.count <= SMP_FEW) return smp_finish(p, sh, q, x, rank, first, row, s);
-        else cut = smp_refine(sh, q, x, rank, nc, turn, false, target);
+        else cut = smp_resolve(sh, q, x, rank, nc, turn, false, target, true);
     }
     if (s.part) {
         // the weights of what top-k kept, by cell; of those at its threshold only the first
-        smp_clear(sh);
+        smp_clear(sh, true);
         x.each([&](float v, int) {
             const unsigned cell = smp_cell(q, v);
             if (v > cut.above && cell < IRX_SMP_BINS) smp_tally(sh, cell, true, smp_weight(q, v));
         });
-        if (cut.above > -INFINITY && rank == 0) {
+        if (cut.ties && rank == 0) {
             __syncthreads();
-            if (threadIdx.x == 0) {
-                const unsigned cell = smp_cell(q, cut.above);
-                const uint64_t w = cut.ties * smp_weight(q, cut.above), sum = ((uint64_t)sh.hi[cell] << 32 | sh.lo[cell]) + w;
-                if (cell < IRX_SMP_BINS) {
-                    sh.cnt[cell] += cut.ties;
-                    sh.lo[cell] = (unsigned)sum;
-                    sh.hi[cell] = (unsigned)(sum >> 32);
-                }
+            const unsigned cell = smp_cell(q, cut.above);
+            if (threadIdx.x == 0 && cell < IRX_SMP_BINS) {
+                const uint64_t sum = ((uint64_t)sh.hi[cell] << 32 | sh.lo[cell]) + cut.ties * smp_weight(q, cut.above);
+                sh.lo[cell] = (unsigned)sum;
+                sh.hi[cell] = (unsigned)(sum >> 32);
             }
         }
         uint64_t target = 0;
         smp_find(sh, rank, nc, turn, true, target, s.part);
-        if (!s.k && sh.above + sh.count <= SMP_FEW) {
-            for (unsigned r = 0; r < nc; r++) s.whole += sh.xa[turn][r];
-            return smp_finish(p, sh, q, x, rank, first, row, s);
+        if (!s.k) {
+            // tokens in that cell and above weigh at least what the next cell's first number does
+            const unsigned cell = sh.cell;
+            const unsigned lo = smp_last(smp_least<T>(q), ty::key(q.maxf), [&](unsigned key) { return smp_cell(q, ty::value(key)) > cell; });
+            const uint64_t w = smp_weight(q, ty::value(lo));
+            if (w && (sh.before + sh.weight) / w <= SMP_FEW) {
+                for (unsigned r = 0; r < nc; r++) s.whole += sh.xa[turn][r];
+                return smp_finish(p, sh, q, x, rank, first, row, s);
+            }
         }
-        const smp_cut c = smp_refine(sh, q, x, rank, nc, turn, true, target);
-        if (c.above > cut.above) cut = c;
-        else cut.ties = min(cut.ties, c.ties);
+        const smp_cut c = smp_resolve(sh, q, x, rank, nc, turn, true, target, !s.k);
+        if (c.above > cut.above || (c.above == cut.above && c.ties < cut.ties)) cut = c;
+    }
+    if (s.least) {                                       // min-p as a threshold: the last number that weighs too little
+        const unsigned key = smp_last(smp_least<T>(q), ty::key(q.maxf), [&](unsigned kk) { return smp_weight(q, ty::value(kk)) < s.least; });
+        const float v = ty::value(key);
+        if (v >= cut.above) cut = {v, 0};
     }
 
     // the kept weights of every thread's stretch of the row, and where u times their total falls
-    const uint64_t w_cut = cut.above > -INFINITY ? smp_weight(q, cut.above) : 0, w_eq = w_cut >= s.least ? w_cut : 0;
+    const uint64_t w_eq = cut.ties ? smp_weight(q, cut.above) : 0;
     uint64_t w = 0;
     unsigned eq = 0;
-    x.each([&](float v, int) {
-        const uint64_t e = v > cut.above ? smp_weight(q, v) : 0;
-        if (e >= s.least) w += e;
+    if (cut.ties) x.each([&](float v, int) {
+        if (v > cut.above) w += smp_weight(q, v);
         eq += v == cut.above;
     });
-    if (cut.above == -INFINITY) eq = 0;
+    else x.each([&](float v, int) { if (v > cut.above) w += smp_weight(q, v); });
     const uint64_t w_mine = w;
     const unsigned eq_mine = eq;
     smp_block_sums(sh, w, eq);
@@ -635,21 +700,20 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
     const int who = __ffs(__ballot_sync(0xffffffffu, run + sum > at)) - 1;             // the lane whose stretch it is
     run = __shfl_sync(0xffffffffu, run + sum - kept, who);
     left = __shfl_sync(0xffffffffu, left, who);
-    const smp_data<T, FAR> y = {data + (warp * 32 + who) * p.words, src + (int64_t)(warp * 32 + who) * p.words * ty::N,
-                                p.n - base - (int64_t)(warp * 32 + who) * p.words * ty::N, p.words};
+    const int64_t off = (int64_t)(warp * 32 + who) * p.words;
+    const smp_data<T, FAR> y = {data + off, src + off * ty::N, p.n - base - off * ty::N, p.words, x.mode, x.top};
     for (int i0 = 0; i0 < p.words * ty::N; i0 += 32) {
         const int i = i0 + lane;
         const float v = i < p.words * ty::N ? ty::get(y.word(i / ty::N), i % ty::N) : -INFINITY;
-        const bool same = v == cut.above && v > -INFINITY;
+        const bool same = cut.ties && v == cut.above;
         const unsigned all = __ballot_sync(0xffffffffu, same);
-        uint64_t e = v > cut.above || (same && __popc(all & ((1u << lane) - 1u)) < left) ? smp_weight(q, v) : 0;
-        if (e < s.least) e = 0;
+        const uint64_t e = v > cut.above || (same && __popc(all & ((1u << lane) - 1u)) < left) ? smp_weight(q, v) : 0;
         left -= min(left, (unsigned)__popc(all));
         const uint64_t up = smp_warp_scan(e);
         const unsigned past = __ballot_sync(0xffffffffu, run + up > at);
         if (past) {
             if (lane == __ffs(past) - 1) {
-                p.token[row] = (int)(base + (int64_t)(warp * 32 + who) * p.words * ty::N + i);
+                p.token[row] = (int)(base + off * ty::N + i);
                 if (p.logprob) p.logprob[row] = (float)log((double)e / (double)total);
             }
             return;
