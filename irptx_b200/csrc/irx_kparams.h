@@ -227,7 +227,7 @@ typedef struct {
 /* The draw of a token: one cluster a row; a thread of a block holds `words` words of 4 bytes, an odd number. */
 #define IRX_SMP_BINS 2048
 #define IRX_SMP_THREADS 512
-#define IRX_SMP_FIXED (IRX_SMP_BINS * 12 + 2048)   /* shared memory beside the row: histogram, reductions */
+#define IRX_SMP_FIXED (IRX_SMP_BINS * 12 + 2560)   /* shared memory beside the row: histogram, reductions */
 
 typedef struct {
     const void *x;
@@ -240,7 +240,9 @@ typedef struct {
     int32_t     words;
     int32_t     kbits;              /* a weight of 1 is 2^kbits, at most 2^46 */
     uint8_t     vec, pad[7];        /* rows of logits begin on 16 bytes */
-    double      tab[32];            /* 2^(kbits + j / 32) */
+    /* constants of the weights' exponential, here so that instructions read them in place: 1.5 * 2^52, 2^52,
+     * (ln 2 / 128)^i / i! for i = 1 to 4, and 2^(kbits + j / 128) */
+    double      big, two52, series[4], tab[128];
 } irx_ksmp_t;
 
 #endif /* IRX_KPARAMS_H */

@@ -48,9 +48,9 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
 {
     constexpr int NB = DP / 64, TILE = NB * PT_HALF;
     irx_pdl_enter();
-    extern __shared__ __align__(1024) unsigned char smem_raw[];
-    unsigned char *sq = smem_raw, *sk = sq + 2 * TILE, *sv = sk + 2 * TILE;
-    if (irx_smem_u32(smem_raw) & 1023u) {
+    extern __shared__ __align__(1024) unsigned char pt_smem[];
+    unsigned char *sq = pt_smem, *sk = sq + 2 * TILE, *sv = sk + 2 * TILE;
+    if (irx_smem_u32(pt_smem) & 1023u) {
         if (threadIdx.x == 0) atomicOr(p.err, IRX_KERR_TIMEOUT);
         return;
     }

@@ -21,13 +21,14 @@
 
 #define SMP_WARPS (IRX_SMP_THREADS / 32)
 #define SMP_FEW 1024                     // tokens that one block finishes alone
+#define SMP_STEP 4                       // words that a thread takes at a time
 
 struct smp_shared {
     union {
         struct { unsigned cnt[IRX_SMP_BINS], lo[IRX_SMP_BINS], hi[IRX_SMP_BINS]; };   // a cell's tokens, or its weight in two words
         struct { uint64_t mine[SMP_FEW], list[SMP_FEW], weight_of[SMP_FEW]; };        // few tokens: this block's, the row's, their weights
     };
-    double tab[32];
+    double tab[128];
     uint64_t red[SMP_WARPS], xa[2][8];   // warps' parts; what every block of the cluster posted, two exchanges of it
     unsigned redc[SMP_WARPS], xc[2][8];
     uint64_t before, weight;             // the cell found: the weight above it, its own
@@ -55,6 +56,7 @@ __device__ __forceinline__ float smp_shift(float x, int mode, float top)
 template <class T> struct smp_type;
 template <> struct smp_type<float> {
     static const int N = 1;
+    static const unsigned PAD = 0xff800000u;             // -infinity
     __device__ static __forceinline__ float get(unsigned w, int) { return __uint_as_float(w); }
     __device__ static __forceinline__ unsigned put(float a, float) { return __float_as_uint(a); }
     __device__ static __forceinline__ unsigned key(float x)
@@ -66,6 +68,7 @@ template <> struct smp_type<float> {
 };
 template <> struct smp_type<__nv_bfloat16> {
     static const int N = 2;
+    static const unsigned PAD = 0xff80ff80u;
     __device__ static __forceinline__ float get(unsigned w, int h) { return __uint_as_float(h ? w & 0xffff0000u : w << 16); }
     __device__ static __forceinline__ unsigned put(float a, float b) { return __float_as_uint(a) >> 16 | (__float_as_uint(b) & 0xffff0000u); }
     __device__ static __forceinline__ unsigned key(float x)
@@ -77,30 +80,34 @@ template <> struct smp_type<__nv_bfloat16> {
 };
 
 struct smp_row {
-    double max, c;                       // a weight is 2^(kbits + (x - max) c / 32)
+    double c, at_max;                    // a weight is 2^(kbits + (x c - at_max) / 128)
     float maxf, floor, step;             // at the floor and below it rounds to 0; cells: (max - x) / 2 * step
-    uint64_t one;                        // 2^kbits
+    uint64_t one;                        // the largest logit's weight
     const double *tab;
+    const irx_ksmp_t *p;
 };
 
-// The weight of a logit. 2^(z / 32) = 2^(i / 32) 2^(r / 32), i = round(z), |r| <= 1/2: a table of 32, kbits in it, and
-// the exponential series to r^5, whose rest is below 2^-48. The last sum, with 2^52, leaves the rounded integer in
-// the low bits. The floor keeps i above -7000 (see T below), so that exponents are added without a check.
-__device__ __forceinline__ uint64_t smp_weight(const smp_row &q, float x)
+// The weight of a logit above the floor, in the low 52 bits under those of 2^52. 2^(z / 128) = 2^(i / 128) 2^(r / 128),
+// i = round(z), |r| <= 1/2: a table of 128, kbits in it, and the exponential series to r^4, whose rest is below 2^-49.
+// The last sum, with 2^52, leaves the rounded integer. at_max is rounded once a row, which scales all its weights
+// alike. The floor keeps i above -30000 (see T below), so that exponents are added without a check.
+__device__ __forceinline__ uint64_t smp_raw(const smp_row &q, float x)
 {
-    const double z = ((double)fmaxf(x, q.floor) - q.max) * q.c;
-    const double big = 6755399441055744.0, l = 0.021660849392498290;                // 1.5 * 2^52, ln 2 / 32
-    const double f = z + big;
+    const irx_ksmp_t &p = *q.p;
+    const double z = fma((double)x, q.c, -q.at_max);
+    const double f = z + p.big;
     const int i = __double2loint(f);
-    const double r = z - (f - big), t = q.tab[i & 31];
-    double e = fma(r, l * l * l * l * l / 120.0, l * l * l * l / 24.0);
-    e = fma(e, r, l * l * l / 6.0);
-    e = fma(e, r, l * l / 2.0);
-    e = fma(e, r, l);
+    const double r = z - (f - p.big), t = q.tab[i & 127];
+    double e = fma(r, p.series[3], p.series[2]);
+    e = fma(e, r, p.series[1]);
+    e = fma(e, r, p.series[0]);
     e = fma(e, r, 1.0);
-    e = fma(e, __hiloint2double(__double2hiint(t) + (i & ~31) * (1 << 15), __double2loint(t)), 4503599627370496.0);
-    return (uint64_t)__double_as_longlong(e) & 0xfffffffffffffull;
+    e = fma(e, __hiloint2double(__double2hiint(t) + (i & ~127) * (1 << 13), __double2loint(t)), p.two52);
+    return (uint64_t)__double_as_longlong(e);
 }
+#define SMP_RAW 0x4330000000000000ull    // the bits of 2^52: a sum of n raw weights has n of them too many
+
+__device__ __forceinline__ uint64_t smp_weight(const smp_row &q, float x) { return smp_raw(q, fmaxf(x, q.floor)) - SMP_RAW; }
 
 // The cell of the first histogram, at least IRX_SMP_BINS for what has no weight. Never falls as x falls.
 __device__ __forceinline__ unsigned smp_cell(const smp_row &q, float x)
@@ -512,9 +519,9 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
 {
     typedef smp_type<T> ty;
     irx_pdl_enter();
-    extern __shared__ __align__(16) unsigned char smp_raw[];
-    smp_shared &sh = *reinterpret_cast<smp_shared *>(smp_raw);
-    unsigned *data = reinterpret_cast<unsigned *>(smp_raw + IRX_SMP_FIXED);
+    extern __shared__ __align__(16) unsigned char smp_bytes[];
+    smp_shared &sh = *reinterpret_cast<smp_shared *>(smp_bytes);
+    unsigned *data = reinterpret_cast<unsigned *>(smp_bytes + IRX_SMP_FIXED);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     unsigned rank = cluster_rank(), nc, turn = 0;
     asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(nc));
@@ -528,7 +535,7 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
 
     // the row into shared memory, padded with -infinity
     unsigned bytes = 0;
-    if (threadIdx.x < 32) sh.tab[threadIdx.x] = p.tab[threadIdx.x];
+    if (threadIdx.x < 128) sh.tab[threadIdx.x] = p.tab[threadIdx.x];
     if (threadIdx.x == 0) sh.few = sh.listed = 0;
     if (!FAR) {
         bytes = p.vec ? (unsigned)(here * sizeof(T)) & ~15u : 0;
@@ -601,10 +608,11 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
     const float reach = __double2float_ru((p.kbits + 2) * 0.69314718055994531 * temp);
     q.tab = sh.tab;
     q.maxf = top;
-    q.max = (double)top;
-    q.c = 46.166241308446828384 / temp;                  // 32 log2(e) / T
+    q.p = &p;
+    q.c = 184.66496523378731354 / temp;                  // 128 log2(e) / T
+    q.at_max = (double)top * q.c;
     q.floor = __fsub_rd(top, reach);
-    q.one = 1ull << p.kbits;
+    q.one = smp_weight(q, top);
     q.step = (float)fmin(2.0 * 2047.6 / (double)reach, 3.0e38);
     smp_settings s;
     s.k = k > 0 && k < p.n ? k : 0;
@@ -662,15 +670,29 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
         if (v >= cut.above) cut = {v, 0};
     }
 
-    // the kept weights of every thread's stretch of the row, and where u times their total falls
+    // the kept weights of every thread's stretch of the row, and where u times their total falls. What is not kept counts as
+    // at the floor, with no weight; eight numbers of which no lane of a warp keeps any are passed over.
     const uint64_t w_eq = cut.ties ? smp_weight(q, cut.above) : 0;
     uint64_t w = 0;
     unsigned eq = 0;
-    if (cut.ties) x.each([&](float v, int) {
-        if (v > cut.above) w += smp_weight(q, v);
-        eq += v == cut.above;
-    });
-    else x.each([&](float v, int) { if (v > cut.above) w += smp_weight(q, v); });
+    for (int j0 = 0; j0 < x.words; j0 += SMP_STEP) {
+        float v[SMP_STEP * ty::N], most = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < SMP_STEP; j++) {
+            const unsigned word = j0 + j < x.words ? x.word(j0 + j) : ty::PAD;
+#pragma unroll
+            for (int h = 0; h < ty::N; h++) {
+                v[j * ty::N + h] = ty::get(word, h);
+                most = fmaxf(most, v[j * ty::N + h]);
+            }
+        }
+        if (!__any_sync(0xffffffffu, most >= cut.above)) continue;
+        if (cut.ties)
+#pragma unroll
+            for (int j = 0; j < SMP_STEP * ty::N; j++) eq += v[j] == cut.above;
+#pragma unroll
+        for (int j = 0; j < SMP_STEP * ty::N; j++) w += smp_raw(q, v[j] > cut.above ? v[j] : q.floor) - SMP_RAW;
+    }
     const uint64_t w_mine = w;
     const unsigned eq_mine = eq;
     smp_block_sums(sh, w, eq);

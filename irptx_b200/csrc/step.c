@@ -325,7 +325,10 @@ static int launch_sample(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
     while ((1ll << k.kbits) < a->vocab) k.kbits++;
     k.kbits = 62 - k.kbits;                                 /* a row's weights sum to at most 2^62 */
     if (k.kbits > 46) k.kbits = 46;
-    for (j = 0; j < 32; j++) k.tab[j] = ldexp(exp2(j / 32.0), k.kbits);
+    k.big = 6755399441055744.0;
+    k.two52 = 4503599627370496.0;
+    for (j = 0; j < 4; j++) k.series[j] = (j ? k.series[j - 1] : 1.0) * (0.69314718055994530942 / 128.0) / (j + 1);
+    for (j = 0; j < 128; j++) k.tab[j] = ldexp(exp2(j / 128.0), k.kbits);
     k.vec = (uint8_t)(a_to(k.x, 16) && a->stride * 4 / epw % 16 == 0);
     /* blocks of a cluster: the row's elements in their shared memory, at least 4096 each */
     nc = 1;
