@@ -21,6 +21,8 @@
 
 #define SMP_WARPS (IRX_SMP_THREADS / 32)
 #define SMP_FEW 1024                     // tokens that one block finishes alone
+#define SMP_CELLS (IRX_SMP_BINS / IRX_SMP_THREADS)      // cells of a thread, in a cluster of one
+#define SMP_OWN (SMP_FEW / IRX_SMP_THREADS)             // few tokens: a thread's
 #define SMP_STEP 4                       // words that a thread takes at a time
 
 struct smp_shared {
@@ -29,39 +31,36 @@ struct smp_shared {
         struct { uint64_t mine[SMP_FEW], list[SMP_FEW], weight_of[SMP_FEW]; };        // few tokens: this block's, the row's, their weights
     };
     double tab[128];
-    uint64_t red[SMP_WARPS], xa[2][8];   // warps' parts; what every block of the cluster posted, two exchanges of it
+    uint64_t red[3][SMP_WARPS], xa[2][8], xb[2][8], xd[2][8];      // warps' parts; what the cluster's blocks posted, two exchanges of it
     unsigned redc[SMP_WARPS], xc[2][8];
     uint64_t before, weight;             // the cell found: the weight above it, its own
     unsigned above, count, cell;         // tokens above it, its own
-    unsigned few, listed, at, key, ties;
+    unsigned few, key, ties;
     uint64_t bar;
 };
 static_assert(sizeof(smp_shared) <= IRX_SMP_FIXED, "the launcher's size");
 
-// Logits as numbers that order and weigh as defined: NaN as -infinity, both zeros as +0. For rows whose largest is
-// infinite (then such logits are 0 and all others -infinity) or below -1e30 (then the largest is taken away from
-// all: exactly, wherever a weight is left) a second step follows, so that a number far below the largest exists.
+// Logits as numbers that order and weigh as defined: NaN as -infinity. For rows whose largest is infinite (then such
+// logits are 0 and all others -infinity) or below -1e30 (then the largest is taken away from all: exactly, wherever a
+// weight is left) a second step follows, so that a number far below the largest exists.
 enum { SMP_PLAIN, SMP_INFINITE, SMP_LOW };
-__device__ __forceinline__ float smp_clean(float x)
-{
-    x += 0.0f;
-    return x == x ? x : -INFINITY;
-}
 __device__ __forceinline__ float smp_shift(float x, int mode, float top)
 {
     return mode == SMP_INFINITE ? (x == INFINITY ? 0.0f : -INFINITY) : mode == SMP_LOW ? x - top : x;
 }
 
-// Keys order as the numbers do.
+// Keys order as the numbers do, both zeros alike.
 template <class T> struct smp_type;
 template <> struct smp_type<float> {
     static const int N = 1;
     static const unsigned PAD = 0xff800000u;             // -infinity
     __device__ static __forceinline__ float get(unsigned w, int) { return __uint_as_float(w); }
     __device__ static __forceinline__ unsigned put(float a, float) { return __float_as_uint(a); }
+    // the larger of each element; of a number and NaN, the number
+    __device__ static __forceinline__ unsigned most(unsigned a, unsigned b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
     __device__ static __forceinline__ unsigned key(float x)
     {
-        const unsigned u = __float_as_uint(x);
+        const unsigned u = __float_as_uint(x + 0.0f);
         return u & 0x80000000u ? ~u : u | 0x80000000u;
     }
     __device__ static __forceinline__ float value(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
@@ -70,10 +69,15 @@ template <> struct smp_type<__nv_bfloat16> {
     static const int N = 2;
     static const unsigned PAD = 0xff80ff80u;
     __device__ static __forceinline__ float get(unsigned w, int h) { return __uint_as_float(h ? w & 0xffff0000u : w << 16); }
+    __device__ static __forceinline__ unsigned most(unsigned a, unsigned b)
+    {
+        const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
+        return *reinterpret_cast<const unsigned *>(&m);
+    }
     __device__ static __forceinline__ unsigned put(float a, float b) { return __float_as_uint(a) >> 16 | (__float_as_uint(b) & 0xffff0000u); }
     __device__ static __forceinline__ unsigned key(float x)
     {
-        const unsigned u = __float_as_uint(x) >> 16;
+        const unsigned u = __float_as_uint(x + 0.0f) >> 16;
         return u & 0x8000u ? ~u & 0xffffu : u | 0x8000u;
     }
     __device__ static __forceinline__ float value(unsigned k) { return __uint_as_float((k & 0x8000u ? k & 0x7fffu : ~k & 0xffffu) << 16); }
@@ -84,16 +88,14 @@ struct smp_row {
     float maxf, floor, step;             // at the floor and below it rounds to 0; cells: (max - x) / 2 * step
     uint64_t one;                        // the largest logit's weight
     const double *tab;
-    const irx_ksmp_t *p;
 };
 
 // The weight of a logit above the floor, in the low 52 bits under those of 2^52. 2^(z / 128) = 2^(i / 128) 2^(r / 128),
 // i = round(z), |r| <= 1/2: a table of 128, kbits in it, and the exponential series to r^4, whose rest is below 2^-49.
 // The last sum, with 2^52, leaves the rounded integer. at_max is rounded once a row, which scales all its weights
 // alike. The floor keeps i above -30000 (see T below), so that exponents are added without a check.
-__device__ __forceinline__ uint64_t smp_raw(const smp_row &q, float x)
+__device__ __forceinline__ uint64_t smp_raw(const irx_ksmp_t &p, const smp_row &q, float x)
 {
-    const irx_ksmp_t &p = *q.p;
     const double z = fma((double)x, q.c, -q.at_max);
     const double f = z + p.big;
     const int i = __double2loint(f);
@@ -107,7 +109,7 @@ __device__ __forceinline__ uint64_t smp_raw(const smp_row &q, float x)
 }
 #define SMP_RAW 0x4330000000000000ull    // the bits of 2^52: a sum of n raw weights has n of them too many
 
-__device__ __forceinline__ uint64_t smp_weight(const smp_row &q, float x) { return smp_raw(q, fmaxf(x, q.floor)) - SMP_RAW; }
+__device__ __forceinline__ uint64_t smp_weight(const irx_ksmp_t &p, const smp_row &q, float x) { return smp_raw(p, q, fmaxf(x, q.floor)) - SMP_RAW; }
 
 // The cell of the first histogram, at least IRX_SMP_BINS for what has no weight. Never falls as x falls.
 __device__ __forceinline__ unsigned smp_cell(const smp_row &q, float x)
@@ -183,13 +185,16 @@ __device__ __forceinline__ void smp_cluster_sync()
     cluster_sync();
 }
 
-// Every block of the cluster learns every block's (a, c); `turn` alternates, so that one exchange's values
+// Every block of the cluster learns every block's (a, c, b, d); `turn` alternates, so that one exchange's values
 // are not written over before all have read them.
-__device__ __forceinline__ void smp_post(smp_shared &sh, unsigned rank, unsigned nc, unsigned &turn, uint64_t a, unsigned c)
+__device__ __forceinline__ void smp_post(smp_shared &sh, unsigned rank, unsigned nc, unsigned &turn, uint64_t a, unsigned c,
+                                         uint64_t b = 0, uint64_t d = 0)
 {
     turn ^= 1u;
     if (threadIdx.x < nc) {
         smp_st64(&sh.xa[turn][rank], threadIdx.x, a);
+        smp_st64(&sh.xb[turn][rank], threadIdx.x, b);
+        smp_st64(&sh.xd[turn][rank], threadIdx.x, d);
         smp_st32(&sh.xc[turn][rank], threadIdx.x, c);
     }
     smp_cluster_sync();
@@ -208,7 +213,7 @@ template <class T, bool FAR> struct smp_data {
         float e[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int h = 0; h < smp_type<T>::N; h++)
-            if (j * smp_type<T>::N + h < left) e[h] = smp_shift(smp_clean((float)src[(int64_t)j * smp_type<T>::N + h]), mode, top);
+            if (j * smp_type<T>::N + h < left) e[h] = smp_shift(fmaxf((float)src[(int64_t)j * smp_type<T>::N + h], -INFINITY), mode, top);
         return smp_type<T>::put(e[0], e[1]);
     }
     // f(number, index among this thread's elements) for each of them
@@ -225,24 +230,24 @@ template <class T, bool FAR> struct smp_data {
 
 struct smp_cut { float above; unsigned ties; };     // what is kept: what is above, and the first `ties` of those equal
 
-// Sums over the block: of `w` and of `c`, by warp into red and redc. All threads get both totals.
-__device__ __forceinline__ void smp_block_sums(smp_shared &sh, uint64_t &w, unsigned &c)
+// Sums over the block of N numbers and of `c`; the warps' parts stay in red and redc. All threads get the totals.
+template <int N>
+__device__ __forceinline__ void smp_block_sums(smp_shared &sh, uint64_t (&w)[N], unsigned &c)
 {
-    w = smp_warp_sum(w);
+#pragma unroll
+    for (int i = 0; i < N; i++) w[i] = smp_warp_sum(w[i]);
     c = __reduce_add_sync(0xffffffffu, c);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) {
-        sh.red[threadIdx.x >> 5] = w;
+#pragma unroll
+        for (int i = 0; i < N; i++) sh.red[i][threadIdx.x >> 5] = w[i];
         sh.redc[threadIdx.x >> 5] = c;
     }
     __syncthreads();
-    w = 0;
-    c = 0;
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 0; i < SMP_WARPS; i++) {
-        w += sh.red[i];
-        c += sh.redc[i];
-    }
+    for (int i = 0; i < N; i++) w[i] = smp_warp_sum(lane < SMP_WARPS ? sh.red[i][lane] : 0);
+    c = __reduce_add_sync(0xffffffffu, lane < SMP_WARPS ? sh.redc[lane] : 0u);
 }
 
 __device__ __forceinline__ void smp_clear(smp_shared &sh, bool by_weight)
@@ -267,22 +272,25 @@ __device__ __forceinline__ void smp_tally(smp_shared &sh, unsigned cell, bool by
 
 // The cell of the blocks' histograms in which the running count, or weight, reaches `target`, from cell 0 on; false when
 // all of them together do not. With `part`, a share of all: target = the least integer not below part / 2^62 times
-// the whole weight, at least 1. Fills every block's sh.cell, above and count, or before and weight.
+// the whole weight, at least 1. SMP_GUESS: the weights are guessed from the cells' tokens, `bits` being what a cell
+// takes from a weight's logarithm. Fills every block's sh.cell, above and count, before and weight.
+enum { SMP_COUNT, SMP_WEIGHT, SMP_GUESS };
 __device__ __forceinline__ uint64_t smp_part(uint64_t part, uint64_t v, bool up)
 {
     const uint64_t hi = __umul64hi(part, v), lo = part * v;
     return (hi << 2 | lo >> 62) + (up && (lo << 2) != 0);
 }
 
-__device__ __forceinline__ bool smp_find(smp_shared &sh, unsigned rank, unsigned nc, unsigned &turn, bool by_weight, uint64_t &target, uint64_t part)
+__device__ __forceinline__ bool smp_find(smp_shared &sh, unsigned rank, unsigned nc, unsigned &turn, int mode, uint64_t &target, uint64_t part, float bits = 0.0f)
 {
+    const bool by_weight = mode != SMP_COUNT;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int slice = IRX_SMP_BINS / nc, each = (slice + IRX_SMP_THREADS - 1) / IRX_SMP_THREADS;
     smp_cluster_sync();                                  // every block's histogram is whole
-    unsigned c[4], cs = 0;
-    uint64_t w[4], ws = 0;
+    unsigned c[SMP_CELLS], cs = 0;
+    uint64_t w[SMP_CELLS], ws = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < SMP_CELLS; i++) {
         c[i] = 0;
         w[i] = 0;
         const int b = threadIdx.x * each + i;
@@ -293,7 +301,7 @@ __device__ __forceinline__ bool smp_find(smp_shared &sh, unsigned rank, unsigned
             for (int r = 0; r < 8; r++) {
                 a[r] = l[r] = h[r] = 0;
                 if (r >= nc) continue;
-                if (by_weight) {
+                if (mode == SMP_WEIGHT) {
                     l[r] = smp_ld32(&sh.lo[cell], r);
                     h[r] = smp_ld32(&sh.hi[cell], r);
                 } else a[r] = smp_ld32(&sh.cnt[cell], r);
@@ -303,6 +311,7 @@ __device__ __forceinline__ bool smp_find(smp_shared &sh, unsigned rank, unsigned
                 c[i] += a[r];
                 w[i] += (uint64_t)l[r] + ((uint64_t)h[r] << 32);
             }
+            if (mode == SMP_GUESS) w[i] = (uint64_t)((float)c[i] * exp2f(32.0f - bits * (float)cell));
         }
         cs += c[i];
         ws += w[i];
@@ -311,20 +320,15 @@ __device__ __forceinline__ bool smp_find(smp_shared &sh, unsigned rank, unsigned
     const uint64_t wi = by_weight ? smp_warp_scan(ws) : 0;
     if (lane == 31) {
         sh.redc[warp] = ci;
-        sh.red[warp] = wi;
+        sh.red[0][warp] = wi;
     }
     __syncthreads();
-    uint64_t wb = wi - ws, wt = 0;
-    unsigned cb = ci - cs, ct = 0;
-#pragma unroll
-    for (int i = 0; i < SMP_WARPS; i++) {
-        if (i < warp) {
-            cb += sh.redc[i];
-            wb += sh.red[i];
-        }
-        ct += sh.redc[i];
-        wt += sh.red[i];
-    }
+    uint64_t wt = lane < SMP_WARPS ? sh.red[0][lane] : 0;
+    unsigned ct = lane < SMP_WARPS ? sh.redc[lane] : 0;
+    uint64_t wb = wi - ws + smp_warp_sum(lane < warp ? wt : 0);
+    unsigned cb = ci - cs + __reduce_add_sync(0xffffffffu, lane < warp ? ct : 0u);
+    wt = smp_warp_sum(wt);
+    ct = __reduce_add_sync(0xffffffffu, ct);
     smp_post(sh, rank, nc, turn, wt, ct);
     uint64_t all = 0, whole = 0;
     for (unsigned r = 0; r < nc; r++) {
@@ -339,7 +343,7 @@ __device__ __forceinline__ bool smp_find(smp_shared &sh, unsigned rank, unsigned
     }
     if (part) target = max(smp_part(part, whole, true), (uint64_t)1);
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < SMP_CELLS; i++) {
         const uint64_t b = by_weight ? wb : cb, n = by_weight ? w[i] : c[i];
         if (b < target && target <= b + n) {             // one thread of the cluster
             for (unsigned r = 0; r < nc; r++) {
@@ -357,10 +361,90 @@ __device__ __forceinline__ bool smp_find(smp_shared &sh, unsigned rank, unsigned
     return target <= all;
 }
 
-// After a first histogram whose cell has been found: the exact threshold in it. The cell's tokens go to block 0 when
-// they are few, else histograms of its range follow.
+// This block's few tokens (n of them in sh.mine) into block 0's list, behind those of the blocks before it. Ends with a
+// cluster barrier.
+__device__ __forceinline__ void smp_hand_over(smp_shared &sh, unsigned n, unsigned at)
+{
+    for (unsigned i = threadIdx.x; i < n; i += IRX_SMP_THREADS) smp_st64(&sh.list[at + i], 0, sh.mine[i]);
+    smp_cluster_sync();
+}
+
+__device__ __forceinline__ uint64_t smp_token(float v, int64_t i) { return (uint64_t)~smp_type<float>::key(v) << 32 | (unsigned)i; }
+
+__device__ __forceinline__ float smp_number(uint64_t token) { return smp_type<float>::value(~(unsigned)(token >> 32)); }
+
+// The threshold among the m tokens of block 0's list, numbers with keys from lo to hi, of which `left` tokens, or that much
+// weight, are to be kept: histograms of 256 cells of the range, by block 0, until a cell is one number.
+template <class T>
+__device__ __forceinline__ smp_cut smp_among(const irx_ksmp_t &p, smp_shared &sh, const smp_row &q, unsigned rank, unsigned nc, unsigned m,
+                                             unsigned lo, unsigned hi, uint64_t left, bool by_weight)
+{
+    typedef smp_type<T> ty;
+    if (rank == 0) {
+        unsigned *low = reinterpret_cast<unsigned *>(sh.mine), *high = low + 256;        // a cell's sum in two words
+        const int lane = threadIdx.x & 31;
+        unsigned key[SMP_OWN];
+        uint64_t w[SMP_OWN];
+#pragma unroll
+        for (int a = 0; a < SMP_OWN; a++) {
+            const unsigned i = threadIdx.x + a * IRX_SMP_THREADS;
+            const float v = i < m ? smp_number(sh.list[i]) : 0.0f;
+            key[a] = i < m ? ty::key(v) : ~0u;
+            w[a] = i < m ? by_weight ? smp_weight(p, q, v) : 1 : 0;
+        }
+        for (;;) {
+            unsigned shift = 0;
+            while (((hi - lo) >> shift) >= 256) shift++;
+            for (int b = threadIdx.x; b < 512; b += IRX_SMP_THREADS) low[b] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int a = 0; a < SMP_OWN; a++)
+                if (key[a] >= lo && key[a] <= hi) {
+                    const unsigned cell = (hi - key[a]) >> shift, wl = (unsigned)w[a], old = atomicAdd(&low[cell], wl);
+                    const unsigned up = (unsigned)(w[a] >> 32) + (old + wl < old);
+                    if (up) atomicAdd(&high[cell], up);
+                }
+            __syncthreads();
+            if (threadIdx.x < 32) {                      // 8 cells a lane
+                uint64_t c[8], sum = 0;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    c[i] = (uint64_t)high[lane * 8 + i] << 32 | low[lane * 8 + i];
+                    sum += c[i];
+                }
+                uint64_t b = smp_warp_scan(sum) - sum;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if (b < left && left <= b + c[i]) {
+                        sh.cell = lane * 8 + i;
+                        sh.before = b;
+                        sh.weight = c[i];
+                    }
+                    b += c[i];
+                }
+            }
+            __syncthreads();
+            left -= sh.before;
+            hi -= sh.cell << shift;
+            lo = hi - lo > (1u << shift) - 1u ? hi - ((1u << shift) - 1u) : lo;
+            if (lo == hi) break;
+        }
+        if (threadIdx.x < nc) {                          // sh.weight is that of this number's tokens, all alike
+            const uint64_t one = by_weight ? smp_weight(p, q, ty::value(lo)) : 1, ties = (left + one - 1) / one;
+            const bool all = ties * one >= sh.weight;    // none of them is cut off: up to the number below
+            smp_st32(&sh.key, threadIdx.x, all ? lo - 1 : lo);
+            smp_st32(&sh.ties, threadIdx.x, all ? 0 : (unsigned)ties);
+        }
+    }
+    if (threadIdx.x == 0) sh.few = 0;
+    smp_cluster_sync();
+    return {ty::value(sh.key), sh.ties};
+}
+
+// After a first histogram whose cell has been found: the exact threshold in it. The cell's tokens go to block 0 when they
+// are few and all of them count (gather), else histograms of its range follow.
 template <class T, bool FAR>
-__device__ __forceinline__ smp_cut smp_resolve(smp_shared &sh, const smp_row &q, const smp_data<T, FAR> &x, unsigned rank, unsigned nc,
+__device__ __forceinline__ smp_cut smp_resolve(const irx_ksmp_t &p, smp_shared &sh, const smp_row &q, const smp_data<T, FAR> &x, unsigned rank, unsigned nc,
                                                unsigned &turn, bool by_weight, uint64_t target, bool gather)
 {
     typedef smp_type<T> ty;
@@ -369,51 +453,25 @@ __device__ __forceinline__ smp_cut smp_resolve(smp_shared &sh, const smp_row &q,
     unsigned lo = smp_last(least, top, [&](unsigned k) { return smp_cell(q, ty::value(k)) > cell; }) + 1;
     uint64_t count = sh.count;                           // at most
     if (by_weight) {
-        const uint64_t w = smp_weight(q, ty::value(lo));
+        const uint64_t w = smp_weight(p, q, ty::value(lo));
         count = w ? sh.weight / w : ~0ull;
     }
     uint64_t left = target - (by_weight ? sh.before : sh.above);
     if (lo != hi && gather && count <= SMP_FEW) {
         const float from = ty::value(lo), to = ty::value(hi);
-        unsigned *mine = reinterpret_cast<unsigned *>(sh.mine), *list = reinterpret_cast<unsigned *>(sh.list);
         x.each([&](float v, int) {
-            if (v >= from && v <= to) mine[atomicAdd(&sh.few, 1u)] = ty::key(v);
+            if (v >= from && v <= to) sh.mine[atomicAdd(&sh.few, 1u)] = smp_token(v, 0);
         });
         __syncthreads();
         const unsigned n = sh.few;
-        if (threadIdx.x == 0 && n) sh.at = smp_add32(&sh.listed, 0, n);
-        __syncthreads();
-        for (unsigned i = threadIdx.x; i < n; i += IRX_SMP_THREADS) smp_st32(&list[sh.at + i], 0, mine[i]);
-        smp_cluster_sync();
-        if (rank == 0) {
-            const unsigned m = sh.listed;
-            for (unsigned i = threadIdx.x; i < m; i += IRX_SMP_THREADS) sh.weight_of[i] = by_weight ? smp_weight(q, ty::value(list[i])) : 1;
-            __syncthreads();
-            for (unsigned i = threadIdx.x; i < m; i += IRX_SMP_THREADS) {
-                const unsigned k = list[i];
-                uint64_t above = 0;
-                unsigned same = 0;
-#pragma unroll 4
-                for (unsigned j = 0; j < m; j++) {
-                    if (list[j] > k) above += sh.weight_of[j];
-                    same += list[j] == k;
-                }
-                const uint64_t w = sh.weight_of[i];
-                if (above < left && left <= above + same * w) {        // this number's tokens, all alike
-                    const unsigned ties = (unsigned)((left - above + w - 1) / w);
-                    for (unsigned r = 0; r < nc; r++) {                // none of them is cut off: up to the number below
-                        smp_st32(&sh.key, r, ties == same ? k - 1 : k);
-                        smp_st32(&sh.ties, r, ties == same ? 0 : ties);
-                    }
-                }
-            }
+        unsigned at = 0, m = 0;
+        smp_post(sh, rank, nc, turn, 0, n);
+        for (unsigned r = 0; r < nc; r++) {
+            if (r == rank) at = m;
+            m += sh.xc[turn][r];
         }
-        if (threadIdx.x == 0) {
-            sh.few = 0;
-            if (rank == 0) sh.listed = 0;
-        }
-        smp_cluster_sync();
-        return {ty::value(sh.key), sh.ties};
+        smp_hand_over(sh, n, at);
+        return smp_among<T>(p, sh, q, rank, nc, m, lo, hi, left, by_weight);
     }
     while (lo != hi) {
         unsigned shift = 0;
@@ -421,47 +479,32 @@ __device__ __forceinline__ smp_cut smp_resolve(smp_shared &sh, const smp_row &q,
         smp_clear(sh, by_weight);
         const float from = ty::value(lo), to = ty::value(hi);
         x.each([&](float v, int) {
-            if (v >= from && v <= to) smp_tally(sh, (hi - ty::key(v)) >> shift, by_weight, by_weight ? smp_weight(q, v) : 0);
+            if (v >= from && v <= to) smp_tally(sh, (hi - ty::key(v)) >> shift, by_weight, by_weight ? smp_weight(p, q, v) : 0);
         });
-        smp_find(sh, rank, nc, turn, by_weight, left, 0);
+        smp_find(sh, rank, nc, turn, by_weight ? SMP_WEIGHT : SMP_COUNT, left, 0);
         left -= by_weight ? sh.before : sh.above;
         hi -= sh.cell << shift;
-        count = by_weight ? sh.weight / max(smp_weight(q, ty::value(hi)), (uint64_t)1) : sh.count;
+        count = by_weight ? sh.weight / max(smp_weight(p, q, ty::value(hi)), (uint64_t)1) : sh.count;
         lo = hi - lo > (1u << shift) - 1u ? hi - ((1u << shift) - 1u) : lo;
     }
-    const uint64_t w = by_weight ? smp_weight(q, ty::value(lo)) : 1, ties = (left + w - 1) / w;
+    const uint64_t w = by_weight ? smp_weight(p, q, ty::value(lo)) : 1, ties = (left + w - 1) / w;
     // (count is exact here: a single number's tokens weigh the same)
     return ties >= count ? smp_cut{ty::value(lo - 1), 0u} : smp_cut{ty::value(lo), (unsigned)ties};
 }
 
 struct smp_settings { uint64_t k, part, least, whole; float u; };      // part: top-p in 2^-62, 0 off; least: min-p's weight
 
-// The few tokens in cells up to sh.cell, gathered in block 0: all filters and the draw.
-// whole: the row's weight, when top-k is off.
-template <class T, bool FAR>
-__device__ __forceinline__ void smp_finish(const irx_ksmp_t &p, smp_shared &sh, const smp_row &q, const smp_data<T, FAR> &x, unsigned rank,
-                                           int64_t first, int64_t row, const smp_settings &s)
+// Block 0, with all tokens that a filter may keep in its list, m of them: all filters and the draw. s.whole: the row's
+// weight, when top-k is off.
+__device__ __forceinline__ void smp_finish(const irx_ksmp_t &p, smp_shared &sh, const smp_row &q, unsigned m, int64_t row, const smp_settings &s)
 {
-    const unsigned cell = sh.cell;
-    __syncthreads();                                     // (the histograms have been read: smp_find ends with a cluster barrier)
-    x.each([&](float v, int i) {
-        if (smp_cell(q, v) <= cell) sh.mine[atomicAdd(&sh.few, 1u)] = (uint64_t)~smp_type<float>::key(v) << 32 | (unsigned)(first + i);
-    });
-    __syncthreads();
-    const unsigned n = sh.few;
-    if (threadIdx.x == 0 && n) sh.at = smp_add32(&sh.listed, 0, n);
-    __syncthreads();
-    for (unsigned i = threadIdx.x; i < n; i += IRX_SMP_THREADS) smp_st64(&sh.list[sh.at + i], 0, sh.mine[i]);
-    smp_cluster_sync();
-    if (rank) return;
-    const unsigned m = sh.listed;
-    uint64_t me[2], w[2], better[2] = {0, 0};
-    unsigned order[2] = {0, 0}, none = 0;
+    uint64_t me[SMP_OWN], w[SMP_OWN], better[SMP_OWN] = {};
+    unsigned order[SMP_OWN] = {}, none = 0;
 #pragma unroll
-    for (int a = 0; a < 2; a++) {
+    for (int a = 0; a < SMP_OWN; a++) {
         const unsigned i = threadIdx.x + a * IRX_SMP_THREADS;
         me[a] = i < m ? sh.list[i] : ~0ull;
-        w[a] = i < m ? smp_weight(q, smp_type<float>::value(~(unsigned)(me[a] >> 32))) : 0;
+        w[a] = i < m ? smp_weight(p, q, smp_number(me[a])) : 0;
         if (i < m) sh.weight_of[i] = w[a];
     }
     __syncthreads();
@@ -469,45 +512,47 @@ __device__ __forceinline__ void smp_finish(const irx_ksmp_t &p, smp_shared &sh, 
     for (unsigned j = 0; j < m; j++) {                   // how many come before each, and their weight
         const uint64_t other = sh.list[j], ow = sh.weight_of[j];
 #pragma unroll
-        for (int a = 0; a < 2; a++)
+        for (int a = 0; a < SMP_OWN; a++)
             if (other < me[a]) {
                 order[a]++;
                 better[a] += ow;
             }
     }
-    uint64_t whole = s.whole;
-    bool keep[2];
+    uint64_t whole[1] = {s.whole};
+    bool keep[SMP_OWN];
 #pragma unroll
-    for (int a = 0; a < 2; a++) keep[a] = threadIdx.x + a * IRX_SMP_THREADS < m && (!s.k || order[a] < s.k);
+    for (int a = 0; a < SMP_OWN; a++) keep[a] = threadIdx.x + a * IRX_SMP_THREADS < m && (!s.k || order[a] < s.k);
     if (s.k && s.part) {
-        whole = (keep[0] ? w[0] : 0) + (keep[1] ? w[1] : 0);
+        whole[0] = 0;
+#pragma unroll
+        for (int a = 0; a < SMP_OWN; a++) whole[0] += keep[a] ? w[a] : 0;
         smp_block_sums(sh, whole, none);
     }
-    const uint64_t target = s.part ? max(smp_part(s.part, whole, true), (uint64_t)1) : ~0ull;
-    uint64_t total = 0;
+    const uint64_t target = s.part ? max(smp_part(s.part, whole[0], true), (uint64_t)1) : ~0ull;
+    uint64_t all[1] = {0};
 #pragma unroll
-    for (int a = 0; a < 2; a++) {
+    for (int a = 0; a < SMP_OWN; a++) {
         keep[a] = keep[a] && better[a] < target && w[a] >= s.least;
         if (!keep[a]) w[a] = 0;
-        total += w[a];
+        all[0] += w[a];
     }
-    smp_block_sums(sh, total, none);                     // (its barriers: all have read weight_of)
+    smp_block_sums(sh, all, none);                     // (its barriers: all have read weight_of)
 #pragma unroll
-    for (int a = 0; a < 2; a++)
+    for (int a = 0; a < SMP_OWN; a++)
         if (threadIdx.x + a * IRX_SMP_THREADS < m) sh.weight_of[threadIdx.x + a * IRX_SMP_THREADS] = w[a];
     __syncthreads();
-    const uint64_t at = smp_part((uint64_t)((double)s.u * 4611686018427387904.0), total, false);
-    uint64_t run[2] = {0, 0};
+    const uint64_t total = all[0], at = smp_part((uint64_t)((double)s.u * 4611686018427387904.0), total, false);
+    uint64_t run[SMP_OWN] = {};
 #pragma unroll 4
     for (unsigned j = 0; j < m; j++) {                   // the kept weight at lower indexes
         const unsigned other = (unsigned)sh.list[j];
         const uint64_t ow = sh.weight_of[j];
 #pragma unroll
-        for (int a = 0; a < 2; a++)
+        for (int a = 0; a < SMP_OWN; a++)
             if (other < (unsigned)me[a]) run[a] += ow;
     }
 #pragma unroll
-    for (int a = 0; a < 2; a++)
+    for (int a = 0; a < SMP_OWN; a++)
         if (run[a] <= at && at < run[a] + w[a]) {        // one thread
             p.token[row] = (int)(unsigned)me[a];
             if (p.logprob) p.logprob[row] = (float)(log((double)w[a] / (double)total));
@@ -536,7 +581,7 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
     // the row into shared memory, padded with -infinity
     unsigned bytes = 0;
     if (threadIdx.x < 128) sh.tab[threadIdx.x] = p.tab[threadIdx.x];
-    if (threadIdx.x == 0) sh.few = sh.listed = 0;
+    if (threadIdx.x == 0) sh.few = 0;
     if (!FAR) {
         bytes = p.vec ? (unsigned)(here * sizeof(T)) & ~15u : 0;
         if (threadIdx.x == 0) {
@@ -552,18 +597,14 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
     }
     __syncthreads();
     if (bytes && !irx_mbar_wait(&sh.bar, 0) && lane == 0) atomicOr(p.err, IRX_KERR_TIMEOUT);
-    float top = -INFINITY;
+    unsigned high = ty::PAD;
 #pragma unroll 4
     for (int j = 0; j < x.words; j++) {
-        const unsigned w = x.word(j);
-        float e[2];
-#pragma unroll
-        for (int h = 0; h < ty::N; h++) {
-            e[h] = smp_clean(ty::get(w, h));
-            top = fmaxf(top, e[h]);
-        }
-        if (!FAR) x.data[j] = ty::put(e[0], e[ty::N - 1]);
+        const unsigned w = ty::most(x.word(j), ty::PAD);
+        high = ty::most(high, w);
+        if (!FAR) x.data[j] = w;
     }
+    float top = fmaxf(ty::get(high, 0), ty::get(high, ty::N - 1));
     const unsigned tk = __reduce_max_sync(0xffffffffu, smp_type<float>::key(top));
     if (lane == 0) sh.redc[warp] = tk;
     __syncthreads();
@@ -608,11 +649,10 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
     const float reach = __double2float_ru((p.kbits + 2) * 0.69314718055994531 * temp);
     q.tab = sh.tab;
     q.maxf = top;
-    q.p = &p;
     q.c = 184.66496523378731354 / temp;                  // 128 log2(e) / T
     q.at_max = (double)top * q.c;
     q.floor = __fsub_rd(top, reach);
-    q.one = smp_weight(q, top);
+    q.one = smp_weight(p, q, top);
     q.step = (float)fmin(2.0 * 2047.6 / (double)reach, 3.0e38);
     smp_settings s;
     s.k = k > 0 && k < p.n ? k : 0;
@@ -622,81 +662,152 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
     s.whole = 0;
 
     smp_cut cut = {q.floor, 0};                          // (at the floor nothing weighs)
-    if (s.k) {
+    uint64_t kept = 0;                                   // the weight of this thread's tokens above `upto`, once it is known
+    float upto = INFINITY;
+    bool tallied = false;
+    if (s.k || s.part) {
         smp_clear(sh, false);
         x.each([&](float v, int) {
             const unsigned cell = smp_cell(q, v);
             if (cell < IRX_SMP_BINS) smp_tally(sh, cell, false, 0);
         });
-        uint64_t target = s.k;
-        if (!smp_find(sh, rank, nc, turn, false, target, 0)) s.k = 0;      // fewer have any weight: all of those
-        else if (sh.above + sh.count <= SMP_FEW) return smp_finish(p, sh, q, x, rank, first, row, s);
-        else cut = smp_resolve(sh, q, x, rank, nc, turn, false, target, true);
+        tallied = true;
     }
-    if (s.part) {
+    if (s.k) {
+        uint64_t target = s.k;
+        if (!smp_find(sh, rank, nc, turn, SMP_COUNT, target, 0)) s.k = 0;      // fewer have any weight: all of those
+        else if (sh.above + sh.count <= SMP_FEW) {
+            const unsigned cell = sh.cell;
+            x.each([&](float v, int i) {
+                if (smp_cell(q, v) <= cell) sh.mine[atomicAdd(&sh.few, 1u)] = smp_token(v, first + i);
+            });
+            __syncthreads();
+            const unsigned n = sh.few;
+            unsigned at = 0, m = 0;
+            smp_post(sh, rank, nc, turn, 0, n);
+            for (unsigned r = 0; r < nc; r++) {
+                if (r == rank) at = m;
+                m += sh.xc[turn][r];
+            }
+            smp_hand_over(sh, n, at);
+            if (rank == 0) smp_finish(p, sh, q, m, row, s);
+            return;
+        } else {
+            cut = smp_resolve(p, sh, q, x, rank, nc, turn, false, target, true);
+            tallied = false;
+        }
+    }
+    bool found = false;
+    if (s.part && tallied) {
+        // Top-p alone. The cell of its threshold is guessed from the cells' tokens; one pass then adds up the row's weight and
+        // that above the cell, and gathers the tokens in it (in the next one too, when the guess is near its edge). If the
+        // threshold does not lie among them, or they are too many, the weights' own histogram follows. With few tokens
+        // from there up, all of them are gathered.
+        uint64_t target = 0;
+        smp_find(sh, rank, nc, turn, SMP_GUESS, target, s.part, (float)(2.0 * q.c / 128.0 / (double)q.step));
+        const float in_cell = (float)(target - sh.before) / (float)sh.weight;
+        const unsigned least = smp_least<T>(q), tk = ty::key(q.maxf), c0 = sh.cell - (in_cell < 0.2f && sh.cell), c1 = sh.cell + (in_cell > 0.8f);
+        const bool few = sh.above + sh.count <= SMP_FEW / 2;
+        const unsigned kb = smp_last(least, tk, [&](unsigned kk) { return smp_cell(q, ty::value(kk)) > min(c1, IRX_SMP_BINS - 1u); });
+        const unsigned ko = few ? tk : smp_last(least, tk, [&](unsigned kk) { return smp_cell(q, ty::value(kk)) >= c0; });
+        const float below = ty::value(kb), over = ty::value(ko);
+        uint64_t sum[3] = {0, 0, 0};                     // the whole, what is over the gathered cells, what is in them
+        x.each([&](float v, int i) {
+            const uint64_t w = smp_weight(p, q, v);
+            sum[0] += w;
+            sum[1] += v > over ? w : 0;
+            if (v > below && v <= over) {
+                sum[2] += w;
+                const unsigned at = atomicAdd(&sh.few, 1u);
+                if (at < SMP_FEW) sh.mine[at] = smp_token(v, first + i);
+            }
+        });
+        const uint64_t own = sum[1];
+        unsigned none = 0, at = 0, m = 0;
+        smp_block_sums(sh, sum, none);
+        const unsigned n = sh.few;
+        smp_post(sh, rank, nc, turn, sum[0], n, sum[1], sum[2]);
+        uint64_t above = 0, in = 0;
+        for (unsigned r = 0; r < nc; r++) {
+            if (r == rank) at = m;
+            m = min(m + sh.xc[turn][r], SMP_FEW + 1u);
+            s.whole += sh.xa[turn][r];
+            above += sh.xb[turn][r];
+            in += sh.xd[turn][r];
+        }
+        target = max(smp_part(s.part, s.whole, true), (uint64_t)1);
+        found = m <= SMP_FEW && above < target && target <= above + in;
+        if (found) {
+            smp_hand_over(sh, n, at);
+            if (few) {
+                if (rank == 0) smp_finish(p, sh, q, m, row, s);
+                return;
+            }
+            cut = smp_among<T>(p, sh, q, rank, nc, m, kb + 1, ko, target - above, true);
+            if (!s.least) {
+                kept = own;
+                upto = over;
+            }
+        } else {
+            __syncthreads();
+            if (threadIdx.x == 0) sh.few = 0;
+        }
+    }
+    if (s.part && !found) {
         // the weights of what top-k kept, by cell; of those at its threshold only the first
         smp_clear(sh, true);
         x.each([&](float v, int) {
             const unsigned cell = smp_cell(q, v);
-            if (v > cut.above && cell < IRX_SMP_BINS) smp_tally(sh, cell, true, smp_weight(q, v));
+            if (v > cut.above && cell < IRX_SMP_BINS) smp_tally(sh, cell, true, smp_weight(p, q, v));
         });
         if (cut.ties && rank == 0) {
             __syncthreads();
             const unsigned cell = smp_cell(q, cut.above);
             if (threadIdx.x == 0 && cell < IRX_SMP_BINS) {
-                const uint64_t sum = ((uint64_t)sh.hi[cell] << 32 | sh.lo[cell]) + cut.ties * smp_weight(q, cut.above);
+                const uint64_t sum = ((uint64_t)sh.hi[cell] << 32 | sh.lo[cell]) + cut.ties * smp_weight(p, q, cut.above);
                 sh.lo[cell] = (unsigned)sum;
                 sh.hi[cell] = (unsigned)(sum >> 32);
             }
         }
         uint64_t target = 0;
-        smp_find(sh, rank, nc, turn, true, target, s.part);
-        if (!s.k) {
-            // tokens in that cell and above weigh at least what the next cell's first number does
-            const unsigned cell = sh.cell;
-            const unsigned lo = smp_last(smp_least<T>(q), ty::key(q.maxf), [&](unsigned key) { return smp_cell(q, ty::value(key)) > cell; });
-            const uint64_t w = smp_weight(q, ty::value(lo));
-            if (w && (sh.before + sh.weight) / w <= SMP_FEW) {
-                for (unsigned r = 0; r < nc; r++) s.whole += sh.xa[turn][r];
-                return smp_finish(p, sh, q, x, rank, first, row, s);
-            }
-        }
-        const smp_cut c = smp_resolve(sh, q, x, rank, nc, turn, true, target, !s.k);
+        smp_find(sh, rank, nc, turn, SMP_WEIGHT, target, s.part);
+        const smp_cut c = smp_resolve(p, sh, q, x, rank, nc, turn, true, target, !s.k);
         if (c.above > cut.above || (c.above == cut.above && c.ties < cut.ties)) cut = c;
     }
     if (s.least) {                                       // min-p as a threshold: the last number that weighs too little
-        const unsigned key = smp_last(smp_least<T>(q), ty::key(q.maxf), [&](unsigned kk) { return smp_weight(q, ty::value(kk)) < s.least; });
+        const unsigned key = smp_last(smp_least<T>(q), ty::key(q.maxf), [&](unsigned kk) { return smp_weight(p, q, ty::value(kk)) < s.least; });
         const float v = ty::value(key);
         if (v >= cut.above) cut = {v, 0};
     }
 
     // the kept weights of every thread's stretch of the row, and where u times their total falls. What is not kept counts as
-    // at the floor, with no weight; eight numbers of which no lane of a warp keeps any are passed over.
-    const uint64_t w_eq = cut.ties ? smp_weight(q, cut.above) : 0;
-    uint64_t w = 0;
+    // at the floor, with no weight; words of which no lane of a warp keeps any are passed over.
+    const uint64_t w_eq = cut.ties ? smp_weight(p, q, cut.above) : 0;
+    uint64_t sums[1] = {kept};
     unsigned eq = 0;
     for (int j0 = 0; j0 < x.words; j0 += SMP_STEP) {
-        float v[SMP_STEP * ty::N], most = -INFINITY;
+        float v[SMP_STEP * ty::N];
+        bool any = false;
 #pragma unroll
         for (int j = 0; j < SMP_STEP; j++) {
             const unsigned word = j0 + j < x.words ? x.word(j0 + j) : ty::PAD;
 #pragma unroll
             for (int h = 0; h < ty::N; h++) {
                 v[j * ty::N + h] = ty::get(word, h);
-                most = fmaxf(most, v[j * ty::N + h]);
+                any |= v[j * ty::N + h] >= cut.above && v[j * ty::N + h] <= upto;
             }
         }
-        if (!__any_sync(0xffffffffu, most >= cut.above)) continue;
+        if (!__any_sync(0xffffffffu, any)) continue;
         if (cut.ties)
 #pragma unroll
             for (int j = 0; j < SMP_STEP * ty::N; j++) eq += v[j] == cut.above;
 #pragma unroll
-        for (int j = 0; j < SMP_STEP * ty::N; j++) w += smp_raw(q, v[j] > cut.above ? v[j] : q.floor) - SMP_RAW;
+        for (int j = 0; j < SMP_STEP * ty::N; j++) sums[0] += smp_raw(p, q, v[j] > cut.above && v[j] <= upto ? v[j] : q.floor) - SMP_RAW;
     }
-    const uint64_t w_mine = w;
+    const uint64_t w_mine = sums[0];
     const unsigned eq_mine = eq;
-    smp_block_sums(sh, w, eq);
-    smp_post(sh, rank, nc, turn, w, eq);
+    smp_block_sums(sh, sums, eq);
+    smp_post(sh, rank, nc, turn, sums[0], eq);
     uint64_t total = 0, run = 0;
     unsigned ties = cut.ties, left = 0;                  // ties: left to keep; left: of them, for this block
     for (unsigned r = 0; r < nc; r++) {
@@ -709,18 +820,18 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
         ties -= have;
     }
     const uint64_t at = smp_part((uint64_t)((double)s.u * 4611686018427387904.0), total, false);
-    if (at < run || at >= run + w + min(left, eq) * w_eq) return;      // one block goes on
+    if (at < run || at >= run + sums[0] + min(left, eq) * w_eq) return;      // one block goes on
     for (int i = 0; i < warp; i++) {
         const unsigned have = min(left, sh.redc[i]);
-        run += sh.red[i] + have * w_eq;
+        run += sh.red[0][i] + have * w_eq;
         left -= have;
     }
-    if (at < run || at >= run + sh.red[warp] + min(left, sh.redc[warp]) * w_eq) return;      // one warp
+    if (at < run || at >= run + sh.red[0][warp] + min(left, sh.redc[warp]) * w_eq) return;      // one warp
     const unsigned before = (unsigned)smp_warp_scan(eq_mine) - eq_mine;
     left -= min(left, before);
-    const uint64_t kept = w_mine + min(left, eq_mine) * w_eq, sum = smp_warp_scan(kept);
+    const uint64_t own = w_mine + min(left, eq_mine) * w_eq, sum = smp_warp_scan(own);
     const int who = __ffs(__ballot_sync(0xffffffffu, run + sum > at)) - 1;             // the lane whose stretch it is
-    run = __shfl_sync(0xffffffffu, run + sum - kept, who);
+    run = __shfl_sync(0xffffffffu, run + sum - own, who);
     left = __shfl_sync(0xffffffffu, left, who);
     const int64_t off = (int64_t)(warp * 32 + who) * p.words;
     const smp_data<T, FAR> y = {data + off, src + off * ty::N, p.n - base - off * ty::N, p.words, x.mode, x.top};
@@ -729,7 +840,7 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
         const float v = i < p.words * ty::N ? ty::get(y.word(i / ty::N), i % ty::N) : -INFINITY;
         const bool same = cut.ties && v == cut.above;
         const unsigned all = __ballot_sync(0xffffffffu, same);
-        const uint64_t e = v > cut.above || (same && __popc(all & ((1u << lane) - 1u)) < left) ? smp_weight(q, v) : 0;
+        const uint64_t e = v > cut.above || (same && __popc(all & ((1u << lane) - 1u)) < left) ? smp_weight(p, q, v) : 0;
         left -= min(left, (unsigned)__popc(all));
         const uint64_t up = smp_warp_scan(e);
         const unsigned past = __ballot_sync(0xffffffffu, run + up > at);
