@@ -207,7 +207,7 @@ typedef struct {
  * key-value head. Shared memory of the FP32 kernel: three tiles of 64 rows and the weights. */
 #define IRX_PR_ST_SMEM(dp) ((3 * 64 * ((dp) + 4) + 64 * 68) * 4)
 
-#define IRX_PR_TC_SMEM(dp) (6 * 2 * (dp) * 128 + 1024)      /* two tiles each of queries, keys and values; barriers */
+#define IRX_PR_TC_SMEM(dp) (6 * 2 * (dp) * 128 + 1024 + 32768)   /* two tiles each of queries, keys and values; barriers; staged outputs */
 
 typedef struct {
     CUtensorMap tma_q, tma_k, tma_v;  /* matrix instructions: [tokens, kv_heads, group, d] and [tokens, kv_heads, d] views */

@@ -41,52 +41,92 @@ __device__ __forceinline__ int pr_len(const irx_kprm_t &p, int s0, int &highest,
 }
 
 // Tiles of a sequence of n tokens: mul rows a token, per rows a tile.
-__device__ __forceinline__ int pr_tiles(int n, int mul, int per)
-{
-    return (int)(((int64_t)n * mul + per - 1) / per);
-}
+struct pr_rows {
+    int mul, per;
+    __device__ __forceinline__ int tiles(int n) const
+    {
+        if (mul == 1) return (int)(((unsigned)n + (unsigned)per - 1) / (unsigned)per);
+        return (int)(((int64_t)n * mul + per - 1) / per);
+    }
+};
 
-// Per key-value head: units whose tile is number t or later, over all sequences. A whole warp calls it.
-__device__ __forceinline__ int pr_count(const irx_kprm_t &p, int t, int mul, int per, int &most)
+// What a warp knows of all units: the first 32 sequences (one a lane), the most tiles of one, the units.
+struct pr_list {
+    pr_rows rows;
+    int tiles, base, len, highest, most;
+    int64_t units;
+};
+
+// Tiles of sequence s0 + lane, its rows and the state for the next 32.
+__device__ __forceinline__ int pr_chunk(const irx_kprm_t &p, const pr_list &l, int s0, int &highest, int &base, int &len)
 {
-    int n = 0, base, highest = 0x80000000;
+    if (!s0) {
+        highest = l.highest;
+        base = l.base;
+        len = l.len;
+        return l.tiles;
+    }
     bool bad;
-    most = 0;
-    for (int s0 = 0; s0 < p.batch; s0 += 32) {
-        const int nt = pr_tiles(pr_len(p, s0, highest, base, bad), mul, per);
-        n += max(0, nt - t);
-        most = max(most, nt);
-    }
-    most = __reduce_max_sync(0xffffffffu, most);
-    return __reduce_add_sync(0xffffffffu, n);
+    len = pr_len(p, s0, highest, base, bad);
+    return l.rows.tiles(len);
 }
 
-// Unit u, u below pr_count(0) * heads; most: the largest sequence's tiles. A whole warp calls it.
-__device__ __forceinline__ pr_unit pr_find(const irx_kprm_t &p, int64_t u, int most, int mul, int per)
+// A whole warp calls these. pr_start: the list; block 0 reports the sequences that are skipped.
+__device__ __forceinline__ pr_list pr_start(const irx_kprm_t &p, pr_rows rows)
 {
-    const int nh = p.h1 - p.h0;
-    int lo = 0, hi = most, after = 0, m;
-    while (hi - lo > 1) {                                // the last t with u below the units of tiles t and later
-        const int mid = (lo + hi) >> 1, c = pr_count(p, mid, mul, per, m);
-        if ((int64_t)c * nh > u) lo = mid;
-        else {
-            hi = mid;
-            after = c;
-        }
-    }
-    const int64_t off = u - (int64_t)after * nh;
-    int skip = (int)(off / nh), highest = 0x80000000;    // among the sequences that have a tile number lo
-    pr_unit r = {0, 0, lo, p.h0 + (int)(off % nh)};
+    pr_list l;
+    l.rows = rows;
+    l.highest = 0x80000000;
+    int sum = 0, most = 0, highest = 0x80000000, base, len;
     for (int s0 = 0; s0 < p.batch; s0 += 32) {
-        int base;
         bool bad;
-        const int n = pr_len(p, s0, highest, base, bad);
-        const unsigned has = __ballot_sync(0xffffffffu, pr_tiles(n, mul, per) > lo);
+        len = pr_len(p, s0, highest, base, bad);
+        if (bad && blockIdx.x == 0) atomicOr(p.err, IRX_KERR_INDEX);
+        const int n = rows.tiles(len);
+        if (!s0) {
+            l.tiles = n;
+            l.base = base;
+            l.len = len;
+            l.highest = highest;
+        }
+        sum += n;
+        most = max(most, n);
+    }
+    l.most = __reduce_max_sync(0xffffffffu, most);
+    l.units = (int64_t)__reduce_add_sync(0xffffffffu, sum) * (p.h1 - p.h0);
+    return l;
+}
+
+// Unit u, below l.units.
+__device__ __forceinline__ pr_unit pr_find(const irx_kprm_t &p, const pr_list &l, int64_t u)
+{
+    const int nh = p.h1 - p.h0, lane = threadIdx.x & 31;
+    int lo = 0, hi = l.most, after = 0;                  // after: tiles numbered hi and later, a head
+    while (hi - lo > 1) {                                // the last t with u below the units of tiles t and later, 32 guesses at a time
+        const int step = (hi - lo + 31) / 32, t = lo + (lane + 1) * step;
+        int c = 0, highest, base, len;
+        for (int s0 = 0; s0 < p.batch; s0 += 32) {
+            const int nt = pr_chunk(p, l, s0, highest, base, len), n = min(32, p.batch - s0);
+            for (int i = 0; i < n; i++) c += max(0, __shfl_sync(0xffffffffu, nt, i) - t);
+        }
+        const int k = __popc(__ballot_sync(0xffffffffu, t < hi && (int64_t)c * nh > u));
+        if (lo + (k + 1) * step < hi) {
+            hi = lo + (k + 1) * step;
+            after = __shfl_sync(0xffffffffu, c, k);
+        }
+        lo += k * step;
+    }
+    const int off = (int)(u - (int64_t)after * nh);
+    int skip = off / nh, highest;                        // among the sequences that have a tile number lo
+    pr_unit r = {0, 0, lo, p.h0 + off % nh};
+    for (int s0 = 0; s0 < p.batch; s0 += 32) {
+        int base, len;
+        const unsigned has = __ballot_sync(0xffffffffu, pr_chunk(p, l, s0, highest, base, len) > lo);
         const int c = __popc(has);
         if (skip < c) {
             const int at = __fns(has, 0, skip + 1);
             r.base = __shfl_sync(0xffffffffu, base, at);
-            r.len = __shfl_sync(0xffffffffu, n, at);
+            r.len = __shfl_sync(0xffffffffu, len, at);
             break;
         }
         skip -= c;
@@ -98,17 +138,6 @@ __device__ __forceinline__ pr_unit pr_find(const irx_kprm_t &p, int64_t u, int m
 __device__ __forceinline__ int64_t pr_turn(int i)
 {
     return (int64_t)i * gridDim.x + (i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-}
-
-// One warp reports sequences that are skipped.
-__device__ __forceinline__ void pr_report(const irx_kprm_t &p)
-{
-    int base, highest = 0x80000000;
-    for (int s0 = 0; s0 < p.batch; s0 += 32) {
-        bool bad;
-        pr_len(p, s0, highest, base, bad);
-        if (bad) atomicOr(p.err, IRX_KERR_INDEX);
-    }
 }
 
 // ---- FP32 units: f32 rows, and bf16 rows that the matrix instructions do not take ----
@@ -147,13 +176,11 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
     float *sq = ps_smem, *sk = sq + 64 * (DP + 4), *sv = sk + 64 * (DP + 4), *sp = sv + 64 * (DP + 4);
     constexpr int NC = DP / 64;                          // 4-column groups of the output a thread owns
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    int most;
-    const int64_t units = (int64_t)pr_count(p, 0, p.group, PS_ROWS, most) * (p.h1 - p.h0);
-    if (blockIdx.x == 0 && threadIdx.x < 32) pr_report(p);
+    const pr_list list = pr_start(p, pr_rows{p.group, PS_ROWS});
     for (int turn = 0;; turn++) {
         const int64_t u = pr_turn(turn);
-        if (u >= units) break;
-        const pr_unit un = pr_find(p, u, most, p.group, PS_ROWS);
+        if (u >= list.units) break;
+        const pr_unit un = pr_find(p, list, u);
         const int64_t r0 = (int64_t)un.tile * PS_ROWS, rows = (int64_t)un.len * p.group;
         const int nr = (int)min((int64_t)PS_ROWS, rows - r0);
         const int first = (int)(r0 / p.group), last = (int)((r0 + nr - 1) / p.group);

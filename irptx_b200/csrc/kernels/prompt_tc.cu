@@ -41,6 +41,9 @@ __device__ __forceinline__ bool pt_cut(const irx_kprm_t &p, const pt_info &f, in
     return j < f.nsink || kb + 127 > first || (p.window && kb <= last - p.window);
 }
 
+// The lowest n bits, n any number.
+__device__ __forceinline__ uint32_t pt_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
 #define PT_HALF 16384                       // 128 rows of 64 columns
 
 template <int DP>
@@ -88,16 +91,15 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
     if (warp >= 8) {
       at_reg_dec();
       if (warp == 8) {                                        // units and loads
-        int most, kv = 0;
-        const int64_t units = (int64_t)pr_count(p, 0, 1, 2 * tp, most) * (p.h1 - p.h0);
-        if (blockIdx.x == 0) pr_report(p);
+        int kv = 0;
+        const pr_list list = pr_start(p, pr_rows{1, 2 * tp});
         int ok = 1;
         for (int uc = 0; ok; uc++) {
             const int us = uc & 1;
             const int64_t u = pr_turn(uc);
             pt_info f = {};
-            if (u < units) {
-                const pr_unit un = pr_find(p, u, most, 1, 2 * tp);
+            if (u < list.units) {
+                const pr_unit un = pr_find(p, list, u);
                 f.base = un.base; f.len = un.len; f.head = un.head;
                 f.tok0 = un.tile * 2 * tp;
                 const int e0 = min(f.tok0 + tp, f.len), e1 = min(f.tok0 + 2 * tp, f.len);
@@ -225,28 +227,28 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
                 if (pt_cut(p, f, j, f.tok0, f.end - 1)) {
                     const int seen = (j < f.nsink ? f.sk : f.end) - pt_key(f, j);
                     uint4 *v = reinterpret_cast<uint4 *>(sv + (gi & 1) * TILE);
-                    bool odd = false;
+                    uint32_t worst = 0;                       // the largest magnitudes of either half, as integers
 #pragma unroll 4
                     for (int i = 0; i < NB * 16; i++) {       // 4 rows of 8 vectors a step
                         const int row = (warp - 10) * 64 + (i & 15) * 4 + (lane >> 3);
                         uint4 *at = v + (i >> 4) * (PT_HALF / 16) + row * 8 + (lane & 7);
-                        if (row >= seen) {
-                            *at = make_uint4(0u, 0u, 0u, 0u);
-                            continue;
-                        }
                         const uint4 x = *at;
-                        uint32_t w[4] = {x.x, x.y, x.z, x.w}, any = 0;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {         // halves whose exponent is all ones
-                            const uint32_t m = __vcmpeq2(w[e] & 0x7f807f80u, 0x7f807f80u);
-                            any |= m;
-                            w[e] &= ~m;
-                        }
-                        if (any) {
-                            *at = make_uint4(w[0], w[1], w[2], w[3]);
-                            odd = true;
-                        }
+                        if (row >= seen) *at = make_uint4(0u, 0u, 0u, 0u);
+                        else worst = __vmaxu2(__vmaxu2(worst, __vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu)),
+                                              __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
                     }
+                    // an exponent of all ones: find them
+                    const bool odd = __any_sync(0xffffffffu, (worst & 0xffffu) >= 0x7f80u || worst >> 16 >= 0x7f80u);
+                    if (odd)
+                        for (int i = 0; i < NB * 16; i++) {
+                            const int row = (warp - 10) * 64 + (i & 15) * 4 + (lane >> 3);
+                            uint4 *at = v + (i >> 4) * (PT_HALF / 16) + row * 8 + (lane & 7);
+                            const uint4 x = *at;
+                            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                            for (int e = 0; e < 4; e++) w[e] &= ~__vcmpeq2(w[e] & 0x7f807f80u, 0x7f807f80u);
+                            *at = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
                     if (odd) infos[us].dirty = 1;
                     fence_proxy_async_smem();
                 }
@@ -263,6 +265,8 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
         const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tbase + tl + t * 128, tO = tbase + tl + 256 + t * 128;
         const float sl2 = fabsf(p.scale2);
+        uint4 *stage = reinterpret_cast<uint4 *>(sv + 2 * TILE + 1024) + warp * 256;
+        const int inv_g = (65535 + g) / g, tok_stride = p.heads * p.d;        // row / g = (row * inv_g) >> 16 below 128
         const int mytok = t * tp + r / g, myhead = r % g;      // within the unit, within the group
         bool ok = true;
         int it = 0;
@@ -287,17 +291,18 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
                     for (int c = 0; c < 128; c++) v[c] = -v[c];
                 }
                 const int kb = pt_key(f, j);
-                if (j < f.nsink || (p.window && kb <= last - p.window)) {
-                    // columns up to `up`, and of those from `low` on or before `sink`
-                    const int up = (j < f.nsink ? min(tok, f.sk - 1) : tok) - kb, low = tok - p.window + 1 - kb, sink = p.sinks - kb;
+                const bool edge = j >= f.nsink && p.window && kb <= last - p.window;
+                if (edge || j < f.nsink || kb + 127 > first) {
+                    // the columns this row sees, as bits: up to `up`, and with a window from `low` on or before `sink`
+                    const int up = (j < f.nsink ? min(tok, f.sk - 1) : tok) - kb, low = edge ? tok - p.window + 1 - kb : 0, sink = p.sinks - kb;
 #pragma unroll
-                    for (int c = 0; c < 128; c++)
-                        if (c > up || (c < low && c >= sink)) v[c] = -INFINITY;
-                } else if (kb + 127 > first) {
-                    const int up = tok - kb;
+                    for (int k = 0; k < 4; k++) {
+                        uint32_t see = pt_below(up + 1 - 32 * k);
+                        if (edge) see &= ~pt_below(low - 32 * k) | pt_below(sink - 32 * k);
 #pragma unroll
-                    for (int c = 0; c < 128; c++)
-                        if (c > up) v[c] = -INFINITY;
+                        for (int c = 0; c < 32; c++)
+                            if (!(see & (1u << c))) v[k * 32 + c] = -INFINITY;
+                    }
                 }
                 float mk[4];
 #pragma unroll
@@ -348,7 +353,8 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
                 const float inv = m > -2.9e38f ? 1.0f / l : NAN;      // (every score -infinity, or NaN: NaN)
                 const int64_t orow = (int64_t)(f.base + tok) * p.heads + f.head * g + myhead;
                 if (mine && p.lse) p.lse[orow] = m < -2.9e38f ? -INFINITY : (m + log2f(l)) * 0.6931471806f;
-                __nv_bfloat16 *o_at = reinterpret_cast<__nv_bfloat16 *>(p.o) + orow * p.d;
+                __nv_bfloat16 *o_at = reinterpret_cast<__nv_bfloat16 *>(p.o) + ((int64_t)(f.base + first) * p.heads + f.head * g) * p.d;
+                const int rows = (last + 1 - first) * g;      // of this tile
 #pragma unroll 1
                 for (int cc = 0; cc < DP / 32; cc++) {
                     float o[32];
@@ -371,18 +377,23 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
                             }
                         }
                     }
-                    if (mine) {
+                    // 64 columns at a time through the warp's 4 KB, so that a store covers four rows' 128 bytes, not 32 rows'
+                    // 16 (chunks of 16 bytes, swizzled by row)
+                    uint4 *st = stage + lane * 8;
 #pragma unroll
-                        for (int j8 = 0; j8 < 4; j8++) {
-                            if (cc * 32 + j8 * 8 >= p.d) break;
-                            uint4 pk;
-                            pk.x = at_pack_bf16(o[j8 * 8 + 0], o[j8 * 8 + 1]);
-                            pk.y = at_pack_bf16(o[j8 * 8 + 2], o[j8 * 8 + 3]);
-                            pk.z = at_pack_bf16(o[j8 * 8 + 4], o[j8 * 8 + 5]);
-                            pk.w = at_pack_bf16(o[j8 * 8 + 6], o[j8 * 8 + 7]);
-                            *reinterpret_cast<uint4 *>(o_at + cc * 32 + j8 * 8) = pk;
-                        }
+                    for (int j8 = 0; j8 < 4; j8++)
+                        st[((cc & 1) * 4 + j8) ^ (lane & 7)] = make_uint4(at_pack_bf16(o[j8 * 8 + 0], o[j8 * 8 + 1]), at_pack_bf16(o[j8 * 8 + 2], o[j8 * 8 + 3]),
+                                                                          at_pack_bf16(o[j8 * 8 + 4], o[j8 * 8 + 5]), at_pack_bf16(o[j8 * 8 + 6], o[j8 * 8 + 7]));
+                    if (!(cc & 1)) continue;
+                    __syncwarp();
+                    const int col = (cc >> 1) * 64 + (lane & 7) * 8;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int row = i * 4 + (lane >> 3), full = (warp & 3) * 32 + row, tk = (full * inv_g) >> 16;
+                        if (full < rows && col < p.d)
+                            *reinterpret_cast<uint4 *>(o_at + tk * tok_stride + (full - tk * g) * p.d + col) = stage[row * 8 + ((lane & 7) ^ (row & 7))];
                     }
+                    __syncwarp();
                 }
                 tc_fence_before();
                 irx_mbar_arrive(&o_free[t]);

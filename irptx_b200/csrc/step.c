@@ -255,7 +255,7 @@ static int launch_prompt(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
     k.vec = (uint8_t)(a->dim % al == 0 && a->q_stride % al == 0 && a->kv_stride % al == 0 && a_to(k.q, 16) && a_to(k.k, 16) &&
                       a_to(k.v, 16) && a_to(k.o, 16));
     dp = a->dim <= 64 ? 64 : a->dim <= 128 ? 128 : 256;
-    if (a->dt == DT_BF16 && k.vec && dp <= 128 && k.group <= 128 && a->q_stride < MAX_STRIDE / 2 && a->kv_stride < MAX_STRIDE / 2) {
+    if (a->dt == DT_BF16 && k.vec && dp <= 128 && k.group <= 128 && (int64_t)a->heads * a->dim < (1 << 24) && a->q_stride < MAX_STRIDE / 2 && a->kv_stride < MAX_STRIDE / 2) {
         const int tp = 128 / k.group;                      /* tokens of a tile */
         const cuuint64_t es2 = 2, qd[4] = {(cuuint64_t)a->dim, (cuuint64_t)k.group, (cuuint64_t)a->kv_heads, (cuuint64_t)a->tokens};
         const cuuint64_t qs[3] = {qd[0] * es2, qd[0] * qd[1] * es2, (cuuint64_t)a->q_stride * es2};
