@@ -207,7 +207,11 @@ typedef struct {
  * key-value head. Shared memory of the FP32 kernel: three tiles of 64 rows and the weights. */
 #define IRX_PR_ST_SMEM(dp) ((3 * 64 * ((dp) + 4) + 64 * 68) * 4)
 
-#define IRX_PR_TC_SMEM(dp) (6 * 2 * (dp) * 128 + 1024 + 32768)   /* two tiles each of queries, keys and values; barriers; staged outputs */
+/* The matrix instructions' kernels. Head sizes up to 128: two tiles of 128 rows each of queries, keys and values; above: one
+ * of queries, rings of key and value tiles of 64. Then 1 KB of barriers, and 4 KB of staged output a softmax warp. */
+#define IRX_PR_TC_SMEM(dp) (6 * 2 * (dp) * 128 + 1024 + 32768)
+#define IRX_PR_WIDE_RING 2
+#define IRX_PR_WIDE_SMEM ((128 + 2 * IRX_PR_WIDE_RING * 64) * 256 * 2 + 1024 + 16384)
 
 typedef struct {
     CUtensorMap tma_q, tma_k, tma_v;  /* matrix instructions: [tokens, kv_heads, group, d] and [tokens, kv_heads, d] views */

@@ -7,7 +7,8 @@
 // copy. The pipeline is irx_attn_bf16's (attn.cu): scores S_t = Q_t K^T into TMEM, one thread a row for the softmax,
 // P over the scores' columns, O_t += P_t V, each tile's softmax under the other tile's products. What differs:
 //   * warp 8 finds the block's units from `starts` (prompt.cu) and hands them out with the loads;
-//   * key tiles may begin anywhere and are masked by token: a window's edge and the sinks' tiles too;
+//   * key tiles may begin anywhere and are masked by token: a window's edge and the sinks' tiles too. The sinks' tile and
+//     a unit's last one are 64 keys wide when that holds all that is seen of them;
 //   * warps 10 and 11 look through the values of the tiles that a mask cuts. Rows that no query of the unit
 //     sees become zeros, for another sequence's numbers or uninitialised ones may lie there and 0 * NaN is NaN.
 //     Infinities and NaN in the others become zeros too, and the unit is marked: its rows add those that they
@@ -35,6 +36,9 @@ __device__ __forceinline__ float pt_max3(float a, float b, float c)
 // First token of key tile j, and whether some row of tokens [first, last] does not see all of it.
 __device__ __forceinline__ int pt_key(const pt_info &f, int j) { return j < f.nsink ? 128 * j : f.lo + 128 * (j - f.nsink); }
 
+// Whether the unit needs only the first 64 keys of tile j: the sinks' or the last one, when that is all there is.
+__device__ __forceinline__ bool pt_narrow(const pt_info &f, int j) { return (j < f.nsink ? f.sk : f.end) - pt_key(f, j) <= 64; }
+
 __device__ __forceinline__ bool pt_cut(const irx_kprm_t &p, const pt_info &f, int j, int first, int last)
 {
     const int kb = pt_key(f, j);
@@ -45,6 +49,143 @@ __device__ __forceinline__ bool pt_cut(const irx_kprm_t &p, const pt_info &f, in
 __device__ __forceinline__ uint32_t pt_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
 #define PT_HALF 16384                       // 128 rows of 64 columns
+
+// All 64 f32 columns of this thread's TMEM lane, with the wait in the same statement.
+__device__ __forceinline__ void pt_ld64(uint32_t taddr, float (&v)[64])
+{
+    uint32_t r[64];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+                 "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+                 "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+                 "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+                   "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+                   "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+                   "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+                   "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+                 : "r"(taddr) : "memory");
+#pragma unroll
+    for (int i = 0; i < 64; i++) v[i] = __uint_as_float(r[i]);
+}
+
+// 32 packed columns (64 bf16 of P) into this thread's TMEM lane, then wait for the stores.
+__device__ __forceinline__ void pt_st32(uint32_t taddr, const uint32_t (&v)[32])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
+                 "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+                 "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n\t"
+                 "tcgen05.wait::st.sync.aligned;"
+                 :: "r"(taddr),
+                    "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                    "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+                    "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+                    "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+                 : "memory");
+}
+
+// at_softmax_row (attn.cu) for 64 scores: P = 2^(s * sl2 - m) as bf16 pairs, and their sum.
+__device__ __forceinline__ float pt_weights(const float (&v)[64], float sl2, float m, uint32_t (&pk)[32])
+{
+    float2 sa = make_float2(0.0f, 0.0f), sb = make_float2(0.0f, 0.0f);
+    const float2 s2 = make_float2(sl2, sl2), nm = make_float2(-m, -m);
+    const float ks = sl2 * (1.0f / 253.0f), kc = (126.0f - m) * (1.0f / 253.0f);
+    const float2 k253 = make_float2(253.0f, 253.0f), kmg = make_float2(12582912.0f - 126.0f, 12582912.0f - 126.0f);
+#pragma unroll
+    for (int i = 0; i < 32; i++) {
+        if ((i & 3) != 3) {
+            const float2 x = __ffma2_rn(make_float2(v[2 * i], v[2 * i + 1]), s2, nm);
+            const float p0 = at_ex2(x.x), p1 = at_ex2(x.y);
+            pk[i] = at_pack_bf16(p0, p1);
+            sa = __fadd2_rn(sa, make_float2(p0, p1));
+        } else {
+            const float2 y = make_float2(at_ffma_sat(v[2 * i], ks, kc), at_ffma_sat(v[2 * i + 1], ks, kc));
+            const float2 t = __ffma2_rn(y, k253, kmg);
+            const float2 nn = __fadd2_rn(kmg, make_float2(-t.x, -t.y));
+            const float2 f = __ffma2_rn(y, k253, nn);
+            float2 q = __ffma2_rn(make_float2(0.055171319384097875f, 0.055171319384097875f), f,
+                                  make_float2(0.2426105373823389f, 0.2426105373823389f));
+            q = __ffma2_rn(q, f, make_float2(0.6932609854947172f, 0.6932609854947172f));
+            q = __ffma2_rn(q, f, make_float2(0.9999281096694117f, 0.9999281096694117f));
+            const uint32_t r0 = __float_as_uint(q.x) + (__float_as_uint(t.x) << 23);
+            const uint32_t r1 = __float_as_uint(q.y) + (__float_as_uint(t.y) << 23);
+            pk[i] = __byte_perm(r0 + 0x8000u, r1 + 0x8000u, 0x7632);
+            sb = __fadd2_rn(sb, make_float2(__uint_as_float(r0), __uint_as_float(r1)));
+        }
+    }
+    return (sa.x + sa.y) + (sb.x + sb.y);
+}
+
+// One softmax step of a row over W scores: masked, exponentials over the scores' columns, and into m and l. O and l keep a
+// maximum up to a factor of 256 behind (attn.cu); each row decides for itself, so that its bits do not depend on the
+// others of its warp. before(): waits until O is this warp's to rescale.
+struct pt_row {
+    uint32_t tS, tO;
+    int up, low, sink;                          // the columns seen: up to `up`, and from `low` on or before `sink`
+    bool cut, negate, first;
+    float sl2;
+};
+
+template <int DP, int W, class F>
+__device__ __forceinline__ void pt_step(const pt_row &r, float &m, float &l, F before)
+{
+    float v[W];
+    if constexpr (W == 128) tmem_ld128(r.tS, v);
+    else pt_ld64(r.tS, v);
+    if (r.negate) {
+#pragma unroll
+        for (int c = 0; c < W; c++) v[c] = -v[c];
+    }
+    if (r.cut) {
+#pragma unroll
+        for (int k = 0; k < W / 32; k++) {
+            const uint32_t see = pt_below(r.up + 1 - 32 * k) & (~pt_below(r.low - 32 * k) | pt_below(r.sink - 32 * k));
+#pragma unroll
+            for (int c = 0; c < 32; c++)
+                if (!(see & (1u << c))) v[k * 32 + c] = -INFINITY;
+        }
+    }
+    float mk[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        mk[k] = pt_max3(v[k * (W / 4)], v[k * (W / 4) + 1], v[k * (W / 4) + 2]);
+#pragma unroll
+        for (int c = 3; c < W / 4 - 1; c += 2) mk[k] = pt_max3(mk[k], v[k * (W / 4) + c], v[k * (W / 4) + c + 1]);
+    }
+    mk[0] = pt_max3(mk[0], v[W / 4 - 1], v[W / 2 - 1]);
+    mk[1] = pt_max3(mk[1], v[3 * W / 4 - 1], v[W - 1]);
+    float mnew = pt_max3(m, pt_max3(mk[0], mk[1], mk[2]) * r.sl2, mk[3] * r.sl2);
+    mnew = mnew < INFINITY ? mnew : NAN;          // a score that is NaN or infinite: the row is NaN
+    const bool grown = !(mnew <= m + 8.0f);
+    if (r.first) {
+        m = mnew;
+    } else if (__any_sync(0xffffffffu, grown)) {
+        if (!before()) return;
+        const float alpha = grown ? at_ex2(m - mnew) : 1.0f;
+        if (grown) m = mnew;
+        l *= alpha;
+#pragma unroll 1
+        for (int cc = 0; cc < DP / 32; cc++) {
+            float o[32];
+            tmem_ld32(r.tO + cc * 32, o);
+#pragma unroll
+            for (int e = 0; e < 32; e++) o[e] *= alpha;
+            tmem_st32(r.tO + cc * 32, o);
+        }
+    }
+    uint32_t pk[W / 2];
+    if constexpr (W == 128) {
+        l += at_softmax_row(v, r.sl2, m, pk);
+        tmem_st64(r.tS, pk);
+    } else {
+        l += pt_weights(v, r.sl2, m, pk);
+        pt_st32(r.tS, pk);
+    }
+}
 
 template <int DP>
 __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
@@ -151,14 +292,15 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
         }
       } else if (warp == 9) {
         if (elect_one()) {                                    // MMA: P0 V, S0', P1 V, S1' per key tile
-            const uint32_t id_qk = umma_idesc_bf16(128, 128, 0), id_pv = umma_idesc_bf16(128, DP, 1);
+            const uint32_t id_qk = umma_idesc_bf16(128, 128, 0), id_qk64 = umma_idesc_bf16(128, 64, 0), id_pv = umma_idesc_bf16(128, DP, 1);
             const uint32_t sq_a = irx_smem_u32(sq), sk_a = irx_smem_u32(sk), sv_a = irx_smem_u32(sv);
             bool ok = true;
             int kv = 0, it0 = 0, it1 = 0, uo0 = 0, uo1 = 0;
             for (int uc = 0; ok; uc++) {
                 const int us = uc & 1;
                 if (!(ok = at_wait(&u_full[us], (uc >> 1) & 1, p.err))) break;
-                const int n0 = infos[us].n0, n1 = infos[us].n1, nmax = max(n0, n1);
+                const pt_info f = read(us);
+                const int n0 = f.n0, n1 = f.n1, nmax = max(n0, n1);
                 irx_mbar_arrive(&u_empty[us]);
                 if (!n0) break;
                 int sleft = n0 + n1;                          // score products of this unit still to issue
@@ -176,20 +318,22 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
                             if (!(ok = at_wait(&v_ok[gi & 1], (gi >> 1) & 1, p.err))) break;
                             tc_fence_after();
                             const uint32_t bv = sv_a + (gi & 1) * TILE;
+                            const bool narrow = pt_narrow(f, j);
 #pragma unroll
                             for (int kk = 0; kk < 8; kk++)
-                                umma_bf16_tmem_a(tbase + 256 + t * 128, tbase + t * 128 + kk * 8,
-                                                 umma_desc_sw128(bv + kk * 16 * 128, PT_HALF, 1024), id_pv, (j | kk) != 0);
+                                if (kk < 4 || !narrow)
+                                    umma_bf16_tmem_a(tbase + 256 + t * 128, tbase + t * 128 + kk * 8,
+                                                     umma_desc_sw128(bv + kk * 16 * 128, PT_HALF, 1024), id_pv, (j | kk) != 0);
                             umma_commit(&pv_done[t]);
                         }
                         if (j + 1 < nt) {                     // S_t = Q_t K_{j+1}^T
                             const int gi = kv + j + 1;
                             if (!(ok = at_wait(&k_full[gi & 1], (gi >> 1) & 1, p.err))) break;
                             tc_fence_after();
-                            const uint32_t aq = sq_a + t * TILE, bk = sk_a + (gi & 1) * TILE;
+                            const uint32_t aq = sq_a + t * TILE, bk = sk_a + (gi & 1) * TILE, id = pt_narrow(f, j + 1) ? id_qk64 : id_qk;
 #pragma unroll
                             for (int kk = 0; kk < DP / 16; kk++)
-                                umma_bf16(tbase + t * 128, at_kmajor_desc(aq, kk), at_kmajor_desc(bk, kk), id_qk, kk > 0);
+                                umma_bf16(tbase + t * 128, at_kmajor_desc(aq, kk), at_kmajor_desc(bk, kk), id, kk > 0);
                             umma_commit(&s_full[t]);
                             if (--sleft == 0) umma_commit(q_empty);
                         }
@@ -227,11 +371,12 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
                 if (pt_cut(p, f, j, f.tok0, f.end - 1)) {
                     const int seen = (j < f.nsink ? f.sk : f.end) - pt_key(f, j);
                     uint4 *v = reinterpret_cast<uint4 *>(sv + (gi & 1) * TILE);
+                    const int quads = pt_narrow(f, j) ? 8 : 16;       // rows are looked at in fours: half of them by each warp
                     uint32_t worst = 0;                       // the largest magnitudes of either half, as integers
 #pragma unroll 4
-                    for (int i = 0; i < NB * 16; i++) {       // 4 rows of 8 vectors a step
-                        const int row = (warp - 10) * 64 + (i & 15) * 4 + (lane >> 3);
-                        uint4 *at = v + (i >> 4) * (PT_HALF / 16) + row * 8 + (lane & 7);
+                    for (int i = 0; i < NB * quads; i++) {
+                        const int blk = i >= quads, row = ((warp - 10) * quads + i - blk * quads) * 4 + (lane >> 3);
+                        uint4 *at = v + blk * (PT_HALF / 16) + row * 8 + (lane & 7);
                         const uint4 x = *at;
                         if (row >= seen) *at = make_uint4(0u, 0u, 0u, 0u);
                         else worst = __vmaxu2(__vmaxu2(worst, __vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu)),
@@ -240,9 +385,9 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
                     // an exponent of all ones: find them
                     const bool odd = __any_sync(0xffffffffu, (worst & 0xffffu) >= 0x7f80u || worst >> 16 >= 0x7f80u);
                     if (odd)
-                        for (int i = 0; i < NB * 16; i++) {
-                            const int row = (warp - 10) * 64 + (i & 15) * 4 + (lane >> 3);
-                            uint4 *at = v + (i >> 4) * (PT_HALF / 16) + row * 8 + (lane & 7);
+                        for (int i = 0; i < NB * quads; i++) {
+                            const int blk = i >= quads, row = ((warp - 10) * quads + i - blk * quads) * 4 + (lane >> 3);
+                            uint4 *at = v + blk * (PT_HALF / 16) + row * 8 + (lane & 7);
                             const uint4 x = *at;
                             uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -284,61 +429,18 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
                 ok = __all_sync(0xffffffffu, at_wait(&s_full[t], (it + j) & 1, p.err));
                 if (!ok) break;
                 tc_fence_after();
-                float v[128];
-                tmem_ld128(tS, v);
-                if (p.scale2 < 0.0f) {
-#pragma unroll
-                    for (int c = 0; c < 128; c++) v[c] = -v[c];
-                }
                 const int kb = pt_key(f, j);
                 const bool edge = j >= f.nsink && p.window && kb <= last - p.window;
-                if (edge || j < f.nsink || kb + 127 > first) {
-                    // the columns this row sees, as bits: up to `up`, and with a window from `low` on or before `sink`
-                    const int up = (j < f.nsink ? min(tok, f.sk - 1) : tok) - kb, low = edge ? tok - p.window + 1 - kb : 0, sink = p.sinks - kb;
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        uint32_t see = pt_below(up + 1 - 32 * k);
-                        if (edge) see &= ~pt_below(low - 32 * k) | pt_below(sink - 32 * k);
-#pragma unroll
-                        for (int c = 0; c < 32; c++)
-                            if (!(see & (1u << c))) v[k * 32 + c] = -INFINITY;
-                    }
-                }
-                float mk[4];
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    mk[k] = pt_max3(v[k * 32], v[k * 32 + 1], v[k * 32 + 2]);
-#pragma unroll
-                    for (int c = 3; c < 31; c += 2) mk[k] = pt_max3(mk[k], v[k * 32 + c], v[k * 32 + c + 1]);
-                }
-                mk[0] = pt_max3(mk[0], v[31], v[63]);
-                mk[1] = pt_max3(mk[1], v[95], v[127]);
-                float mnew = pt_max3(m, pt_max3(mk[0], mk[1], mk[2]) * sl2, mk[3] * sl2);
-                mnew = mnew < INFINITY ? mnew : NAN;          // a score that is NaN or infinite: the row is NaN
-                // O and l keep a maximum up to a factor of 256 behind (attn.cu); each row decides for itself, so that
-                // its bits do not depend on the others of its warp
-                const bool grown = !(mnew <= m + 8.0f);
-                if (j == 0) {
-                    m = mnew;
-                } else if (__any_sync(0xffffffffu, grown)) {
+                const int up = (j < f.nsink ? min(tok, f.sk - 1) : tok) - kb, low = edge ? tok - p.window + 1 - kb : -0x40000000;
+                auto done_before = [&]() {                    // the product of the step before, which writes O
                     ok = __all_sync(0xffffffffu, at_wait(&pv_done[t], (it + j - 1) & 1, p.err));
-                    if (!ok) break;
                     tc_fence_after();
-                    const float alpha = grown ? at_ex2(m - mnew) : 1.0f;
-                    if (grown) m = mnew;
-                    l *= alpha;
-#pragma unroll 1
-                    for (int cc = 0; cc < DP / 32; cc++) {
-                        float o[32];
-                        tmem_ld32(tO + cc * 32, o);
-#pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] *= alpha;
-                        tmem_st32(tO + cc * 32, o);
-                    }
-                }
-                uint32_t pk[64];
-                l += at_softmax_row(v, sl2, m, pk);
-                tmem_st64(tS, pk);
+                    return ok;
+                };
+                const pt_row row = {tS, tO, up, low, p.sinks - kb, edge || j < f.nsink || kb + 127 > first, p.scale2 < 0.0f, j == 0, sl2};
+                if (pt_narrow(f, j)) pt_step<DP, 64>(row, m, l, done_before);
+                else pt_step<DP, 128>(row, m, l, done_before);
+                if (!ok) break;
                 tc_fence_before();
                 irx_mbar_arrive(&p_full[t]);
             }

@@ -255,18 +255,19 @@ static int launch_prompt(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
     k.vec = (uint8_t)(a->dim % al == 0 && a->q_stride % al == 0 && a->kv_stride % al == 0 && a_to(k.q, 16) && a_to(k.k, 16) &&
                       a_to(k.v, 16) && a_to(k.o, 16));
     dp = a->dim <= 64 ? 64 : a->dim <= 128 ? 128 : 256;
-    if (a->dt == DT_BF16 && k.vec && dp <= 128 && k.group <= 128 && (int64_t)a->heads * a->dim < (1 << 24) && a->q_stride < MAX_STRIDE / 2 && a->kv_stride < MAX_STRIDE / 2) {
-        const int tp = 128 / k.group;                      /* tokens of a tile */
+    if (a->dt == DT_BF16 && k.vec && k.group <= 128 && (int64_t)a->heads * a->dim < (1 << 24) && a->q_stride < MAX_STRIDE / 2 && a->kv_stride < MAX_STRIDE / 2) {
+        const int tp = 128 / k.group, nt = dp == 256 ? 1 : 2;  /* tokens of a tile, tiles of a unit */
         const cuuint64_t es2 = 2, qd[4] = {(cuuint64_t)a->dim, (cuuint64_t)k.group, (cuuint64_t)a->kv_heads, (cuuint64_t)a->tokens};
         const cuuint64_t qs[3] = {qd[0] * es2, qd[0] * qd[1] * es2, (cuuint64_t)a->q_stride * es2};
         const cuuint64_t kd[3] = {qd[0], qd[2], qd[3]}, ks[2] = {qd[0] * es2, (cuuint64_t)a->kv_stride * es2};
-        const cuuint32_t qb[4] = {64, (cuuint32_t)k.group, 1, (cuuint32_t)tp}, kb[3] = {64, 1, 128};
+        const cuuint32_t qb[4] = {64, (cuuint32_t)k.group, 1, (cuuint32_t)tp}, kb[3] = {64, 1, dp == 256 ? 64 : 128};
         if (irx_dev_tmap(&k.tma_q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void *)(size_t)k.q, qd, qs, qb, CU_TENSOR_MAP_SWIZZLE_128B) ||
             irx_dev_tmap(&k.tma_k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, (void *)(size_t)k.k, kd, ks, kb, CU_TENSOR_MAP_SWIZZLE_128B) ||
             irx_dev_tmap(&k.tma_v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, (void *)(size_t)k.v, kd, ks, kb, CU_TENSOR_MAP_SWIZZLE_128B))
             return 1;
-        want = ((a->tokens + 2 * tp - 1) / (2 * tp) + a->batch) * (u1 - u0);
-        return irx_dev_launch(d, K_PR_TC + (dp == 128), (unsigned)(want < d->sms ? want : d->sms), 384, IRX_PR_TC_SMEM(dp), 1, st, &k);
+        want = ((a->tokens + nt * tp - 1) / (nt * tp) + a->batch) * (u1 - u0);
+        return irx_dev_launch(d, K_PR_TC + (dp == 64 ? 0 : dp == 128 ? 1 : 2), (unsigned)(want < d->sms ? want : d->sms), 128 * nt + 128,
+                              (unsigned)(dp == 256 ? IRX_PR_WIDE_SMEM : IRX_PR_TC_SMEM(dp)), 1, st, &k);
     }
     kk = K_PR_ST + (dp == 64 ? 0 : dp == 128 ? 1 : 2);
     want = ((a->tokens * k.group + 63) / 64 + a->batch) * (u1 - u0);
