@@ -142,10 +142,11 @@ __device__ __forceinline__ int64_t pr_turn(int i)
 
 // ---- FP32 units: f32 rows, and bf16 rows that the matrix instructions do not take ----
 //
-// 64 query rows against tiles of 64 keys, all as f32 in shared memory; 256 threads hold 4 x 4 scores and
-// 4 rows x DP / 16 columns of the output each, in registers. Rows of Q and K are padded by four
-// floats, so that the 16 key rows read together fall into different banks. Bound by the FP32 units
-// and the shared memory that feeds them.
+// 64 query rows against tiles of 64 keys, as f32 in shared memory, keys and values in turn in one buffer, so that two
+// blocks fit an SM up to 128 columns and one loads while the other multiplies; 256 threads hold 4 x 4 scores and 4 rows
+// x DP / 16 columns of the output each, in registers, and multiply two numbers an instruction. Rows are padded by
+// four floats, so that the 16 key rows read together fall into different banks. Bound by the FP32 units and the
+// shared memory that feeds them.
 #define PS_ROWS 64
 #define PS_KEYS 64
 
@@ -173,7 +174,7 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
 {
     irx_pdl_enter();
     extern __shared__ __align__(16) float ps_smem[];
-    float *sq = ps_smem, *sk = sq + 64 * (DP + 4), *sv = sk + 64 * (DP + 4), *sp = sv + 64 * (DP + 4);
+    float *sq = ps_smem, *sk = sq + 64 * (DP + 4), *sp = sk + 64 * (DP + 4);          // queries; keys, then values; weights
     constexpr int NC = DP / 64;                          // 4-column groups of the output a thread owns
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const pr_list list = pr_start(p, pr_rows{p.group, PS_ROWS});
@@ -196,7 +197,8 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
             sq[r * (DP + 4) + c] = x;
         }
         int tok[4];
-        float m[4], l[4], o[4][NC * 4];
+        float m[4], l[4];
+        float2 o[4][NC * 2];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int r = min(ty * 4 + i, nr - 1);
@@ -204,7 +206,7 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
             m[i] = -3.0e38f;
             l[i] = 0.0f;
 #pragma unroll
-            for (int c = 0; c < NC * 4; c++) o[i][c] = 0.0f;
+            for (int c = 0; c < NC * 2; c++) o[i][c] = make_float2(0.0f, 0.0f);
         }
         const int lo = p.window ? max(0, first - p.window + 1) : 0, sinks = min(p.sinks, lo);
         const int nsink = (sinks + PS_KEYS - 1) / PS_KEYS, ntiles = nsink + (last - lo) / PS_KEYS + 1;
@@ -215,13 +217,12 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
             const bool cut = kt < nsink || nk < PS_KEYS || kb + PS_KEYS - 1 > first || (p.window && kb <= last - p.window);
             __syncthreads();
             ps_fill<DP>(sk, p.k, p.dt, un.base + kb, p.kv_stride, (int64_t)un.head * p.d, nk, p.d, p.vec);
-            ps_fill<DP>(sv, p.v, p.dt, un.base + kb, p.kv_stride, (int64_t)un.head * p.d, nk, p.d, p.vec);
             __syncthreads();
-            float s[4][4];
+            float2 s2[4][4];
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) s[i][j] = 0.0f;
+                for (int j = 0; j < 4; j++) s2[i][j] = make_float2(0.0f, 0.0f);
 #pragma unroll 2
             for (int c = 0; c < DP; c += 4) {
                 float4 a[4], b[4];
@@ -234,15 +235,19 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
                 for (int i = 0; i < 4; i++)
 #pragma unroll
                     for (int j = 0; j < 4; j++)
-                        s[i][j] = fmaf(a[i].w, b[j].w, fmaf(a[i].z, b[j].z, fmaf(a[i].y, b[j].y, fmaf(a[i].x, b[j].x, s[i][j]))));
+                        s2[i][j] = __ffma2_rn(make_float2(a[i].z, a[i].w), make_float2(b[j].z, b[j].w),
+                                              __ffma2_rn(make_float2(a[i].x, a[i].y), make_float2(b[j].x, b[j].y), s2[i][j]));
             }
+            __syncthreads();                             // the keys are done with
+            ps_fill<DP>(sk, p.v, p.dt, un.base + kb, p.kv_stride, (int64_t)un.head * p.d, nk, p.d, p.vec);
+            float s[4][4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 float mx = -3.0e38f;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const int key = kb + tx + 16 * j;
-                    s[i][j] *= p.scale2;
+                    s[i][j] = (s2[i][j].x + s2[i][j].y) * p.scale2;
                     if (cut && (key >= kend || key > tok[i] || (p.window && key <= tok[i] - p.window && key >= p.sinks))) s[i][j] = -INFINITY;
                     mx = s[i][j] > mx || s[i][j] != s[i][j] ? s[i][j] : mx;      // a NaN stays
                 }
@@ -264,27 +269,24 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
                 m[i] = mn;
                 l[i] = l[i] * r + sum;
 #pragma unroll
-                for (int c = 0; c < NC * 4; c++) o[i][c] *= r;
+                for (int c = 0; c < NC * 2; c++) o[i][c] = __fmul2_rn(o[i][c], make_float2(r, r));
             }
-            __syncwarp();                                // a row's weights are made and read by one half warp
+            __syncthreads();                             // the values are there (a row's weights are made and read by one half warp)
             for (int j = 0; j < PS_KEYS; j++) {
                 float w[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) w[i] = sp[(ty * 4 + i) * 68 + j];
 #pragma unroll
                 for (int g = 0; g < NC; g++) {
-                    const float4 x = *reinterpret_cast<const float4 *>(sv + j * (DP + 4) + g * 64 + tx * 4);
+                    const float4 x = *reinterpret_cast<const float4 *>(sk + j * (DP + 4) + g * 64 + tx * 4);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         if (cut && w[i] == 0.0f) continue;
-                        o[i][g * 4] = fmaf(w[i], x.x, o[i][g * 4]);
-                        o[i][g * 4 + 1] = fmaf(w[i], x.y, o[i][g * 4 + 1]);
-                        o[i][g * 4 + 2] = fmaf(w[i], x.z, o[i][g * 4 + 2]);
-                        o[i][g * 4 + 3] = fmaf(w[i], x.w, o[i][g * 4 + 3]);
+                        o[i][g * 2] = __ffma2_rn(make_float2(w[i], w[i]), make_float2(x.x, x.y), o[i][g * 2]);
+                        o[i][g * 2 + 1] = __ffma2_rn(make_float2(w[i], w[i]), make_float2(x.z, x.w), o[i][g * 2 + 1]);
                     }
                 }
             }
-            __syncwarp();
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -299,12 +301,12 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     const int col = g * 64 + tx * 4 + c;
-                    if (col < p.d) irx_st1(p.o, p.dt, row * p.d + col, o[i][g * 4 + c] * inv);
+                    if (col < p.d) irx_st1(p.o, p.dt, row * p.d + col, (c & 1 ? o[i][g * 2 + c / 2].y : o[i][g * 2 + c / 2].x) * inv);
                 }
         }
     }
 }
 
-extern "C" __global__ void __launch_bounds__(256) irx_prompt_st_64(const __grid_constant__ irx_kprm_t p) { ps_body<64>(p); }
-extern "C" __global__ void __launch_bounds__(256) irx_prompt_st_128(const __grid_constant__ irx_kprm_t p) { ps_body<128>(p); }
+extern "C" __global__ void __launch_bounds__(256, 2) irx_prompt_st_64(const __grid_constant__ irx_kprm_t p) { ps_body<64>(p); }
+extern "C" __global__ void __launch_bounds__(256, 2) irx_prompt_st_128(const __grid_constant__ irx_kprm_t p) { ps_body<128>(p); }
 extern "C" __global__ void __launch_bounds__(256) irx_prompt_st_256(const __grid_constant__ irx_kprm_t p) { ps_body<256>(p); }

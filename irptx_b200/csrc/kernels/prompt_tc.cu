@@ -7,8 +7,8 @@
 // copy. The pipeline is irx_attn_bf16's (attn.cu): scores S_t = Q_t K^T into TMEM, one thread a row for the softmax,
 // P over the scores' columns, O_t += P_t V, each tile's softmax under the other tile's products. What differs:
 //   * warp 8 finds the block's units from `starts` (prompt.cu) and hands them out with the loads;
-//   * key tiles may begin anywhere and are masked by token: a window's edge and the sinks' tiles too. The sinks' tile and
-//     a unit's last one are 64 keys wide when that holds all that is seen of them;
+//   * key tiles may begin anywhere and are masked by token: a window's edge and the sinks' tiles too. With heads above 64
+//     the sinks' tile and a unit's last one are 64 keys wide when that holds all that is seen of them;
 //   * warps 10 and 11 look through the values of the tiles that a mask cuts. Rows that no query of the unit
 //     sees become zeros, for another sequence's numbers or uninitialised ones may lie there and 0 * NaN is NaN.
 //     Infinities and NaN in the others become zeros too, and the unit is marked: its rows add those that they
@@ -36,8 +36,11 @@ __device__ __forceinline__ float pt_max3(float a, float b, float c)
 // First token of key tile j, and whether some row of tokens [first, last] does not see all of it.
 __device__ __forceinline__ int pt_key(const pt_info &f, int j) { return j < f.nsink ? 128 * j : f.lo + 128 * (j - f.nsink); }
 
-// Whether the unit needs only the first 64 keys of tile j: the sinks' or the last one, when that is all there is.
-__device__ __forceinline__ bool pt_narrow(const pt_info &f, int j) { return (j < f.nsink ? f.sk : f.end) - pt_key(f, j) <= 64; }
+// Whether the unit needs only the first 64 keys of tile j: the sinks' or the last one, when that is all there is. Not for
+// head sizes up to 64, whose softmax bounds them: a second form of its step in the loop costs the first more than
+// it saves (window with sinks 395 us with it, 344 without).
+template <int DP>
+__device__ __forceinline__ bool pt_narrow(const pt_info &f, int j) { return DP != 64 && (j < f.nsink ? f.sk : f.end) - pt_key(f, j) <= 64; }
 
 __device__ __forceinline__ bool pt_cut(const irx_kprm_t &p, const pt_info &f, int j, int first, int last)
 {
@@ -318,7 +321,7 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
                             if (!(ok = at_wait(&v_ok[gi & 1], (gi >> 1) & 1, p.err))) break;
                             tc_fence_after();
                             const uint32_t bv = sv_a + (gi & 1) * TILE;
-                            const bool narrow = pt_narrow(f, j);
+                            const bool narrow = pt_narrow<DP>(f, j);
 #pragma unroll
                             for (int kk = 0; kk < 8; kk++)
                                 if (kk < 4 || !narrow)
@@ -330,7 +333,7 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
                             const int gi = kv + j + 1;
                             if (!(ok = at_wait(&k_full[gi & 1], (gi >> 1) & 1, p.err))) break;
                             tc_fence_after();
-                            const uint32_t aq = sq_a + t * TILE, bk = sk_a + (gi & 1) * TILE, id = pt_narrow(f, j + 1) ? id_qk64 : id_qk;
+                            const uint32_t aq = sq_a + t * TILE, bk = sk_a + (gi & 1) * TILE, id = pt_narrow<DP>(f, j + 1) ? id_qk64 : id_qk;
 #pragma unroll
                             for (int kk = 0; kk < DP / 16; kk++)
                                 umma_bf16(tbase + t * 128, at_kmajor_desc(aq, kk), at_kmajor_desc(bk, kk), id, kk > 0);
@@ -371,7 +374,7 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
                 if (pt_cut(p, f, j, f.tok0, f.end - 1)) {
                     const int seen = (j < f.nsink ? f.sk : f.end) - pt_key(f, j);
                     uint4 *v = reinterpret_cast<uint4 *>(sv + (gi & 1) * TILE);
-                    const int quads = pt_narrow(f, j) ? 8 : 16;       // rows are looked at in fours: half of them by each warp
+                    const int quads = pt_narrow<DP>(f, j) ? 8 : 16;       // rows are looked at in fours: half of them by each warp
                     uint32_t worst = 0;                       // the largest magnitudes of either half, as integers
 #pragma unroll 4
                     for (int i = 0; i < NB * quads; i++) {
@@ -438,7 +441,7 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
                     return ok;
                 };
                 const pt_row row = {tS, tO, up, low, p.sinks - kb, edge || j < f.nsink || kb + 127 > first, p.scale2 < 0.0f, j == 0, sl2};
-                if (pt_narrow(f, j)) pt_step<DP, 64>(row, m, l, done_before);
+                if (pt_narrow<DP>(f, j)) pt_step<DP, 64>(row, m, l, done_before);
                 else pt_step<DP, 128>(row, m, l, done_before);
                 if (!ok) break;
                 tc_fence_before();

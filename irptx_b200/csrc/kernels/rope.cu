@@ -20,8 +20,8 @@
 template <class T, int V> struct rope_vec;
 template <> struct rope_vec<__nv_bfloat16, 8> {
     uint4 r;
-    __device__ __forceinline__ void load(const __nv_bfloat16 *p) { r = *reinterpret_cast<const uint4 *>(p); }
-    __device__ __forceinline__ void store(__nv_bfloat16 *p) const { *reinterpret_cast<uint4 *>(p) = r; }
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p) { r = __ldcs(reinterpret_cast<const uint4 *>(p)); }
+    __device__ __forceinline__ void store(__nv_bfloat16 *p) const { __stcs(reinterpret_cast<uint4 *>(p), r); }
     __device__ __forceinline__ void get(float (&o)[8]) const
     {
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
@@ -44,8 +44,8 @@ template <> struct rope_vec<__nv_bfloat16, 8> {
 };
 template <> struct rope_vec<float, 4> {
     float4 r;
-    __device__ __forceinline__ void load(const float *p) { r = *reinterpret_cast<const float4 *>(p); }
-    __device__ __forceinline__ void store(float *p) const { *reinterpret_cast<float4 *>(p) = r; }
+    __device__ __forceinline__ void load(const float *p) { r = __ldcs(reinterpret_cast<const float4 *>(p)); }
+    __device__ __forceinline__ void store(float *p) const { __stcs(reinterpret_cast<float4 *>(p), r); }
     __device__ __forceinline__ void get(float (&o)[4]) const { o[0] = r.x; o[1] = r.y; o[2] = r.z; o[3] = r.w; }
     __device__ __forceinline__ void set(const float (&o)[4]) { r = make_float4(o[0], o[1], o[2], o[3]); }
 };
