@@ -181,13 +181,23 @@ __device__ __forceinline__ void pt_step(const pt_row &r, float &m, float &l, F b
         }
     }
     uint32_t pk[W / 2];
-    if constexpr (W == 128) {
+    if (r.cut) {                                  // all on the MUFU: the FMA pipe's pairs give 2^-126 for -infinity, which a value could lift
+        float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < W / 2; i++) {
+            const float2 x = __ffma2_rn(make_float2(v[2 * i], v[2 * i + 1]), make_float2(r.sl2, r.sl2), make_float2(-m, -m));
+            const float p0 = at_ex2(x.x), p1 = at_ex2(x.y);
+            pk[i] = at_pack_bf16(p0, p1);
+            sum = __fadd2_rn(sum, make_float2(p0, p1));
+        }
+        l += sum.x + sum.y;
+    } else if constexpr (W == 128) {
         l += at_softmax_row(v, r.sl2, m, pk);
-        tmem_st64(r.tS, pk);
     } else {
         l += pt_weights(v, r.sl2, m, pk);
-        pt_st32(r.tS, pk);
     }
+    if constexpr (W == 128) tmem_st64(r.tS, pk);
+    else pt_st32(r.tS, pk);
 }
 
 template <int DP>

@@ -195,7 +195,8 @@ int irx_compile_prompt(const irx_prompt_t *m, irx_plan_t *plan)
     a = &p->u.pr;
     if (!m) return irx_fail(E093, "a prompt of no descriptor");
     if (!float_dt(m->dtype)) return irx_fail(E024, "a prompt whose dtype is not f32 or bf16");
-    if (m->tokens < 1 || m->tokens > MAX_COUNT || m->batch < 1) return irx_fail(E042, "a prompt of no tokens or sequences");
+    if (m->tokens < 1 || m->tokens > (1 << 30)) return irx_fail(E042, "prompts' tokens outside 1 to 2^30");
+    if (m->batch < 1 || m->batch > (1 << 16)) return irx_fail(E042, "sequences outside 1 to 2^16");
     if (m->head_dim < 1 || m->head_dim > MAX_DIM) return irx_fail(E042, "a head size outside 1 to 256");
     if (m->kv_heads < 1 || m->heads < 1 || m->heads % m->kv_heads) return irx_fail(E042, "query heads that are not a multiple of the key-value heads");
     if (m->window < 0 || m->sinks < 0) return irx_fail(E042, "a window or sink count below 0");
@@ -250,6 +251,7 @@ static int launch_prompt(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
     k.window = a->window; k.sinks = a->sinks;
     /* a masked score is -inf times this, so it must not be 0; 2^-120 of a finite score is as good as 0 */
     k.scale2 = (float)((double)scale * 1.4426950408889634);
+    if (!isfinite(k.scale2)) k.scale2 = scale < 0 ? -3.4028234663852886e38f : 3.4028234663852886e38f;
     if (fabsf(k.scale2) < 7.5e-37f) k.scale2 = k.scale2 < 0 ? -7.5e-37f : 7.5e-37f;
     k.dt = a->dt;
     k.vec = (uint8_t)(a->dim % al == 0 && a->q_stride % al == 0 && a->kv_stride % al == 0 && a_to(k.q, 16) && a_to(k.k, 16) &&

@@ -305,6 +305,26 @@ def test_prompt_hidden_values_have_no_effect(cuda, irx, dtype, window, sinks, he
     assert bool(out[own].isnan().all())
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 2)])
+@pytest.mark.parametrize("heads,kv,d", [(4, 1, 128), (2, 2, 64), (2, 1, 256)])
+def test_prompt_hidden_large_values_have_no_effect(cuda, irx, dtype, window, sinks, heads, kv, d):
+    """The type's largest numbers in a token that the others do not see: their bits are those without it."""
+    torch = cuda
+    c = prompt_case(torch, irx, dtype, heads, kv, d, [190, 60], window=window, sinks=sinks)
+    plain = prompt_run(torch, irx, c)
+    for at in (189, 249):                                # the last tokens: only their own rows see them
+        c["v"][at] = torch.finfo(c["v"].dtype).max
+    if window:
+        c["v"][5] = torch.finfo(c["v"].dtype).max         # seen by tokens 5 to 44
+    out, lse = prompt_run(torch, irx, c)
+    own = torch.zeros(c["t"], dtype=torch.bool, device="cuda")
+    own[[189, 249]] = True
+    if window:
+        own[5:45] = True
+    assert torch.equal(out[~own], plain[0][~own]) and torch.equal(lse, plain[1])
+
+
 def test_prompt_reports_bad_starts(cuda, irx):
     torch = cuda
     c = prompt_case(torch, irx, "bf16", 4, 2, 64, [50, 60, 70])

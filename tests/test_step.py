@@ -61,7 +61,7 @@ def test_refusals(irx):
     refused(irx, 24, irx.rope_append, cache(irx, dtype="f16"), 2, 4, f)
     for k in (dict(tokens=0), dict(batch=0), dict(heads=0), dict(kv_heads=0), dict(heads=5), dict(head_dim=0), dict(head_dim=257),
               dict(window=-1), dict(sinks=-1), dict(sinks=1), dict(scale=NAN), dict(scale=INF), dict(q_stride=255), dict(kv_stride=127),
-              dict(tokens=1 << 31), dict(batch=1 << 30, heads=64, kv_heads=64), dict(q_stride=1 << 41)):
+              dict(tokens=(1 << 30) + 1), dict(batch=(1 << 16) + 1), dict(tokens=1 << 30, heads=256, kv_heads=2), dict(q_stride=1 << 41)):
         refused(irx, 42, irx.prompt, **{**dict(tokens=9, batch=2, heads=4, kv_heads=2, head_dim=64), **k})
     refused(irx, 24, irx.prompt, 9, 2, 4, 2, 64, dtype="f64")
     for k in (dict(rows=0), dict(vocab=0), dict(vocab=(1 << 30) + 1), dict(rows=1 << 28), dict(stride=99), dict(stride=1 << 41)):
