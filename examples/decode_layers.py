@@ -132,6 +132,10 @@ class Decoder:
 
         return s, self.forward(self.embed[torch.tensor(tokens, device="cuda")], seq, pos, attention)[-1]
 
+    def choose(self, logits):
+        """Every slot's next token."""
+        return logits.float().argmax(-1)
+
     def start(self, state):
         """Record a decoding step over all slots; `state` holds each slot's token and position (-1: none)."""
         self.token, self.pos = state
@@ -147,7 +151,7 @@ class Decoder:
         def step():
             self.lens.copy_(self.pos + 1)
             logits = self.forward(self.embed[self.token.clamp_min(0)], self.seq, self.pos, attention)
-            self.token.copy_(logits.float().argmax(-1))
+            self.token.copy_(self.choose(logits))
             self.pos.add_((self.pos >= 0).to(torch.int32))
             return logits
 
@@ -173,6 +177,10 @@ class Decoder:
 
     # ---- the check ----
 
+    def turned(self, x):
+        """What the positions do to queries and keys [heads, tokens, dim]: nothing here."""
+        return x
+
     def dense(self, tokens):
         """The last token's logits of the same model, computed over the whole sequence in 64 bits."""
         def norm(x, w):
@@ -181,6 +189,7 @@ class Decoder:
         mask = torch.ones(n, n, device="cuda", dtype=torch.bool).tril()
         for b in self.blocks:
             q, k, v = (norm(x, b["n1"]) @ b["qkv"].dense.T).unflatten(1, (-1, self.dim)).transpose(0, 1).split([self.heads, self.kv, self.kv])
+            q, k = self.turned(q), self.turned(k)
             k, v = k.repeat_interleave(self.heads // self.kv, 0), v.repeat_interleave(self.heads // self.kv, 0)
             p = (q @ k.transpose(1, 2) / math.sqrt(self.dim)).masked_fill(~mask, -math.inf).softmax(-1)
             x = x + (p @ v).transpose(0, 1).reshape(n, -1) @ b["o"].dense.T
