@@ -272,20 +272,26 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
                 for (int c = 0; c < NC * 2; c++) o[i][c] = __fmul2_rn(o[i][c], make_float2(r, r));
             }
             __syncthreads();                             // the values are there (a row's weights are made and read by one half warp)
-            for (int j = 0; j < PS_KEYS; j++) {
-                float w[4];
+#pragma unroll 1
+            for (int j0 = 0; j0 < PS_KEYS; j0 += 4) {
+                float w[4][4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) w[i] = sp[(ty * 4 + i) * 68 + j];
-#pragma unroll
-                for (int g = 0; g < NC; g++) {
-                    const float4 x = *reinterpret_cast<const float4 *>(sk + j * (DP + 4) + g * 64 + tx * 4);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        if (cut && w[i] == 0.0f) continue;
-                        o[i][g * 2] = __ffma2_rn(make_float2(w[i], w[i]), make_float2(x.x, x.y), o[i][g * 2]);
-                        o[i][g * 2 + 1] = __ffma2_rn(make_float2(w[i], w[i]), make_float2(x.z, x.w), o[i][g * 2 + 1]);
-                    }
+                for (int i = 0; i < 4; i++) {
+                    const float4 x = *reinterpret_cast<const float4 *>(sp + (ty * 4 + i) * 68 + j0);
+                    w[i][0] = x.x; w[i][1] = x.y; w[i][2] = x.z; w[i][3] = x.w;
                 }
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int g = 0; g < NC; g++) {
+                        const float4 x = *reinterpret_cast<const float4 *>(sk + (j0 + j) * (DP + 4) + g * 64 + tx * 4);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            if (cut && w[i][j] == 0.0f) continue;
+                            o[i][g * 2] = __ffma2_rn(make_float2(w[i][j], w[i][j]), make_float2(x.x, x.y), o[i][g * 2]);
+                            o[i][g * 2 + 1] = __ffma2_rn(make_float2(w[i][j], w[i][j]), make_float2(x.z, x.w), o[i][g * 2 + 1]);
+                        }
+                    }
             }
         }
 #pragma unroll

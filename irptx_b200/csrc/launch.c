@@ -166,7 +166,7 @@ static const char *const KNAMES[K_COUNT] = {
     "irx_mv4_bf16_32_1", "irx_mv4_bf16_32_2", "irx_mv4_bf16_64_1", "irx_mv4_bf16_64_2", "irx_mv4_bf16_128_1", "irx_mv4_bf16_128_2",
     "irx_mv4_f32_32_1", "irx_mv4_f32_32_2", "irx_mv4_f32_64_1", "irx_mv4_f32_64_2", "irx_mv4_f32_128_1", "irx_mv4_f32_128_2",
     "irx_mv4_any",
-    "irx_rope_bf16_8", "irx_rope_bf16_1", "irx_rope_f32_4", "irx_rope_f32_1",
+    "irx_rope_bf16_lane", "irx_rope_bf16_8", "irx_rope_bf16_1", "irx_rope_f32_lane", "irx_rope_f32_4", "irx_rope_f32_1",
     "irx_prompt_st_64", "irx_prompt_st_128", "irx_prompt_st_256", "irx_prompt_tc_64", "irx_prompt_tc_128", "irx_prompt_tc_256",
     "irx_sample_bf16", "irx_sample_bf16_far", "irx_sample_f32", "irx_sample_f32_far"
 };

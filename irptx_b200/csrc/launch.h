@@ -18,7 +18,7 @@ enum {
     K_DEC_TC, K_DEC_ST = K_DEC_TC + 5, K_KV_APPEND = K_DEC_ST + 6, K_KV_COPY = K_KV_APPEND + 3,
     K_MV4 = K_KV_COPY + 3, K_MV4_ANY = K_MV4 + 12,
     /* rotary positions by type and vector, prompt attention by padded head size, the draw by type and residence */
-    K_ROPE, K_PR_ST = K_ROPE + 4, K_PR_TC = K_PR_ST + 3, K_SMP = K_PR_TC + 3,
+    K_ROPE, K_PR_ST = K_ROPE + 6, K_PR_TC = K_PR_ST + 3, K_SMP = K_PR_TC + 3,
     K_COUNT = K_SMP + 4
 };
 

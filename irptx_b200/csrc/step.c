@@ -171,7 +171,7 @@ static int launch_rope(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsign
           ((size_t)k.x_stride | (size_t)k.kv_stride | (size_t)k.y_stride | (size_t)k.page_stride | (size_t)k.head_stride |
            (size_t)k.token_stride | (size_t)k.d | (size_t)a->pairs) * (size_t)es;
     v = mix % 16 == 0 ? vmax : 1;
-    k.items = k.pairs / v + (k.d - 2 * k.pairs) / v;
+    k.items = k.pairs / v + (k.d - 2 * k.pairs + 2 * v - 1) / (2 * v);      /* two vectors each */
     /* A warp for each token shares the token's angles; with few tokens more warps each (down to one item a
      * lane), until the GPU has sixteen for every SM. */
     n = (int64_t)(k.heads + 2 * k.kv) * k.items;
@@ -181,7 +181,7 @@ static int launch_rope(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsign
     k.parts = (int32_t)((n + k.chunk - 1) / k.chunk);
     warps = (u1 - u0) * k.parts;
     if ((warps + 3) / 4 > MAX_COUNT) return irx_fail(E042, "a rotation past one launch's blocks");
-    return irx_dev_launch(d, K_ROPE + (c->dt == DT_BF16 ? 0 : 2) + (v == 1), (unsigned)((warps + 3) / 4), 128, 0, 1, st, &k);
+    return irx_dev_launch(d, K_ROPE + (c->dt == DT_BF16 ? 0 : 3) + (v == 1 ? 2 : 32 % k.items ? 1 : 0), (unsigned)((warps + 3) / 4), 128, 0, 1, st, &k);
 }
 
 /* ---- attention over packed prompts ---- */
