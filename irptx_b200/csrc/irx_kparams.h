@@ -231,7 +231,7 @@ typedef struct {
 /* The draw of a token: one cluster a row; a thread of a block holds `words` words of 4 bytes, an odd number. */
 #define IRX_SMP_BINS 2048
 #define IRX_SMP_THREADS 512
-#define IRX_SMP_FIXED (IRX_SMP_BINS * 12 + 2560)   /* shared memory beside the row: histogram, reductions */
+#define IRX_SMP_FIXED (IRX_SMP_BINS * 12 + 2816)   /* shared memory beside the row: histogram, reductions */
 
 typedef struct {
     const void *x;

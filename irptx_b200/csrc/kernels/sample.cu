@@ -27,7 +27,7 @@
 
 struct smp_shared {
     union {
-        struct { unsigned cnt[IRX_SMP_BINS], lo[IRX_SMP_BINS], hi[IRX_SMP_BINS]; };   // a cell's tokens, or its weight in two words
+        struct { unsigned cnt[IRX_SMP_BINS + 32], lo[IRX_SMP_BINS], hi[IRX_SMP_BINS]; };   // a cell's tokens, or its weight in two words
         struct { uint64_t mine[SMP_FEW], list[SMP_FEW], weight_of[SMP_FEW]; };        // few tokens: this block's, the row's, their weights
     };
     double tab[128];
@@ -111,11 +111,11 @@ __device__ __forceinline__ uint64_t smp_raw(const irx_ksmp_t &p, const smp_row &
 
 __device__ __forceinline__ uint64_t smp_weight(const irx_ksmp_t &p, const smp_row &q, float x) { return smp_raw(p, q, fmaxf(x, q.floor)) - SMP_RAW; }
 
-// The cell of the first histogram, at least IRX_SMP_BINS for what has no weight. Never falls as x falls.
-__device__ __forceinline__ unsigned smp_cell(const smp_row &q, float x)
+// The cell of the first histogram, `none` (at least IRX_SMP_BINS) for what has no weight. Never falls as x falls.
+__device__ __forceinline__ unsigned smp_cell(const smp_row &q, float x, unsigned none = IRX_SMP_BINS)
 {
     const float f = fmaf(fmaf(-0.5f, x, 0.5f * q.maxf), q.step, 8388608.0f);         // 2^23: the sum's low bits are the cell
-    return x > q.floor && f < 8388608.0f + IRX_SMP_BINS ? __float_as_uint(f) - 0x4b000000u : IRX_SMP_BINS;
+    return x > q.floor && f < 8388608.0f + IRX_SMP_BINS ? __float_as_uint(f) - 0x4b000000u : none;
 }
 
 // A key whose number is the floor or lies below it.
@@ -227,6 +227,29 @@ template <class T, bool FAR> struct smp_data {
         }
     }
 };
+
+// f(number, index) for the few numbers above `from` and up to `to`: looked for SMP_STEP words at a time, with one branch.
+template <class T, bool FAR, class F>
+__device__ __forceinline__ void smp_pick(const smp_data<T, FAR> &x, float from, float to, F f)
+{
+    typedef smp_type<T> ty;
+    for (int j0 = 0; j0 < x.words; j0 += SMP_STEP) {
+        unsigned hits = 0;
+#pragma unroll
+        for (int j = 0; j < SMP_STEP; j++) {
+            const unsigned w = j0 + j < x.words ? x.word(j0 + j) : ty::PAD;
+#pragma unroll
+            for (int h = 0; h < ty::N; h++) {
+                const float v = ty::get(w, h);
+                if (v > from && v <= to) hits |= 1u << (j * ty::N + h);
+            }
+        }
+        for (; hits; hits &= hits - 1) {
+            const int b = __ffs(hits) - 1;
+            f(ty::get(x.word(j0 + b / ty::N), b % ty::N), j0 * ty::N + b);
+        }
+    }
+}
 
 struct smp_cut { float above; unsigned ties; };     // what is kept: what is above, and the first `ties` of those equal
 
@@ -458,10 +481,7 @@ __device__ __forceinline__ smp_cut smp_resolve(const irx_ksmp_t &p, smp_shared &
     }
     uint64_t left = target - (by_weight ? sh.before : sh.above);
     if (lo != hi && gather && count <= SMP_FEW) {
-        const float from = ty::value(lo), to = ty::value(hi);
-        x.each([&](float v, int) {
-            if (v >= from && v <= to) sh.mine[atomicAdd(&sh.few, 1u)] = smp_token(v, 0);
-        });
+        smp_pick(x, ty::value(lo - 1), ty::value(hi), [&](float v, int) { sh.mine[atomicAdd(&sh.few, 1u)] = smp_token(v, 0); });
         __syncthreads();
         const unsigned n = sh.few;
         unsigned at = 0, m = 0;
@@ -667,20 +687,16 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
     bool tallied = false;
     if (s.k || s.part) {
         smp_clear(sh, false);
-        x.each([&](float v, int) {
-            const unsigned cell = smp_cell(q, v);
-            if (cell < IRX_SMP_BINS) smp_tally(sh, cell, false, 0);
-        });
+        unsigned *cells = sh.cnt;                        // what has no weight goes behind them, each lane to a place of its own
+        x.each([&](float v, int) { atomicAdd(cells + smp_cell(q, v, IRX_SMP_BINS + lane), 1u); });
         tallied = true;
     }
     if (s.k) {
         uint64_t target = s.k;
         if (!smp_find(sh, rank, nc, turn, SMP_COUNT, target, 0)) s.k = 0;      // fewer have any weight: all of those
         else if (sh.above + sh.count <= SMP_FEW) {
-            const unsigned cell = sh.cell;
-            x.each([&](float v, int i) {
-                if (smp_cell(q, v) <= cell) sh.mine[atomicAdd(&sh.few, 1u)] = smp_token(v, first + i);
-            });
+            const unsigned cell = sh.cell, below = smp_last(smp_least<T>(q), ty::key(q.maxf), [&](unsigned kk) { return smp_cell(q, ty::value(kk)) > cell; });
+            smp_pick(x, ty::value(below), INFINITY, [&](float v, int i) { sh.mine[atomicAdd(&sh.few, 1u)] = smp_token(v, first + i); });
             __syncthreads();
             const unsigned n = sh.few;
             unsigned at = 0, m = 0;
@@ -712,15 +728,17 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
         const unsigned ko = few ? tk : smp_last(least, tk, [&](unsigned kk) { return smp_cell(q, ty::value(kk)) >= c0; });
         const float below = ty::value(kb), over = ty::value(ko);
         uint64_t sum[3] = {0, 0, 0};                     // the whole, what is over the gathered cells, what is in them
-        x.each([&](float v, int i) {
-            const uint64_t w = smp_weight(p, q, v);
+        x.each([&](float v, int) {
+            const uint64_t w = smp_raw(p, q, fmaxf(v, q.floor));
             sum[0] += w;
-            sum[1] += v > over ? w : 0;
-            if (v > below && v <= over) {
-                sum[2] += w;
-                const unsigned at = atomicAdd(&sh.few, 1u);
-                if (at < SMP_FEW) sh.mine[at] = smp_token(v, first + i);
-            }
+            sum[1] += v > over ? w : SMP_RAW;
+        });
+        sum[0] -= (uint64_t)(x.words * ty::N) * SMP_RAW;
+        sum[1] -= (uint64_t)(x.words * ty::N) * SMP_RAW;
+        smp_pick(x, below, over, [&](float v, int i) {
+            sum[2] += smp_weight(p, q, v);
+            const unsigned at = atomicAdd(&sh.few, 1u);
+            if (at < SMP_FEW) sh.mine[at] = smp_token(v, first + i);
         });
         const uint64_t own = sum[1];
         unsigned none = 0, at = 0, m = 0;
@@ -785,7 +803,11 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
     const uint64_t w_eq = cut.ties ? smp_weight(p, q, cut.above) : 0;
     uint64_t sums[1] = {kept};
     unsigned eq = 0;
-    for (int j0 = 0; j0 < x.words; j0 += SMP_STEP) {
+    const bool whole = cut.above == q.floor && upto == INFINITY;       // nothing is cut: no floor but the weights' own
+    if (whole) {
+        x.each([&](float v, int) { sums[0] += smp_raw(p, q, fmaxf(v, q.floor)); });
+        sums[0] -= (uint64_t)(x.words * ty::N) * SMP_RAW;
+    } else for (int j0 = 0; j0 < x.words; j0 += SMP_STEP) {
         float v[SMP_STEP * ty::N];
         bool any = false;
 #pragma unroll
