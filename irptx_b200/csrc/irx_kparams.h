@@ -243,7 +243,6 @@ typedef struct {
     int64_t     r0, stride, n;
     int32_t     words;
     int32_t     kbits;              /* a weight of 1 is 2^kbits, at most 2^46 */
-    uint8_t     vec, pad[7];        /* rows of logits begin on 16 bytes */
     /* constants of the weights' exponential, here so that instructions read them in place: 1.5 * 2^52, 2^52,
      * (ln 2 / 128)^i / i! for i = 1 to 4, and 2^(kbits + j / 128) */
     double      big, two52, series[4], tab[128];

@@ -590,30 +590,38 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     unsigned rank = cluster_rank(), nc, turn = 0;
     asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(nc));
-    const int64_t row = p.r0 + blockIdx.x / nc, per = (int64_t)p.words * IRX_SMP_THREADS * ty::N, base = (int64_t)rank * per;
-    const int64_t here = max((int64_t)0, min(per, p.n - base));
-    const T *src = reinterpret_cast<const T *>(p.x) + row * p.stride + base;
+    const int64_t row = p.r0 + blockIdx.x / nc, per = (int64_t)p.words * IRX_SMP_THREADS * ty::N;
+    const T *line = reinterpret_cast<const T *>(p.x) + row * p.stride;
+    // a row that begins inside a word: its words count from there, with one element of nothing first
+    const int lead = !FAR && ((size_t)line & 3) ? 1 : 0;
+    const int64_t base = (int64_t)rank * per - lead, here = max((int64_t)0, min(per, p.n - base));
+    const T *src = line + base;
+    if (!FAR) data += ((size_t)src & 15) / 4;            // as far past 16 bytes as in memory
     const int64_t first = base + (int64_t)threadIdx.x * p.words * ty::N;               // this thread's first element
     smp_data<T, FAR> x = {data + threadIdx.x * p.words, src + (int64_t)threadIdx.x * p.words * ty::N, p.n - first, p.words, SMP_PLAIN, 0.0f};
     const float t = p.temperature[row], tp = p.top_p[row], mp = p.min_p[row], un = p.u[row];
     const int k = p.top_k[row];
 
-    // the row into shared memory, padded with -infinity
+    // the row into shared memory, padded with -infinity: what lies between multiples of 16 bytes in one copy
     unsigned bytes = 0;
     if (threadIdx.x < 128) sh.tab[threadIdx.x] = p.tab[threadIdx.x];
     if (threadIdx.x == 0) sh.few = 0;
     if (!FAR) {
-        bytes = p.vec ? (unsigned)(here * sizeof(T)) & ~15u : 0;
+        const size_t a0 = (size_t)src, from = (a0 + (base < 0 ? sizeof(T) : 0) + 15) & ~(size_t)15, to = (a0 + here * sizeof(T)) & ~(size_t)15;
+        bytes = to > from ? (unsigned)(to - from) : 0;
         if (threadIdx.x == 0) {
             irx_mbar_init(&sh.bar, 1);
             irx_fence_mbar_init();
             if (bytes) {
                 irx_mbar_expect_tx(&sh.bar, bytes);
-                irx_bulk_g2s(data, src, bytes, &sh.bar);
+                irx_bulk_g2s(reinterpret_cast<unsigned char *>(data) + (from - a0), reinterpret_cast<const void *>(from), bytes, &sh.bar);
             }
         }
         T *e = reinterpret_cast<T *>(data);
-        for (int64_t i = bytes / sizeof(T) + threadIdx.x; i < per; i += IRX_SMP_THREADS) e[i] = i < here ? src[i] : (T)-INFINITY;
+        const int64_t i0 = (int64_t)(from - a0) / (int64_t)sizeof(T), i1 = i0 + bytes / sizeof(T);       // copied
+        if (threadIdx.x < i0 && bytes) e[threadIdx.x] = base + threadIdx.x >= 0 ? src[threadIdx.x] : (T)-INFINITY;
+        for (int64_t i = (bytes ? i1 : 0) + threadIdx.x; i < per; i += IRX_SMP_THREADS)
+            e[i] = i < here && base + i >= 0 ? src[i] : (T)-INFINITY;
     }
     __syncthreads();
     if (bytes && !irx_mbar_wait(&sh.bar, 0) && lane == 0) atomicOr(p.err, IRX_KERR_TIMEOUT);

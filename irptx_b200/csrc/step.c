@@ -313,7 +313,7 @@ static int launch_sample(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
     const int epw = a->dt == DT_BF16 ? 2 : 1;              /* elements of a word */
     static irx_ksmp_t k;
     long long u0, u1;
-    int64_t nc, words, room = (d->smem_optin - IRX_SMP_FIXED) / 4;
+    int64_t nc, words, room = (d->smem_optin - IRX_SMP_FIXED - 16) / 4;
     int far, j;
     memset(&k, 0, sizeof k);
     irx_unit_range(a->rows, s, ns, &u0, &u1);
@@ -332,13 +332,12 @@ static int launch_sample(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
     k.two52 = 4503599627370496.0;
     for (j = 0; j < 4; j++) k.series[j] = (j ? k.series[j - 1] : 1.0) * (0.69314718055994530942 / 128.0) / (j + 1);
     for (j = 0; j < 128; j++) k.tab[j] = ldexp(exp2(j / 128.0), k.kbits);
-    k.vec = (uint8_t)(a_to(k.x, 16) && a->stride * 4 / epw % 16 == 0);
     /* Blocks of a cluster: as few as hold the row in their shared memory, since every block pays for the row's settings
      * and exchanges. With few rows more, down to 4096 elements each, as long as all rows' blocks run at once; with many,
      * as many as let two blocks share an SM. Measured (128001 bf16 logits, top-k and top-p, 64 rows): 2 blocks 31 us,
      * 4 37, 8 54; one row: 30, 22, 18; 256 rows of 151999, top-p: 243, 219, 288. */
     for (nc = 1;; nc *= 2) {
-        words = (a->vocab + nc * epw * IRX_SMP_THREADS - 1) / (nc * epw * IRX_SMP_THREADS) | 1;
+        words = (a->vocab + epw - 1 + nc * epw * IRX_SMP_THREADS - 1) / (nc * epw * IRX_SMP_THREADS) | 1;
         if (nc == 8) break;
         if (words * IRX_SMP_THREADS > room) continue;
         if (words * epw * IRX_SMP_THREADS <= 4096) break;
@@ -347,7 +346,7 @@ static int launch_sample(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
     k.words = (int32_t)words;
     far = words * IRX_SMP_THREADS > room;
     return irx_dev_launch(d, K_SMP + (a->dt == DT_BF16 ? 0 : 2) + far, (unsigned)((u1 - u0) * nc), IRX_SMP_THREADS,
-                          (unsigned)(IRX_SMP_FIXED + (far ? 0 : words * IRX_SMP_THREADS * 4)), (unsigned)nc, st, &k);
+                          (unsigned)(IRX_SMP_FIXED + (far ? 0 : words * IRX_SMP_THREADS * 4 + 16)), (unsigned)nc, st, &k);
 }
 
 /* ---- one entry for the launch switch, and the plans' descriptions ---- */
