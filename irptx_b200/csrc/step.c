@@ -333,15 +333,14 @@ static int launch_sample(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
     for (j = 0; j < 4; j++) k.series[j] = (j ? k.series[j - 1] : 1.0) * (0.69314718055994530942 / 128.0) / (j + 1);
     for (j = 0; j < 128; j++) k.tab[j] = ldexp(exp2(j / 128.0), k.kbits);
     /* Blocks of a cluster: as few as hold the row in their shared memory, since every block pays for the row's settings
-     * and exchanges. With few rows more, down to 4096 elements each, as long as all rows' blocks run at once; with many,
-     * as many as let two blocks share an SM. Measured (128001 bf16 logits, top-k and top-p, 64 rows): 2 blocks 31 us,
-     * 4 37, 8 54; one row: 30, 22, 18; 256 rows of 151999, top-p: 243, 219, 288. */
+     * and exchanges. With few rows more, down to 4096 elements each, as long as all rows' blocks run at once. Measured
+     * with 2, 4 and 8 blocks: 64 rows of 128001 bf16 logits, top-k and top-p, 23, 29, 49 us; f32 (2 do not hold it) 40 with 4, 52
+     * with 8; 256 rows of 151999, top-p, bf16 185, 192, 267, f32 260 with 4, 286 with 8; one row of 128001 30, 22, 17. */
     for (nc = 1;; nc *= 2) {
         words = (a->vocab + epw - 1 + nc * epw * IRX_SMP_THREADS - 1) / (nc * epw * IRX_SMP_THREADS) | 1;
         if (nc == 8) break;
         if (words * IRX_SMP_THREADS > room) continue;
-        if (words * epw * IRX_SMP_THREADS <= 4096) break;
-        if ((u1 - u0) * nc * 2 > d->sms && ((u1 - u0) * nc < 2 * d->sms || words * IRX_SMP_THREADS * 4 + IRX_SMP_FIXED <= 113 * 1024)) break;
+        if (words * epw * IRX_SMP_THREADS <= 4096 || (u1 - u0) * nc * 2 > d->sms) break;
     }
     k.words = (int32_t)words;
     far = words * IRX_SMP_THREADS > room;
