@@ -14,8 +14,11 @@
 // weights round to zero, or their weights, show the cell in which a filter ends. When that cell and those
 // above it hold few tokens (top-k, or a peaked row), they go to the first block, which finishes alone. Otherwise the
 // cell's own tokens are resolved, by the first block when they are few, else by histograms of the cell's
-// range, and every thread adds up its stretch's kept weights. What bounds large calls is instructions, about
-// 25 of them for each weight.
+// range, and every thread adds up its stretch's kept weights.
+//
+// Bound by instructions for many rows (31 an element without filters, 82 with top-p: 128 rows of 151999 bf16
+// logits 51 and 154 us, against 6 us for reading them) and by its exchanges and passes, one after another, for
+// few (one row of 128001, top-k and top-p: 15 to 17 us).
 #pragma once
 #include "tc.cuh"
 
