@@ -16,8 +16,8 @@
 // cell's own tokens are resolved, by the first block when they are few, else by histograms of the cell's
 // range, and every thread adds up its stretch's kept weights.
 //
-// Bound by instructions for many rows (31 an element without filters, 82 with top-p: 128 rows of 151999 bf16
-// logits 51 and 154 us, against 6 us for reading them) and by its exchanges and passes, one after another, for
+// Bound by instructions for many rows (30 an element without filters, 67 with top-p: 128 rows of 151999 bf16
+// logits 38 and 85 us, against 6 us for reading them) and by its exchanges and passes, one after another, for
 // few (one row of 128001, top-k and top-p: 15 to 17 us).
 #pragma once
 #include "tc.cuh"
@@ -42,6 +42,7 @@ struct smp_shared {
     uint64_t bar;
 };
 static_assert(sizeof(smp_shared) <= IRX_SMP_FIXED, "the launcher's size");
+static_assert(3 * IRX_SMP_THREADS * sizeof(unsigned) <= SMP_FEW * sizeof(uint64_t), "three words a thread in the list's place");
 
 // Logits as numbers that order and weigh as defined: NaN as -infinity. For rows whose largest is infinite (then such
 // logits are 0 and all others -infinity) or below -1e30 (then the largest is taken away from all: exactly, wherever a
@@ -407,7 +408,7 @@ __device__ __forceinline__ smp_cut smp_among(const irx_ksmp_t &p, smp_shared &sh
 {
     typedef smp_type<T> ty;
     if (rank == 0) {
-        unsigned *low = reinterpret_cast<unsigned *>(sh.mine), *high = low + 256;        // a cell's sum in two words
+        unsigned *low = reinterpret_cast<unsigned *>(sh.weight_of), *high = low + 256;   // a cell's sum in two words
         const int lane = threadIdx.x & 31;
         unsigned key[SMP_OWN];
         uint64_t w[SMP_OWN];
@@ -693,9 +694,9 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
     s.whole = 0;
 
     smp_cut cut = {q.floor, 0};                          // (at the floor nothing weighs)
-    uint64_t kept = 0;                                   // the weight of this thread's tokens above `upto`, once it is known
-    float upto = INFINITY;
-    bool tallied = false;
+    uint64_t kept = 0;                                   // this thread's kept weight and its tokens at the threshold, when `known`
+    unsigned at_cut = 0;
+    bool tallied = false, known = false;
     if (s.k || s.part) {
         smp_clear(sh, false);
         unsigned *cells = sh.cnt;                        // what has no weight goes behind them, each lane to a place of its own
@@ -739,18 +740,31 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
         const unsigned ko = few ? tk : smp_last(least, tk, [&](unsigned kk) { return smp_cell(q, ty::value(kk)) >= c0; });
         const float below = ty::value(kb), over = ty::value(ko);
         uint64_t sum[3] = {0, 0, 0};                     // the whole, what is over the gathered cells, what is in them
-        x.each([&](float v, int) {
-            const uint64_t w = smp_raw(p, q, fmaxf(v, q.floor));
-            sum[0] += w;
-            sum[1] += v > over ? w : SMP_RAW;
-        });
-        sum[0] -= (uint64_t)(x.words * ty::N) * SMP_RAW;
-        sum[1] -= (uint64_t)(x.words * ty::N) * SMP_RAW;
-        smp_pick(x, below, over, [&](float v, int i) {
-            sum[2] += smp_weight(p, q, v);
-            const unsigned at = atomicAdd(&sh.few, 1u);
-            if (at < SMP_FEW) sh.mine[at] = smp_token(v, first + i);
-        });
+        for (int j0 = 0; j0 < x.words; j0 += SMP_STEP) {
+            unsigned hits = 0;
+#pragma unroll
+            for (int j = 0; j < SMP_STEP; j++) {
+                const unsigned word = j0 + j < x.words ? x.word(j0 + j) : ty::PAD;
+#pragma unroll
+                for (int h = 0; h < ty::N; h++) {
+                    const float v = ty::get(word, h);
+                    const uint64_t w = smp_raw(p, q, fmaxf(v, q.floor));
+                    sum[0] += w;
+                    sum[1] += v > over ? w : SMP_RAW;
+                    if (v > below && v <= over) hits |= 1u << (j * ty::N + h);
+                }
+            }
+            for (; hits; hits &= hits - 1) {
+                const int b = __ffs(hits) - 1;
+                const float v = ty::get(x.word(j0 + b / ty::N), b % ty::N);
+                sum[2] += smp_weight(p, q, v);
+                const unsigned at = atomicAdd(&sh.few, 1u);
+                if (at < SMP_FEW) sh.mine[at] = smp_token(v, first + j0 * ty::N + b);
+            }
+        }
+        const uint64_t read = (uint64_t)((x.words + SMP_STEP - 1) / SMP_STEP * SMP_STEP * ty::N) * SMP_RAW;
+        sum[0] -= read;
+        sum[1] -= read;
         const uint64_t own = sum[1];
         unsigned none = 0, at = 0, m = 0;
         smp_block_sums(sh, sum, none);
@@ -773,9 +787,23 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
                 return;
             }
             cut = smp_among<T>(p, sh, q, rank, nc, m, kb + 1, ko, target - above, true);
-            if (!s.least) {
-                kept = own;
-                upto = over;
+            if (!s.least) {                              // what is kept of the gathered cells, to the threads that it came from
+                unsigned *lo = reinterpret_cast<unsigned *>(sh.list), *hi = lo + IRX_SMP_THREADS, *eq = hi + IRX_SMP_THREADS;
+                lo[threadIdx.x] = hi[threadIdx.x] = eq[threadIdx.x] = 0;
+                __syncthreads();
+                for (unsigned i = threadIdx.x; i < n; i += IRX_SMP_THREADS) {
+                    const float v = smp_number(sh.mine[i]);
+                    const int whose = (int)((unsigned)sh.mine[i] - base) / (p.words * ty::N);
+                    if (v > cut.above) {
+                        const uint64_t w = smp_weight(p, q, v);
+                        const unsigned wl = (unsigned)w, old = atomicAdd(&lo[whose], wl);
+                        atomicAdd(&hi[whose], (unsigned)(w >> 32) + (old + wl < old));
+                    } else if (cut.ties && v == cut.above) atomicAdd(&eq[whose], 1u);
+                }
+                __syncthreads();
+                kept = own + ((uint64_t)hi[threadIdx.x] << 32 | lo[threadIdx.x]);
+                at_cut = eq[threadIdx.x];
+                known = true;
             }
         } else {
             __syncthreads();
@@ -813,9 +841,9 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
     // at the floor, with no weight; words of which no lane of a warp keeps any are passed over.
     const uint64_t w_eq = cut.ties ? smp_weight(p, q, cut.above) : 0;
     uint64_t sums[1] = {kept};
-    unsigned eq = 0;
-    const bool whole = cut.above == q.floor && upto == INFINITY;       // nothing is cut: no floor but the weights' own
-    if (whole) {
+    unsigned eq = at_cut;
+    if (known) {
+    } else if (cut.above == q.floor) {                   // nothing is cut: no floor but the weights' own
         x.each([&](float v, int) { sums[0] += smp_raw(p, q, fmaxf(v, q.floor)); });
         sums[0] -= (uint64_t)(x.words * ty::N) * SMP_RAW;
     } else for (int j0 = 0; j0 < x.words; j0 += SMP_STEP) {
@@ -827,7 +855,7 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
 #pragma unroll
             for (int h = 0; h < ty::N; h++) {
                 v[j * ty::N + h] = ty::get(word, h);
-                any |= v[j * ty::N + h] >= cut.above && v[j * ty::N + h] <= upto;
+                any |= v[j * ty::N + h] >= cut.above;
             }
         }
         if (!__any_sync(0xffffffffu, any)) continue;
@@ -835,7 +863,7 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
 #pragma unroll
             for (int j = 0; j < SMP_STEP * ty::N; j++) eq += v[j] == cut.above;
 #pragma unroll
-        for (int j = 0; j < SMP_STEP * ty::N; j++) sums[0] += smp_raw(p, q, v[j] > cut.above && v[j] <= upto ? v[j] : q.floor) - SMP_RAW;
+        for (int j = 0; j < SMP_STEP * ty::N; j++) sums[0] += smp_raw(p, q, v[j] > cut.above ? v[j] : q.floor) - SMP_RAW;
     }
     const uint64_t w_mine = sums[0];
     const unsigned eq_mine = eq;
