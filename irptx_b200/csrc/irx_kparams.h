@@ -204,8 +204,8 @@ typedef struct {
 } irx_krope_t;
 
 /* Attention over packed prompts. Units: tiles of query rows (token, head of the group) of a sequence and a
- * key-value head. Shared memory of the FP32 kernel: two tiles of 64 rows and the weights. */
-#define IRX_PR_ST_SMEM(dp) ((2 * 64 * ((dp) + 4) + 64 * 68) * 4)
+ * key-value head. Shared memory of the FP32 kernel: 64 rows each of queries, keys and values, and the weights. */
+#define IRX_PR_ST_SMEM(dp) ((3 * 64 * (dp) + 64 * 64) * 4)
 
 /* The matrix instructions' kernels. Head sizes up to 128: two tiles of 128 rows each of queries, keys and values; above: one
  * of queries, rings of key and value tiles of 64. Then 1 KB of barriers, and 4 KB of staged output a softmax warp. */

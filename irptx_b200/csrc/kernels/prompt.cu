@@ -142,30 +142,31 @@ __device__ __forceinline__ int64_t pr_turn(int i)
 
 // ---- FP32 units: f32 rows, and bf16 rows that the matrix instructions do not take ----
 //
-// 64 query rows against tiles of 64 keys, as f32 in shared memory, keys and values in turn in one buffer, so that two
-// blocks fit an SM up to 128 columns and one loads while the other multiplies; 256 threads hold 4 x 4 scores and 4 rows
-// x DP / 16 columns of the output each, in registers, and multiply two numbers an instruction. Rows are padded by
-// four floats, so that the 16 key rows read together fall into different banks. Bound by the FP32 units and the
-// shared memory that feeds them.
+// 64 query rows against tiles of 64 keys, as f32 in shared memory: keys and values each in a buffer of their own, so that
+// values arrive while scores are computed and the next keys during the second product; two blocks fit an SM up to 128
+// columns. 256 threads hold 4 x 4 scores and 4 rows x DP / 16 columns of the output each, in registers, and multiply two
+// numbers an instruction. A key row's groups of four floats are permuted by the row's place in its eight, so that the 16 key
+// rows read together fall into different banks. Bound by the FP32 units and the shared memory that feeds them.
 #define PS_ROWS 64
 #define PS_KEYS 64
 
-template <int DP>
+// n rows of d numbers into 64 rows of DP, zeros behind both; f32 rows of whole 16 bytes asynchronously
+template <int DP, bool SWZ>
 __device__ __forceinline__ void ps_fill(float *dst, const void *src, int dt, int64_t row0, int64_t stride, int64_t off, int n, int d, bool vec)
 {
-    // n rows of d numbers into 64 rows of DP + 4, zeros behind both
     if (vec && dt == DT_F32) {
-        for (int e = threadIdx.x; e < 64 * (DP / 4); e += 256) {
-            const int r = e / (DP / 4), c = (e % (DP / 4)) * 4;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < n && c < d) x = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(src) + (row0 + r) * stride + off + c);
-            *reinterpret_cast<float4 *>(dst + r * (DP + 4) + c) = x;
+        const float *from = reinterpret_cast<const float *>(src) + row0 * stride + off;
+#pragma unroll
+        for (int e0 = 0; e0 < 64 * (DP / 4); e0 += 256) {
+            const int e = e0 + threadIdx.x, r = e / (DP / 4), c = (e % (DP / 4)) * 4;
+            const bool there = r < n && c < d;
+            cp16(irx_smem_u32(dst + r * DP + (SWZ ? c ^ (r & 7) << 2 : c)), there ? from + r * stride + c : from, there ? 16 : 0);
         }
         return;
     }
     for (int e = threadIdx.x; e < 64 * DP; e += 256) {
         const int r = e / DP, c = e % DP;
-        dst[r * (DP + 4) + c] = r < n && c < d ? irx_ld1(src, dt, (row0 + r) * stride + off + c) : 0.0f;
+        dst[r * DP + (SWZ ? c ^ (r & 7) << 2 : c)] = r < n && c < d ? irx_ld1(src, dt, (row0 + r) * stride + off + c) : 0.0f;
     }
 }
 
@@ -174,50 +175,62 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
 {
     irx_pdl_enter();
     extern __shared__ __align__(16) float ps_smem[];
-    float *sq = ps_smem, *sk = sq + 64 * (DP + 4), *sp = sk + 64 * (DP + 4);          // queries; keys, then values; weights
+    float *sq = ps_smem, *sk = sq + 64 * DP, *sv = sk + 64 * DP, *sp = sv + 64 * DP;       // queries, keys, values, weights
     constexpr int NC = DP / 64;                          // 4-column groups of the output a thread owns
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const pr_list list = pr_start(p, pr_rows{p.group, PS_ROWS});
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, odd = ty & 1;      // of a warp's two fours of rows, the second has
+    const pr_list list = pr_start(p, pr_rows{p.group, PS_ROWS});               // its queries and weights in other banks
     for (int turn = 0;; turn++) {
         const int64_t u = pr_turn(turn);
         if (u >= list.units) break;
         const pr_unit un = pr_find(p, list, u);
         const int64_t r0 = (int64_t)un.tile * PS_ROWS, rows = (int64_t)un.len * p.group;
         const int nr = (int)min((int64_t)PS_ROWS, rows - r0);
-        const int first = (int)(r0 / p.group), last = (int)((r0 + nr - 1) / p.group);
-        __syncthreads();                                 // the tile before is done with
-        for (int e = threadIdx.x; e < 64 * DP; e += 256) {
-            const int r = e / DP, c = e % DP;
-            float x = 0.0f;
-            if (r < nr && c < p.d) {
-                const int64_t tok = (r0 + r) / p.group;
-                const int h = un.head * p.group + (int)((r0 + r) - tok * p.group);
-                x = irx_ld1(p.q, p.dt, (un.base + tok) * p.q_stride + (int64_t)h * p.d + c);
+        const int first = (int)(r0 / p.group), skip = (int)(r0 - (int64_t)first * p.group), last = first + (skip + nr - 1) / p.group;
+        const int lo = p.window ? max(0, first - p.window + 1) : 0, sinks = min(p.sinks, lo);
+        const int nsink = (sinks + PS_KEYS - 1) / PS_KEYS, ntiles = nsink + (last - lo) / PS_KEYS + 1;
+        auto begin = [&](int kt) { return kt < nsink ? kt * PS_KEYS : lo + (kt - nsink) * PS_KEYS; };
+        auto end = [&](int kt) { return kt < nsink ? sinks : last + 1; };
+        auto keys = [&](int kt) {
+            ps_fill<DP, true>(sk, p.k, p.dt, un.base + begin(kt), p.kv_stride, (int64_t)un.head * p.d, min(PS_KEYS, end(kt) - begin(kt)), p.d, p.vec);
+            cp_commit();
+        };
+        __syncthreads();                                 // the unit before is done with
+        if (p.vec && p.dt == DT_F32) {
+#pragma unroll
+            for (int e0 = 0; e0 < 64 * (DP / 4); e0 += 256) {
+                const int e = e0 + threadIdx.x, r = e / (DP / 4), c = (e % (DP / 4)) * 4, t = (skip + r) / p.group;
+                const bool there = r < nr && c < p.d;
+                const float *from = reinterpret_cast<const float *>(p.q) + (un.base + first + t) * p.q_stride
+                                    + (int64_t)(un.head * p.group + skip + r - t * p.group) * p.d + c;
+                cp16(irx_smem_u32(sq + r * DP + (c ^ (r & 4))), there ? (const void *)from : p.q, there ? 16 : 0);
             }
-            sq[r * (DP + 4) + c] = x;
-        }
+        } else
+            for (int e = threadIdx.x; e < 64 * DP; e += 256) {
+                const int r = e / DP, c = e % DP, t = (skip + r) / p.group;
+                sq[r * DP + (c ^ (r & 4))] = r < nr && c < p.d ? irx_ld1(p.q, p.dt, (un.base + first + t) * p.q_stride
+                                                                         + (int64_t)(un.head * p.group + skip + r - t * p.group) * p.d + c) : 0.0f;
+            }
+        keys(0);
         int tok[4];
         float m[4], l[4];
         float2 o[4][NC * 2];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int r = min(ty * 4 + i, nr - 1);
-            tok[i] = (int)((r0 + r) / p.group);
+            tok[i] = first + (skip + r) / p.group;
             m[i] = -3.0e38f;
             l[i] = 0.0f;
 #pragma unroll
             for (int c = 0; c < NC * 2; c++) o[i][c] = make_float2(0.0f, 0.0f);
         }
-        const int lo = p.window ? max(0, first - p.window + 1) : 0, sinks = min(p.sinks, lo);
-        const int nsink = (sinks + PS_KEYS - 1) / PS_KEYS, ntiles = nsink + (last - lo) / PS_KEYS + 1;
         for (int kt = 0; kt < ntiles; kt++) {
-            const int kb = kt < nsink ? kt * PS_KEYS : lo + (kt - nsink) * PS_KEYS;
-            const int kend = kt < nsink ? sinks : last + 1, nk = min(PS_KEYS, kend - kb);
+            const int kb = begin(kt), kend = end(kt), nk = min(PS_KEYS, kend - kb);
             // a tile that some row does not see in whole: masked, and its weights of zero add nothing
             const bool cut = kt < nsink || nk < PS_KEYS || kb + PS_KEYS - 1 > first || (p.window && kb <= last - p.window);
-            __syncthreads();
-            ps_fill<DP>(sk, p.k, p.dt, un.base + kb, p.kv_stride, (int64_t)un.head * p.d, nk, p.d, p.vec);
-            __syncthreads();
+            cp_wait<0>();
+            __syncthreads();                             // the keys are there, the values before are done with
+            ps_fill<DP, false>(sv, p.v, p.dt, un.base + kb, p.kv_stride, (int64_t)un.head * p.d, nk, p.d, p.vec);
+            cp_commit();
             float2 s2[4][4];
 #pragma unroll
             for (int i = 0; i < 4; i++)
@@ -228,8 +241,8 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
                 float4 a[4], b[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    a[i] = *reinterpret_cast<const float4 *>(sq + (ty * 4 + i) * (DP + 4) + c);
-                    b[i] = *reinterpret_cast<const float4 *>(sk + (tx + 16 * i) * (DP + 4) + c);
+                    a[i] = *reinterpret_cast<const float4 *>(sq + (ty * 4 + i) * DP + (c ^ odd << 2));
+                    b[i] = *reinterpret_cast<const float4 *>(sk + (tx + 16 * i) * DP + (c ^ (tx & 7) << 2));
                 }
 #pragma unroll
                 for (int i = 0; i < 4; i++)
@@ -238,8 +251,6 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
                         s2[i][j] = __ffma2_rn(make_float2(a[i].z, a[i].w), make_float2(b[j].z, b[j].w),
                                               __ffma2_rn(make_float2(a[i].x, a[i].y), make_float2(b[j].x, b[j].y), s2[i][j]));
             }
-            __syncthreads();                             // the keys are done with
-            ps_fill<DP>(sk, p.v, p.dt, un.base + kb, p.kv_stride, (int64_t)un.head * p.d, nk, p.d, p.vec);
             float s[4][4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -262,7 +273,7 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
                 for (int j = 0; j < 4; j++) {
                     s[i][j] = exp2f(s[i][j] - mn);
                     sum += s[i][j];
-                    sp[(ty * 4 + i) * 68 + tx + 16 * j] = s[i][j];
+                    sp[(ty * 4 + i) * 64 + tx + (16 * j ^ odd << 4)] = s[i][j];
                 }
 #pragma unroll
                 for (int x = 8; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
@@ -271,20 +282,22 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
 #pragma unroll
                 for (int c = 0; c < NC * 2; c++) o[i][c] = __fmul2_rn(o[i][c], make_float2(r, r));
             }
-            __syncthreads();                             // the values are there (a row's weights are made and read by one half warp)
+            cp_wait<0>();
+            __syncthreads();                             // the values are there, the keys done with (a row's weights are made and read by one half warp)
+            if (kt + 1 < ntiles) keys(kt + 1);
 #pragma unroll 1
             for (int j0 = 0; j0 < PS_KEYS; j0 += 4) {
                 float w[4][4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float4 x = *reinterpret_cast<const float4 *>(sp + (ty * 4 + i) * 68 + j0);
+                    const float4 x = *reinterpret_cast<const float4 *>(sp + (ty * 4 + i) * 64 + (j0 ^ odd << 4));
                     w[i][0] = x.x; w[i][1] = x.y; w[i][2] = x.z; w[i][3] = x.w;
                 }
 #pragma unroll
                 for (int j = 0; j < 4; j++)
 #pragma unroll
                     for (int g = 0; g < NC; g++) {
-                        const float4 x = *reinterpret_cast<const float4 *>(sk + (j0 + j) * (DP + 4) + g * 64 + tx * 4);
+                        const float4 x = *reinterpret_cast<const float4 *>(sv + (j0 + j) * DP + g * 64 + tx * 4);
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             if (cut && w[i][j] == 0.0f) continue;
@@ -298,7 +311,7 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
         for (int i = 0; i < 4; i++) {
             const int r = ty * 4 + i;
             if (r >= nr) continue;
-            const int h = un.head * p.group + (int)((r0 + r) - (int64_t)tok[i] * p.group);
+            const int h = un.head * p.group + skip + r - (tok[i] - first) * p.group;
             const int64_t row = (int64_t)(un.base + tok[i]) * p.heads + h;
             const float inv = 1.0f / l[i];
             if (p.lse && tx == 0) p.lse[row] = (m[i] + log2f(l[i])) * 0.6931471806f;
