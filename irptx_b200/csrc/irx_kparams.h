@@ -205,6 +205,7 @@ typedef struct {
 
 /* Attention over packed prompts. Units: tiles of query rows (token, head of the group) of a sequence and a
  * key-value head. Shared memory of the FP32 kernel: 64 rows each of queries, keys and values, and the weights. */
+#define IRX_PR_ST_THREADS(dp) ((dp) == 128 ? 128 : 256)
 #define IRX_PR_ST_SMEM(dp) ((3 * 64 * (dp) + 64 * 64) * 4)
 
 /* The matrix instructions' kernels. Head sizes up to 128: two tiles of 128 rows each of queries, keys and values; above: one

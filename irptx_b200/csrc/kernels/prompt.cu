@@ -144,39 +144,42 @@ __device__ __forceinline__ int64_t pr_turn(int i)
 //
 // 64 query rows against tiles of 64 keys, as f32 in shared memory: keys and values each in a buffer of their own, so that
 // values arrive while scores are computed and the next keys during the second product; two blocks fit an SM up to 128
-// columns. 256 threads hold 4 x 4 scores and 4 rows x DP / 16 columns of the output each, in registers, and multiply two
-// numbers an instruction. A key row's groups of four floats are permuted by the row's place in its eight, so that the 16 key
-// rows read together fall into different banks. Bound by the FP32 units and the shared memory that feeds them.
+// columns. A thread holds R x 4 scores and R rows x DP / 16 columns of the output in registers and multiplies two numbers an
+// instruction; a 16-byte read costs its four accesses of the shared memory also where lanes read the same, so at R = 4 that
+// memory is as busy as the FP32 units (71 and 61 %). R = 8 (128 threads) reads less and has half the warps: 161 against 170 us
+// for 2222 tokens in five prompts, 16 heads on 4 of 128; at 64 columns 122 against 95, so 4 there, and above 128, where the
+// registers end. A key row's groups of four floats are permuted by the row's place in its eight, so that the 16 key
+// rows read together fall into different banks.
 #define PS_ROWS 64
 #define PS_KEYS 64
 
 // n rows of d numbers into 64 rows of DP, zeros behind both; f32 rows of whole 16 bytes asynchronously
-template <int DP, bool SWZ>
+template <int DP, int NT, bool SWZ>
 __device__ __forceinline__ void ps_fill(float *dst, const void *src, int dt, int64_t row0, int64_t stride, int64_t off, int n, int d, bool vec)
 {
     if (vec && dt == DT_F32) {
         const float *from = reinterpret_cast<const float *>(src) + row0 * stride + off;
 #pragma unroll
-        for (int e0 = 0; e0 < 64 * (DP / 4); e0 += 256) {
+        for (int e0 = 0; e0 < 64 * (DP / 4); e0 += NT) {
             const int e = e0 + threadIdx.x, r = e / (DP / 4), c = (e % (DP / 4)) * 4;
             const bool there = r < n && c < d;
             cp16(irx_smem_u32(dst + r * DP + (SWZ ? c ^ (r & 7) << 2 : c)), there ? from + r * stride + c : from, there ? 16 : 0);
         }
         return;
     }
-    for (int e = threadIdx.x; e < 64 * DP; e += 256) {
+    for (int e = threadIdx.x; e < 64 * DP; e += NT) {
         const int r = e / DP, c = e % DP;
         dst[r * DP + (SWZ ? c ^ (r & 7) << 2 : c)] = r < n && c < d ? irx_ld1(src, dt, (row0 + r) * stride + off + c) : 0.0f;
     }
 }
 
-template <int DP>
+template <int DP, int R>
 __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
 {
     irx_pdl_enter();
     extern __shared__ __align__(16) float ps_smem[];
     float *sq = ps_smem, *sk = sq + 64 * DP, *sv = sk + 64 * DP, *sp = sv + 64 * DP;       // queries, keys, values, weights
-    constexpr int NC = DP / 64;                          // 4-column groups of the output a thread owns
+    constexpr int NC = DP / 64, NT = 1024 / R;           // 4-column groups of the output a thread owns; threads
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, odd = ty & 1;      // of a warp's two fours of rows, the second has
     const pr_list list = pr_start(p, pr_rows{p.group, PS_ROWS});               // its queries and weights in other banks
     for (int turn = 0;; turn++) {
@@ -191,32 +194,32 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
         auto begin = [&](int kt) { return kt < nsink ? kt * PS_KEYS : lo + (kt - nsink) * PS_KEYS; };
         auto end = [&](int kt) { return kt < nsink ? sinks : last + 1; };
         auto keys = [&](int kt) {
-            ps_fill<DP, true>(sk, p.k, p.dt, un.base + begin(kt), p.kv_stride, (int64_t)un.head * p.d, min(PS_KEYS, end(kt) - begin(kt)), p.d, p.vec);
+            ps_fill<DP, NT, true>(sk, p.k, p.dt, un.base + begin(kt), p.kv_stride, (int64_t)un.head * p.d, min(PS_KEYS, end(kt) - begin(kt)), p.d, p.vec);
             cp_commit();
         };
         __syncthreads();                                 // the unit before is done with
         if (p.vec && p.dt == DT_F32) {
 #pragma unroll
-            for (int e0 = 0; e0 < 64 * (DP / 4); e0 += 256) {
+            for (int e0 = 0; e0 < 64 * (DP / 4); e0 += NT) {
                 const int e = e0 + threadIdx.x, r = e / (DP / 4), c = (e % (DP / 4)) * 4, t = (skip + r) / p.group;
                 const bool there = r < nr && c < p.d;
                 const float *from = reinterpret_cast<const float *>(p.q) + (un.base + first + t) * p.q_stride
                                     + (int64_t)(un.head * p.group + skip + r - t * p.group) * p.d + c;
-                cp16(irx_smem_u32(sq + r * DP + (c ^ (r & 4))), there ? (const void *)from : p.q, there ? 16 : 0);
+                cp16(irx_smem_u32(sq + r * DP + (c ^ (r / R & 1) << 2)), there ? (const void *)from : p.q, there ? 16 : 0);
             }
         } else
-            for (int e = threadIdx.x; e < 64 * DP; e += 256) {
+            for (int e = threadIdx.x; e < 64 * DP; e += NT) {
                 const int r = e / DP, c = e % DP, t = (skip + r) / p.group;
-                sq[r * DP + (c ^ (r & 4))] = r < nr && c < p.d ? irx_ld1(p.q, p.dt, (un.base + first + t) * p.q_stride
+                sq[r * DP + (c ^ (r / R & 1) << 2)] = r < nr && c < p.d ? irx_ld1(p.q, p.dt, (un.base + first + t) * p.q_stride
                                                                          + (int64_t)(un.head * p.group + skip + r - t * p.group) * p.d + c) : 0.0f;
             }
         keys(0);
-        int tok[4];
-        float m[4], l[4];
-        float2 o[4][NC * 2];
+        int tok[R];
+        float m[R], l[R];
+        float2 o[R][NC * 2];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = min(ty * 4 + i, nr - 1);
+        for (int i = 0; i < R; i++) {
+            const int r = min(ty * R + i, nr - 1);
             tok[i] = first + (skip + r) / p.group;
             m[i] = -3.0e38f;
             l[i] = 0.0f;
@@ -229,31 +232,32 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
             const bool cut = kt < nsink || nk < PS_KEYS || kb + PS_KEYS - 1 > first || (p.window && kb <= last - p.window);
             cp_wait<0>();
             __syncthreads();                             // the keys are there, the values before are done with
-            ps_fill<DP, false>(sv, p.v, p.dt, un.base + kb, p.kv_stride, (int64_t)un.head * p.d, nk, p.d, p.vec);
+            ps_fill<DP, NT, false>(sv, p.v, p.dt, un.base + kb, p.kv_stride, (int64_t)un.head * p.d, nk, p.d, p.vec);
             cp_commit();
-            float2 s2[4][4];
+            float2 s2[R][4];
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < R; i++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) s2[i][j] = make_float2(0.0f, 0.0f);
-#pragma unroll 2
+#pragma unroll (R == 8 ? 2 : 4)
             for (int c = 0; c < DP; c += 4) {
-                float4 a[4], b[4];
+                float4 a[R], b[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    a[i] = *reinterpret_cast<const float4 *>(sq + (ty * 4 + i) * DP + (c ^ odd << 2));
-                    b[i] = *reinterpret_cast<const float4 *>(sk + (tx + 16 * i) * DP + (c ^ (tx & 7) << 2));
-                }
+                for (int i = 0; i < R; i++)
+                    a[i] = *reinterpret_cast<const float4 *>(sq + (ty * R + i) * DP + (c ^ odd << 2));
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+                for (int j = 0; j < 4; j++)
+                    b[j] = *reinterpret_cast<const float4 *>(sk + (tx + 16 * j) * DP + (c ^ (tx & 7) << 2));
+#pragma unroll
+                for (int i = 0; i < R; i++)
 #pragma unroll
                     for (int j = 0; j < 4; j++)
                         s2[i][j] = __ffma2_rn(make_float2(a[i].z, a[i].w), make_float2(b[j].z, b[j].w),
                                               __ffma2_rn(make_float2(a[i].x, a[i].y), make_float2(b[j].x, b[j].y), s2[i][j]));
             }
-            float s[4][4];
+            float s[R][4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
+            for (int i = 0; i < R; i++) {
                 float mx = -3.0e38f;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
@@ -273,24 +277,22 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
                 for (int j = 0; j < 4; j++) {
                     s[i][j] = exp2f(s[i][j] - mn);
                     sum += s[i][j];
-                    sp[(ty * 4 + i) * 64 + tx + (16 * j ^ odd << 4)] = s[i][j];
+                    sp[(ty * R + i) * 64 + tx + (16 * j ^ odd << 4)] = s[i][j];
                 }
-#pragma unroll
-                for (int x = 8; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
                 m[i] = mn;
-                l[i] = l[i] * r + sum;
+                l[i] = l[i] * r + sum;                   // of this lane's keys: joined at the end
 #pragma unroll
                 for (int c = 0; c < NC * 2; c++) o[i][c] = __fmul2_rn(o[i][c], make_float2(r, r));
             }
             cp_wait<0>();
             __syncthreads();                             // the values are there, the keys done with (a row's weights are made and read by one half warp)
             if (kt + 1 < ntiles) keys(kt + 1);
-#pragma unroll 1
+#pragma unroll 2
             for (int j0 = 0; j0 < PS_KEYS; j0 += 4) {
-                float w[4][4];
+                float w[R][4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float4 x = *reinterpret_cast<const float4 *>(sp + (ty * 4 + i) * 64 + (j0 ^ odd << 4));
+                for (int i = 0; i < R; i++) {
+                    const float4 x = *reinterpret_cast<const float4 *>(sp + (ty * R + i) * 64 + (j0 ^ odd << 4));
                     w[i][0] = x.x; w[i][1] = x.y; w[i][2] = x.z; w[i][3] = x.w;
                 }
 #pragma unroll
@@ -299,7 +301,7 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
                     for (int g = 0; g < NC; g++) {
                         const float4 x = *reinterpret_cast<const float4 *>(sv + (j0 + j) * DP + g * 64 + tx * 4);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
+                        for (int i = 0; i < R; i++) {
                             if (cut && w[i][j] == 0.0f) continue;
                             o[i][g * 2] = __ffma2_rn(make_float2(w[i][j], w[i][j]), make_float2(x.x, x.y), o[i][g * 2]);
                             o[i][g * 2 + 1] = __ffma2_rn(make_float2(w[i][j], w[i][j]), make_float2(x.z, x.w), o[i][g * 2 + 1]);
@@ -308,8 +310,10 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
             }
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = ty * 4 + i;
+        for (int i = 0; i < R; i++) {
+            const int r = ty * R + i;
+#pragma unroll
+            for (int x = 8; x; x >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
             if (r >= nr) continue;
             const int h = un.head * p.group + skip + r - (tok[i] - first) * p.group;
             const int64_t row = (int64_t)(un.base + tok[i]) * p.heads + h;
@@ -326,6 +330,7 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
     }
 }
 
-extern "C" __global__ void __launch_bounds__(256, 2) irx_prompt_st_64(const __grid_constant__ irx_kprm_t p) { ps_body<64>(p); }
-extern "C" __global__ void __launch_bounds__(256, 2) irx_prompt_st_128(const __grid_constant__ irx_kprm_t p) { ps_body<128>(p); }
-extern "C" __global__ void __launch_bounds__(256) irx_prompt_st_256(const __grid_constant__ irx_kprm_t p) { ps_body<256>(p); }
+#define PS_KERNEL(DP, B) extern "C" __global__ void __launch_bounds__(IRX_PR_ST_THREADS(DP), B) irx_prompt_st_##DP(const __grid_constant__ irx_kprm_t p) { ps_body<DP, 1024 / IRX_PR_ST_THREADS(DP)>(p); }
+PS_KERNEL(64, 2)
+PS_KERNEL(128, 2)
+PS_KERNEL(256, 1)

@@ -273,8 +273,8 @@ static int launch_prompt(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
     }
     kk = K_PR_ST + (dp == 64 ? 0 : dp == 128 ? 1 : 2);
     want = ((a->tokens * k.group + 63) / 64 + a->batch) * (u1 - u0);
-    if (irx_serve_grid(d, kk, 256, IRX_PR_ST_SMEM(dp), want, &grid)) return 1;
-    return irx_dev_launch(d, kk, (unsigned)grid, 256, IRX_PR_ST_SMEM(dp), 1, st, &k);
+    if (irx_serve_grid(d, kk, IRX_PR_ST_THREADS(dp), IRX_PR_ST_SMEM(dp), want, &grid)) return 1;
+    return irx_dev_launch(d, kk, (unsigned)grid, IRX_PR_ST_THREADS(dp), IRX_PR_ST_SMEM(dp), 1, st, &k);
 }
 
 /* ---- the draw of a token ---- */
