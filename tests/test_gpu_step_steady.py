@@ -115,6 +115,25 @@ def test_sample_flat_and_steep_rows(cuda, irx):
                 draw_check(torch, irx, torch.stack(rows), [(t, k, p, m, u)] * len(rows))
 
 
+@pytest.mark.parametrize("rows", [1, 4, 48])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_sample_ends_among_equal_logits(cuda, irx, dtype, rows):
+    """top-p alone ends inside 700 equal logits below 3000 others: too many for one block to finish, few enough to be gathered,
+    and held by every block of the row. Where the running sum ends is half a token's weight away from the next one."""
+    torch = cuda
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    n, x = 20011, torch.full((20011,), -30.0, device="cuda")
+    place = torch.randperm(n, generator=gen, device="cuda")
+    x[place[:3000]] = torch.empty(3000, device="cuda").uniform_(1.2, 1.8, generator=gen)
+    x[place[3000:3700]] = 1.0
+    x = x.to(tdt(torch, dtype))
+    e = torch.exp(x.double() - x.double().max())
+    above, one = float(e[place[:3000]].sum()), float(e[place[3000]])
+    for kept in (0.5, 99.5, 350.5, 699.5):
+        p = (above + kept * one) / float(e.sum())
+        draw_check(torch, irx, x.expand(rows, n).contiguous(), [(1.0, 0, p, 0.0, (i + 0.45) / rows) for i in range(rows)])
+
+
 def test_sample_many_short_rows(cuda, irx):
     torch = cuda
     gen, rnd = torch.Generator(device="cuda").manual_seed(9), random.Random(9)
