@@ -588,6 +588,7 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
 {
     typedef smp_type<T> ty;
     irx_pdl_enter();
+    cluster_arrive();                                    // (waited for before the first exchange)
     extern __shared__ __align__(16) unsigned char smp_bytes[];
     smp_shared &sh = *reinterpret_cast<smp_shared *>(smp_bytes);
     unsigned *data = reinterpret_cast<unsigned *>(smp_bytes + IRX_SMP_FIXED);
@@ -643,6 +644,8 @@ __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
     unsigned best = 0;
 #pragma unroll
     for (int i = 0; i < SMP_WARPS; i++) best = max(best, sh.redc[i]);
+    __syncwarp();
+    cluster_wait();                                      // every block of the cluster has begun: its shared memory may be written
     smp_post(sh, rank, nc, turn, 0, best);
     for (unsigned r = 0; r < nc; r++) best = max(best, sh.xc[turn][r]);
     top = smp_type<float>::value(best);

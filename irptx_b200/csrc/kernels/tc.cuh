@@ -158,6 +158,11 @@ __device__ __forceinline__ void cluster_sync()
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// The same barrier in two parts, for work between them: until the wait has ended, other blocks of the cluster may not
+// have begun, and their shared memory must not be touched.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // One arrival on an mbarrier anywhere in the cluster (a shared::cluster address), ordered after
 // this thread's earlier work at CTA scope: for signals that publish no ordinary memory to the
 // other CTA (tensor-memory hand-offs are ordered by the tcgen05 fences around the barrier).
