@@ -53,7 +53,9 @@ __device__ __forceinline__ float smp_shift(float x, int mode, float top)
     return mode == SMP_INFINITE ? (x == INFINITY ? 0.0f : -INFINITY) : mode == SMP_LOW ? x - top : x;
 }
 
-// Keys order as the numbers do, both zeros alike.
+// Keys order as the numbers do: the magnitude's bits, counted up or down from 2^31 (bf16: 2^15), which is the key of both
+// zeros. Neighbouring keys are neighbouring numbers, none is left out: "above the number of the key below" and "from this
+// key on" are the same everywhere, at 0 too.
 template <class T> struct smp_type;
 template <> struct smp_type<float> {
     static const int N = 1;
@@ -64,10 +66,10 @@ template <> struct smp_type<float> {
     __device__ static __forceinline__ unsigned most(unsigned a, unsigned b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
     __device__ static __forceinline__ unsigned key(float x)
     {
-        const unsigned u = __float_as_uint(x + 0.0f);
-        return u & 0x80000000u ? ~u : u | 0x80000000u;
+        const unsigned u = __float_as_uint(x);
+        return u & 0x80000000u ? 0u - u : u | 0x80000000u;
     }
-    __device__ static __forceinline__ float value(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+    __device__ static __forceinline__ float value(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : 0u - k); }
 };
 template <> struct smp_type<__nv_bfloat16> {
     static const int N = 2;
@@ -81,10 +83,10 @@ template <> struct smp_type<__nv_bfloat16> {
     __device__ static __forceinline__ unsigned put(float a, float b) { return __float_as_uint(a) >> 16 | (__float_as_uint(b) & 0xffff0000u); }
     __device__ static __forceinline__ unsigned key(float x)
     {
-        const unsigned u = __float_as_uint(x + 0.0f) >> 16;
-        return u & 0x8000u ? ~u & 0xffffu : u | 0x8000u;
+        const unsigned u = __float_as_uint(x) >> 16;
+        return u & 0x8000u ? (0u - u) & 0xffffu : u | 0x8000u;
     }
-    __device__ static __forceinline__ float value(unsigned k) { return __uint_as_float((k & 0x8000u ? k & 0x7fffu : ~k & 0xffffu) << 16); }
+    __device__ static __forceinline__ float value(unsigned k) { return __uint_as_float((k & 0x8000u ? k & 0x7fffu : (0u - k) & 0xffffu) << 16); }
 };
 
 struct smp_row {
