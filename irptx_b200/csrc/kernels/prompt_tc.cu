@@ -91,15 +91,26 @@ __device__ __forceinline__ void pt_st32(uint32_t taddr, const uint32_t (&v)[32])
                  : "memory");
 }
 
-// at_softmax_row (attn.cu) for 64 scores: P = 2^(s * sl2 - m) as bf16 pairs, and their sum.
-__device__ __forceinline__ float pt_weights(const float (&v)[64], float sl2, float m, uint32_t (&pk)[32])
+// Two bf16 numbers less 2^-126 each.
+__device__ __forceinline__ uint32_t pt_less(uint32_t x)
+{
+    uint32_t d;
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(0x00800080u));
+    return d;
+}
+
+// at_softmax_row (attn.cu) for W scores: P = 2^(s * sl2 - m) as bf16 pairs, and their sum. What differs: the FMA pipe's
+// pairs, which end at 2^-126, lose that much once rounded, so that a weight below it is 0 on either pipe and adds nothing, however
+// large its value. (Half a step of a bf16 weight from 2^-116 on is more than that: those are the same bits.)
+template <int W>
+__device__ __forceinline__ float pt_weights(const float (&v)[W], float sl2, float m, uint32_t (&pk)[W / 2])
 {
     float2 sa = make_float2(0.0f, 0.0f), sb = make_float2(0.0f, 0.0f);
     const float2 s2 = make_float2(sl2, sl2), nm = make_float2(-m, -m);
     const float ks = sl2 * (1.0f / 253.0f), kc = (126.0f - m) * (1.0f / 253.0f);
     const float2 k253 = make_float2(253.0f, 253.0f), kmg = make_float2(12582912.0f - 126.0f, 12582912.0f - 126.0f);
 #pragma unroll
-    for (int i = 0; i < 32; i++) {
+    for (int i = 0; i < W / 2; i++) {
         if ((i & 3) != 3) {
             const float2 x = __ffma2_rn(make_float2(v[2 * i], v[2 * i + 1]), s2, nm);
             const float p0 = at_ex2(x.x), p1 = at_ex2(x.y);
@@ -116,7 +127,7 @@ __device__ __forceinline__ float pt_weights(const float (&v)[64], float sl2, flo
             q = __ffma2_rn(q, f, make_float2(0.9999281096694117f, 0.9999281096694117f));
             const uint32_t r0 = __float_as_uint(q.x) + (__float_as_uint(t.x) << 23);
             const uint32_t r1 = __float_as_uint(q.y) + (__float_as_uint(t.y) << 23);
-            pk[i] = __byte_perm(r0 + 0x8000u, r1 + 0x8000u, 0x7632);
+            pk[i] = pt_less(__byte_perm(r0 + 0x8000u, r1 + 0x8000u, 0x7632));
             sb = __fadd2_rn(sb, make_float2(__uint_as_float(r0), __uint_as_float(r1)));
         }
     }
@@ -181,7 +192,7 @@ __device__ __forceinline__ void pt_step(const pt_row &r, float &m, float &l, F b
         }
     }
     uint32_t pk[W / 2];
-    if (r.cut) {                                  // all on the MUFU: the FMA pipe's pairs give 2^-126 for -infinity, which a value could lift
+    if (r.cut) {                                  // all on the MUFU, whose weight of a hidden key, 2^-infinity, is exactly 0
         float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int i = 0; i < W / 2; i++) {
@@ -191,10 +202,8 @@ __device__ __forceinline__ void pt_step(const pt_row &r, float &m, float &l, F b
             sum = __fadd2_rn(sum, make_float2(p0, p1));
         }
         l += sum.x + sum.y;
-    } else if constexpr (W == 128) {
-        l += at_softmax_row(v, r.sl2, m, pk);
     } else {
-        l += pt_weights(v, r.sl2, m, pk);
+        l += pt_weights<W>(v, r.sl2, m, pk);
     }
     if constexpr (W == 128) tmem_st64(r.tS, pk);
     else pt_st32(r.tS, pk);
