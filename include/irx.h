@@ -217,9 +217,9 @@ IRX_API int irx_compile_rope_append(const irx_kv_cache_t *cache, const irx_rope_
  * or leave the rows, or that begins below an earlier start, is skipped and reported; one of no tokens is none. What a
  * mask hides has no effect, infinities and NaN among it. bf16 with head_dim a multiple of 8 and 16-byte aligned rows
  * takes the matrix instructions (weights rounded to bf16, sums f32), everything else f32 units. A weight below 2^-126 of
- * the row's largest may count as zero, and then adds nothing, however large its value. Values times the keys seen have to
- * stay in f32's range. head_dim up to 256, tokens up to 2^30, batch up to 2^16. A row's bits depend on its own sequence
- * alone. Units: key-value heads. */
+ * the row's largest may count as zero, and then adds nothing, however large its value; one that is infinite or NaN makes
+ * every row that sees it infinite or NaN. Values times the keys seen have to stay in f32's range. head_dim up to 256, tokens
+ * up to 2^30, batch up to 2^16. A row's bits depend on its own sequence alone. Units: key-value heads. */
 typedef struct irx_prompt {
     int dtype;
     long long tokens;

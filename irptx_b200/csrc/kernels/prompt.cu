@@ -228,7 +228,7 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
         }
         for (int kt = 0; kt < ntiles; kt++) {
             const int kb = begin(kt), kend = end(kt), nk = min(PS_KEYS, kend - kb);
-            // a tile that some row does not see in whole: masked, and its weights of zero add nothing
+            // a tile that some row does not see in whole: masked, and what is hidden passed over
             const bool cut = kt < nsink || nk < PS_KEYS || kb + PS_KEYS - 1 > first || (p.window && kb <= last - p.window);
             cp_wait<0>();
             __syncthreads();                             // the keys are there, the values before are done with
@@ -275,9 +275,9 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
                 float sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    s[i][j] = exp2f(s[i][j] - mn);
-                    sum += s[i][j];
-                    sp[(ty * R + i) * 64 + tx + (16 * j ^ odd << 4)] = s[i][j];
+                    const float w = exp2f(s[i][j] - mn);
+                    sum += w;                            // a weight of -0: of a score of -infinity, not one that vanished
+                    sp[(ty * R + i) * 64 + tx + (16 * j ^ odd << 4)] = s[i][j] == -INFINITY ? -0.0f : w;
                 }
                 m[i] = mn;
                 l[i] = l[i] * r + sum;                   // of this lane's keys: joined at the end
@@ -302,7 +302,7 @@ __device__ __forceinline__ void ps_body(const irx_kprm_t &p)
                         const float4 x = *reinterpret_cast<const float4 *>(sv + (j0 + j) * DP + g * 64 + tx * 4);
 #pragma unroll
                         for (int i = 0; i < R; i++) {
-                            if (cut && w[i][j] == 0.0f) continue;
+                            if (cut && __float_as_uint(w[i][j]) == 0x80000000u) continue;
                             o[i][g * 2] = __ffma2_rn(make_float2(w[i][j], w[i][j]), make_float2(x.x, x.y), o[i][g * 2]);
                             o[i][g * 2 + 1] = __ffma2_rn(make_float2(w[i][j], w[i][j]), make_float2(x.z, x.w), o[i][g * 2 + 1]);
                         }

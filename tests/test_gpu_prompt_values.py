@@ -36,3 +36,18 @@ def test_a_large_value_of_no_weight(cuda, irx, dtype, heads, d, window, at):
     out, lse = attend(cuda, irx, dtype, heads, d, n, [0.0 if j == at else -300.0 for j in range(n)], values, window)
     see = slice(at, at + window if window else n)
     assert bool((out[see] == 1.0).all()) and bool((lse[see].abs() <= (7.6e-5 if dtype == "bf16" else 0.0)).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("heads,d", [(1, 64), (4, 128), (3, 80), (2, 256), (1, 33)])
+@pytest.mark.parametrize("window,at", [(0, 5), (0, 130), (0, 400), (400, 150)])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_an_infinite_value_shows_in_every_row_that_sees_it(cuda, irx, dtype, heads, d, window, at, value):
+    """Key 0 has the score 0, the others -300: `value` stands behind a weight that vanishes, in tiles seen in part and in
+    whole. Rows that see it are infinite or NaN, the others 1."""
+    n = 700
+    out, lse = attend(cuda, irx, dtype, heads, d, n, [0.0] + [-300.0] * (n - 1), [value if j == at else 1.0 for j in range(n)], window)
+    see = cuda.zeros(n, dtype=cuda.bool, device="cuda")
+    see[at:at + window if window else n] = True
+    assert not bool(out[see].isfinite().any()) and bool((out[~see] == 1.0).all())
+    assert bool(lse.isfinite().all())
