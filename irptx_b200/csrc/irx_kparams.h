@@ -225,7 +225,7 @@ typedef struct {
     int32_t     batch, heads, kv_heads, group, d;
     int32_t     h0, h1;             /* kv heads of this launch (a shard) */
     int32_t     window, sinks;
-    float       scale2;             /* scale * log2(e), not zero */
+    float       scale2;             /* scale * log2(e) */
     uint8_t     dt, vec, pad[2];
 } irx_kprm_t;
 

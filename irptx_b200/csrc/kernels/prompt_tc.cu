@@ -140,9 +140,10 @@ __device__ __forceinline__ float pt_weights(const float (&v)[W], float sl2, floa
 struct pt_row {
     uint32_t tS, tO;
     int up, low, sink;                          // the columns seen: up to `up`, and from `low` on or before `sink`
-    bool cut, negate, first;
-    float sl2;
+    bool cut, other, first;                     // other: a scale that is not above 0
+    float scale2, sl2;                          // sl2: above 0, since hidden scores are -infinity times it
 };
+__device__ __forceinline__ float pt_sl2(float scale2) { return scale2 == 0.0f ? 1.0f : fabsf(scale2); }
 
 template <int DP, int W, class F>
 __device__ __forceinline__ void pt_step(const pt_row &r, float &m, float &l, F before)
@@ -150,9 +151,10 @@ __device__ __forceinline__ void pt_step(const pt_row &r, float &m, float &l, F b
     float v[W];
     if constexpr (W == 128) tmem_ld128(r.tS, v);
     else pt_ld64(r.tS, v);
-    if (r.negate) {
+    if (r.other) {                                // the rest of the scale: a sign, or 0
+        const float by = r.scale2 < 0.0f ? -1.0f : 0.0f;
 #pragma unroll
-        for (int c = 0; c < W; c++) v[c] = -v[c];
+        for (int c = 0; c < W; c++) v[c] *= by;
     }
     if (r.cut) {
 #pragma unroll
@@ -431,7 +433,7 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
         const int t = warp >> 2, r = (warp & 3) * 32 + lane;
         const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tbase + tl + t * 128, tO = tbase + tl + 256 + t * 128;
-        const float sl2 = fabsf(p.scale2);
+        const float sl2 = pt_sl2(p.scale2);
         uint4 *stage = reinterpret_cast<uint4 *>(sv + 2 * TILE + 1024) + warp * 256;
         const int inv_g = (65535 + g) / g, tok_stride = p.heads * p.d;        // row / g = (row * inv_g) >> 16 below 128
         const int mytok = t * tp + r / g, myhead = r % g;      // within the unit, within the group
@@ -459,7 +461,7 @@ __device__ __forceinline__ void pt_body(const irx_kprm_t &p)
                     tc_fence_after();
                     return ok;
                 };
-                const pt_row row = {tS, tO, up, low, p.sinks - kb, edge || j < f.nsink || kb + 127 > first, p.scale2 < 0.0f, j == 0, sl2};
+                const pt_row row = {tS, tO, up, low, p.sinks - kb, edge || j < f.nsink || kb + 127 > first, !(p.scale2 > 0.0f), j == 0, p.scale2, sl2};
                 if (pt_narrow<DP>(f, j)) pt_step<DP, 64>(row, m, l, done_before);
                 else pt_step<DP, 128>(row, m, l, done_before);
                 if (!ok) break;

@@ -225,7 +225,7 @@ extern "C" __global__ void __launch_bounds__(256, 1) irx_prompt_tc_256(const __g
     } else {                                                   // softmax: four warps a tile
         const int r = warp * 32 + lane;
         const uint32_t tS = tbase + ((uint32_t)(warp * 32) << 16), tO = tS + 256;
-        const float sl2 = fabsf(p.scale2);
+        const float sl2 = pt_sl2(p.scale2);
         uint4 *stage = reinterpret_cast<uint4 *>(sv + RING * KT + 1024) + warp * 256;
         const int inv_g = (65535 + g) / g, tok_stride = p.heads * p.d;        // row / g = (row * inv_g) >> 16 below 128
         const int mytok = r / g, myhead = r % g;               // within the unit, within the group
@@ -252,7 +252,7 @@ extern "C" __global__ void __launch_bounds__(256, 1) irx_prompt_tc_256(const __g
                     tc_fence_after();
                     return ok;
                 };
-                const pt_row row = {tS + b * 64, tO, up, low, p.sinks - kb, edge || j < f.nsink || kb + 63 > first, p.scale2 < 0.0f, j == 0, sl2};
+                const pt_row row = {tS + b * 64, tO, up, low, p.sinks - kb, edge || j < f.nsink || kb + 63 > first, !(p.scale2 > 0.0f), j == 0, p.scale2, sl2};
                 pt_step<DP, 64>(row, m, l, done_before);
                 if (!ok) break;
                 tc_fence_before();

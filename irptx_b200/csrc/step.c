@@ -249,10 +249,8 @@ static int launch_prompt(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
     k.batch = a->batch; k.heads = a->heads; k.kv_heads = a->kv_heads; k.group = a->heads / a->kv_heads; k.d = a->dim;
     k.h0 = (int32_t)u0; k.h1 = (int32_t)u1;
     k.window = a->window; k.sinks = a->sinks;
-    /* a masked score is -inf times this, so it must not be 0; 2^-120 of a finite score is as good as 0 */
     k.scale2 = (float)((double)scale * 1.4426950408889634);
     if (!isfinite(k.scale2)) k.scale2 = scale < 0 ? -3.4028234663852886e38f : 3.4028234663852886e38f;
-    if (fabsf(k.scale2) < 7.5e-37f) k.scale2 = k.scale2 < 0 ? -7.5e-37f : 7.5e-37f;
     k.dt = a->dt;
     k.vec = (uint8_t)(a->dim % al == 0 && a->q_stride % al == 0 && a->kv_stride % al == 0 && a_to(k.q, 16) && a_to(k.k, 16) &&
                       a_to(k.v, 16) && a_to(k.o, 16));
