@@ -136,7 +136,7 @@ typedef struct irx_kv_cache {
  * each. Keys whose table entry names no page of the pool are left out as the mask's are (a sequence
  * that keeps none of its keys: NaN, and -inf), and a length outside 0 to table_cols * page_size
  * counts as the nearer end; both are reported. Sums of weights times values are f32 and divided at
- * the end: values times the keys seen have to stay in its range. The result is the same bits for the
+ * the end: values times the keys seen have to stay in its range; a scale past 2.35e38 is refused. The result is the same bits for the
  * same inputs on the same GPU; a sequence's last places depend on where the others' lengths, and a
  * shard's heads, place its cuts. Units: key-value heads. */
 IRX_API int irx_compile_decode(const irx_kv_cache_t *cache, int heads, long long q_stride, float scale, int window, int sinks,
@@ -218,8 +218,9 @@ IRX_API int irx_compile_rope_append(const irx_kv_cache_t *cache, const irx_rope_
  * mask hides has no effect, infinities and NaN among it. bf16 with head_dim a multiple of 8 and 16-byte aligned rows
  * takes the matrix instructions (weights rounded to bf16, sums f32), everything else f32 units. A weight below 2^-126 of
  * the row's largest may count as zero, and then adds nothing, however large its value; one that is infinite or NaN makes
- * every row that sees it infinite or NaN. Values times the keys seen have to stay in f32's range. head_dim up to 256, tokens
- * up to 2^30, batch up to 2^16. A row's bits depend on its own sequence alone. Units: key-value heads. */
+ * every row that sees it infinite or NaN. Products of queries and keys, scores and values times the keys seen have to stay in
+ * f32's range; a scale past 2.35e38 is refused. head_dim up to 256, tokens up to 2^30, batch up to 2^16. A row's bits depend
+ * on its own sequence alone. Units: key-value heads. */
 typedef struct irx_prompt {
     int dtype;
     long long tokens;

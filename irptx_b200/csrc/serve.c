@@ -93,6 +93,7 @@ int irx_compile_decode(const irx_kv_cache_t *cache, int heads, long long q_strid
     if (window < 0 || sinks < 0) return irx_fail(E042, "a window or sink count below 0");
     if (sinks && !window) return irx_fail(E042, "sinks without a window");
     if (!(scale == scale) || scale - scale != 0.0f) return irx_fail(E042, "a scale that is not finite");
+    if (scale > MAX_SCALE || scale < -MAX_SCALE) return irx_fail(E042, "a scale past 2.35e38, which f32 does not hold times log2(e)");
     qrow = (int64_t)heads * a->c.dim;
     if (q_stride < 0 || q_stride > MAX_STRIDE || (q_stride && q_stride < qrow))
         return irx_fail(E042, "query rows that overlap");

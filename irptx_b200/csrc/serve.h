@@ -12,6 +12,7 @@
 #define MAX_DIM 256
 #define MAX_COUNT 0x7fffffffll
 #define MAX_STRIDE (1ll << 40)
+#define MAX_SCALE 2.35e38f                 /* of scores: times log2(e) still an f32 number */
 #define MAX_SPAN 9e17                      /* elements; sums of a few stay below 2^63 */
 
 static inline int esz(int dt) { return dt == DT_BF16 ? 2 : dt == DT_U8 ? 1 : 4; }

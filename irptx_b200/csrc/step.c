@@ -202,6 +202,7 @@ int irx_compile_prompt(const irx_prompt_t *m, irx_plan_t *plan)
     if (m->window < 0 || m->sinks < 0) return irx_fail(E042, "a window or sink count below 0");
     if (m->sinks && !m->window) return irx_fail(E042, "sinks without a window");
     if (!isfinite(m->scale)) return irx_fail(E042, "a scale that is not finite");
+    if (fabsf(m->scale) > MAX_SCALE) return irx_fail(E042, "a scale past 2.35e38, which f32 does not hold times log2(e)");
     qrow = (int64_t)m->heads * m->head_dim;
     krow = (int64_t)m->kv_heads * m->head_dim;
     if (m->q_stride < 0 || m->q_stride > MAX_STRIDE || (m->q_stride && m->q_stride < qrow) || m->kv_stride < 0 ||
@@ -250,7 +251,6 @@ static int launch_prompt(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
     k.h0 = (int32_t)u0; k.h1 = (int32_t)u1;
     k.window = a->window; k.sinks = a->sinks;
     k.scale2 = (float)((double)scale * 1.4426950408889634);
-    if (!isfinite(k.scale2)) k.scale2 = scale < 0 ? -3.4028234663852886e38f : 3.4028234663852886e38f;
     k.dt = a->dt;
     k.vec = (uint8_t)(a->dim % al == 0 && a->q_stride % al == 0 && a->kv_stride % al == 0 && a_to(k.q, 16) && a_to(k.k, 16) &&
                       a_to(k.v, 16) && a_to(k.o, 16));
