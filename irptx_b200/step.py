@@ -49,12 +49,15 @@ def _number(name: str, v) -> float:
 
 
 def rope_freqs(rot: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, original: float = 0,
-               fast: float = 32.0, slow: float = 1.0) -> list[float]:
+               fast: float | None = None, slow: float = 1.0) -> list[float]:
     """The rot / 2 rotation frequencies base ** (-2 i / rot), in radians a position, scaled for a context ``factor``
-    times the ``original`` one: "linear", "ntk", "yarn" or "bands" (``irx_rope_freqs``). YaRN's
+    times the ``original`` one: "linear", "ntk", "yarn" or "bands" (``irx_rope_freqs``). Pairs that turn more than
+    ``fast`` times within the original context are kept: 32 unless given, with "bands" 4. YaRN's
     amplitude, 0.1 ln(factor) + 1, is the caller's to give to :func:`rope`."""
     if scaling not in _SCALING:
         _refuse(42, f"a scaling {scaling!r} ({', '.join(_SCALING)})")
+    if fast is None:
+        fast = 4.0 if scaling == "bands" else 32.0
     out = (ctypes.c_double * max(1, min(_int("rot", rot), 256)))()
     if _irx._lib().irx_rope_freqs(_int("rot", rot), float(base), _SCALING[scaling], float(factor), float(original), float(fast),
                                   float(slow), out):
