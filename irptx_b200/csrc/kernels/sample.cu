@@ -589,8 +589,8 @@ template <class T, bool FAR>
 __device__ __forceinline__ void smp_body(const irx_ksmp_t &p)
 {
     typedef smp_type<T> ty;
-    irx_pdl_enter();
     cluster_arrive();                                    // (waited for before the first exchange)
+    irx_pdl_enter();
     extern __shared__ __align__(16) unsigned char smp_bytes[];
     smp_shared &sh = *reinterpret_cast<smp_shared *>(smp_bytes);
     unsigned *data = reinterpret_cast<unsigned *>(smp_bytes + IRX_SMP_FIXED);
