@@ -146,8 +146,8 @@ __device__ __forceinline__ int64_t pr_turn(int i)
 // values arrive while scores are computed and the next keys during the second product; two blocks fit an SM up to 128
 // columns. A thread holds R x 4 scores and R rows x DP / 16 columns of the output in registers and multiplies two numbers an
 // instruction; a 16-byte read costs its four accesses of the shared memory also where lanes read the same, so at R = 4 that
-// memory is busier than the FP32 units (71 and 61 %). R = 8 (128 threads) reads less (44 and 56 %) and has half the warps: 161 against 170 us
-// for 2222 tokens in five prompts, 16 heads on 4 of 128; at 64 columns 122 against 95, so 4 there, and above 128, where the
+// memory is busier than the FP32 units (71 and 61 %). R = 8 (128 threads) reads less (44 and 56 %) and has half the warps: 147 against 154 us
+// for 2093 tokens in five prompts, 16 heads on 4 of 128; at 64 columns 87 against 86, so 4 there, and above 128, where the
 // registers end. A key row's groups of four floats are permuted by the row's place in its eight, so that the 16 key
 // rows read together fall into different banks.
 #define PS_ROWS 64

@@ -38,7 +38,7 @@ __device__ __forceinline__ int pt_key(const pt_info &f, int j) { return j < f.ns
 
 // Whether the unit needs only the first 64 keys of tile j: the sinks' or the last one, when that is all there is. Not for
 // head sizes up to 64, whose softmax bounds them: a second form of its step in the loop costs the first more than
-// it saves (window with sinks 395 us with it, 344 without).
+// it saves (window with sinks 365 us with it, 352 without).
 template <int DP>
 __device__ __forceinline__ bool pt_narrow(const pt_info &f, int j) { return DP != 64 && (j < f.nsink ? f.sk : f.end) - pt_key(f, j) <= 64; }
 
@@ -99,9 +99,17 @@ __device__ __forceinline__ uint32_t pt_less(uint32_t x)
     return d;
 }
 
-// at_softmax_row (attn.cu) for W scores: P = 2^(s * sl2 - m) as bf16 pairs, and their sum. What differs: the FMA pipe's
-// pairs, which end at 2^-126, lose that much once rounded, so that a weight below it is 0 on either pipe and adds nothing, however
-// large its value. (Half a step of a bf16 weight from 2^-116 on is more than that: those are the same bits.)
+// at_softmax_row (attn.cu) for W scores: P = 2^(s * sl2 - m) as bf16 pairs, and their sum.
+//
+// Weights are rounded to bf16, the product's type; the row's sum is of the weights as they were. The output is then 0.0018 to
+// 0.0022 off the definition (norms), where its own rounding makes 0.0016. Weights as two bf16 numbers and two products, as the
+// decode kernel has, for which they are no work, bring that to 0.0016 but cost a third to four fifths here: 16001 tokens 3310 us
+// against 2115, a ragged batch 415 against 232, a window with sinks 470 against 358, 37 tokens 10.2 against 8.0 (the second
+// halves in the scores' other columns).
+//
+// What differs from at_softmax_row: the FMA pipe's pairs, which end at 2^-126, lose that much once rounded, so that a weight
+// below it is 0 on either pipe and adds nothing, however large its value. (From 2^-116 on that is less than half a step of a
+// bf16 weight: those are the same bits.)
 template <int W>
 __device__ __forceinline__ float pt_weights(const float (&v)[W], float sl2, float m, uint32_t (&pk)[W / 2])
 {

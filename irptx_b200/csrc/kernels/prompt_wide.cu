@@ -5,7 +5,8 @@
 // there, the other tile's products, is here the tile's own: its scores have two buffers, and those of the next step
 // are computed during a step's softmax. (For head sizes up to 128 this form is the slower one: a product 64 keys
 // wide takes as long as one of 128, its queries' rows being what it waits for. 16001 tokens of 128: 2.38 against 2.10 ms.)
-// Before it, these head sizes took FP32 units: 2000 tokens, 8 heads of 256, 1135 us, now 45.
+// Before it, these head sizes took FP32 units: 2000 tokens, 8 heads of 256, 1135 us, now 42; 8000 tokens, 16 heads on 4 of 256,
+// 528 us (992 TFLOP/s), of 192, computed as 256, 487.
 #pragma once
 #include "prompt_tc.cu"
 

@@ -332,8 +332,9 @@ static int launch_sample(const irx_plan_int_t *p, irx_dev_t *d, unsigned s, unsi
     for (j = 0; j < 128; j++) k.tab[j] = ldexp(exp2(j / 128.0), k.kbits);
     /* Blocks of a cluster: as few as hold the row in their shared memory, since every block pays for the row's settings
      * and exchanges. With few rows more, down to 4096 elements each, as long as all rows' blocks run at once. Measured
-     * with 2, 4 and 8 blocks: 64 rows of 128001 bf16 logits, top-k and top-p, 23, 29, 49 us; f32 (2 do not hold it) 40 with 4, 52
-     * with 8; 256 rows of 151999, top-p, bf16 185, 192, 267, f32 260 with 4, 286 with 8; one row of 128001 30, 22, 17. */
+     * with 2, 4 and 8 blocks: 64 rows of 128001 bf16 logits, top-k and top-p, 28, 38, 55 us; f32 (2 do not hold it) 52 with 4, 61
+     * with 8; 256 rows of 151999, top-p, bf16 216, 202, 267 (the filters are on the device: the rule does not see them), f32 293
+     * with 4, 318 with 8; one row of 128001 f32 17.7 with 4, 15.4 with 8. */
     for (nc = 1;; nc *= 2) {
         words = (a->vocab + epw - 1 + nc * epw * IRX_SMP_THREADS - 1) / (nc * epw * IRX_SMP_THREADS) | 1;
         if (nc == 8) break;
