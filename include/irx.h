@@ -216,7 +216,7 @@ IRX_API int irx_compile_rope_append(const irx_kv_cache_t *cache, const irx_rope_
  * rows outside every sequence are not read into any result and are left as they were. A sequence whose starts fall
  * or leave the rows, or that begins below an earlier start, is skipped and reported; one of no tokens is none. What a
  * mask hides has no effect, infinities and NaN among it. bf16 with head_dim a multiple of 8 and 16-byte aligned rows
- * takes the matrix instructions (weights rounded to bf16, sums f32), everything else f32 units. A weight below 2^-126 of
+ * takes the matrix instructions (weights rounded to bf16, sums f32), everything else f32 units. A weight below 2^-118 of
  * the row's largest may count as zero, and then adds nothing, however large its value; one that is infinite or NaN makes
  * every row that sees it infinite or NaN. Products of queries and keys, scores and values times the keys seen have to stay in
  * f32's range; a scale past 2.35e38 is refused. head_dim up to 256, tokens up to 2^30, batch up to 2^16. A row's bits depend

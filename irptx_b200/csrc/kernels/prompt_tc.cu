@@ -142,9 +142,11 @@ __device__ __forceinline__ float pt_weights(const float (&v)[W], float sl2, floa
     return (sa.x + sa.y) + (sb.x + sb.y);
 }
 
-// One softmax step of a row over W scores: masked, exponentials over the scores' columns, and into m and l. O and l keep a
-// maximum up to a factor of 256 behind (attn.cu); each row decides for itself, so that its bits do not depend on the
-// others of its warp. before(): waits until O is this warp's to rescale.
+// One softmax step of a row over W scores: masked, exponentials 2^(x - m) over the scores' columns, and into m and l. m is set
+// PT_LAG above a maximum and moves when one passes it (attn.cu's lag of a factor of 256, from above: no weight is over 1, and O
+// stays within the values' sum). Each row decides for itself, so that its bits do not depend on the others of its warp. before(): waits
+// until O is this warp's to rescale.
+#define PT_LAG 8.0f
 struct pt_row {
     uint32_t tS, tO;
     int up, low, sink;                          // the columns seen: up to `up`, and from `low` on or before `sink`
@@ -182,15 +184,15 @@ __device__ __forceinline__ void pt_step(const pt_row &r, float &m, float &l, F b
     }
     mk[0] = pt_max3(mk[0], v[W / 4 - 1], v[W / 2 - 1]);
     mk[1] = pt_max3(mk[1], v[3 * W / 4 - 1], v[W - 1]);
-    float mnew = pt_max3(m, pt_max3(mk[0], mk[1], mk[2]) * r.sl2, mk[3] * r.sl2);
-    mnew = mnew < INFINITY ? mnew : NAN;          // a score that is NaN or infinite: the row is NaN
-    const bool grown = !(mnew <= m + 8.0f);
+    float top = pt_max3(-3.0e38f, pt_max3(mk[0], mk[1], mk[2]) * r.sl2, mk[3] * r.sl2);
+    top = top < INFINITY ? top : NAN;            // a score that is NaN or infinite: the row is NaN
+    const bool grown = !(top <= m);
     if (r.first) {
-        m = mnew;
+        m = top + PT_LAG;
     } else if (__any_sync(0xffffffffu, grown)) {
         if (!before()) return;
-        const float alpha = grown ? at_ex2(m - mnew) : 1.0f;
-        if (grown) m = mnew;
+        const float alpha = grown ? at_ex2(m - (top + PT_LAG)) : 1.0f;
+        if (grown) m = top + PT_LAG;
         l *= alpha;
 #pragma unroll 1
         for (int cc = 0; cc < DP / 32; cc++) {

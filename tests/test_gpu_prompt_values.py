@@ -51,3 +51,17 @@ def test_an_infinite_value_shows_in_every_row_that_sees_it(cuda, irx, dtype, hea
     see[at:at + window if window else n] = True
     assert not bool(out[see].isfinite().any()) and bool((out[~see] == 1.0).all())
     assert bool(lse.isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("heads,d", [(1, 64), (4, 128), (3, 80), (2, 256), (1, 33)])
+@pytest.mark.parametrize("step", [0.0, 5.5, 11.0, -5.5])
+def test_values_times_keys_within_the_range(cuda, irx, dtype, heads, d, step):
+    """300 values of 2^119 have a sum below 2^128. Scores that rise by 5.5 after every 128 keys (weights 245 times those before, which
+    the running maximum may lag behind) leave it there: every row's result is the value."""
+    n = 300
+    out, lse = attend(cuda, irx, dtype, heads, d, n, [step * (j // 128) for j in range(n)], [2.0 ** 119] * n)
+    # equal values: the weights' sum over itself, n + 2 roundings of 2^-24 in f32; on the matrix path weights 2^-9 and 1e-4 off and
+    # the result's half step, 2^-9 below or at 2^119 and 2^-8 above
+    off = 2.0 ** -8 + 2.0 ** -9 + 1e-4 if dtype == "bf16" else (n + 2) * 2.0 ** -24 * 2
+    assert bool(((out.double() / 2.0 ** 119 - 1.0).abs() <= off).all()) and bool(lse.isfinite().all())
