@@ -219,9 +219,9 @@ IRX_API int irx_compile_rope_append(const irx_kv_cache_t *cache, const irx_rope_
  * 128 query heads a key-value head takes the matrix instructions (weights rounded to bf16, sums f32), everything else f32
  * units. A weight below 2^-118 of the row's largest may count as zero, and then adds nothing, however large its value; a value
  * that is infinite or NaN makes every row that sees it infinite or NaN. Products of queries and keys and values times the
- * keys seen have to stay in f32's range, scores within 2e38; a scale past 2.35e38 is refused. head_dim up to 256, tokens up to 2^30, batch up to
- * 2^16 (each block looks through all starts for each of its units: thousands of short sequences cost that). A row's bits
- * depend on its own sequence alone. Units: key-value heads. */
+ * keys seen have to stay in f32's range, scores within 2e38; a scale past 2.35e38 is refused. head_dim up to 256, tokens up
+ * to 2^30, batch up to 2^16 (each block looks through all starts for each of its units: thousands of short sequences cost
+ * that). A row's bits depend on its own sequence alone. Units: key-value heads. */
 typedef struct irx_prompt {
     int dtype;
     long long tokens;
